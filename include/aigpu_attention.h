@@ -514,6 +514,142 @@ typedef struct AiGpuSelectKeys {
 AIGPU_ABI int aigpu_select_keys(const AiGpuSelectKeys* args);
 
 /* ------------------------------------------------------------------------ */
+/* 11. Rotary positions (the inlined loop of LocalModel.hpp:2624-2648 as an  */
+/*    operator of its own, for q and keys that go to aigpu_attention_device).*/
+/*    Per token at position p and head, with n = rotaryDims / 2 and pair j   */
+/*    made of elements (j, j + n), or (2j, 2j + 1) when interleaved:         */
+/*      a = p frequencies[j]                                                 */
+/*      (u, w) -> amplitude (u cos a - w sin a, w cos a + u sin a)           */
+/*    and elements from rotaryDims on copied. transpose = 1 turns by -a (the */
+/*    amplitude still multiplies): the gradient of x from the gradient of    */
+/*    out. The angle is formed in 64 bits, so far positions keep their       */
+/*    fp32-exact cosine (the reference, and the entries above, round it to   */
+/*    fp32 first: 3e-3 radians at position 100000); the rotation itself is   */
+/*    fp32, rounded once to `type`. out may be x (same strides); other       */
+/*    overlaps are refused. Asynchronous; needs no scratch, so calls on      */
+/*    different streams are not ordered by the backend.                      */
+/* ------------------------------------------------------------------------ */
+typedef struct AiGpuRotary {
+    const void* x;            /* element (token, head, d) at token*tokenStride + head*headStride + d, type */
+    void* out;                /* the same with the out strides, type */
+    const uint32_t* positions;/* [count], or NULL: start, start + 1, ... */
+    const float* frequencies; /* [rotaryDims/2] */
+    float amplitude;          /* of cos and sin (scaled long contexts); 0 means 1 */
+    uint32_t rotaryDims;      /* even, 2 .. dim */
+    uint32_t type;            /* AIGPU_F32 / AIGPU_BF16 */
+    uint32_t interleaved, transpose, reserved;
+    uint64_t count, start, heads, dim;
+    uint64_t tokenStride, headStride;       /* 0 mean heads*headStride and dim */
+    uint64_t outTokenStride, outHeadStride; /* 0 likewise */
+    void* stream;
+} AiGpuRotary;
+AIGPU_ABI int aigpu_rotary(const AiGpuRotary* args);
+
+/* The frequency table that rotations take, on the host (LocalModel.hpp:807-820
+   builds the first, second and fourth kind; computed here in 64 bits and
+   rounded once). With f_j = base^(-2j / dims):
+     NONE    f_j
+     LINEAR  f_j / factor
+     NTK     f_j with base * factor^(dims / (dims - 2)) as the base
+     LLAMA3  f_j / factor where a turn takes more than original / low
+             positions, f_j below original / high, blended between
+     YARN    f_j / factor for pairs of at most `low` turns over `original`
+             positions, f_j from `high` turns on, a ramp over the pair index
+             between; amplitude 0.1 ln(factor) + 1
+   *amplitude (optional) is what the rotations' amplitude takes. Needs no
+   device. */
+enum { AIGPU_ROTARY_NONE = 0, AIGPU_ROTARY_LINEAR = 1, AIGPU_ROTARY_NTK = 2, AIGPU_ROTARY_LLAMA3 = 3,
+       AIGPU_ROTARY_YARN = 4 };
+typedef struct AiGpuRotaryScaling {
+    uint32_t kind;            /* AIGPU_ROTARY_* */
+    uint32_t dims;            /* rotaryDims: even, at least 2 (4 for NTK) */
+    double base;              /* ropeTheta, > 1 */
+    double factor;            /* >= 1 (LINEAR and later) */
+    double original;          /* trained context (LLAMA3, YARN) */
+    double low, high;         /* LLAMA3: 1 and 4; YARN: 1 and 32 */
+} AiGpuRotaryScaling;
+AIGPU_ABI int aigpu_rotary_frequencies(const AiGpuRotaryScaling* scaling, float* frequencies, float* amplitude);
+
+/* ------------------------------------------------------------------------ */
+/* 12. A paged KV cache: the sequences of a batch keep their positions in    */
+/*    pages of pageSize positions from one pool, found through a table.      */
+/*    Position i of sequence b lies in page table[b][i / pageSize], row      */
+/*    i % pageSize. No counterpart in the reference, whose cache is one      */
+/*    contiguous run per layer. lengths[b] counts the cached positions with  */
+/*    the newest token's, for both entries: a step adds its tokens to the    */
+/*    lengths, then appends, then decodes. A length of 0 is an empty place   */
+/*    of a padded batch. A table entry is read only where a position of the  */
+/*    sequence needs it; the rest may hold anything.                         */
+/* ------------------------------------------------------------------------ */
+typedef struct AiGpuPagedCache {
+    void* keys;               /* bf16; element (page, head, row, d) at page*pageStride +       */
+    void* values;             /*   head*headStride + row*rowStride + d                         */
+    const uint32_t* table;    /* [batch][tableStride], the first tableWidth of each row */
+    const uint32_t* lengths;  /* [batch] */
+    uint64_t batch, pages, pageSize, kvHeads, dim;  /* dim 64, 96, 128, 192 or 256 */
+    uint64_t tableWidth, tableStride;               /* tableStride 0 means tableWidth */
+    uint64_t pageStride, headStride, rowStride;     /* all 0: [pages][kvHeads][pageSize][dim] */
+} AiGpuPagedCache;
+
+/* The newest tokens' k (normed and rotated on the way) and v into the pages,
+   rounded to bf16. Without `starts` there is one token a sequence (count =
+   batch). With it, rows starts[b] .. starts[b + 1] - 1 of k and v are the last
+   starts[b + 1] - starts[b] positions of sequence b, and rows before starts[0]
+   or from starts[batch] on are not read. A token whose position is negative
+   (a length below its new tokens), beyond the table or in a page outside the
+   pool is not written; a decode over such a length answers NaN. No two
+   tokens may share a row: a page shared by sequences is copied before either
+   writes to it. Asynchronous; needs no scratch, so calls on different streams
+   are not ordered by the backend. */
+typedef struct AiGpuPagedAppend {
+    AiGpuPagedCache cache;
+    const void* k;            /* [count][kvHeads][dim], inType; token t at t*kStride */
+    const void* v;            /* the same at t*vStride */
+    const uint32_t* starts;   /* [batch + 1], not decreasing, or NULL */
+    const float* kNorm;       /* [dim] gamma, NULL = no norm (LocalModel.hpp:2609-2617) */
+    const float* rotaryFrequencies; /* [rotaryDims/2], NULL = no rotation */
+    float epsilon, normOffset;
+    float amplitude;          /* as AiGpuRotary::amplitude */
+    uint32_t rotaryDims, interleaved, inType;
+    uint64_t count, kStride, vStride; /* strides 0 mean kvHeads*dim */
+    void* stream;
+} AiGpuPagedAppend;
+AIGPU_ABI int aigpu_paged_append(const AiGpuPagedAppend* args);
+
+/* Attention of the newest token of each sequence over its cached positions
+   (its own included: append first), q normed and rotated at position
+   lengths[b] - 1 on load. fp32 throughout but for the cache's bf16: q and the
+   softmax's weights enter the products in three bf16 terms each. A sequence of
+   length 0 gets zeros; one whose length exceeds maxLength, or that needs a page
+   outside the pool, gets NaN. Attended rows have to be finite (a value that is
+   not makes the heads that read it NaN); rows that no position covers may hold
+   anything. */
+typedef struct AiGpuPagedDecode {
+    AiGpuPagedCache cache;
+    const void* q;            /* [batch][heads][qStride], inType; sequence b at b*qTokenStride */
+    float* out;               /* [batch][heads][dim] fp32 */
+    const float* qNorm;
+    const float* rotaryFrequencies;
+    float epsilon, normOffset, amplitude;
+    float scale;              /* of the scores; 0 means 1/sqrt(dim) */
+    uint32_t rotaryDims, interleaved, inType;
+    uint32_t outputGate;      /* as AiGpuPrefill::outputGate */
+    uint32_t maxLength;       /* >= every lengths[b]; sizes the launch */
+    uint32_t reserved;
+    uint64_t heads, qStride, qTokenStride;  /* qStride 0 means dim, qTokenStride 0 heads*qStride */
+    uint64_t window;          /* the last `window` positions only; 0 = all */
+    void* workspace;          /* device, 256-byte aligned, or NULL: the backend's own scratch */
+    uint64_t workspaceBytes;
+    void* stream;
+} AiGpuPagedDecode;
+AIGPU_ABI int aigpu_paged_decode(const AiGpuPagedDecode* args);
+/* The workspace bytes that a call with these sizes needs at most (0: none),
+   whatever the lengths hold. Calls that may run at once need a workspace each.
+   A call captured into a graph has to bring one where this is not 0: the
+   backend's scratch may move. */
+AIGPU_ABI uint64_t aigpu_paged_decode_workspace(const AiGpuPagedDecode* args);
+
+/* ------------------------------------------------------------------------ */
 /* Per-kernel timing. With profiling on, every launch is bracketed by a pair */
 /* of hipEvents on the stream it runs on; aigpu_profile_read synchronises    */
 /* and reports the summed device time and launch count of kernels whose name */

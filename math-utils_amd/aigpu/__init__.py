@@ -12,6 +12,9 @@ Device forms (torch tensors on the GPU):
     prefill(...)            attentionMixer norm -> RoPE -> append -> attention
     decode(...)             batched ragged decode with norm/RoPE on load
     gated_delta_rule(...)   gatedDeltaNetMixer recurrence (chunked scan)
+    rotary(...)             rotary positions of strided heads, both pair layouts
+    paged_append(...)       new keys and values into a paged cache
+    paged_decode(...)       one token's attention over a paged cache
 """
 import ctypes as C
 import os
@@ -806,3 +809,251 @@ def select_keys(h, q_resid, weights, k_norm, k_norm_bias, ape, index_keys, index
                            startPos=start_pos, hidden=hidden, qRank=q_resid.shape[1], heads=heads, dim=dim,
                            topK=top_k, pool=pool, capacity=index_keys.shape[0], stream=_stream(stream))
     _check(lib().aigpu_select_keys(C.byref(args)))
+
+
+# ------------------------------------------------- 11 + 12. rotary positions, the paged cache
+class AiGpuRotary(C.Structure):
+    _fields_ = [("x", _vp), ("out", _vp), ("positions", _vp), ("frequencies", _vp), ("amplitude", _f32),
+                ("rotaryDims", _u32), ("type", _u32), ("interleaved", _u32), ("transpose", _u32), ("reserved", _u32),
+                ("count", _u64), ("start", _u64), ("heads", _u64), ("dim", _u64), ("tokenStride", _u64),
+                ("headStride", _u64), ("outTokenStride", _u64), ("outHeadStride", _u64), ("stream", _vp)]
+
+
+class AiGpuRotaryScaling(C.Structure):
+    _fields_ = [("kind", _u32), ("dims", _u32), ("base", C.c_double), ("factor", C.c_double),
+                ("original", C.c_double), ("low", C.c_double), ("high", C.c_double)]
+
+
+class AiGpuPagedCache(C.Structure):
+    _fields_ = [("keys", _vp), ("values", _vp), ("table", _vp), ("lengths", _vp), ("batch", _u64), ("pages", _u64),
+                ("pageSize", _u64), ("kvHeads", _u64), ("dim", _u64), ("tableWidth", _u64), ("tableStride", _u64),
+                ("pageStride", _u64), ("headStride", _u64), ("rowStride", _u64)]
+
+
+class AiGpuPagedAppend(C.Structure):
+    _fields_ = [("cache", AiGpuPagedCache), ("k", _vp), ("v", _vp), ("starts", _vp), ("kNorm", _vp),
+                ("rotaryFrequencies", _vp), ("epsilon", _f32), ("normOffset", _f32), ("amplitude", _f32),
+                ("rotaryDims", _u32), ("interleaved", _u32), ("inType", _u32), ("count", _u64), ("kStride", _u64),
+                ("vStride", _u64), ("stream", _vp)]
+
+
+class AiGpuPagedDecode(C.Structure):
+    _fields_ = [("cache", AiGpuPagedCache), ("q", _vp), ("out", _vp), ("qNorm", _vp), ("rotaryFrequencies", _vp),
+                ("epsilon", _f32), ("normOffset", _f32), ("amplitude", _f32), ("scale", _f32), ("rotaryDims", _u32),
+                ("interleaved", _u32), ("inType", _u32), ("outputGate", _u32), ("maxLength", _u32),
+                ("reserved", _u32), ("heads", _u64), ("qStride", _u64), ("qTokenStride", _u64), ("window", _u64),
+                ("workspace", _vp), ("workspaceBytes", _u64), ("stream", _vp)]
+
+
+SIGNATURES.update({
+    "aigpu_rotary": (C.c_int, [C.POINTER(AiGpuRotary)]),
+    "aigpu_rotary_frequencies": (C.c_int, [C.POINTER(AiGpuRotaryScaling), _vp, C.POINTER(_f32)]),
+    "aigpu_paged_append": (C.c_int, [C.POINTER(AiGpuPagedAppend)]),
+    "aigpu_paged_decode": (C.c_int, [C.POINTER(AiGpuPagedDecode)]),
+    "aigpu_paged_decode_workspace": (_u64, [C.POINTER(AiGpuPagedDecode)]),
+})
+
+ROTARY_KINDS = {None: 0, "none": 0, "linear": 1, "ntk": 2, "llama3": 3, "yarn": 4}
+
+
+def rotary_frequencies(rotary_dims, theta, scaling=None, factor=1.0, original=0.0, low=1.0, high=None):
+    """(fp32 numpy table of rotary_dims / 2 frequencies, amplitude) of
+    aigpu_rotary_frequencies; high defaults to 4 ("llama3") or 32 ("yarn")."""
+    if high is None:
+        high = 32.0 if scaling == "yarn" else 4.0
+    out, amplitude = np.zeros(max(rotary_dims // 2, 1), np.float32), _f32()
+    s = AiGpuRotaryScaling(ROTARY_KINDS[scaling], rotary_dims, theta, factor, original, low, high)
+    _check(lib().aigpu_rotary_frequencies(C.byref(s), out.ctypes.data, C.byref(amplitude)))
+    return out, amplitude.value
+
+
+def _same_device(first, name, *others):
+    """every tensor on the backend's device; `others` are (tensor or None, name)"""
+    import torch
+    for t, n in ((first, name),) + others:
+        if t is None:
+            continue
+        if not isinstance(t, torch.Tensor):
+            raise TypeError(f"{n} must be a torch.Tensor")
+        if not t.is_cuda or t.get_device() != 0:
+            raise ValueError(f"{n} must be on the backend's GPU, cuda:0")
+
+
+def _own_stream(stream):
+    """the stream given, or torch's current one of the backend's device"""
+    if stream is not None:
+        return stream
+    import torch
+    return torch.cuda.current_stream(0).cuda_stream
+
+
+def _whole(value, name, most=0xFFFFFFFFFFFFFFFF):
+    """the C structures would wrap what is out of range"""
+    if not 0 <= value <= most:
+        raise ValueError(f"{name} must be 0 .. {most}, not {value}")
+
+
+def _vector(t, name, least, exact=False):
+    """an fp32 vector of at least (or exactly) `least` elements, or None; its address"""
+    import torch
+    if t is None:
+        return None
+    if t.dtype != torch.float32 or t.dim() != 1 or (t.stride(0) != 1 and t.shape[0] > 1):
+        raise TypeError(f"{name} must be a contiguous float32 vector")
+    if t.shape[0] < least or (exact and t.shape[0] != least):
+        raise ValueError(f"{name} has {t.shape[0]} elements, {least} are needed")
+    return t.data_ptr()
+
+
+def _indices(t, name, dims, shape=None):
+    """an int32 (or uint32) tensor of `dims` dimensions with unit stride in the last; its address"""
+    import torch
+    if t.dtype not in (torch.int32, torch.uint32) or t.dim() != dims or (t.stride(-1) != 1 and t.shape[-1] > 1):
+        raise TypeError(f"{name} must be an int32 tensor of {dims} dimensions with unit stride")
+    if shape is not None and t.shape[0] != shape:
+        raise ValueError(f"{name} has {t.shape[0]} entries, {shape} are needed")
+    return t.data_ptr()
+
+
+def _strides(t, name):
+    """(token, head) element strides of a [tokens][heads][dim] tensor with
+    unit stride in the last dimension; a dimension of one has its dense one"""
+    n, heads, dim = t.shape
+    if t.stride(2) != 1 and dim > 1:
+        raise ValueError(f"{name} must have unit stride in its last dimension")
+    hs = t.stride(1) if heads > 1 else dim
+    ts = t.stride(0) if n > 1 else heads * hs
+    if ts <= 0 or hs <= 0:
+        raise ValueError(f"{name} must not be a broadcast view")
+    return ts, hs
+
+
+def rotary(x, out, freqs, positions=None, start=0, rotary_dims=None, interleaved=False, amplitude=1.0,
+           backward=False, stream=None):
+    """Rotary positions of x [tokens][heads][dim] (fp32 or bf16, any token and
+    head strides) into out (the same shape and type; may be x): pair j of the
+    first rotary_dims elements (default 2 len(freqs)) turns by position *
+    freqs[j], halves paired or neighbours (interleaved); the rest is copied.
+    positions [tokens] int32, or start, start + 1, ... backward=True gives x's
+    gradient from out's (the transposed rotation). Asynchronous."""
+    _same_device(x, "x", (out, "out"), (freqs, "freqs"), (positions, "positions"))
+    if x.dim() != 3 or out.shape != x.shape or out.dtype != x.dtype:
+        raise ValueError("x must be [tokens][heads][dim], and out of its shape and type")
+    count, heads, dim = x.shape
+    rot = 2 * freqs.shape[0] if rotary_dims is None else rotary_dims
+    _whole(rot, "rotary_dims", 4096)
+    _whole(start, "start", 0xFFFFFFFF)
+    if x.numel() == 0:
+        return out
+    ts, hs = _strides(x, "x")
+    ots, ohs = _strides(out, "out")
+    a = AiGpuRotary(x.data_ptr(), out.data_ptr(),
+                    None if positions is None else _indices(positions, "positions", 1, count),
+                    _vector(freqs, "freqs", rot // 2), amplitude, rot, _dtype_tag(x), 1 if interleaved else 0,
+                    1 if backward else 0, 0, count, start, heads, dim, ts, hs, ots, ohs, _own_stream(stream))
+    _check(lib().aigpu_rotary(C.byref(a)))
+    return out
+
+
+def _paged_cache(keys, values, table, lengths):
+    import torch
+    if keys.dtype != torch.bfloat16 or values.dtype != torch.bfloat16:
+        raise TypeError("the pages must be bfloat16")
+    if keys.dim() != 4 or values.shape != keys.shape or values.stride() != keys.stride():
+        raise ValueError("key and value pages must be [pages][kv_heads][page_size][dim] with the same strides")
+    pages, kv_heads, size, dim = keys.shape
+    ps, hs, rs, one = keys.stride()
+    if one != 1 and dim > 1:
+        raise ValueError("the pages must have unit stride in their last dimension")
+    # a dimension of one may carry any stride: give it one that is in range
+    rs = rs if size > 1 else dim
+    hs = hs if kv_heads > 1 else dim
+    ps = ps if pages > 1 else dim
+    batch = lengths.shape[0] if lengths.dim() == 1 else -1
+    width = table.shape[1] if table.dim() == 2 else 0
+    return AiGpuPagedCache(keys.data_ptr(), values.data_ptr(), _indices(table, "table", 2, batch),
+                           _indices(lengths, "lengths", 1), batch, pages, size, kv_heads, dim, width,
+                           table.stride(0) if batch > 1 else width, ps, hs, rs)
+
+
+def paged_append(k, v, key_pages, value_pages, table, lengths, starts=None, k_norm=None, eps=1e-6, norm_offset=0.0,
+                 freqs=None, rotary_dims=None, interleaved=False, amplitude=1.0, stream=None):
+    """The newest tokens' k (normed, rotated) and v [tokens][kv_heads][dim]
+    (fp32 or bf16, any token stride) into the bf16 pages
+    [pages][kv_heads][page_size][dim] (or a view with other strides), at the
+    places that table [batch][width] and lengths [batch] (the new tokens
+    included) say; starts [batch + 1] where a sequence has other than one.
+    Asynchronous."""
+    _same_device(k, "k", (v, "v"), (key_pages, "key_pages"), (value_pages, "value_pages"), (table, "table"),
+                 (lengths, "lengths"), (starts, "starts"), (k_norm, "k_norm"), (freqs, "freqs"))
+    cache = _paged_cache(key_pages, value_pages, table, lengths)
+    count = k.shape[0]
+    if k.dim() != 3 or k.shape[1] != cache.kvHeads or k.shape[2] != cache.dim or v.shape != k.shape \
+            or v.dtype != k.dtype:
+        raise ValueError("k and v must be [tokens][kv_heads][dim] of one type, as the pages have them")
+    if count == 0:
+        return
+    (ks, kh), (vs, vh) = _strides(k, "k"), _strides(v, "v")
+    if kh != cache.dim or vh != cache.dim:
+        raise ValueError("the heads of a token's k and v must lie one after the other")
+    rot = 0 if freqs is None else (2 * freqs.shape[0] if rotary_dims is None else rotary_dims)
+    _whole(rot, "rotary_dims", 4096)
+    a = AiGpuPagedAppend(cache, k.data_ptr(), v.data_ptr(),
+                         None if starts is None else _indices(starts, "starts", 1, cache.batch + 1),
+                         _vector(k_norm, "k_norm", cache.dim, True), _vector(freqs, "freqs", rot // 2), eps,
+                         norm_offset, amplitude, rot, 1 if interleaved else 0, _dtype_tag(k), count, ks, vs,
+                         _own_stream(stream))
+    _check(lib().aigpu_paged_append(C.byref(a)))
+
+
+def _paged_decode(q, out, key_pages, value_pages, table, lengths, max_length, q_norm, eps, norm_offset, freqs,
+                  rotary_dims, interleaved, amplitude, scale, window, output_gate, workspace, stream):
+    import torch
+    _same_device(q, "q", (out, "out"), (key_pages, "key_pages"), (value_pages, "value_pages"), (table, "table"),
+                 (lengths, "lengths"), (q_norm, "q_norm"), (freqs, "freqs"), (workspace, "workspace"))
+    cache = _paged_cache(key_pages, value_pages, table, lengths)
+    if q.dim() != 3 or q.shape[0] != cache.batch or q.shape[2] < cache.dim:
+        raise ValueError("q must be [batch][heads][at least dim]")
+    heads = q.shape[1]
+    if out.dtype != torch.float32 or tuple(out.shape) != (cache.batch, heads, cache.dim) or not out.is_contiguous():
+        raise ValueError("out must be a contiguous float32 [batch][heads][dim]")
+    ts, hs = _strides(q, "q") if q.numel() else (1, q.shape[2])
+    rot = 0 if freqs is None else (2 * freqs.shape[0] if rotary_dims is None else rotary_dims)
+    room, nbytes = None, 0
+    if workspace is not None:
+        if not workspace.is_contiguous():
+            raise ValueError("workspace must be contiguous")
+        room, nbytes = workspace.data_ptr(), workspace.numel() * workspace.element_size()
+    if max_length is None:
+        max_length = min(cache.tableWidth * cache.pageSize, 0xFFFFFFFF)
+    _whole(max_length, "max_length", 0xFFFFFFFF)
+    _whole(window, "window")
+    _whole(rot, "rotary_dims", 4096)
+    return AiGpuPagedDecode(cache, q.data_ptr(), out.data_ptr(), _vector(q_norm, "q_norm", cache.dim, True),
+                            _vector(freqs, "freqs", rot // 2), eps, norm_offset, amplitude, scale, rot,
+                            1 if interleaved else 0, _dtype_tag(q), 1 if output_gate else 0, max_length, 0, heads, hs,
+                            ts, window, room, nbytes, _own_stream(stream))
+
+
+def paged_decode(q, out, key_pages, value_pages, table, lengths, max_length=None, q_norm=None, eps=1e-6,
+                 norm_offset=0.0, freqs=None, rotary_dims=None, interleaved=False, amplitude=1.0, scale=0.0, window=0,
+                 output_gate=False, workspace=None, stream=None):
+    """Attention of each sequence's newest token over its cached positions:
+    q [batch][heads][dim] (fp32 or bf16; 2 dim wide with output_gate), normed
+    and rotated at lengths[b] - 1 on load; out [batch][heads][dim] fp32; the
+    pages, table and lengths as paged_append left them. max_length (default:
+    what the table can hold) is at least every length. A call captured into a
+    graph brings a workspace of paged_decode_workspace(...) bytes.
+    Asynchronous."""
+    a = _paged_decode(q, out, key_pages, value_pages, table, lengths, max_length, q_norm, eps, norm_offset, freqs,
+                      rotary_dims, interleaved, amplitude, scale, window, output_gate, workspace, stream)
+    if lengths.shape[0]:
+        _check(lib().aigpu_paged_decode(C.byref(a)))
+    return out
+
+
+def paged_decode_workspace(q, out, key_pages, value_pages, table, lengths, max_length=None):
+    """the bytes of a workspace for paged_decode calls of these sizes, whatever the lengths hold"""
+    a = _paged_decode(q, out, key_pages, value_pages, table, lengths, max_length, None, 1e-6, 0.0, None, None, False,
+                      1.0, 0.0, 0, False, None, None)
+    return int(lib().aigpu_paged_decode_workspace(C.byref(a)))

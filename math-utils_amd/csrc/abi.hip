@@ -1032,3 +1032,196 @@ AIGPU_ABI int aigpu_latent_attention(const AiGpuLatentAttention* args) {
 }
 
 } // extern "C"
+
+/* --------------------------------------------------------------- 11 + 12 */
+
+namespace {
+
+/* the backend's device current for the length of a call: the context is the
+   first device's, whatever device the calling thread has made current since */
+struct OnDevice {
+    int before = 0;
+    bool moved = false;
+    OnDevice() {
+        if (hipGetDevice(&before) == hipSuccess && before != 0) moved = hipSetDevice(0) == hipSuccess;
+    }
+    ~OnDevice() {
+        if (moved) (void)hipSetDevice(before);
+    }
+    OnDevice(const OnDevice&) = delete;
+    OnDevice& operator=(const OnDevice&) = delete;
+};
+
+/* argument errors are told first, so that they need no device to be seen */
+bool usable(Context& ctx, const char* who) {
+    return ctx.ok || ctx.fail(std::string(who) + ": no usable gfx950 device");
+}
+
+/* the cache as the kernels take it; sizes past these limits have no use and
+   would overflow the index arithmetic */
+bool paged_cache(Context& ctx, const char* who, const AiGpuPagedCache& a, aigpu::PagedCache& c) {
+    const std::string w = std::string(who) + ": ";
+    if (a.batch > (1u << 20) || a.kvHeads > 65535 || a.dim > 4096 || a.pages > 0x7FFFFFFFu)
+        return ctx.fail(w + "sizes out of range");
+    if (a.kvHeads == 0 || a.dim == 0 || a.pages == 0) return ctx.fail(w + "an empty pool");
+    if (a.pageSize == 0 || a.pageSize > (1u << 24)) return ctx.fail(w + "pageSize must be 1 .. 2^24");
+    if (a.tableWidth == 0 || a.tableWidth > 0x7FFFFFFFu) return ctx.fail(w + "tableWidth must be 1 .. 2^31 - 1");
+    c.tableStride = a.tableStride ? a.tableStride : a.tableWidth;
+    if (c.tableStride >= (uint64_t(1) << 40)) return ctx.fail(w + "tableStride out of range");
+    c.pageStride = a.pageStride;
+    c.headStride = a.headStride;
+    c.rowStride = a.rowStride;
+    if (a.pageStride == 0 && a.headStride == 0 && a.rowStride == 0) {
+        c.rowStride = a.dim;
+        c.headStride = a.pageSize * a.dim;
+        c.pageStride = a.kvHeads * c.headStride;
+    }
+    // the last element of the pool within 2^62
+    const uint64_t top = uint64_t(1) << 60;
+    if (c.rowStride > top / a.pageSize || c.headStride > top / a.kvHeads || c.pageStride > top / a.pages)
+        return ctx.fail(w + "page strides out of range");
+    c.keys = static_cast<uint16_t*>(a.keys);
+    c.values = static_cast<uint16_t*>(a.values);
+    c.table = a.table;
+    c.lengths = a.lengths;
+    c.batch = uint32_t(a.batch);
+    c.pages = uint32_t(a.pages);
+    c.pageSize = uint32_t(a.pageSize);
+    c.kvHeads = uint32_t(a.kvHeads);
+    c.dim = uint32_t(a.dim);
+    c.tableWidth = uint32_t(a.tableWidth);
+    return true;
+}
+
+bool paged_decode_params(Context& ctx, const AiGpuPagedDecode* args, aigpu::PagedDecodeParams& p) {
+    if (!paged_cache(ctx, "paged decode", args->cache, p.c)) return false;
+    if (args->heads > 65535) return ctx.fail("paged decode: heads out of range");
+    p.q = args->q;
+    p.out = args->out;
+    p.gamma = args->qNorm;
+    p.freqs = args->rotaryFrequencies;
+    p.eps = args->epsilon;
+    p.offset = args->normOffset;
+    p.amplitude = args->amplitude == 0.0f ? 1.0f : args->amplitude;
+    p.scale = args->scale == 0.0f ? 1.0f / sqrtf(float(args->cache.dim)) : args->scale;
+    p.rot = args->rotaryDims > 4096 ? -1 : int(args->rotaryDims);
+    p.interleaved = args->interleaved ? 1 : 0;
+    p.inType = args->inType > 1 ? -1 : int(args->inType);
+    p.outputGate = args->outputGate ? 1 : 0;
+    p.maxLength = args->maxLength;
+    p.heads = uint32_t(args->heads);
+    p.qStride = args->qStride ? args->qStride : args->cache.dim;
+    p.qTokenStride = args->qTokenStride ? args->qTokenStride : args->heads * p.qStride;
+    if (p.qStride >= (uint64_t(1) << 40) || p.qTokenStride >= (uint64_t(1) << 40))
+        return ctx.fail("paged decode: a stride of q is out of range");
+    p.window = args->window;
+    return aigpu::check_paged_decode(p);
+}
+
+} // namespace
+
+extern "C" {
+
+AIGPU_ABI int aigpu_rotary(const AiGpuRotary* args) {
+    Context& ctx = Context::instance();
+    std::lock_guard<std::recursive_mutex> lock(ctx.gate);
+    if (!args) return ctx.fail("rotary: null arguments"), 0;
+    aigpu::RotaryParams p{};
+    p.x = args->x;
+    p.out = args->out;
+    p.positions = args->positions;
+    p.freqs = args->frequencies;
+    p.amplitude = args->amplitude == 0.0f ? 1.0f : args->amplitude;
+    p.type = args->type > 1 ? -1 : int(args->type);
+    p.interleaved = args->interleaved ? 1 : 0;
+    p.transpose = args->transpose ? 1 : 0;
+    p.rot = args->rotaryDims;
+    p.count = args->count;
+    p.start = args->start;
+    p.heads = args->heads;
+    p.dim = args->dim;
+    p.headStride = args->headStride ? args->headStride : args->dim;
+    p.outHeadStride = args->outHeadStride ? args->outHeadStride : args->dim;
+    p.tokenStride = args->tokenStride ? args->tokenStride : args->heads * p.headStride;
+    p.outTokenStride = args->outTokenStride ? args->outTokenStride : args->heads * p.outHeadStride;
+    if (!aigpu::check_rotary(p) || !usable(ctx, "rotary")) return 0;
+    const OnDevice device;
+    return aigpu::launch_rotary(p, as_stream(args->stream)) ? 1 : 0;
+}
+
+AIGPU_ABI int aigpu_rotary_frequencies(const AiGpuRotaryScaling* s, float* frequencies, float* amplitude) {
+    Context& ctx = Context::instance();
+    std::lock_guard<std::recursive_mutex> lock(ctx.gate);
+    if (!s || !frequencies) return ctx.fail("rotary frequencies: null arguments"), 0;
+    float a = 1.0f;
+    if (!aigpu::rotary_frequencies(*s, frequencies, &a)) return 0;
+    if (amplitude) *amplitude = a;
+    return 1;
+}
+
+AIGPU_ABI int aigpu_paged_append(const AiGpuPagedAppend* args) {
+    Context& ctx = Context::instance();
+    std::lock_guard<std::recursive_mutex> lock(ctx.gate);
+    if (!args) return ctx.fail("paged append: null arguments"), 0;
+    aigpu::PagedAppendParams p{};
+    if (!paged_cache(ctx, "paged append", args->cache, p.c)) return 0;
+    const uint64_t row = args->cache.kvHeads * args->cache.dim;
+    p.k = args->k;
+    p.v = args->v;
+    p.starts = args->starts;
+    p.gamma = args->kNorm;
+    p.freqs = args->rotaryFrequencies;
+    p.eps = args->epsilon;
+    p.offset = args->normOffset;
+    p.amplitude = args->amplitude == 0.0f ? 1.0f : args->amplitude;
+    p.rot = args->rotaryDims > 4096 ? -1 : int(args->rotaryDims);
+    p.interleaved = args->interleaved ? 1 : 0;
+    p.inType = args->inType > 1 ? -1 : int(args->inType);
+    p.count = args->count;
+    p.kStride = args->kStride ? args->kStride : row;
+    p.vStride = args->vStride ? args->vStride : row;
+    if (p.kStride >= (uint64_t(1) << 40) || p.vStride >= (uint64_t(1) << 40))
+        return ctx.fail("paged append: a stride of k or v is out of range"), 0;
+    if (!aigpu::check_paged_append(p) || !usable(ctx, "paged append")) return 0;
+    const OnDevice device;
+    return aigpu::launch_paged_append(p, as_stream(args->stream)) ? 1 : 0;
+}
+
+AIGPU_ABI uint64_t aigpu_paged_decode_workspace(const AiGpuPagedDecode* args) {
+    Context& ctx = Context::instance();
+    std::lock_guard<std::recursive_mutex> lock(ctx.gate);
+    if (!args) return ctx.fail("paged decode: null arguments"), 0;
+    aigpu::PagedDecodeParams p{};
+    return paged_decode_params(ctx, args, p) ? aigpu::paged_decode_workspace(p) : 0;
+}
+
+AIGPU_ABI int aigpu_paged_decode(const AiGpuPagedDecode* args) {
+    Context& ctx = Context::instance();
+    std::lock_guard<std::recursive_mutex> lock(ctx.gate);
+    if (!args) return ctx.fail("paged decode: null arguments"), 0;
+    aigpu::PagedDecodeParams p{};
+    if (!paged_decode_params(ctx, args, p)) return 0;
+    const size_t need = aigpu::paged_decode_workspace(p);
+    if (args->workspace) {
+        if (reinterpret_cast<uintptr_t>(args->workspace) & 255)
+            return ctx.fail("paged decode: the workspace must be 256-byte aligned"), 0;
+        if (args->workspaceBytes < need)
+            return ctx.fail("paged decode: the workspace holds " + std::to_string(args->workspaceBytes) +
+                            " bytes, the call needs " + std::to_string(need)),
+                   0;
+    }
+    if (!usable(ctx, "paged decode")) return 0;
+    const OnDevice device;
+    hipStream_t stream = as_stream(args->stream);
+    if (args->workspace) return aigpu::launch_paged_decode(p, args->workspace, stream) ? 1 : 0;
+    if (need == 0) return aigpu::launch_paged_decode(p, nullptr, stream) ? 1 : 0;
+    if (aigpu::capturing(stream))
+        return ctx.fail("paged decode: a captured call needs a workspace of its own (" + std::to_string(need) +
+                        " bytes)"),
+               0;
+    const StreamOrder order(ctx, stream);
+    void* work = ctx.grow(aigpu::SLOT_PAGED, need);
+    return work && aigpu::launch_paged_decode(p, work, stream) ? 1 : 0;
+}
+
+} // extern "C"

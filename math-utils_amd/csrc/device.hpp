@@ -108,6 +108,14 @@ __device__ __forceinline__ void norm_rope_row(float* x, int dim, const float* ga
     }
 }
 
+/* cos and sin of pos * freq radians. The product and its reduction to a turn
+   are in 64 bits (in fp32 the angle of position 100000 is already 3e-3 radians
+   off), the functions in fp32 of the remaining half turn. */
+__device__ __forceinline__ void rotation_at(uint32_t pos, float freq, float& cs, float& sn) {
+    const double turns = double(pos) * double(freq) * 0.15915494309189535;   // 1 / (2 pi)
+    sincospif(2.0f * float(turns - rint(turns)), &sn, &cs);
+}
+
 /* fp16 of a finite fp32 value, noting in `bad` when it does not fit fp16's
    range (|x| >= 65520 rounds to infinity); infinite or NaN inputs stay what
    they are and are not noted (a NaN converts to a NaN, never to an infinity) */

@@ -7,6 +7,8 @@
 #include <hip/hip_runtime.h>
 #include <stdint.h>
 
+#include "../../include/aigpu_attention.h"
+
 namespace aigpu {
 
 // ---- generic fp32 attention (kernels::attention semantics) ---------------
@@ -260,6 +262,62 @@ struct GdnGatedNormParams {
     uint64_t count, valueHeads, valueDim;
 };
 bool launch_gdn_gated_norm(const GdnGatedNormParams& p, hipStream_t stream);
+
+// ---- rotary positions ----
+struct RotaryParams {
+    const void* x;
+    void* out;
+    const uint32_t* positions;  // or null: start + token
+    const float* freqs;         // [rot / 2]
+    float amplitude;
+    int type, interleaved, transpose;
+    uint32_t rot;
+    uint64_t count, start, heads, dim;
+    uint64_t tokenStride, headStride, outTokenStride, outHeadStride;
+};
+// check_*: the argument checks, which need no device; launch_* assume them
+bool check_rotary(const RotaryParams& p);
+bool launch_rotary(const RotaryParams& p, hipStream_t stream);
+// the table of a scaling (host work), and the amplitude that goes with it
+bool rotary_frequencies(const AiGpuRotaryScaling& s, float* frequencies, float* amplitude);
+
+// ---- the paged cache: append, and one token's attention over it ----
+struct PagedCache {
+    uint16_t* keys;
+    uint16_t* values;
+    const uint32_t* table;
+    const uint32_t* lengths;
+    uint64_t pageStride, headStride, rowStride, tableStride;
+    uint32_t batch, pages, pageSize, kvHeads, dim, tableWidth;
+};
+struct PagedAppendParams {
+    PagedCache c;
+    const void* k;
+    const void* v;
+    const uint32_t* starts;     // [batch + 1], or null: one token a sequence
+    const float* gamma;
+    const float* freqs;
+    float eps, offset, amplitude;
+    int rot, interleaved, inType;
+    uint64_t count, kStride, vStride;
+};
+bool check_paged_append(const PagedAppendParams& p);
+bool launch_paged_append(const PagedAppendParams& p, hipStream_t stream);
+struct PagedDecodeParams {
+    PagedCache c;
+    const void* q;
+    float* out;
+    const float* gamma;
+    const float* freqs;
+    float eps, offset, amplitude, scale;
+    int rot, interleaved, inType, outputGate;
+    uint32_t maxLength, heads;
+    uint64_t qStride, qTokenStride, window;
+};
+bool check_paged_decode(const PagedDecodeParams& p);
+size_t paged_decode_workspace(const PagedDecodeParams& p);
+// work: paged_decode_workspace(p) bytes, or null where that is 0
+bool launch_paged_decode(const PagedDecodeParams& p, void* work, hipStream_t stream);
 
 // ---- a plain streaming device copy (the bench's achievable-bandwidth line) ----
 bool launch_copy(void* dst, const void* src, uint64_t bytes, hipStream_t stream);

@@ -65,6 +65,11 @@ AIGPU_ABI void aigpu_dense_release(void*) {}
 AIGPU_ABI void aigpu_dense_decode(void*, const float*, float*, uint32_t) {}
 AIGPU_ABI void aigpu_dense_read_cache(void*, float* const*, float* const*, uint32_t) {}
 AIGPU_ABI int aigpu_gdn_gated_norm(const AiGpuGdnGatedNorm*) { return 0; }
+AIGPU_ABI int aigpu_rotary(const AiGpuRotary*) { return 0; }
+AIGPU_ABI int aigpu_rotary_frequencies(const AiGpuRotaryScaling*, float*, float*) { return 0; }
+AIGPU_ABI int aigpu_paged_append(const AiGpuPagedAppend*) { return 0; }
+AIGPU_ABI int aigpu_paged_decode(const AiGpuPagedDecode*) { return 0; }
+AIGPU_ABI uint64_t aigpu_paged_decode_workspace(const AiGpuPagedDecode*) { return 0; }
 
 AIGPU_ABI void aigpu_profile(int) {}
 AIGPU_ABI int aigpu_profile_read(const char*, double* ms, uint64_t* n) {
