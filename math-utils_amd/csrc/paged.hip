@@ -1,6 +1,7 @@
 // paged.hip - a paged KV cache: appending the newest tokens, and one token's
 // attention over each sequence's pages.
 #include <cmath>
+#include <type_traits>
 
 #include "context.hpp"
 #include "device.hpp"
@@ -180,85 +181,663 @@ __global__ __launch_bounds__(THREADS) void paged_append_kernel(AppendArgs a) {
 }
 
 /*
-    One token's attention, the plain way: a workgroup a (sequence, query head),
-    its four waves taking every fourth position, each with a running maximum and
-    sum, joined at the end.
+    One token's attention over the pages, in two launches.
+
+    The batch is cut into slabs of 32 positions of one sequence, one kv head and
+    up to 16 of its query heads, listed sequence by sequence, and the list into
+    one even run a wave: whatever the lengths, every wave reads the same number of
+    slabs within one, and the work is bounded by the keys and values read once
+    (HBM). paged_attention_kernel works a run off as one software pipeline over
+    its slabs, whichever sequence they belong to: page ids are read two slabs
+    ahead, keys (registers) and values (DMA into LDS) one slab ahead, so loads
+    stay in flight while a sequence ends and the next one's queries are prepared.
+      scores   v_mfma_f32_16x16x32_bf16, 16 keys as A, the heads' queries as B, in
+               three terms of 8 bits each (x = hi + mid + lo exactly: fp32 is 24
+               bits), so the products are fp32's; three instructions a tile cost
+               11% of the matrix rate at full HBM bandwidth
+      softmax  a running maximum and sum a head; lane l holds head l % 16
+      p v      the weights in three terms likewise, as A, exactly the scores the
+               lane holds; values as B through ds_read_b64_tr_b16
+    A sequence's head wholly in one run is written at once. What is left at the
+    end of a run is joined over the workgroup's waves in LDS; pairs that span
+    workgroups leave (max, sum, weighted values) records, two a wave at most, that
+    paged_merge_kernel joins in their order, so results do not depend on timing.
 */
-__global__ __launch_bounds__(THREADS) void paged_decode_kernel(PagedDecodeParams p) {
-    constexpr int WAVES = THREADS / WAVE, PER = 4;   // elements of a row a lane holds at most
-    __shared__ float q[256], acc[WAVES][256], wm[WAVES], wl[WAVES];
-    __shared__ int bad;
+constexpr int SLAB = 32;
+constexpr int WAVES = 4;
+constexpr int ROWS = 16;             // query heads of a group
+constexpr uint32_t MAXB = 512;       // sequences of a launch
+
+struct DecodeArgs {
+    PagedDecodeParams p;
+    uint32_t* plan;                  // [MAXB + 1] slabs before each sequence, and in all
+    float* records;                  // [waves][2]: (m, l)[perGroup], then [perGroup][dim]
+    uint32_t groups, perGroup;       // of one kv head's query heads
+    float scaleLog2;
+    int wideQ;                       // q rows can be read 16 bytes at a time
+};
+
+typedef __bf16 bf16v4 __attribute__((__vector_size__(4 * sizeof(__bf16))));
+
+/* ds_read_b64_tr_b16: within each 16-lane group, lane i receives element i % 4
+   of the 8-byte rows addressed by lanes i/4, i/4 + 4, i/4 + 8, i/4 + 12 */
+__device__ __forceinline__ bf16v4 read_transposed(const uint16_t* lds) {
+    typedef __attribute__((address_space(3))) bf16v4 lds_bf16v4;
+    return __builtin_amdgcn_ds_read_tr16_b64_v4bf16((lds_bf16v4*)(lds));
+}
+
+/* s_waitcnt vmcnt(N) alone */
+template <int N>
+__device__ __forceinline__ void wait_loads() {
+    static_assert(N >= 0 && N < 64, "vmcnt range");
+    __builtin_amdgcn_s_waitcnt((N & 15) | (7 << 4) | (15 << 8) | ((N >> 4) << 14));
+}
+
+__device__ __forceinline__ uint32_t uniform(uint32_t x) { return __builtin_amdgcn_readfirstlane(x); }
+
+/* x, hidden from the compiler: what is derived from it is formed where it is
+   used. The pipeline's loop would otherwise hold every address and mask of its
+   rare parts in registers (a hundred of them, spilled). */
+__device__ __forceinline__ int fresh_lane(int x) {
+    asm volatile("" : "+v"(x));
+    return x;
+}
+__device__ __forceinline__ uint32_t fresh_uniform(uint32_t x) {
+    asm volatile("" : "+s"(x));
+    return x;
+}
+
+/* the eight rows of 32 bytes that 32 lanes read transposed lie in distinct
+   banks (64 of 4 bytes): block x of 16 bytes of row r sits at x ^ this */
+template <int D>
+__device__ __forceinline__ int value_swizzle(int r) {
+    if constexpr (D % 128 == 0) return 2 * (r & 7);        // rows start in the same bank
+    else if constexpr (D % 64 == 0) return 2 * ((r >> 1) & 3);
+    else return 2 * ((r >> 2) & 1);
+}
+
+__device__ __forceinline__ uint32_t first_of(const PagedDecodeParams& p, uint32_t len) {
+    return p.window && len > p.window ? uint32_t(len - p.window) : 0u;
+}
+
+__device__ __forceinline__ uint32_t slabs_of(const PagedDecodeParams& p, uint32_t len) {
+    return len == 0 || len > p.maxLength ? 0u : (len + SLAB - 1) / SLAB - first_of(p, len) / SLAB;
+}
+
+/* the even cut of `total` slabs into runs: run w's first slab, and a slab's run */
+struct Cut {
+    uint32_t runs, each, extra;      // the first `extra` runs have one more
+    __device__ __forceinline__ Cut(uint32_t total, uint32_t waves) {
+        runs = total < waves ? total : waves;
+        each = runs ? total / runs : 0;
+        extra = runs ? total % runs : 0;
+    }
+    __device__ __forceinline__ uint32_t begin(uint32_t w) const {
+        return w < runs ? w * each + (w < extra ? w : extra) : runs * each + extra;
+    }
+    __device__ __forceinline__ uint32_t run_of(uint32_t slab) const {
+        const uint32_t longer = extra * (each + 1);
+        return slab < longer ? slab / (each + 1) : extra + (slab - longer) / each;
+    }
+};
+
+struct Slab {
+    uint32_t b, pair;                // pair: kv head * groups + group
+    uint32_t pos, first, len;        // its first position; the attended range
+    uint32_t is;                     // of BEGINS .. CLOSES
+};
+enum : uint32_t {
+    BEGINS = 1, ENDS = 2,            // the pair's first slab, its last
+    OPENS = 4, CLOSES = 8,           // the first of the pair in this run, the last
+};
+
+/* fp32 to three bf16 terms whose sum it is: each takes the next 8 bits */
+__device__ __forceinline__ void split3(const float (&x)[8], u32x4 (&t)[3]) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        float a = x[2 * i], b = x[2 * i + 1];
+#pragma unroll
+        for (int k = 0; k < 3; ++k) {
+            const uint32_t ua = __float_as_uint(a), ub = __float_as_uint(b);
+            t[k][i] = __builtin_amdgcn_perm(ub, ua, 0x07060302);    // the high halves
+            a -= __uint_as_float(ua & 0xFFFF0000u);
+            b -= __uint_as_float(ub & 0xFFFF0000u);
+        }
+    }
+}
+
+/* x times sigmoid of the gate half of its q row when the output gate is on */
+__device__ __forceinline__ float gated(const PagedDecodeParams& p, uint32_t b, uint32_t head, uint32_t d, float x) {
+    if (!p.outputGate) return x;
+    return x * sigmoid_of(load_elem(p.q, b * p.qTokenStride + head * p.qStride + p.c.dim + d, p.inType));
+}
+
+constexpr int occupancy(int D) { return D <= 128 ? 2 : 1; }
+
+template <int D, bool BF>
+__global__ __launch_bounds__(THREADS, occupancy(D)) void paged_attention_kernel(DecodeArgs a) {
+    constexpr int DB = D / 32, CT = D / 16, BPR = D / 8;
+    constexpr int VLOADS = SLAB * BPR / WAVE;
+    const PagedDecodeParams& p = a.p;
     const PagedCache& c = p.c;
-    const uint32_t b = blockIdx.x / p.heads, head = blockIdx.x % p.heads, D = c.dim;
-    const uint32_t kvh = head / (p.heads / c.kvHeads);
-    const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
-    const uint32_t len = c.lengths[b];
-    float* out = p.out + (size_t(b) * p.heads + head) * D;
-    if (len == 0 || len > p.maxLength) {
-        for (uint32_t d = threadIdx.x; d < D; d += THREADS) out[d] = len ? __builtin_nanf("") : 0.0f;
-        return;
-    }
-    const size_t qrow = b * p.qTokenStride + head * p.qStride;
-    if (threadIdx.x == 0) bad = 0;
-    if (w == 0) {
-        float ss = 0.0f;
-        for (uint32_t d = lane; d < D; d += WAVE) {
-            q[d] = load_elem(p.q, qrow + d, p.inType);
-            ss += q[d] * q[d];
+    const int lane = threadIdx.x & 63, w = int(uniform(threadIdx.x >> 6));
+    const int g = lane >> 4, c16 = lane & 15;
+    const uint32_t B = c.batch, pairs = c.kvHeads * a.groups, G = p.heads / c.kvHeads;
+
+    __shared__ uint32_t pre[MAXB + 1], lens[MAXB], sums[WAVES];
+    __shared__ uint64_t place[WAVES][SLAB];
+    __shared__ float2 turns[WAVES][D / 2];
+    __shared__ float gamma[D];
+    __shared__ float wm[WAVES][ROWS], wl[WAVES][ROWS];
+    __shared__ uint32_t left[WAVES];              // the pair a wave's run leaves open (b * pairs + pair), or NOWHERE
+    __shared__ uint32_t leftEnds[WAVES];          // bit 0: from the pair's first slab, bit 1: to its last
+    __shared__ __attribute__((aligned(16))) uint16_t vbuf[WAVES][2][SLAB * D];
+
+    // ---- the list: slabs before each sequence ----
+    {
+        uint32_t own[2];
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+            const uint32_t b = 2 * threadIdx.x + i;
+            const uint32_t len = b < B ? c.lengths[b] : 0u;
+            if (b < B) lens[b] = len;
+            own[i] = slabs_of(p, len) * pairs;
         }
+        if (p.gamma)
+            for (int d = threadIdx.x; d < D; d += THREADS) gamma[d] = p.gamma[d] + p.offset;
+        uint32_t x = own[0] + own[1];
+#pragma unroll
+        for (int o = 1; o < WAVE; o <<= 1) {
+            const uint32_t y = __shfl_up(x, o, WAVE);
+            if (lane >= o) x += y;
+        }
+        if (lane == 63) sums[w] = x;
+        __syncthreads();
+        uint32_t before = x - own[0] - own[1];
+        for (int k = 0; k < w; ++k) before += sums[k];
+        const uint32_t b = 2 * threadIdx.x;
+        if (b <= B) pre[b] = before;
+        if (b + 1 <= B) pre[b + 1] = before + own[0];
+        if (threadIdx.x == THREADS - 1 && B == MAXB) pre[B] = before + own[0] + own[1];
+        __syncthreads();
+    }
+    if (blockIdx.x == 0)
+        for (uint32_t i = threadIdx.x; i <= B; i += THREADS) a.plan[i] = pre[i];
+    // sequences without a slab: empty ones, and those that cannot be
+    for (uint32_t b = blockIdx.x; b < B; b += gridDim.x) {
+        if (pre[b] != pre[b + 1]) continue;
+        const float x = lens[b] ? __builtin_nanf("") : 0.0f;
+        for (uint32_t i = threadIdx.x; i < p.heads * D; i += THREADS) p.out[size_t(b) * p.heads * D + i] = x;
+    }
+
+    const Cut cut(uniform(pre[B]), gridDim.x * WAVES);
+    const uint32_t run = blockIdx.x * WAVES + w;
+    const uint32_t runEnd = cut.begin(run + 1);
+    uint32_t at = cut.begin(run);                 // the next slab to list
+    const uint32_t count = runEnd - at;
+    uint32_t seq = 0, pair = 0, slab = 0, slabs = 1, len = 0;
+    if (count) {
+        uint32_t lo = 0, hi = B;                  // pre[lo] <= at < pre[hi]
+        while (hi - lo > 1) {
+            const uint32_t mid = (lo + hi) / 2;
+            if (uniform(pre[mid]) <= at) lo = mid;
+            else hi = mid;
+        }
+        seq = lo;
+        len = uniform(lens[seq]);
+        slabs = slabs_of(p, len);
+        const uint32_t in = at - uniform(pre[seq]);
+        pair = in / slabs;
+        slab = in % slabs;
+    }
+    auto list = [&](Slab& s) {
+        s.b = seq;
+        s.pair = pair;
+        s.first = first_of(p, len);
+        s.len = len;
+        s.pos = (s.first / SLAB + slab) * SLAB;
+        s.is = slab == 0 ? BEGINS | OPENS : 0u;
+        if (at == runEnd - count) s.is |= OPENS;
+        if (slab + 1 == slabs) s.is |= ENDS | CLOSES;
+        if (at + 1 == runEnd) s.is |= CLOSES;
+        ++at;
+        if (++slab == slabs && at < runEnd) {
+            slab = 0;
+            if (++pair == pairs) {
+                pair = 0;
+                do ++seq;                         // at < pre[B]: a later sequence has slabs
+                while (uniform(pre[seq]) == uniform(pre[seq + 1]));
+                len = uniform(lens[seq]);
+                slabs = slabs_of(p, len);
+            }
+        }
+    };
+
+    // ---- the stages of a slab ----
+    u32x4 kr[2][DB];                 // keys: rows 16 rb + c16
+    // its page ids: lane r (of 32) holds row r's; rows outside the attended
+    // range stand at its ends, so that nothing else is read
+    struct Rows { uint32_t page, row; };
+    auto find = [&](const Slab& s, Rows& r) {
+        uint32_t pos = s.pos + (lane & 31);
+        pos = pos < s.first ? s.first : (pos < s.len ? pos : s.len - 1);
+        const uint32_t slot = pos / c.pageSize;
+        r.row = pos - slot * c.pageSize;
+        r.page = c.table[s.b * c.tableStride + slot];
+    };
+    // its keys into registers (A operands: row lane % 16, 8 elements a lane),
+    // its values into LDS; false where a page lies outside the pool (its rows
+    // are then read from page 0)
+    auto issue = [&](const Slab& s, const Rows& r, int half) -> bool {
+        const int lane = fresh_lane(threadIdx.x & 63), g = lane >> 4, c16 = lane & 15;
+        const bool ok = r.page < c.pages;
+        const uint64_t mine = (ok ? uint64_t(r.page) * c.pageStride + uint64_t(r.row) * c.rowStride : 0) +
+                              uint64_t(s.pair / a.groups) * c.headStride;
+        wave_sync();
+        if (lane < SLAB) place[w][lane] = mine;
+        wave_sync();
+#pragma unroll
+        for (int rb = 0; rb < 2; ++rb) {
+            const uint16_t* k = c.keys + place[w][16 * rb + c16] + 8 * g;
+#pragma unroll
+            for (int db = 0; db < DB; ++db) kr[rb][db] = *reinterpret_cast<const u32x4*>(k + 32 * db);
+        }
+        uint16_t* to = vbuf[w][half];
+#pragma unroll
+        for (int j = 0; j < VLOADS; ++j) {
+            const int i = j * WAVE + lane, row = i / BPR, block = (i % BPR) ^ value_swizzle<D>(row);
+            // cache policy 2: nontemporal (each value is read once)
+            __builtin_amdgcn_global_load_lds(c.values + place[w][row] + 8 * block,
+                                             (__attribute__((address_space(3))) void*)(to + j * WAVE * 8), 16, 0, 2);
+        }
+        return __all(ok);
+    };
+    // the raw queries of a pair, lane (c16, g) holding head c16's elements
+    // 32 db + 8 g + 0..7: the B operand's layout
+    constexpr int RAW = BF ? 1 : 2;
+    u32x4 raw[DB][RAW];
+    auto ask = [&](const Slab& s) {
+        const int lane = fresh_lane(threadIdx.x & 63), g = lane >> 4, c16 = lane & 15;
+        const uint32_t group = s.pair % a.groups, kvh = s.pair / a.groups;
+        const uint32_t h = group * a.perGroup + c16;
+        const uint32_t head = kvh * G + (c16 < a.perGroup && h < G ? h : group * a.perGroup);
+        const size_t row = s.b * p.qTokenStride + head * p.qStride + 8 * g;
+#pragma unroll
+        for (int db = 0; db < DB; ++db) {
+            if (a.wideQ) {
+                const u32x4* src = reinterpret_cast<const u32x4*>(static_cast<const char*>(p.q) +
+                                                                  (row + 32 * db) * (BF ? 2 : 4));
+#pragma unroll
+                for (int i = 0; i < RAW; ++i) raw[db][i] = src[i];
+            } else if constexpr (BF) {
+                const uint16_t* src = static_cast<const uint16_t*>(p.q) + row + 32 * db;
+#pragma unroll
+                for (int i = 0; i < 4; ++i) raw[db][0][i] = src[2 * i] | uint32_t(src[2 * i + 1]) << 16;
+            } else {
+                const uint32_t* src = static_cast<const uint32_t*>(p.q) + row + 32 * db;
+#pragma unroll
+                for (int i = 0; i < 8; ++i) raw[db][i / 4][i % 4] = src[i];
+            }
+        }
+    };
+    const uint32_t turnedDims = p.freqs ? uint32_t(p.rot) : 0;
+    float freq[(D / 2 + WAVE - 1) / WAVE];
+#pragma unroll
+    for (uint32_t i = 0; i < sizeof(freq) / 4; ++i)
+        freq[i] = lane + i * WAVE < turnedDims / 2 ? p.freqs[lane + i * WAVE] : 0.0f;
+
+    bf16x8 qb[DB][3];
+    uint32_t turned = NOWHERE;
+    // raw to the three-term B operands: norm, rotation at len - 1, scale;
+    // `spare`: 16 rows in LDS
+    auto prepare = [&](const Slab& s, float* spare) {
+        const uint32_t group = s.pair % a.groups, rot = fresh_uniform(turnedDims), half = rot / 2;
+        const int lane = fresh_lane(threadIdx.x & 63), g = lane >> 4, c16 = lane & 15;
+        const bool live = c16 < a.perGroup && group * a.perGroup + c16 < G;
+        float x[DB][8];
+#pragma unroll
+        for (int db = 0; db < DB; ++db)
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+                uint32_t bits;
+                if constexpr (BF) bits = e & 1 ? raw[db][0][e / 2] & 0xFFFF0000u : raw[db][0][e / 2] << 16;
+                else bits = raw[db][e / 4][e % 4];
+                x[db][e] = live ? __uint_as_float(bits) : 0.0f;
+            }
+        float inv = 1.0f;
         if (p.gamma) {
-            const float inv = 1.0f / sqrtf(wave_sum(ss) / float(D) + p.eps);
-            for (uint32_t d = lane; d < D; d += WAVE) q[d] = q[d] * inv * (p.gamma[d] + p.offset);
+            float ss = 0.0f;
+#pragma unroll
+            for (int db = 0; db < DB; ++db)
+#pragma unroll
+                for (int e = 0; e < 8; ++e) ss += x[db][e] * x[db][e];
+            ss += __shfl_xor(ss, 16, WAVE);
+            ss += __shfl_xor(ss, 32, WAVE);
+            inv = 1.0f / sqrtf(ss / float(D) + p.eps);
+#pragma unroll
+            for (int db = 0; db < DB; ++db)
+#pragma unroll
+                for (int e = 0; e < 8; ++e) x[db][e] = x[db][e] * inv * gamma[32 * db + 8 * g + e];
         }
-        wave_sync();
-        const uint32_t half = p.freqs ? p.rot / 2 : 0;
-        for (uint32_t j = lane; j < half; j += WAVE) {
-            const uint32_t i0 = p.interleaved ? 2 * j : j, i1 = p.interleaved ? 2 * j + 1 : j + half;
-            float cs, sn;
-            rotation_at(len - 1, p.freqs[j], cs, sn);
-            const float u = q[i0], v = q[i1];
-            q[i0] = (u * cs - v * sn) * p.amplitude;
-            q[i1] = (v * cs + u * sn) * p.amplitude;
+        if (rot) {
+            if (turned != s.b) {
+                wave_sync();
+#pragma unroll
+                for (uint32_t i = 0; i < sizeof(freq) / 4; ++i) {
+                    float cs, sn;
+                    rotation_at(s.len - 1, freq[i], cs, sn);
+                    if (lane + i * WAVE < half) turns[w][lane + i * WAVE] = float2{cs * p.amplitude, sn * p.amplitude};
+                }
+                wave_sync();
+                turned = s.b;
+            }
+            if (p.interleaved) {
+#pragma unroll
+                for (int db = 0; db < DB; ++db)
+#pragma unroll
+                    for (int e = 0; e < 8; e += 2) {
+                        const uint32_t d = 32 * db + 8 * g + e;
+                        if (d < rot) {
+                            const float2 cs = turns[w][d / 2];
+                            const float u = x[db][e], v = x[db][e + 1];
+                            x[db][e] = u * cs.x - v * cs.y;
+                            x[db][e + 1] = v * cs.x + u * cs.y;
+                        }
+                    }
+            } else if (half % 32 == 0) {
+                // the partner 32 k elements on is this lane's too
+#pragma unroll
+                for (int k = 1; k <= DB / 2; ++k) {
+                    if (half != 32u * k) continue;
+#pragma unroll
+                    for (int db = 0; db < k; ++db)
+#pragma unroll
+                        for (int e = 0; e < 8; ++e) {
+                            const float2 cs = turns[w][32 * db + 8 * g + e];
+                            const float u = x[db][e], v = x[db + k][e];
+                            x[db][e] = u * cs.x - v * cs.y;
+                            x[db + k][e] = v * cs.x + u * cs.y;
+                        }
+                }
+            } else {
+                // elsewhere it is another lane's: through the values' idle half
+                float* row = spare + c16 * D;
+#pragma unroll
+                for (int db = 0; db < DB; ++db)
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) row[32 * db + 8 * g + e] = x[db][e];
+                wave_sync();
+#pragma unroll
+                for (int db = 0; db < DB; ++db) {
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) {
+                        const uint32_t d = 32 * db + 8 * g + e;
+                        const bool late = d >= half;
+                        const uint32_t o = late ? d - half : d + half;
+                        if (d < rot) {
+                            const float2 cs = turns[w][late ? o : d];
+                            x[db][e] = late ? x[db][e] * cs.x + row[o] * cs.y : x[db][e] * cs.x - row[o] * cs.y;
+                        }
+                    }
+                    __builtin_amdgcn_sched_barrier(0);
+                }
+                wave_sync();
+            }
         }
+#pragma unroll
+        for (int db = 0; db < DB; ++db) {
+#pragma unroll
+            for (int e = 0; e < 8; ++e) x[db][e] *= a.scaleLog2;
+            u32x4 t[3];
+            split3(x[db], t);
+#pragma unroll
+            for (int k = 0; k < 3; ++k) qb[db][k] = __builtin_bit_cast(bf16x8, t[k]);
+        }
+    };
+
+    float m = -INFINITY, l = 0.0f;   // of head c16; l of this lane's positions
+    floatx4 acc[CT];                 // [tile][r]: head 4 g + r, column 16 tile + c16
+    bool bad = false, begun = false;
+    float sv[2][4];                  // scores: of head c16 at positions 16 rb + 4 g + i
+    auto score = [&](const Slab& s) {
+        const int lane = fresh_lane(threadIdx.x & 63), g = lane >> 4;
+#pragma unroll
+        for (int rb = 0; rb < 2; ++rb) {
+            floatx4 sc = floatx4{0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+            for (int k = 2; k >= 0; --k)
+#pragma unroll
+                for (int db = 0; db < DB; ++db)
+                    sc = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, kr[rb][db]), qb[db][k], sc,
+                                                                 0, 0, 0);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const uint32_t pos = s.pos + 16 * rb + 4 * g + i;
+                sv[rb][i] = pos >= s.first && pos < s.len ? sc[i] : -INFINITY;
+            }
+        }
+    };
+    auto weigh = [&](int bufHalf, bool nextInFlight) {
+        const int lane = fresh_lane(threadIdx.x & 63), g = lane >> 4, c16 = lane & 15;
+        float top = -INFINITY;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) top = fmaxf(top, sv[i >> 2][i & 3]);
+        top = fmaxf(top, __shfl_xor(top, 16, WAVE));
+        top = fmaxf(top, __shfl_xor(top, 32, WAVE));
+        const float next = fmaxf(m, top), base = next == -INFINITY ? 0.0f : next;
+        const float keep = exp2f(m - base);
+        float pv[8], sum = 0.0f;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            pv[i] = exp2f(sv[i >> 2][i & 3] - base);
+            sum += pv[i];
+        }
+        l = l * keep + sum;
+        m = next;
+        float rk[4];
+#pragma unroll
+        for (int r = 0; r < 4; ++r) rk[r] = __shfl(keep, 4 * g + r, WAVE);
+#pragma unroll
+        for (int t = 0; t < CT; ++t)
+#pragma unroll
+            for (int r = 0; r < 4; ++r) acc[t][r] *= rk[r];
+        u32x4 pa[3];
+        split3(pv, pa);
+        // this slab's values have landed: at most the next slab's loads are out
+        if (nextInFlight) wait_loads<2 * DB + VLOADS>();
+        else wait_loads<0>();
         wave_sync();
-        for (uint32_t d = lane; d < D; d += WAVE) q[d] *= p.scale * LOG2E;
+        const uint16_t* vs = vbuf[w][bufHalf];
+#pragma unroll
+        for (int t = 0; t < CT; ++t) {
+            // lane c16 of group g gets column 16 t + c16 of rows 4 g + 0..3, then 16 + 4 g + 0..3
+            const int r0 = 4 * g + (c16 >> 2), r1 = r0 + 16;
+            const int x = 2 * t + ((c16 >> 1) & 1), sub = 4 * (c16 & 1);
+            const bf16v4 lo = read_transposed(vs + r0 * D + 8 * (x ^ value_swizzle<D>(r0)) + sub);
+            const bf16v4 hi = read_transposed(vs + r1 * D + 8 * (x ^ value_swizzle<D>(r1)) + sub);
+            const bf16x8 vb = __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
+#pragma unroll
+            for (int k = 2; k >= 0; --k)
+                acc[t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, pa[k]), vb, acc[t], 0, 0, 0);
+        }
+    };
+    // a pair's last slab of this run: the sum over lanes, then its output or,
+    // where other runs have parts of it, a record (the run's last stays in the
+    // registers, for the workgroup's join)
+    auto finish = [&](const Slab& s, bool last) {
+        const int lane = fresh_lane(threadIdx.x & 63), g = lane >> 4, c16 = lane & 15;
+        l += __shfl_xor(l, 16, WAVE);
+        l += __shfl_xor(l, 32, WAVE);
+        if (bad) l = __builtin_nanf("");
+        const bool whole = begun && (s.is & ENDS);
+        if (last && !whole) return;
+        const uint32_t group = s.pair % a.groups, kvh = s.pair / a.groups, h0 = group * a.perGroup;
+        const uint32_t rows = a.perGroup < G - h0 ? a.perGroup : G - h0;
+        float* rec = a.records + size_t(run) * 2 * a.perGroup * (D + 2);
+        float* accRows = rec + 2 * a.perGroup;
+        if (!whole && g == 0 && uint32_t(c16) < rows) {
+            rec[c16] = m;
+            rec[a.perGroup + c16] = l;
+        }
+        float* to = whole ? p.out + (size_t(s.b) * p.heads + kvh * G + h0) * D : accRows;
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+            const uint32_t row = 4 * g + r;
+            const float total = __shfl(l, row, WAVE), by = whole ? 1.0f / total : 1.0f;
+            if (row < rows) {
+#pragma unroll
+                for (int t = 0; t < CT; ++t) to[row * D + 16 * t + c16] = acc[t][r] * by;
+            }
+        }
+        if (whole && p.outputGate) {
+#pragma unroll 1
+            for (uint32_t i = c16; i < 4 * D; i += 16) {      // this lane's own elements again
+                const uint32_t row = 4 * g + i / D, d = i % D;
+                if (row < rows) to[row * D + d] = gated(p, s.b, kvh * G + h0 + row, d, to[row * D + d]);
+            }
+        }
+    };
+
+    // ---- the pipeline ----
+    Slab s0{}, s1{}, s2{};           // computed, in flight, its pages asked for
+    Rows r1{}, r2{};
+    bool ok0 = true;
+    if (count) {
+        list(s0);
+        ask(s0);
+        Rows r0;
+        find(s0, r0);
+        if (count > 1) list(s1), find(s1, r1);
+        ok0 = issue(s0, r0, 0);
+    }
+    __builtin_amdgcn_sched_barrier(0);
+#pragma unroll 1
+    for (uint32_t i = 0; i < count; ++i) {
+        const int at = i & 1;
+        const bool more = i + 1 < count;
+        wave_sync();                 // the other buffer's reads are done
+        if (s0.is & OPENS) {
+            prepare(s0, reinterpret_cast<float*>(vbuf[w][at ^ 1]));
+            m = -INFINITY;
+            l = 0.0f;
+#pragma unroll
+            for (int t = 0; t < CT; ++t) acc[t] = floatx4{0.0f, 0.0f, 0.0f, 0.0f};
+            bad = false;
+            begun = s0.is & BEGINS;
+        }
+        bad |= !ok0;
+        score(s0);
+        __builtin_amdgcn_sched_barrier(0);
+        if (more) {
+            if (i + 2 < count) list(s2), find(s2, r2);
+            if (s1.is & OPENS) ask(s1);
+            ok0 = issue(s1, r1, at ^ 1);
+        }
+        __builtin_amdgcn_sched_barrier(0);
+        weigh(at, more);
+        if (s0.is & CLOSES) finish(s0, !more);
+        if (more) {
+            s0 = s1;
+            s1 = s2;
+            r1 = r2;
+        }
+    }
+
+    // ---- the runs' open ends, joined over the workgroup ----
+    const bool open = count && !(begun && (s0.is & ENDS));
+    if (lane == 0) {
+        left[w] = open ? s0.b * pairs + s0.pair : NOWHERE;
+        leftEnds[w] = (begun ? 1u : 0u) | (s0.is & ENDS ? 2u : 0u);
+    }
+    if (open) {
+        if (g == 0) wm[w][c16] = m, wl[w][c16] = l;
+        float* rows = reinterpret_cast<float*>(vbuf[w]);
+        wave_sync();
+#pragma unroll
+        for (int t = 0; t < CT; ++t)
+#pragma unroll
+            for (int r = 0; r < 4; ++r) rows[(4 * g + r) * D + 16 * t + c16] = acc[t][r];
     }
     __syncthreads();
-    const uint32_t first = p.window && len > p.window ? uint32_t(len - p.window) : 0u;
-    float m = -INFINITY, l = 0.0f, o[PER] = {};
-    for (uint64_t pos = first + w; pos < len; pos += WAVES) {
-        const uint64_t at = row_offset(c, b, pos, kvh);
-        if (at == ~uint64_t(0)) {
-            if (lane == 0) bad = 1;
-            continue;
+    for (int from = 0, to; from < WAVES; from = to) {
+        const uint32_t id = left[from];
+        for (to = from + 1; to < WAVES && left[to] == id; ++to) {}
+        if (id == NOWHERE) continue;
+        const bool whole = (leftEnds[from] & 1) && (leftEnds[to - 1] & 2);
+        const uint32_t b = id / pairs, pr = id % pairs, kvh = pr / a.groups, h0 = pr % a.groups * a.perGroup;
+        const uint32_t rows = a.perGroup < G - h0 ? a.perGroup : G - h0;
+        float* rec = a.records + (size_t(blockIdx.x * WAVES + from) * 2 + 1) * a.perGroup * (D + 2);
+        float* out = p.out + (size_t(b) * p.heads + kvh * G + h0) * D;
+        for (uint32_t i = threadIdx.x; i < rows * D; i += THREADS) {
+            const uint32_t row = i / D, d = i % D;
+            float top = -INFINITY, sum = 0.0f, x = 0.0f;
+            for (int k = from; k < to; ++k) top = fmaxf(top, wm[k][row]);
+            const float base = top == -INFINITY ? 0.0f : top;
+            for (int k = from; k < to; ++k) {
+                const float f = exp2f(wm[k][row] - base);
+                sum += wl[k][row] * f;
+                x += reinterpret_cast<const float*>(vbuf[k])[i] * f;
+            }
+            if (whole) {
+                out[i] = gated(p, b, kvh * G + h0 + row, d, x / sum);
+            } else {
+                rec[2 * a.perGroup + i] = x;
+                if (d == 0) rec[row] = top, rec[a.perGroup + row] = sum;
+            }
         }
-        float s = 0.0f;
-        for (uint32_t d = lane; d < D; d += WAVE) s += q[d] * bf16_bits_to_float(c.keys[at + d]);
-        s = wave_sum(s);
-        const float top = fmaxf(m, s), keep = exp2f(m - top), weight = exp2f(s - top);
-        l = l * keep + weight;
-        for (uint32_t i = 0; i < PER; ++i) {
-            const uint32_t d = lane + i * WAVE;
-            if (d < D) o[i] = o[i] * keep + weight * bf16_bits_to_float(c.values[at + d]);
-        }
-        m = top;
     }
-    for (uint32_t i = 0; i < PER; ++i)
-        if (lane + i * WAVE < D) acc[w][lane + i * WAVE] = o[i];
-    if (lane == 0) wm[w] = m, wl[w] = l;
-    __syncthreads();
-    const float top = fmaxf(fmaxf(wm[0], wm[1]), fmaxf(wm[2], wm[3]));
-    for (uint32_t d = threadIdx.x; d < D; d += THREADS) {
-        float sum = 0.0f, x = 0.0f;
-        for (int k = 0; k < WAVES; ++k) {
-            const float f = wm[k] == -INFINITY ? 0.0f : exp2f(wm[k] - top);
-            sum += wl[k] * f;
-            x += acc[k][d] * f;
+}
+
+/* joins the records of the (sequence, query head) pairs that span workgroups:
+   one a workgroup for the runs it joined, and one of the run that went on to
+   another pair. Thread d owns column d; a tile of records is read at once. */
+template <int D>
+__global__ __launch_bounds__(D) void paged_merge_kernel(DecodeArgs a, uint32_t waves) {
+    constexpr int TILE = 16;
+    const PagedDecodeParams& p = a.p;
+    const uint32_t b = blockIdx.x / p.heads, head = blockIdx.x % p.heads, G = p.heads / p.c.kvHeads;
+    const uint32_t group = head % G / a.perGroup, row = head % G % a.perGroup;
+    const uint32_t pairs = p.c.kvHeads * a.groups, pair = head / G * a.groups + group;
+    const uint32_t begin = a.plan[b], slabs = (a.plan[b + 1] - begin) / pairs;
+    if (slabs == 0) return;
+    const Cut cut(a.plan[p.c.batch], waves);
+    const uint32_t first = begin + pair * slabs, end = first + slabs;
+    const uint32_t from = cut.run_of(first), to = cut.run_of(end - 1);
+    const bool toEnd = end == cut.begin(to + 1);       // the last run ends with the pair
+    if (from == to || (from / WAVES == to / WAVES && toEnd)) return;
+    const uint32_t wg = from / WAVES;
+    // joined records: of every workgroup but the last one where that holds no more than the run that went on
+    const uint32_t joined = to / WAVES - wg + (toEnd || to % WAVES > (to / WAVES == wg ? from % WAVES : 0u) ? 1 : 0);
+    const uint32_t total = joined + (toEnd ? 0 : 1);
+    const size_t size = size_t(a.perGroup) * (D + 2);
+    const uint32_t d = threadIdx.x;
+    float top = -INFINITY, sum = 0.0f, x = 0.0f;
+    for (uint32_t k0 = 0; k0 < total; k0 += TILE) {
+        float mk[TILE], lk[TILE], xk[TILE];
+#pragma unroll
+        for (int i = 0; i < TILE; ++i) {
+            const uint32_t k = k0 + i < total ? k0 + i : total - 1;
+            const uint32_t slot = k < joined ? ((wg + k) * WAVES + (k ? 0 : from % WAVES)) * 2 + 1 : to * 2;
+            const float* rec = a.records + slot * size;
+            mk[i] = k0 + i < total ? rec[row] : -INFINITY;
+            lk[i] = k0 + i < total ? rec[a.perGroup + row] : 0.0f;
+            xk[i] = rec[2 * a.perGroup + row * D + d];
         }
-        x = bad ? __builtin_nanf("") : x / sum;
-        if (p.outputGate) x *= sigmoid_of(load_elem(p.q, qrow + D + d, p.inType));
-        out[d] = x;
+        float next = top;
+#pragma unroll
+        for (int i = 0; i < TILE; ++i) next = fmaxf(next, mk[i]);
+        const float base = next == -INFINITY ? 0.0f : next, keep = exp2f(top - base);
+        sum *= keep;
+        x *= keep;
+#pragma unroll
+        for (int i = 0; i < TILE; ++i) {
+            const float f = exp2f(mk[i] - base);
+            sum += lk[i] * f;
+            x += xk[i] * f;
+        }
+        top = next;
     }
+    p.out[(size_t(b) * p.heads + head) * D + d] = gated(p, b, head, d, x / sum);
 }
 
 bool rotation_ok(Context& ctx, const char* who, const float* freqs, int rot, uint32_t dim, float amplitude) {
@@ -326,6 +905,36 @@ bool launch_paged_append(const PagedAppendParams& p, hipStream_t stream) {
     });
 }
 
+namespace {
+
+/* how a decode is launched */
+struct DecodeShape {
+    uint32_t groups, perGroup;       // of a kv head's query heads
+    uint32_t slice;                  // sequences of a launch; 0: one is too much
+    uint32_t grid;
+};
+
+DecodeShape decode_shape(const PagedDecodeParams& p) {
+    DecodeShape s{};
+    const uint32_t G = p.heads / p.c.kvHeads;
+    s.groups = (G + ROWS - 1) / ROWS;
+    s.perGroup = (G + s.groups - 1) / s.groups;
+    uint64_t slabs = (uint64_t(p.maxLength) + SLAB - 1) / SLAB;
+    if (p.window && p.window / SLAB + 2 < slabs) slabs = p.window / SLAB + 2;
+    const uint64_t each = slabs * p.c.kvHeads * s.groups, most = uint64_t(1) << 31;   // slabs are counted in 32 bits
+    uint64_t slice = p.c.batch < MAXB ? p.c.batch : MAXB;
+    if (each && slice > most / each) slice = most / each;
+    s.slice = uint32_t(slice);
+    const int cus = Context::instance().cus ? Context::instance().cus : 256;
+    const uint64_t most_grid = uint64_t(cus) * occupancy(int(p.c.dim)), want = (slice * each + WAVES - 1) / WAVES;
+    s.grid = uint32_t(want < most_grid ? (want ? want : 1) : most_grid);
+    return s;
+}
+
+constexpr size_t PLAN_BYTES = (MAXB + 1) * 4 + 252 & ~size_t(255);
+
+} // namespace
+
 bool check_paged_decode(const PagedDecodeParams& p) {
     Context& ctx = Context::instance();
     if (!cache_ok(ctx, "paged decode", p.c)) return false;
@@ -342,18 +951,62 @@ bool check_paged_decode(const PagedDecodeParams& p) {
         return ctx.fail("paged decode: the scale must be positive and finite");
     if (p.maxLength > uint64_t(p.c.tableWidth) * p.c.pageSize)
         return ctx.fail("paged decode: maxLength exceeds the positions of the table");
+    if (p.maxLength > (1u << 31)) return ctx.fail("paged decode: maxLength must be at most 2^31");
+    if (p.c.batch && decode_shape(p).slice == 0) return ctx.fail("paged decode: one sequence is too much work");
     return true;
 }
 
-size_t paged_decode_workspace(const PagedDecodeParams& p) { return 0; }
+size_t paged_decode_workspace(const PagedDecodeParams& p) {
+    if (p.c.batch == 0) return 0;
+    const DecodeShape s = decode_shape(p);
+    return PLAN_BYTES + size_t(s.grid) * WAVES * 2 * s.perGroup * (p.c.dim + 2) * sizeof(float);
+}
 
 bool launch_paged_decode(const PagedDecodeParams& p, void* work, hipStream_t stream) {
     Context& ctx = Context::instance();
     if (p.c.batch == 0) return true;
-    const unsigned grid = p.c.batch * p.heads;
-    return ctx.launch("paged_decode_kernel", stream, [&] {
-        hipLaunchKernelGGL(paged_decode_kernel, dim3(grid), dim3(THREADS), 0, stream, p);
-    });
+    const DecodeShape s = decode_shape(p);
+    DecodeArgs a{};
+    a.p = p;
+    a.plan = static_cast<uint32_t*>(work);
+    a.records = reinterpret_cast<float*>(static_cast<char*>(work) + PLAN_BYTES);
+    a.groups = s.groups;
+    a.perGroup = s.perGroup;
+    a.scaleLog2 = p.scale * LOG2E;
+    const size_t es = p.inType == 1 ? 2 : 4;
+    a.wideQ = (reinterpret_cast<uintptr_t>(p.q) & 15) == 0 && (p.heads == 1 || p.qStride % (16 / es) == 0) &&
+              (p.c.batch == 1 || p.qTokenStride % (16 / es) == 0);
+    for (uint32_t b0 = 0; b0 < p.c.batch; b0 += s.slice) {
+        a.p.c.batch = p.c.batch - b0 < s.slice ? p.c.batch - b0 : s.slice;
+        a.p.c.table = p.c.table + b0 * p.c.tableStride;
+        a.p.c.lengths = p.c.lengths + b0;
+        a.p.q = static_cast<const char*>(p.q) + b0 * p.qTokenStride * es;
+        a.p.out = p.out + size_t(b0) * p.heads * p.c.dim;
+        auto go = [&](auto attention, auto merge) {
+            return ctx.launch("paged_attention_kernel", stream, [&] {
+                       hipLaunchKernelGGL(attention, dim3(s.grid), dim3(THREADS), 0, stream, a);
+                   }) &&
+                   ctx.launch("paged_merge_kernel", stream, [&] {
+                       hipLaunchKernelGGL(merge, dim3(a.p.c.batch * p.heads), dim3(p.c.dim), 0, stream, a,
+                                          s.grid * WAVES);
+                   });
+        };
+        bool ok = false;
+        auto of = [&](auto dim) {
+            constexpr int D = decltype(dim)::value;
+            ok = p.inType == 1 ? go(paged_attention_kernel<D, true>, paged_merge_kernel<D>)
+                               : go(paged_attention_kernel<D, false>, paged_merge_kernel<D>);
+        };
+        switch (p.c.dim) {
+            case 64: of(std::integral_constant<int, 64>{}); break;
+            case 96: of(std::integral_constant<int, 96>{}); break;
+            case 128: of(std::integral_constant<int, 128>{}); break;
+            case 192: of(std::integral_constant<int, 192>{}); break;
+            default: of(std::integral_constant<int, 256>{}); break;
+        }
+        if (!ok) return false;
+    }
+    return true;
 }
 
 } // namespace aigpu
