@@ -638,15 +638,17 @@ typedef struct AiGpuPagedDecode {
     uint32_t reserved;
     uint64_t heads, qStride, qTokenStride;  /* qStride 0 means dim, qTokenStride 0 heads*qStride */
     uint64_t window;          /* the last `window` positions only; 0 = all */
-    void* workspace;          /* device, 256-byte aligned, or NULL: the backend's own scratch */
+    void* workspace;          /* device, 256-byte aligned, zero-filled at first; NULL: the backend's scratch */
     uint64_t workspaceBytes;
     void* stream;
 } AiGpuPagedDecode;
 AIGPU_ABI int aigpu_paged_decode(const AiGpuPagedDecode* args);
 /* The workspace bytes that a call with these sizes needs at most (0: none),
-   whatever the lengths hold. Calls that may run at once need a workspace each.
-   A call captured into a graph has to bring one where this is not 0: the
-   backend's scratch may move. */
+   whatever the lengths hold. The workspace is zero-filled before its first use
+   (as aigpu_allocate leaves it); every call leaves the part that matters zero
+   again, so calls of any sizes may follow one another in it, but calls that may
+   run at once need one each. A call captured into a graph has to bring one
+   where this is not 0: the backend's scratch may move. */
 AIGPU_ABI uint64_t aigpu_paged_decode_workspace(const AiGpuPagedDecode* args);
 
 /* ------------------------------------------------------------------------ */

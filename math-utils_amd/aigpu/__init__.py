@@ -18,6 +18,7 @@ Device forms (torch tensors on the GPU):
 """
 import ctypes as C
 import os
+import struct as _struct
 
 import numpy as np
 
@@ -867,16 +868,44 @@ def rotary_frequencies(rotary_dims, theta, scaling=None, factor=1.0, original=0.
     return out, amplitude.value
 
 
-def _same_device(first, name, *others):
-    """every tensor on the backend's device; `others` are (tensor or None, name)"""
-    import torch
-    for t, n in ((first, name),) + others:
-        if t is None:
-            continue
-        if not isinstance(t, torch.Tensor):
-            raise TypeError(f"{n} must be a torch.Tensor")
-        if not t.is_cuda or t.get_device() != 0:
-            raise ValueError(f"{n} must be on the backend's GPU, cuda:0")
+# These calls are short enough on the GPU that the binding shows: their
+# structures are packed in one go (2 us less than filling a ctypes Structure of
+# thirty fields) and passed to the entry points as bytes.
+_CACHE = "4P10Q"
+_PACK = {"aigpu_rotary": _struct.Struct("4Pf5I8QP"),
+         "aigpu_paged_append": _struct.Struct(_CACHE + "5P3f3I3QP"),
+         "aigpu_paged_decode": _struct.Struct(_CACHE + "4P4f6I4QPQP")}
+_entries = {}
+
+
+def _entry(name):
+    """the entry point taking its structure as bytes"""
+    fn = _entries.get(name)
+    if fn is None:
+        fn = lib()[name]         # a function object of its own beside the one that SIGNATURES declares
+        fn.restype, fn.argtypes = C.c_int, [C.c_char_p]
+        _entries[name] = fn
+    return fn
+
+
+def _packed(name, *values):
+    try:
+        return _PACK[name].pack(*values)
+    except _struct.error as e:
+        raise ValueError(f"{name}: an argument is out of range: {e}") from None
+
+
+def _at(t, name):
+    """the address of a tensor of the backend's device, or 0 for None"""
+    if t is None:
+        return 0
+    try:
+        device = t.get_device()
+    except AttributeError:
+        raise TypeError(f"{name} must be a torch.Tensor") from None
+    if device != 0:
+        raise ValueError(f"{name} must be on the backend's GPU, cuda:0")
+    return t.data_ptr()
 
 
 def _own_stream(stream):
@@ -884,45 +913,55 @@ def _own_stream(stream):
     if stream is not None:
         return stream
     import torch
-    return torch.cuda.current_stream(0).cuda_stream
+    raw = getattr(torch._C, "_cuda_getCurrentRawStream", None)   # without a Stream object built round it
+    return raw(0) if raw else torch.cuda.current_stream(0).cuda_stream
 
 
-def _whole(value, name, most=0xFFFFFFFFFFFFFFFF):
-    """the C structures would wrap what is out of range"""
-    if not 0 <= value <= most:
-        raise ValueError(f"{name} must be 0 .. {most}, not {value}")
+def _kind(t):
+    """the type tag of a float32 or bfloat16 tensor"""
+    import torch
+    if t.dtype is torch.bfloat16:
+        return BF16
+    if t.dtype is torch.float32:
+        return F32
+    raise TypeError(f"unsupported dtype {t.dtype}: float32 or bfloat16")
 
 
 def _vector(t, name, least, exact=False):
-    """an fp32 vector of at least (or exactly) `least` elements, or None; its address"""
-    import torch
+    """the address of an fp32 vector of at least (or exactly) `least` elements, or 0 for None"""
     if t is None:
-        return None
-    if t.dtype != torch.float32 or t.dim() != 1 or (t.stride(0) != 1 and t.shape[0] > 1):
+        return 0
+    at = _at(t, name)
+    if _kind(t) != F32 or t.dim() != 1 or not t.is_contiguous():
         raise TypeError(f"{name} must be a contiguous float32 vector")
-    if t.shape[0] < least or (exact and t.shape[0] != least):
-        raise ValueError(f"{name} has {t.shape[0]} elements, {least} are needed")
-    return t.data_ptr()
+    n = t.shape[0]
+    if n < least or (exact and n != least):
+        raise ValueError(f"{name} has {n} elements, {least} are needed")
+    return at
 
 
-def _indices(t, name, dims, shape=None):
-    """an int32 (or uint32) tensor of `dims` dimensions with unit stride in the last; its address"""
+def _indices(t, name, dims, entries=None):
+    """the address of an int32 (or uint32) tensor of `dims` dimensions with unit stride in the last"""
     import torch
+    at = _at(t, name)
     if t.dtype not in (torch.int32, torch.uint32) or t.dim() != dims or (t.stride(-1) != 1 and t.shape[-1] > 1):
         raise TypeError(f"{name} must be an int32 tensor of {dims} dimensions with unit stride")
-    if shape is not None and t.shape[0] != shape:
-        raise ValueError(f"{name} has {t.shape[0]} entries, {shape} are needed")
-    return t.data_ptr()
+    if entries is not None and t.shape[0] != entries:
+        raise ValueError(f"{name} has {t.shape[0]} entries, {entries} are needed")
+    return at
 
 
 def _strides(t, name):
     """(token, head) element strides of a [tokens][heads][dim] tensor with
     unit stride in the last dimension; a dimension of one has its dense one"""
     n, heads, dim = t.shape
-    if t.stride(2) != 1 and dim > 1:
+    ts, hs, one = t.stride()
+    if one != 1 and dim > 1:
         raise ValueError(f"{name} must have unit stride in its last dimension")
-    hs = t.stride(1) if heads > 1 else dim
-    ts = t.stride(0) if n > 1 else heads * hs
+    if heads == 1:
+        hs = dim
+    if n == 1:
+        ts = heads * hs
     if ts <= 0 or hs <= 0:
         raise ValueError(f"{name} must not be a broadcast view")
     return ts, hs
@@ -936,44 +975,41 @@ def rotary(x, out, freqs, positions=None, start=0, rotary_dims=None, interleaved
     freqs[j], halves paired or neighbours (interleaved); the rest is copied.
     positions [tokens] int32, or start, start + 1, ... backward=True gives x's
     gradient from out's (the transposed rotation). Asynchronous."""
-    _same_device(x, "x", (out, "out"), (freqs, "freqs"), (positions, "positions"))
+    of, to = _at(x, "x"), _at(out, "out")
     if x.dim() != 3 or out.shape != x.shape or out.dtype != x.dtype:
         raise ValueError("x must be [tokens][heads][dim], and out of its shape and type")
     count, heads, dim = x.shape
     rot = 2 * freqs.shape[0] if rotary_dims is None else rotary_dims
-    _whole(rot, "rotary_dims", 4096)
-    _whole(start, "start", 0xFFFFFFFF)
+    turns = _vector(freqs, "freqs", rot // 2)
+    where = 0 if positions is None else _indices(positions, "positions", 1, count)
     if x.numel() == 0:
         return out
     ts, hs = _strides(x, "x")
     ots, ohs = _strides(out, "out")
-    a = AiGpuRotary(x.data_ptr(), out.data_ptr(),
-                    None if positions is None else _indices(positions, "positions", 1, count),
-                    _vector(freqs, "freqs", rot // 2), amplitude, rot, _dtype_tag(x), 1 if interleaved else 0,
-                    1 if backward else 0, 0, count, start, heads, dim, ts, hs, ots, ohs, _own_stream(stream))
-    _check(lib().aigpu_rotary(C.byref(a)))
+    args = _packed("aigpu_rotary", of, to, where, turns, amplitude, rot, _kind(x), 1 if interleaved else 0,
+                   1 if backward else 0, 0, count, start, heads, dim, ts, hs, ots, ohs, _own_stream(stream))
+    _check(_entry("aigpu_rotary")(args))
     return out
 
 
 def _paged_cache(keys, values, table, lengths):
-    import torch
-    if keys.dtype != torch.bfloat16 or values.dtype != torch.bfloat16:
+    """AiGpuPagedCache's fields"""
+    at = _at(keys, "key_pages"), _at(values, "value_pages"), _indices(table, "table", 2), _indices(lengths, "lengths", 1)
+    if _kind(keys) != BF16 or _kind(values) != BF16:
         raise TypeError("the pages must be bfloat16")
-    if keys.dim() != 4 or values.shape != keys.shape or values.stride() != keys.stride():
+    strides = keys.stride()
+    if len(strides) != 4 or values.shape != keys.shape or values.stride() != strides:
         raise ValueError("key and value pages must be [pages][kv_heads][page_size][dim] with the same strides")
     pages, kv_heads, size, dim = keys.shape
-    ps, hs, rs, one = keys.stride()
+    ps, hs, rs, one = strides
     if one != 1 and dim > 1:
         raise ValueError("the pages must have unit stride in their last dimension")
     # a dimension of one may carry any stride: give it one that is in range
-    rs = rs if size > 1 else dim
-    hs = hs if kv_heads > 1 else dim
-    ps = ps if pages > 1 else dim
-    batch = lengths.shape[0] if lengths.dim() == 1 else -1
-    width = table.shape[1] if table.dim() == 2 else 0
-    return AiGpuPagedCache(keys.data_ptr(), values.data_ptr(), _indices(table, "table", 2, batch),
-                           _indices(lengths, "lengths", 1), batch, pages, size, kv_heads, dim, width,
-                           table.stride(0) if batch > 1 else width, ps, hs, rs)
+    batch, (rows, width) = lengths.shape[0], table.shape
+    if rows != batch:
+        raise ValueError(f"table has {rows} entries, {batch} are needed")
+    return at + (batch, pages, size, kv_heads, dim, width, table.stride(0) if batch > 1 else width,
+                 ps if pages > 1 else dim, hs if kv_heads > 1 else dim, rs if size > 1 else dim)
 
 
 def paged_append(k, v, key_pages, value_pages, table, lengths, starts=None, k_norm=None, eps=1e-6, norm_offset=0.0,
@@ -984,55 +1020,46 @@ def paged_append(k, v, key_pages, value_pages, table, lengths, starts=None, k_no
     places that table [batch][width] and lengths [batch] (the new tokens
     included) say; starts [batch + 1] where a sequence has other than one.
     Asynchronous."""
-    _same_device(k, "k", (v, "v"), (key_pages, "key_pages"), (value_pages, "value_pages"), (table, "table"),
-                 (lengths, "lengths"), (starts, "starts"), (k_norm, "k_norm"), (freqs, "freqs"))
     cache = _paged_cache(key_pages, value_pages, table, lengths)
-    count = k.shape[0]
-    if k.dim() != 3 or k.shape[1] != cache.kvHeads or k.shape[2] != cache.dim or v.shape != k.shape \
-            or v.dtype != k.dtype:
+    of_k, of_v, batch, kv_heads, dim = _at(k, "k"), _at(v, "v"), cache[4], cache[7], cache[8]
+    shape = k.shape
+    if len(shape) != 3 or shape[1] != kv_heads or shape[2] != dim or v.shape != shape or v.dtype != k.dtype:
         raise ValueError("k and v must be [tokens][kv_heads][dim] of one type, as the pages have them")
-    if count == 0:
+    begins = 0 if starts is None else _indices(starts, "starts", 1, batch + 1)
+    rot = 0 if freqs is None else (2 * freqs.shape[0] if rotary_dims is None else rotary_dims)
+    turns, gamma = _vector(freqs, "freqs", rot // 2), _vector(k_norm, "k_norm", dim, True)
+    if shape[0] == 0:
         return
     (ks, kh), (vs, vh) = _strides(k, "k"), _strides(v, "v")
-    if kh != cache.dim or vh != cache.dim:
+    if kh != dim or vh != dim:
         raise ValueError("the heads of a token's k and v must lie one after the other")
-    rot = 0 if freqs is None else (2 * freqs.shape[0] if rotary_dims is None else rotary_dims)
-    _whole(rot, "rotary_dims", 4096)
-    a = AiGpuPagedAppend(cache, k.data_ptr(), v.data_ptr(),
-                         None if starts is None else _indices(starts, "starts", 1, cache.batch + 1),
-                         _vector(k_norm, "k_norm", cache.dim, True), _vector(freqs, "freqs", rot // 2), eps,
-                         norm_offset, amplitude, rot, 1 if interleaved else 0, _dtype_tag(k), count, ks, vs,
-                         _own_stream(stream))
-    _check(lib().aigpu_paged_append(C.byref(a)))
+    args = _packed("aigpu_paged_append", *cache, of_k, of_v, begins, gamma, turns, eps, norm_offset, amplitude, rot,
+                   1 if interleaved else 0, _kind(k), shape[0], ks, vs, _own_stream(stream))
+    _check(_entry("aigpu_paged_append")(args))
 
 
 def _paged_decode(q, out, key_pages, value_pages, table, lengths, max_length, q_norm, eps, norm_offset, freqs,
                   rotary_dims, interleaved, amplitude, scale, window, output_gate, workspace, stream):
-    import torch
-    _same_device(q, "q", (out, "out"), (key_pages, "key_pages"), (value_pages, "value_pages"), (table, "table"),
-                 (lengths, "lengths"), (q_norm, "q_norm"), (freqs, "freqs"), (workspace, "workspace"))
     cache = _paged_cache(key_pages, value_pages, table, lengths)
-    if q.dim() != 3 or q.shape[0] != cache.batch or q.shape[2] < cache.dim:
+    of_q, to, batch, dim = _at(q, "q"), _at(out, "out"), cache[4], cache[8]
+    if q.dim() != 3 or q.shape[0] != batch or q.shape[2] < dim:
         raise ValueError("q must be [batch][heads][at least dim]")
     heads = q.shape[1]
-    if out.dtype != torch.float32 or tuple(out.shape) != (cache.batch, heads, cache.dim) or not out.is_contiguous():
+    if _kind(out) != F32 or tuple(out.shape) != (batch, heads, dim) or not out.is_contiguous():
         raise ValueError("out must be a contiguous float32 [batch][heads][dim]")
     ts, hs = _strides(q, "q") if q.numel() else (1, q.shape[2])
     rot = 0 if freqs is None else (2 * freqs.shape[0] if rotary_dims is None else rotary_dims)
-    room, nbytes = None, 0
+    room, nbytes = 0, 0
     if workspace is not None:
         if not workspace.is_contiguous():
             raise ValueError("workspace must be contiguous")
-        room, nbytes = workspace.data_ptr(), workspace.numel() * workspace.element_size()
+        room, nbytes = _at(workspace, "workspace"), workspace.numel() * workspace.element_size()
     if max_length is None:
-        max_length = min(cache.tableWidth * cache.pageSize, 0xFFFFFFFF)
-    _whole(max_length, "max_length", 0xFFFFFFFF)
-    _whole(window, "window")
-    _whole(rot, "rotary_dims", 4096)
-    return AiGpuPagedDecode(cache, q.data_ptr(), out.data_ptr(), _vector(q_norm, "q_norm", cache.dim, True),
-                            _vector(freqs, "freqs", rot // 2), eps, norm_offset, amplitude, scale, rot,
-                            1 if interleaved else 0, _dtype_tag(q), 1 if output_gate else 0, max_length, 0, heads, hs,
-                            ts, window, room, nbytes, _own_stream(stream))
+        max_length = min(cache[9] * cache[6], 0xFFFFFFFF)
+    return _packed("aigpu_paged_decode", *cache, of_q, to, _vector(q_norm, "q_norm", dim, True),
+                   _vector(freqs, "freqs", rot // 2), eps, norm_offset, amplitude, scale, rot,
+                   1 if interleaved else 0, _kind(q), 1 if output_gate else 0, max_length, 0, heads, hs, ts, window,
+                   room, nbytes, _own_stream(stream))
 
 
 def paged_decode(q, out, key_pages, value_pages, table, lengths, max_length=None, q_norm=None, eps=1e-6,
@@ -1043,17 +1070,20 @@ def paged_decode(q, out, key_pages, value_pages, table, lengths, max_length=None
     and rotated at lengths[b] - 1 on load; out [batch][heads][dim] fp32; the
     pages, table and lengths as paged_append left them. max_length (default:
     what the table can hold) is at least every length. A call captured into a
-    graph brings a workspace of paged_decode_workspace(...) bytes.
-    Asynchronous."""
-    a = _paged_decode(q, out, key_pages, value_pages, table, lengths, max_length, q_norm, eps, norm_offset, freqs,
-                      rotary_dims, interleaved, amplitude, scale, window, output_gate, workspace, stream)
-    if lengths.shape[0]:
-        _check(lib().aigpu_paged_decode(C.byref(a)))
+    graph brings a workspace (paged_decode_workspace), its own where calls may
+    run at once. Asynchronous."""
+    args = _paged_decode(q, out, key_pages, value_pages, table, lengths, max_length, q_norm, eps, norm_offset, freqs,
+                         rotary_dims, interleaved, amplitude, scale, window, output_gate, workspace, stream)
+    if q.shape[0]:
+        _check(_entry("aigpu_paged_decode")(args))
     return out
 
 
 def paged_decode_workspace(q, out, key_pages, value_pages, table, lengths, max_length=None):
-    """the bytes of a workspace for paged_decode calls of these sizes, whatever the lengths hold"""
-    a = _paged_decode(q, out, key_pages, value_pages, table, lengths, max_length, None, 1e-6, 0.0, None, None, False,
-                      1.0, 0.0, 0, False, None, None)
-    return int(lib().aigpu_paged_decode_workspace(C.byref(a)))
+    """a workspace (zero-filled uint8 tensor) for paged_decode calls of these
+    sizes or smaller ones of the same heads and dim, whatever the lengths hold"""
+    import torch
+    args = _paged_decode(q, out, key_pages, value_pages, table, lengths, max_length, None, 1e-6, 0.0, None, None,
+                         False, 1.0, 0.0, 0, False, None, None)
+    need = lib().aigpu_paged_decode_workspace(C.cast(C.c_char_p(args), C.POINTER(AiGpuPagedDecode)))
+    return torch.zeros(int(need), dtype=torch.uint8, device=q.device)

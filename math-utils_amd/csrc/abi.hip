@@ -150,7 +150,8 @@ void* Context::grow(ScratchSlot slot, size_t bytes) {
 void* Context::growZeroed(ScratchSlot slot, size_t bytes) {
     const bool fresh = scratchBytes[slot] < (bytes ? bytes : 256);
     void* p = grow(slot, bytes);
-    if (p && fresh && hipMemset(p, 0, scratchBytes[slot]) != hipSuccess) {
+    // waited for: the call's own stream need not follow the one of the memset
+    if (p && fresh && (hipMemset(p, 0, scratchBytes[slot]) != hipSuccess || hipDeviceSynchronize() != hipSuccess)) {
         (void)hipGetLastError();
         error = "hipMemset of scratch failed";
         return nullptr;
@@ -1220,7 +1221,7 @@ AIGPU_ABI int aigpu_paged_decode(const AiGpuPagedDecode* args) {
                         " bytes)"),
                0;
     const StreamOrder order(ctx, stream);
-    void* work = ctx.grow(aigpu::SLOT_PAGED, need);
+    void* work = ctx.growZeroed(aigpu::SLOT_PAGED, need);
     return work && aigpu::launch_paged_decode(p, work, stream) ? 1 : 0;
 }
 

@@ -181,16 +181,17 @@ __global__ __launch_bounds__(THREADS) void paged_append_kernel(AppendArgs a) {
 }
 
 /*
-    One token's attention over the pages, in two launches.
+    One token's attention over the pages.
 
     The batch is cut into slabs of 32 positions of one sequence, one kv head and
-    up to 16 of its query heads, listed sequence by sequence, and the list into
-    one even run a wave: whatever the lengths, every wave reads the same number of
-    slabs within one, and the work is bounded by the keys and values read once
-    (HBM). paged_attention_kernel works a run off as one software pipeline over
-    its slabs, whichever sequence they belong to: page ids are read two slabs
-    ahead, keys (registers) and values (DMA into LDS) one slab ahead, so loads
-    stay in flight while a sequence ends and the next one's queries are prepared.
+    up to 16 of its query heads (a pair: sequence, heads), listed pair by pair,
+    and the list into one even run a wave: whatever the lengths, every wave reads
+    as many slabs, within one, and the work is bounded by the keys and values,
+    read once (HBM). paged_attention_kernel works a run off as one software
+    pipeline over its slabs, whichever pair they belong to: page ids are read two
+    slabs ahead, keys (registers) and values (DMA into LDS) one slab ahead, so
+    loads stay in flight while a pair ends and the next one's queries are
+    prepared.
       scores   v_mfma_f32_16x16x32_bf16, 16 keys as A, the heads' queries as B, in
                three terms of 8 bits each (x = hi + mid + lo exactly: fp32 is 24
                bits), so the products are fp32's; three instructions a tile cost
@@ -198,20 +199,28 @@ __global__ __launch_bounds__(THREADS) void paged_append_kernel(AppendArgs a) {
       softmax  a running maximum and sum a head; lane l holds head l % 16
       p v      the weights in three terms likewise, as A, exactly the scores the
                lane holds; values as B through ds_read_b64_tr_b16
-    A sequence's head wholly in one run is written at once. What is left at the
-    end of a run is joined over the workgroup's waves in LDS; pairs that span
-    workgroups leave (max, sum, weighted values) records, two a wave at most, that
-    paged_merge_kernel joins in their order, so results do not depend on timing.
+    A pair wholly in one run is written at once. What is left at the end of a run
+    is joined over the workgroup's waves in LDS; pairs that span workgroups leave
+    (max, sum, weighted values) records, two a wave at most, that are joined in
+    their order, so results do not depend on timing: by the workgroup that finds
+    itself the last of the pair's (a counter that it sets back to zero), or, where
+    a pair's records are more than one workgroup should read, by
+    paged_merge_kernel.
 */
 constexpr int SLAB = 32;
 constexpr int WAVES = 4;
 constexpr int ROWS = 16;             // query heads of a group
 constexpr uint32_t MAXB = 512;       // sequences of a launch
+constexpr uint32_t MAX_RUNS = 4096;
+// A pair's queries and its end cost about what a slab's loads do when many are
+// short, so the list counts a unit for them before its slabs' units.
+constexpr uint32_t OPENING = 1;
 
 struct DecodeArgs {
     PagedDecodeParams p;
-    uint32_t* plan;                  // [MAXB + 1] slabs before each sequence, and in all
-    float* records;                  // [waves][2]: (m, l)[perGroup], then [perGroup][dim]
+    uint32_t* arrived;               // [runs] by a pair's last run; zero between calls
+    uint32_t* plan;                  // [MAXB + 1] units before each sequence, and in all; null: joined in the kernel
+    float* records;                  // [runs][2] of record_floats
     uint32_t groups, perGroup;       // of one kv head's query heads
     float scaleLog2;
     int wideQ;                       // q rows can be read 16 bytes at a time
@@ -264,7 +273,7 @@ __device__ __forceinline__ uint32_t slabs_of(const PagedDecodeParams& p, uint32_
     return len == 0 || len > p.maxLength ? 0u : (len + SLAB - 1) / SLAB - first_of(p, len) / SLAB;
 }
 
-/* the even cut of `total` slabs into runs: run w's first slab, and a slab's run */
+/* the even cut of `total` units into runs: run w's first unit, and a unit's run */
 struct Cut {
     uint32_t runs, each, extra;      // the first `extra` runs have one more
     __device__ __forceinline__ Cut(uint32_t total, uint32_t waves) {
@@ -275,10 +284,51 @@ struct Cut {
     __device__ __forceinline__ uint32_t begin(uint32_t w) const {
         return w < runs ? w * each + (w < extra ? w : extra) : runs * each + extra;
     }
-    __device__ __forceinline__ uint32_t run_of(uint32_t slab) const {
+    __device__ __forceinline__ uint32_t run_of(uint32_t unit) const {
         const uint32_t longer = extra * (each + 1);
-        return slab < longer ? slab / (each + 1) : extra + (slab - longer) / each;
+        return unit < longer ? unit / (each + 1) : extra + (unit - longer) / each;
     }
+};
+
+/* a record: the rows' maxima and sums, padded to 16 bytes, then [perGroup][D] */
+__host__ __device__ constexpr uint32_t record_heads(uint32_t rows) { return (2 * rows + 3) / 4 * 4; }
+__host__ __device__ constexpr uint32_t record_floats(uint32_t rows, uint32_t D) { return record_heads(rows) + rows * D; }
+
+/* The parts of a pair whose units are begin .. end - 1: `joined` records of
+   workgroups wg, wg + 1, ... over their runs, then one of run `to` if that went
+   on to another pair. Of one part alone there is no record: its wave or its
+   workgroup wrote the output. */
+struct Parts {
+    uint32_t from, to, joined, total;
+    Parts() = default;
+    __device__ __forceinline__ Parts(const Cut& cut, uint32_t begin, uint32_t end) {
+        from = cut.run_of(begin + OPENING);
+        to = cut.run_of(end - 1);
+        const bool toEnd = end + OPENING >= cut.begin(to + 1);     // no later slab in run `to`
+        const uint32_t wg = from / WAVES, last = to / WAVES;
+        joined = last - wg + (toEnd || to % WAVES > (last == wg ? from % WAVES : 0u) ? 1 : 0);
+        total = joined + (toEnd ? 0 : 1);
+        if (from == to) total = 1;
+    }
+    // the place of part k's record in [runs][2]
+    __device__ __forceinline__ uint32_t slot(uint32_t k) const {
+        return k == joined ? to * 2 : ((from / WAVES + k) * WAVES + (k ? 0 : from % WAVES)) * 2 + 1;
+    }
+};
+
+/* Records go from one workgroup to another within a launch, perhaps between
+   XCDs, whose L2s do not see each other's lines: written and read past the L2
+   (device scope), which spares the fences that would write back and invalidate
+   it whole. Their order: the writer's stores are waited for before it counts
+   itself in, and the reader reads after the last count. */
+constexpr int PAST_L2 = 16;          // the buffer instructions' sc1 bit
+__device__ __forceinline__ __amdgpu_buffer_rsrc_t buffer_of(float* base) {
+    return __builtin_amdgcn_make_buffer_rsrc(base, 0, -1, 0x00027000);
+}
+
+struct Piece {
+    uint32_t begin, end;             // the pair's units; begin NOWHERE: none
+    uint32_t b, head, rows;          // its query heads: head .. head + rows - 1 of sequence b
 };
 
 struct Slab {
@@ -312,6 +362,121 @@ __device__ __forceinline__ float gated(const PagedDecodeParams& p, uint32_t b, u
     return x * sigmoid_of(load_elem(p.q, b * p.qTokenStride + head * p.qStride + p.c.dim + d, p.inType));
 }
 
+/*
+    Joins rows `row0` .. of a pair's records into the output of query heads
+    `head` .. of sequence b, by TEAM threads: a workgroup or a wave, with the same
+    sums in the same order. A thread takes four columns of a row and adds the
+    parts up, a tile of them (one trip to memory) at a time; or, where that takes
+    fewer trips, the parts are dealt to WAVES shares, a wave of the workgroup each
+    (a wave alone takes them one after the other), that meet in `room`.
+*/
+constexpr int JOIN_FLOATS = 6;
+constexpr uint32_t FEW = 8, MANY = 16;   // parts of a tile: of all of them, of a share
+template <int D, int TEAM>
+__device__ __forceinline__ void join_parts(const DecodeArgs& a, const Parts& parts, uint32_t b, uint32_t head,
+                                           uint32_t row0, uint32_t rows, float* room) {
+    const PagedDecodeParams& p = a.p;
+    const uint32_t size = record_floats(a.perGroup, D), skip = record_heads(a.perGroup), units = rows * (D / 4);
+    const auto records = buffer_of(a.records);
+    float top, sum;
+    floatx4 x;
+    auto clear = [&] {
+        top = -INFINITY;
+        sum = 0.0f;
+        x = floatx4{0.0f, 0.0f, 0.0f, 0.0f};
+    };
+    auto word = [&](uint32_t at) {
+        return __uint_as_float(__builtin_amdgcn_raw_buffer_load_b32(records, at * 4, 0, PAST_L2));
+    };
+    // parts k0, k0 + step, ... `count` of them, of columns `unit`
+    auto add = [&](auto count, uint32_t unit, uint32_t k0, uint32_t step) {
+        constexpr uint32_t N = decltype(count)::value;
+        const uint32_t row = row0 + unit / (D / 4), d = unit % (D / 4) * 4;
+        float mk[N], lk[N];
+        u32x4 xk[N];
+#pragma unroll
+        for (uint32_t i = 0; i < N; ++i) {
+            const uint32_t k = k0 + i * step, at = parts.slot(k < parts.total ? k : k0) * size;
+            mk[i] = word(at + row);
+            lk[i] = word(at + a.perGroup + row);
+            xk[i] = __builtin_amdgcn_raw_buffer_load_b128(records, (at + skip + row * D + d) * 4, 0, PAST_L2);
+        }
+        float next = top;
+#pragma unroll
+        for (uint32_t i = 0; i < N; ++i)
+            if (k0 + i * step < parts.total) next = fmaxf(next, mk[i]);
+        const float base = next == -INFINITY ? 0.0f : next, keep = exp2f(top - base);
+        sum *= keep;
+        x *= keep;
+#pragma unroll
+        for (uint32_t i = 0; i < N; ++i) {
+            if (k0 + i * step >= parts.total) break;
+            const float f = exp2f(mk[i] - base);
+            sum += lk[i] * f;
+            x += __builtin_bit_cast(floatx4, xk[i]) * f;
+        }
+        top = next;
+    };
+    auto write = [&](uint32_t unit) {
+        const uint32_t h = head + unit / (D / 4), d = unit % (D / 4) * 4;
+        const float by = 1.0f / sum;
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+            p.out[(size_t(b) * p.heads + h) * D + d + i] = gated(p, b, h, d + i, x[i] * by);
+    };
+    const uint32_t trips = (units + THREADS - 1) / THREADS * ((parts.total + FEW - 1) / FEW);
+    const uint32_t shared = (units + WAVE - 1) / WAVE * ((parts.total + WAVES * MANY - 1) / (WAVES * MANY));
+    if (trips <= shared) {
+#pragma unroll 1
+        for (uint32_t unit = threadIdx.x % TEAM; unit < units; unit += TEAM) {
+            clear();
+#pragma unroll 1
+            for (uint32_t k0 = 0; k0 < parts.total; k0 += FEW)
+                add(std::integral_constant<uint32_t, FEW>{}, unit, k0, 1);
+            write(unit);
+        }
+        return;
+    }
+    auto meet = [] {
+        if constexpr (TEAM == WAVE) wave_sync();
+        else __syncthreads();
+    };
+    const uint32_t lane = threadIdx.x % WAVE, wave = TEAM == WAVE ? 0 : uniform(threadIdx.x / WAVE);
+#pragma unroll 1
+    for (uint32_t u0 = 0; u0 < units; u0 += WAVE) {
+        const uint32_t unit = u0 + lane;
+#pragma unroll 1
+        for (uint32_t q = wave; q < WAVES; q += TEAM / WAVE) {
+            if (unit >= units) continue;
+            clear();
+#pragma unroll 1
+            for (uint32_t k0 = q; k0 < parts.total; k0 += WAVES * MANY)
+                add(std::integral_constant<uint32_t, MANY>{}, unit, k0, WAVES);
+            float* mine = room + (q * WAVE + lane) * JOIN_FLOATS;
+            mine[0] = top;
+            mine[1] = sum;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) mine[2 + i] = x[i];
+        }
+        meet();
+        if (wave == 0 && unit < units) {
+            clear();
+#pragma unroll
+            for (uint32_t o = 0; o < WAVES; ++o) {
+                const float* theirs = room + (o * WAVE + lane) * JOIN_FLOATS;
+                const float next = fmaxf(top, theirs[0]), base = next == -INFINITY ? 0.0f : next;
+                const float keep = exp2f(top - base), f = exp2f(theirs[0] - base);
+                sum = sum * keep + theirs[1] * f;
+#pragma unroll
+                for (int i = 0; i < 4; ++i) x[i] = x[i] * keep + theirs[2 + i] * f;
+                top = next;
+            }
+            write(unit);
+        }
+        meet();
+    }
+}
+
 constexpr int occupancy(int D) { return D <= 128 ? 2 : 1; }
 
 template <int D, bool BF>
@@ -321,19 +486,21 @@ __global__ __launch_bounds__(THREADS, occupancy(D)) void paged_attention_kernel(
     const PagedDecodeParams& p = a.p;
     const PagedCache& c = p.c;
     const int lane = threadIdx.x & 63, w = int(uniform(threadIdx.x >> 6));
-    const int g = lane >> 4, c16 = lane & 15;
     const uint32_t B = c.batch, pairs = c.kvHeads * a.groups, G = p.heads / c.kvHeads;
 
     __shared__ uint32_t pre[MAXB + 1], lens[MAXB], sums[WAVES];
     __shared__ uint64_t place[WAVES][SLAB];
     __shared__ float2 turns[WAVES][D / 2];
     __shared__ float gamma[D];
-    __shared__ float wm[WAVES][ROWS], wl[WAVES][ROWS];
-    __shared__ uint32_t left[WAVES];              // the pair a wave's run leaves open (b * pairs + pair), or NOWHERE
+    __shared__ float wm[WAVES][ROWS], wl[WAVES][ROWS], total[ROWS];
+    // pairs that waves leave in parts: [w] in the record of a run that went on to
+    // another pair, [WAVES + w] open at the run's end
+    __shared__ Piece pieces[2 * WAVES];
+    __shared__ Parts joins[2 * WAVES];            // those that this workgroup joins; total 0: none
     __shared__ uint32_t leftEnds[WAVES];          // bit 0: from the pair's first slab, bit 1: to its last
     __shared__ __attribute__((aligned(16))) uint16_t vbuf[WAVES][2][SLAB * D];
 
-    // ---- the list: slabs before each sequence ----
+    // ---- the list: units before each sequence ----
     {
         uint32_t own[2];
 #pragma unroll
@@ -341,10 +508,12 @@ __global__ __launch_bounds__(THREADS, occupancy(D)) void paged_attention_kernel(
             const uint32_t b = 2 * threadIdx.x + i;
             const uint32_t len = b < B ? c.lengths[b] : 0u;
             if (b < B) lens[b] = len;
-            own[i] = slabs_of(p, len) * pairs;
+            const uint32_t slabs = slabs_of(p, len);
+            own[i] = slabs ? (slabs + OPENING) * pairs : 0u;
         }
         if (p.gamma)
             for (int d = threadIdx.x; d < D; d += THREADS) gamma[d] = p.gamma[d] + p.offset;
+        if (lane < 2) pieces[w + lane * WAVES].begin = NOWHERE;
         uint32_t x = own[0] + own[1];
 #pragma unroll
         for (int o = 1; o < WAVE; o <<= 1) {
@@ -361,7 +530,7 @@ __global__ __launch_bounds__(THREADS, occupancy(D)) void paged_attention_kernel(
         if (threadIdx.x == THREADS - 1 && B == MAXB) pre[B] = before + own[0] + own[1];
         __syncthreads();
     }
-    if (blockIdx.x == 0)
+    if (a.plan && blockIdx.x == 0)
         for (uint32_t i = threadIdx.x; i <= B; i += THREADS) a.plan[i] = pre[i];
     // sequences without a slab: empty ones, and those that cannot be
     for (uint32_t b = blockIdx.x; b < B; b += gridDim.x) {
@@ -373,10 +542,21 @@ __global__ __launch_bounds__(THREADS, occupancy(D)) void paged_attention_kernel(
     const Cut cut(uniform(pre[B]), gridDim.x * WAVES);
     const uint32_t run = blockIdx.x * WAVES + w;
     const uint32_t runEnd = cut.begin(run + 1);
-    uint32_t at = cut.begin(run);                 // the next slab to list
-    const uint32_t count = runEnd - at;
-    uint32_t seq = 0, pair = 0, slab = 0, slabs = 1, len = 0;
-    if (count) {
+    uint32_t at = cut.begin(run);                 // the next slab's unit
+    uint32_t seq = 0, pair = 0, slab = 0, slabs = 1, len = 0, fresh = OPENS;
+    // to the next pair's first slab, if the run reaches it
+    auto next_pair = [&] {
+        at += OPENING;
+        slab = 0;
+        if (at < runEnd && ++pair == pairs) {
+            pair = 0;
+            do ++seq;                             // at < pre[B]: a later sequence has slabs
+            while (uniform(pre[seq]) == uniform(pre[seq + 1]));
+            len = uniform(lens[seq]);
+            slabs = slabs_of(p, len);
+        }
+    };
+    if (at < runEnd) {
         uint32_t lo = 0, hi = B;                  // pre[lo] <= at < pre[hi]
         while (hi - lo > 1) {
             const uint32_t mid = (lo + hi) / 2;
@@ -387,34 +567,27 @@ __global__ __launch_bounds__(THREADS, occupancy(D)) void paged_attention_kernel(
         len = uniform(lens[seq]);
         slabs = slabs_of(p, len);
         const uint32_t in = at - uniform(pre[seq]);
-        pair = in / slabs;
-        slab = in % slabs;
+        pair = in / (slabs + OPENING);
+        slab = in % (slabs + OPENING);
+        if (slab < OPENING) at += OPENING - slab, slab = 0;
+        else slab -= OPENING;
     }
-    auto list = [&](Slab& s) {
+    auto list = [&](Slab& s) -> bool {
+        if (at >= runEnd) return false;
         s.b = seq;
         s.pair = pair;
         s.first = first_of(p, len);
         s.len = len;
         s.pos = (s.first / SLAB + slab) * SLAB;
-        s.is = slab == 0 ? BEGINS | OPENS : 0u;
-        if (at == runEnd - count) s.is |= OPENS;
-        if (slab + 1 == slabs) s.is |= ENDS | CLOSES;
-        if (at + 1 == runEnd) s.is |= CLOSES;
+        s.is = fresh | (slab == 0 ? BEGINS | OPENS : 0u) | (slab + 1 == slabs ? ENDS | CLOSES : 0u) |
+               (at + 1 >= runEnd ? CLOSES : 0u);
+        fresh = 0;
         ++at;
-        if (++slab == slabs && at < runEnd) {
-            slab = 0;
-            if (++pair == pairs) {
-                pair = 0;
-                do ++seq;                         // at < pre[B]: a later sequence has slabs
-                while (uniform(pre[seq]) == uniform(pre[seq + 1]));
-                len = uniform(lens[seq]);
-                slabs = slabs_of(p, len);
-            }
-        }
+        if (++slab == slabs) next_pair();
+        return true;
     };
 
     // ---- the stages of a slab ----
-    u32x4 kr[2][DB];                 // keys: rows 16 rb + c16
     // its page ids: lane r (of 32) holds row r's; rows outside the attended
     // range stand at its ends, so that nothing else is read
     struct Rows { uint32_t page, row; };
@@ -428,6 +601,7 @@ __global__ __launch_bounds__(THREADS, occupancy(D)) void paged_attention_kernel(
     // its keys into registers (A operands: row lane % 16, 8 elements a lane),
     // its values into LDS; false where a page lies outside the pool (its rows
     // are then read from page 0)
+    u32x4 kr[2][DB];                 // keys: rows 16 rb + lane % 16
     auto issue = [&](const Slab& s, const Rows& r, int half) -> bool {
         const int lane = fresh_lane(threadIdx.x & 63), g = lane >> 4, c16 = lane & 15;
         const bool ok = r.page < c.pages;
@@ -460,40 +634,43 @@ __global__ __launch_bounds__(THREADS, occupancy(D)) void paged_attention_kernel(
         const int lane = fresh_lane(threadIdx.x & 63), g = lane >> 4, c16 = lane & 15;
         const uint32_t group = s.pair % a.groups, kvh = s.pair / a.groups;
         const uint32_t h = group * a.perGroup + c16;
-        const uint32_t head = kvh * G + (c16 < a.perGroup && h < G ? h : group * a.perGroup);
+        const uint32_t head = kvh * G + (uint32_t(c16) < a.perGroup && h < G ? h : group * a.perGroup);
         const size_t row = s.b * p.qTokenStride + head * p.qStride + 8 * g;
+        if (a.wideQ) {
+            const u32x4* src = reinterpret_cast<const u32x4*>(static_cast<const char*>(p.q) + row * (BF ? 2 : 4));
 #pragma unroll
-        for (int db = 0; db < DB; ++db) {
-            if (a.wideQ) {
-                const u32x4* src = reinterpret_cast<const u32x4*>(static_cast<const char*>(p.q) +
-                                                                  (row + 32 * db) * (BF ? 2 : 4));
+            for (int db = 0; db < DB; ++db)
 #pragma unroll
-                for (int i = 0; i < RAW; ++i) raw[db][i] = src[i];
-            } else if constexpr (BF) {
-                const uint16_t* src = static_cast<const uint16_t*>(p.q) + row + 32 * db;
+                for (int i = 0; i < RAW; ++i) raw[db][i] = src[db * 4 * RAW + i];
+        } else if constexpr (BF) {
+            const uint16_t* src = static_cast<const uint16_t*>(p.q) + row;
 #pragma unroll
-                for (int i = 0; i < 4; ++i) raw[db][0][i] = src[2 * i] | uint32_t(src[2 * i + 1]) << 16;
-            } else {
-                const uint32_t* src = static_cast<const uint32_t*>(p.q) + row + 32 * db;
+            for (int db = 0; db < DB; ++db)
 #pragma unroll
-                for (int i = 0; i < 8; ++i) raw[db][i / 4][i % 4] = src[i];
-            }
+                for (int i = 0; i < 4; ++i)
+                    raw[db][0][i] = src[32 * db + 2 * i] | uint32_t(src[32 * db + 2 * i + 1]) << 16;
+        } else {
+            const uint32_t* src = static_cast<const uint32_t*>(p.q) + row;
+#pragma unroll
+            for (int db = 0; db < DB; ++db)
+#pragma unroll
+                for (int i = 0; i < 8; ++i) raw[db][i / 4][i % 4] = src[32 * db + i];
         }
     };
-    const uint32_t turnedDims = p.freqs ? uint32_t(p.rot) : 0;
+    const uint32_t rot = p.freqs ? uint32_t(p.rot) : 0;
     float freq[(D / 2 + WAVE - 1) / WAVE];
 #pragma unroll
-    for (uint32_t i = 0; i < sizeof(freq) / 4; ++i)
-        freq[i] = lane + i * WAVE < turnedDims / 2 ? p.freqs[lane + i * WAVE] : 0.0f;
+    for (uint32_t i = 0; i < sizeof(freq) / 4; ++i) freq[i] = lane + i * WAVE < rot / 2 ? p.freqs[lane + i * WAVE] : 0.0f;
 
     bf16x8 qb[DB][3];
     uint32_t turned = NOWHERE;
-    // raw to the three-term B operands: norm, rotation at len - 1, scale;
-    // `spare`: 16 rows in LDS
+    // raw to the three-term B operands: norm, rotation at len - 1, scale.
+    // `spare` holds 16 rows in LDS, element d of row r at d ^ 4 (r % 8), so that
+    // a column of them is spread over the banks
     auto prepare = [&](const Slab& s, float* spare) {
-        const uint32_t group = s.pair % a.groups, rot = fresh_uniform(turnedDims), half = rot / 2;
         const int lane = fresh_lane(threadIdx.x & 63), g = lane >> 4, c16 = lane & 15;
-        const bool live = c16 < a.perGroup && group * a.perGroup + c16 < G;
+        const uint32_t group = s.pair % a.groups;
+        const bool live = uint32_t(c16) < a.perGroup && group * a.perGroup + c16 < G;
         float x[DB][8];
 #pragma unroll
         for (int db = 0; db < DB; ++db)
@@ -504,7 +681,6 @@ __global__ __launch_bounds__(THREADS, occupancy(D)) void paged_attention_kernel(
                 else bits = raw[db][e / 4][e % 4];
                 x[db][e] = live ? __uint_as_float(bits) : 0.0f;
             }
-        float inv = 1.0f;
         if (p.gamma) {
             float ss = 0.0f;
 #pragma unroll
@@ -513,13 +689,14 @@ __global__ __launch_bounds__(THREADS, occupancy(D)) void paged_attention_kernel(
                 for (int e = 0; e < 8; ++e) ss += x[db][e] * x[db][e];
             ss += __shfl_xor(ss, 16, WAVE);
             ss += __shfl_xor(ss, 32, WAVE);
-            inv = 1.0f / sqrtf(ss / float(D) + p.eps);
+            const float inv = 1.0f / sqrtf(ss / float(D) + p.eps);
 #pragma unroll
             for (int db = 0; db < DB; ++db)
 #pragma unroll
                 for (int e = 0; e < 8; ++e) x[db][e] = x[db][e] * inv * gamma[32 * db + 8 * g + e];
         }
         if (rot) {
+            const uint32_t half = rot / 2;
             if (turned != s.b) {
                 wave_sync();
 #pragma unroll
@@ -528,59 +705,61 @@ __global__ __launch_bounds__(THREADS, occupancy(D)) void paged_attention_kernel(
                     rotation_at(s.len - 1, freq[i], cs, sn);
                     if (lane + i * WAVE < half) turns[w][lane + i * WAVE] = float2{cs * p.amplitude, sn * p.amplitude};
                 }
-                wave_sync();
                 turned = s.b;
             }
+            wave_sync();
             if (p.interleaved) {
 #pragma unroll
                 for (int db = 0; db < DB; ++db)
 #pragma unroll
                     for (int e = 0; e < 8; e += 2) {
                         const uint32_t d = 32 * db + 8 * g + e;
-                        if (d < rot) {
-                            const float2 cs = turns[w][d / 2];
-                            const float u = x[db][e], v = x[db][e + 1];
-                            x[db][e] = u * cs.x - v * cs.y;
-                            x[db][e + 1] = v * cs.x + u * cs.y;
-                        }
+                        const float2 cs = turns[w][d / 2];
+                        const float u = x[db][e], v = x[db][e + 1];
+                        x[db][e] = d < rot ? u * cs.x - v * cs.y : u;
+                        x[db][e + 1] = d < rot ? v * cs.x + u * cs.y : v;
                     }
-            } else if (half % 32 == 0) {
-                // the partner 32 k elements on is this lane's too
+            } else if (DB % 2 == 0 && half == D / 2) {
+                // the partner D / 2 elements on is this lane's too
 #pragma unroll
-                for (int k = 1; k <= DB / 2; ++k) {
-                    if (half != 32u * k) continue;
+                for (int db = 0; db < DB / 2; ++db)
 #pragma unroll
-                    for (int db = 0; db < k; ++db)
-#pragma unroll
-                        for (int e = 0; e < 8; ++e) {
-                            const float2 cs = turns[w][32 * db + 8 * g + e];
-                            const float u = x[db][e], v = x[db + k][e];
-                            x[db][e] = u * cs.x - v * cs.y;
-                            x[db + k][e] = v * cs.x + u * cs.y;
-                        }
-                }
+                    for (int e = 0; e < 8; ++e) {
+                        const float2 cs = turns[w][32 * db + 8 * g + e];
+                        const float u = x[db][e], v = x[db + DB / 2][e];
+                        x[db][e] = u * cs.x - v * cs.y;
+                        x[db + DB / 2][e] = v * cs.x + u * cs.y;
+                    }
             } else {
-                // elsewhere it is another lane's: through the values' idle half
+                // elsewhere it is another lane's: through LDS (whose reads wait
+                // for the values on their way there)
+                const int sw = 4 * (c16 & 7);
                 float* row = spare + c16 * D;
 #pragma unroll
                 for (int db = 0; db < DB; ++db)
 #pragma unroll
-                    for (int e = 0; e < 8; ++e) row[32 * db + 8 * g + e] = x[db][e];
+                    for (int i = 0; i < 2; ++i)
+                        *reinterpret_cast<floatx4*>(row + ((32 * db + 8 * g + 4 * i) ^ sw)) =
+                            floatx4{x[db][4 * i], x[db][4 * i + 1], x[db][4 * i + 2], x[db][4 * i + 3]};
+                wave_sync();
+#pragma unroll 8
+                for (uint32_t j = g; j < half; j += 4) {      // the row's pairs, a quarter a lane
+                    float* u = row + ((p.interleaved ? 2 * j : j) ^ sw);
+                    float* v = row + ((p.interleaved ? 2 * j + 1 : j + half) ^ sw);
+                    const float2 cs = turns[w][j];
+                    const float xu = *u, xv = *v;
+                    *u = xu * cs.x - xv * cs.y;
+                    *v = xv * cs.x + xu * cs.y;
+                }
                 wave_sync();
 #pragma unroll
-                for (int db = 0; db < DB; ++db) {
+                for (int db = 0; db < DB; ++db)
 #pragma unroll
-                    for (int e = 0; e < 8; ++e) {
-                        const uint32_t d = 32 * db + 8 * g + e;
-                        const bool late = d >= half;
-                        const uint32_t o = late ? d - half : d + half;
-                        if (d < rot) {
-                            const float2 cs = turns[w][late ? o : d];
-                            x[db][e] = late ? x[db][e] * cs.x + row[o] * cs.y : x[db][e] * cs.x - row[o] * cs.y;
-                        }
+                    for (int i = 0; i < 2; ++i) {
+                        const floatx4 y = *reinterpret_cast<const floatx4*>(row + ((32 * db + 8 * g + 4 * i) ^ sw));
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) x[db][4 * i + e] = y[e];
                     }
-                    __builtin_amdgcn_sched_barrier(0);
-                }
                 wave_sync();
             }
         }
@@ -647,23 +826,38 @@ __global__ __launch_bounds__(THREADS, occupancy(D)) void paged_attention_kernel(
         if (nextInFlight) wait_loads<2 * DB + VLOADS>();
         else wait_loads<0>();
         wave_sync();
+        // lane c16 of group g gets column 16 t + c16 of rows 4 g + 0..3, then 16 + 4 g + 0..3
         const uint16_t* vs = vbuf[w][bufHalf];
+        const int r0 = 4 * g + (c16 >> 2), r1 = r0 + 16, x0 = (c16 >> 1) & 1, sub = 4 * (c16 & 1);
+        constexpr int BATCH = CT % 4 == 0 ? 4 : 2;       // tiles whose reads go out together
 #pragma unroll
-        for (int t = 0; t < CT; ++t) {
-            // lane c16 of group g gets column 16 t + c16 of rows 4 g + 0..3, then 16 + 4 g + 0..3
-            const int r0 = 4 * g + (c16 >> 2), r1 = r0 + 16;
-            const int x = 2 * t + ((c16 >> 1) & 1), sub = 4 * (c16 & 1);
-            const bf16v4 lo = read_transposed(vs + r0 * D + 8 * (x ^ value_swizzle<D>(r0)) + sub);
-            const bf16v4 hi = read_transposed(vs + r1 * D + 8 * (x ^ value_swizzle<D>(r1)) + sub);
-            const bf16x8 vb = __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
+        for (int t0 = 0; t0 < CT; t0 += BATCH) {
+            bf16v4 lo[BATCH], hi[BATCH];
+#pragma unroll
+            for (int t = 0; t < BATCH; ++t) {
+                const int x = 2 * (t0 + t) + x0;
+                lo[t] = read_transposed(vs + r0 * D + 8 * (x ^ value_swizzle<D>(r0)) + sub);
+                hi[t] = read_transposed(vs + r1 * D + 8 * (x ^ value_swizzle<D>(r1)) + sub);
+            }
 #pragma unroll
             for (int k = 2; k >= 0; --k)
-                acc[t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, pa[k]), vb, acc[t], 0, 0, 0);
+#pragma unroll
+                for (int t = 0; t < BATCH; ++t)
+                    acc[t0 + t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(
+                        __builtin_bit_cast(bf16x8, pa[k]), __builtin_shufflevector(lo[t], hi[t], 0, 1, 2, 3, 4, 5, 6, 7),
+                        acc[t0 + t], 0, 0, 0);
         }
     };
     // a pair's last slab of this run: the sum over lanes, then its output or,
     // where other runs have parts of it, a record (the run's last stays in the
     // registers, for the workgroup's join)
+    const auto records = buffer_of(a.records);
+    auto piece_of = [&](const Slab& s) {
+        const uint32_t h0 = s.pair % a.groups * a.perGroup, units = slabs_of(p, s.len) + OPENING;
+        const uint32_t begin = uniform(pre[s.b]) + s.pair * units;
+        return Piece{begin, begin + units, s.b, s.pair / a.groups * G + h0,
+                     a.perGroup < G - h0 ? a.perGroup : G - h0};
+    };
     auto finish = [&](const Slab& s, bool last) {
         const int lane = fresh_lane(threadIdx.x & 63), g = lane >> 4, c16 = lane & 15;
         l += __shfl_xor(l, 16, WAVE);
@@ -671,29 +865,42 @@ __global__ __launch_bounds__(THREADS, occupancy(D)) void paged_attention_kernel(
         if (bad) l = __builtin_nanf("");
         const bool whole = begun && (s.is & ENDS);
         if (last && !whole) return;
-        const uint32_t group = s.pair % a.groups, kvh = s.pair / a.groups, h0 = group * a.perGroup;
-        const uint32_t rows = a.perGroup < G - h0 ? a.perGroup : G - h0;
-        float* rec = a.records + size_t(run) * 2 * a.perGroup * (D + 2);
-        float* accRows = rec + 2 * a.perGroup;
-        if (!whole && g == 0 && uint32_t(c16) < rows) {
-            rec[c16] = m;
-            rec[a.perGroup + c16] = l;
+        const Piece piece = piece_of(s);
+        const uint32_t rows = piece.rows;
+        if (!whole) {
+            const uint32_t rec = run * 2 * record_floats(a.perGroup, D);
+            auto put = [&](uint32_t at, float x) {
+                __builtin_amdgcn_raw_buffer_store_b32(__float_as_uint(x), records, (rec + at) * 4, 0, PAST_L2);
+            };
+            if (g == 0 && uint32_t(c16) < rows) {
+                put(c16, m);
+                put(a.perGroup + c16, l);
+            }
+#pragma unroll
+            for (int r = 0; r < 4; ++r)
+                if (4 * g + r < rows) {
+#pragma unroll
+                    for (int t = 0; t < CT; ++t)
+                        put(record_heads(a.perGroup) + (4 * g + r) * D + 16 * t + c16, acc[t][r]);
+                }
+            if (lane == 0) pieces[w] = piece;
+            return;
         }
-        float* to = whole ? p.out + (size_t(s.b) * p.heads + kvh * G + h0) * D : accRows;
+        float* to = p.out + (size_t(s.b) * p.heads + piece.head) * D;
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
             const uint32_t row = 4 * g + r;
-            const float total = __shfl(l, row, WAVE), by = whole ? 1.0f / total : 1.0f;
+            const float by = 1.0f / __shfl(l, row, WAVE);
             if (row < rows) {
 #pragma unroll
                 for (int t = 0; t < CT; ++t) to[row * D + 16 * t + c16] = acc[t][r] * by;
             }
         }
-        if (whole && p.outputGate) {
+        if (p.outputGate) {
 #pragma unroll 1
             for (uint32_t i = c16; i < 4 * D; i += 16) {      // this lane's own elements again
                 const uint32_t row = 4 * g + i / D, d = i % D;
-                if (row < rows) to[row * D + d] = gated(p, s.b, kvh * G + h0 + row, d, to[row * D + d]);
+                if (row < rows) to[row * D + d] = gated(p, s.b, piece.head + row, d, to[row * D + d]);
             }
         }
     };
@@ -702,22 +909,22 @@ __global__ __launch_bounds__(THREADS, occupancy(D)) void paged_attention_kernel(
     Slab s0{}, s1{}, s2{};           // computed, in flight, its pages asked for
     Rows r1{}, r2{};
     bool ok0 = true;
-    if (count) {
-        list(s0);
-        ask(s0);
+    const bool any = list(s0);
+    bool more = false, moreThen = false;
+    if (any) {
         Rows r0;
         find(s0, r0);
-        if (count > 1) list(s1), find(s1, r1);
+        more = list(s1);
+        if (more) find(s1, r1);
+        ask(s0);
         ok0 = issue(s0, r0, 0);
     }
     __builtin_amdgcn_sched_barrier(0);
 #pragma unroll 1
-    for (uint32_t i = 0; i < count; ++i) {
-        const int at = i & 1;
-        const bool more = i + 1 < count;
+    for (int buf = 0; any; buf ^= 1) {
         wave_sync();                 // the other buffer's reads are done
         if (s0.is & OPENS) {
-            prepare(s0, reinterpret_cast<float*>(vbuf[w][at ^ 1]));
+            prepare(s0, reinterpret_cast<float*>(vbuf[w][buf ^ 1]));
             m = -INFINITY;
             l = 0.0f;
 #pragma unroll
@@ -729,27 +936,29 @@ __global__ __launch_bounds__(THREADS, occupancy(D)) void paged_attention_kernel(
         score(s0);
         __builtin_amdgcn_sched_barrier(0);
         if (more) {
-            if (i + 2 < count) list(s2), find(s2, r2);
+            moreThen = list(s2);
+            if (moreThen) find(s2, r2);
             if (s1.is & OPENS) ask(s1);
-            ok0 = issue(s1, r1, at ^ 1);
+            ok0 = issue(s1, r1, buf ^ 1);
         }
         __builtin_amdgcn_sched_barrier(0);
-        weigh(at, more);
+        weigh(buf, more);
         if (s0.is & CLOSES) finish(s0, !more);
-        if (more) {
-            s0 = s1;
-            s1 = s2;
-            r1 = r2;
-        }
+        if (!more) break;
+        s0 = s1;
+        s1 = s2;
+        r1 = r2;
+        more = moreThen;
     }
 
     // ---- the runs' open ends, joined over the workgroup ----
-    const bool open = count && !(begun && (s0.is & ENDS));
+    const bool open = any && !(begun && (s0.is & ENDS));
     if (lane == 0) {
-        left[w] = open ? s0.b * pairs + s0.pair : NOWHERE;
+        if (open) pieces[WAVES + w] = piece_of(s0);
         leftEnds[w] = (begun ? 1u : 0u) | (s0.is & ENDS ? 2u : 0u);
     }
     if (open) {
+        const int g = lane >> 4, c16 = lane & 15;
         if (g == 0) wm[w][c16] = m, wl[w][c16] = l;
         float* rows = reinterpret_cast<float*>(vbuf[w]);
         wave_sync();
@@ -759,85 +968,106 @@ __global__ __launch_bounds__(THREADS, occupancy(D)) void paged_attention_kernel(
             for (int r = 0; r < 4; ++r) rows[(4 * g + r) * D + 16 * t + c16] = acc[t][r];
     }
     __syncthreads();
-    for (int from = 0, to; from < WAVES; from = to) {
-        const uint32_t id = left[from];
-        for (to = from + 1; to < WAVES && left[to] == id; ++to) {}
-        if (id == NOWHERE) continue;
-        const bool whole = (leftEnds[from] & 1) && (leftEnds[to - 1] & 2);
-        const uint32_t b = id / pairs, pr = id % pairs, kvh = pr / a.groups, h0 = pr % a.groups * a.perGroup;
-        const uint32_t rows = a.perGroup < G - h0 ? a.perGroup : G - h0;
-        float* rec = a.records + (size_t(blockIdx.x * WAVES + from) * 2 + 1) * a.perGroup * (D + 2);
-        float* out = p.out + (size_t(b) * p.heads + kvh * G + h0) * D;
-        for (uint32_t i = threadIdx.x; i < rows * D; i += THREADS) {
-            const uint32_t row = i / D, d = i % D;
-            float top = -INFINITY, sum = 0.0f, x = 0.0f;
+    const Piece* open_ends = pieces + WAVES;
+    bool recorded[WAVES] = {};       // open_ends[w] leads a record of the workgroup's
+#pragma unroll
+    for (int from = 0; from < WAVES; ++from) {
+        const uint32_t id = uniform(open_ends[from].begin);
+        if (id == NOWHERE || (from && uniform(open_ends[from - 1].begin) == id)) continue;
+        int to = from + 1;
+        while (to < WAVES && uniform(open_ends[to].begin) == id) ++to;
+        const bool whole = uniform((leftEnds[from] & 1) && (leftEnds[to - 1] & 2));
+        recorded[from] = !whole;
+        const uint32_t b = uniform(open_ends[from].b), head = uniform(open_ends[from].head),
+                       rows = uniform(open_ends[from].rows);
+        const uint32_t rec = ((blockIdx.x * WAVES + from) * 2 + 1) * record_floats(a.perGroup, D);
+        if (threadIdx.x < rows) {    // each wave's factor, and the sum
+            const uint32_t row = threadIdx.x;
+            float top = -INFINITY, sum = 0.0f;
             for (int k = from; k < to; ++k) top = fmaxf(top, wm[k][row]);
             const float base = top == -INFINITY ? 0.0f : top;
             for (int k = from; k < to; ++k) {
                 const float f = exp2f(wm[k][row] - base);
                 sum += wl[k][row] * f;
-                x += reinterpret_cast<const float*>(vbuf[k])[i] * f;
+                wm[k][row] = f;
             }
-            if (whole) {
-                out[i] = gated(p, b, kvh * G + h0 + row, d, x / sum);
-            } else {
-                rec[2 * a.perGroup + i] = x;
-                if (d == 0) rec[row] = top, rec[a.perGroup + row] = sum;
+            total[row] = sum;
+            if (!whole) {
+                __builtin_amdgcn_raw_buffer_store_b32(__float_as_uint(top), records, (rec + row) * 4, 0, PAST_L2);
+                __builtin_amdgcn_raw_buffer_store_b32(__float_as_uint(sum), records, (rec + a.perGroup + row) * 4, 0,
+                                                      PAST_L2);
             }
         }
+        __syncthreads();
+#pragma unroll 1
+        for (uint32_t i = threadIdx.x; i < rows * (D / 4); i += THREADS) {
+            const uint32_t row = i / (D / 4), d = i % (D / 4) * 4;
+            floatx4 x = floatx4{0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+            for (int k = 0; k < WAVES; ++k)
+                if (k >= from && k < to)
+                    x += *reinterpret_cast<const floatx4*>(reinterpret_cast<const float*>(vbuf[k]) + 4 * i) * wm[k][row];
+            if (whole) {
+                const float by = 1.0f / total[row];
+#pragma unroll
+                for (int e = 0; e < 4; ++e)
+                    p.out[(size_t(b) * p.heads + head + row) * D + d + e] = gated(p, b, head + row, d + e, x[e] * by);
+            } else {
+                __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u32x4, x), records,
+                                                       (rec + record_heads(a.perGroup) + 4 * i) * 4, 0, PAST_L2);
+            }
+        }
+        __syncthreads();             // total and the factors are read
+    }
+    if (a.plan) return;
+
+    // ---- pairs that span workgroups: the last one to arrive joins them ----
+    wait_loads<0>();                 // this wave's records are out
+    __syncthreads();
+    bool mine = false;
+    Parts parts{};
+    if (threadIdx.x < 2 * WAVES) {
+        const Piece& piece = pieces[threadIdx.x];
+        bool counts = piece.begin != NOWHERE;
+#pragma unroll
+        for (int k = 0; k < WAVES; ++k)
+            if (threadIdx.x == WAVES + k) counts = recorded[k];
+        if (counts) {
+            parts = Parts(cut, piece.begin, piece.end);
+            uint32_t* arrived = a.arrived + parts.to;
+            const uint32_t before = __hip_atomic_fetch_add(arrived, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+            mine = before + 1 == parts.total;
+            if (mine) __hip_atomic_store(arrived, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+        }
+        joins[threadIdx.x] = mine ? parts : Parts{};
+    }
+    const int count = __syncthreads_count(mine);
+    if (count == 0) return;
+    // several, of no more columns than a wave takes at once: a wave each
+    const bool apart = count > 1 && a.perGroup * (D / 4) <= WAVE;
+#pragma unroll 1
+    for (int k = apart ? w : 0; k < 2 * WAVES; k += apart ? WAVES : 1) {
+        if (uniform(joins[k].total) == 0) continue;
+        const Piece& piece = pieces[k];
+        if (apart)
+            join_parts<D, WAVE>(a, joins[k], piece.b, piece.head, 0, piece.rows, reinterpret_cast<float*>(vbuf[w]));
+        else
+            join_parts<D, THREADS>(a, joins[k], piece.b, piece.head, 0, piece.rows, reinterpret_cast<float*>(vbuf[0]));
     }
 }
 
-/* joins the records of the (sequence, query head) pairs that span workgroups:
-   one a workgroup for the runs it joined, and one of the run that went on to
-   another pair. Thread d owns column d; a tile of records is read at once. */
+/* joins the records of one (sequence, query head) a workgroup */
 template <int D>
-__global__ __launch_bounds__(D) void paged_merge_kernel(DecodeArgs a, uint32_t waves) {
-    constexpr int TILE = 16;
+__global__ __launch_bounds__(THREADS) void paged_merge_kernel(DecodeArgs a, uint32_t runs) {
+    __shared__ __attribute__((aligned(16))) float room[THREADS * JOIN_FLOATS];
     const PagedDecodeParams& p = a.p;
     const uint32_t b = blockIdx.x / p.heads, head = blockIdx.x % p.heads, G = p.heads / p.c.kvHeads;
-    const uint32_t group = head % G / a.perGroup, row = head % G % a.perGroup;
-    const uint32_t pairs = p.c.kvHeads * a.groups, pair = head / G * a.groups + group;
-    const uint32_t begin = a.plan[b], slabs = (a.plan[b + 1] - begin) / pairs;
-    if (slabs == 0) return;
-    const Cut cut(a.plan[p.c.batch], waves);
-    const uint32_t first = begin + pair * slabs, end = first + slabs;
-    const uint32_t from = cut.run_of(first), to = cut.run_of(end - 1);
-    const bool toEnd = end == cut.begin(to + 1);       // the last run ends with the pair
-    if (from == to || (from / WAVES == to / WAVES && toEnd)) return;
-    const uint32_t wg = from / WAVES;
-    // joined records: of every workgroup but the last one where that holds no more than the run that went on
-    const uint32_t joined = to / WAVES - wg + (toEnd || to % WAVES > (to / WAVES == wg ? from % WAVES : 0u) ? 1 : 0);
-    const uint32_t total = joined + (toEnd ? 0 : 1);
-    const size_t size = size_t(a.perGroup) * (D + 2);
-    const uint32_t d = threadIdx.x;
-    float top = -INFINITY, sum = 0.0f, x = 0.0f;
-    for (uint32_t k0 = 0; k0 < total; k0 += TILE) {
-        float mk[TILE], lk[TILE], xk[TILE];
-#pragma unroll
-        for (int i = 0; i < TILE; ++i) {
-            const uint32_t k = k0 + i < total ? k0 + i : total - 1;
-            const uint32_t slot = k < joined ? ((wg + k) * WAVES + (k ? 0 : from % WAVES)) * 2 + 1 : to * 2;
-            const float* rec = a.records + slot * size;
-            mk[i] = k0 + i < total ? rec[row] : -INFINITY;
-            lk[i] = k0 + i < total ? rec[a.perGroup + row] : 0.0f;
-            xk[i] = rec[2 * a.perGroup + row * D + d];
-        }
-        float next = top;
-#pragma unroll
-        for (int i = 0; i < TILE; ++i) next = fmaxf(next, mk[i]);
-        const float base = next == -INFINITY ? 0.0f : next, keep = exp2f(top - base);
-        sum *= keep;
-        x *= keep;
-#pragma unroll
-        for (int i = 0; i < TILE; ++i) {
-            const float f = exp2f(mk[i] - base);
-            sum += lk[i] * f;
-            x += xk[i] * f;
-        }
-        top = next;
-    }
-    p.out[(size_t(b) * p.heads + head) * D + d] = gated(p, b, head, d, x / sum);
+    const uint32_t pairs = p.c.kvHeads * a.groups, pair = head / G * a.groups + head % G / a.perGroup;
+    const uint32_t before = a.plan[b], units = (a.plan[b + 1] - before) / pairs;
+    if (units == 0) return;
+    const uint32_t begin = before + pair * units;
+    const Parts parts(Cut(a.plan[p.c.batch], runs), begin, begin + units);
+    if (parts.total > 1) join_parts<D, THREADS>(a, parts, b, head, head % G % a.perGroup, 1, room);
 }
 
 bool rotation_ok(Context& ctx, const char* who, const float* freqs, int rot, uint32_t dim, float amplitude) {
@@ -921,17 +1151,28 @@ DecodeShape decode_shape(const PagedDecodeParams& p) {
     s.perGroup = (G + s.groups - 1) / s.groups;
     uint64_t slabs = (uint64_t(p.maxLength) + SLAB - 1) / SLAB;
     if (p.window && p.window / SLAB + 2 < slabs) slabs = p.window / SLAB + 2;
-    const uint64_t each = slabs * p.c.kvHeads * s.groups, most = uint64_t(1) << 31;   // slabs are counted in 32 bits
+    const uint64_t each = (slabs + OPENING) * p.c.kvHeads * s.groups, most = uint64_t(1) << 31;   // units are counted in 32 bits
     uint64_t slice = p.c.batch < MAXB ? p.c.batch : MAXB;
     if (each && slice > most / each) slice = most / each;
     s.slice = uint32_t(slice);
     const int cus = Context::instance().cus ? Context::instance().cus : 256;
-    const uint64_t most_grid = uint64_t(cus) * occupancy(int(p.c.dim)), want = (slice * each + WAVES - 1) / WAVES;
+    uint64_t most_grid = uint64_t(cus) * occupancy(int(p.c.dim));
+    if (most_grid > MAX_RUNS / WAVES) most_grid = MAX_RUNS / WAVES;
+    const uint64_t want = (slice * each + WAVES - 1) / WAVES;
     s.grid = uint32_t(want < most_grid ? (want ? want : 1) : most_grid);
     return s;
 }
 
-constexpr size_t PLAN_BYTES = (MAXB + 1) * 4 + 252 & ~size_t(255);
+// a pair's records that one workgroup joins within the attention's launch; past
+// it, a workgroup a query head of a second launch
+constexpr uint64_t JOIN_BYTES = 256 << 10;
+bool joins_in_kernel(const PagedDecodeParams& p, const DecodeShape& s, uint32_t batch) {
+    const uint64_t parts = s.grid / (uint64_t(batch) * p.c.kvHeads * s.groups) + 1;
+    return parts * s.perGroup * p.c.dim * sizeof(float) <= JOIN_BYTES;
+}
+
+// workspace: a place for arrivals that no call's records overlap, the plan, the records
+constexpr size_t ARRIVED_BYTES = MAX_RUNS * 4, PLAN_BYTES = (MAXB + 1) * 4 + 252 & ~size_t(255);
 
 } // namespace
 
@@ -959,7 +1200,8 @@ bool check_paged_decode(const PagedDecodeParams& p) {
 size_t paged_decode_workspace(const PagedDecodeParams& p) {
     if (p.c.batch == 0) return 0;
     const DecodeShape s = decode_shape(p);
-    return PLAN_BYTES + size_t(s.grid) * WAVES * 2 * s.perGroup * (p.c.dim + 2) * sizeof(float);
+    return ARRIVED_BYTES + PLAN_BYTES +
+           size_t(s.grid) * WAVES * 2 * record_floats(s.perGroup, p.c.dim) * sizeof(float);
 }
 
 bool launch_paged_decode(const PagedDecodeParams& p, void* work, hipStream_t stream) {
@@ -968,8 +1210,8 @@ bool launch_paged_decode(const PagedDecodeParams& p, void* work, hipStream_t str
     const DecodeShape s = decode_shape(p);
     DecodeArgs a{};
     a.p = p;
-    a.plan = static_cast<uint32_t*>(work);
-    a.records = reinterpret_cast<float*>(static_cast<char*>(work) + PLAN_BYTES);
+    a.arrived = static_cast<uint32_t*>(work);
+    a.records = reinterpret_cast<float*>(static_cast<char*>(work) + ARRIVED_BYTES + PLAN_BYTES);
     a.groups = s.groups;
     a.perGroup = s.perGroup;
     a.scaleLog2 = p.scale * LOG2E;
@@ -982,14 +1224,17 @@ bool launch_paged_decode(const PagedDecodeParams& p, void* work, hipStream_t str
         a.p.c.lengths = p.c.lengths + b0;
         a.p.q = static_cast<const char*>(p.q) + b0 * p.qTokenStride * es;
         a.p.out = p.out + size_t(b0) * p.heads * p.c.dim;
+        a.plan = joins_in_kernel(p, s, a.p.c.batch)
+                     ? nullptr
+                     : reinterpret_cast<uint32_t*>(static_cast<char*>(work) + ARRIVED_BYTES);
         auto go = [&](auto attention, auto merge) {
             return ctx.launch("paged_attention_kernel", stream, [&] {
                        hipLaunchKernelGGL(attention, dim3(s.grid), dim3(THREADS), 0, stream, a);
                    }) &&
-                   ctx.launch("paged_merge_kernel", stream, [&] {
-                       hipLaunchKernelGGL(merge, dim3(a.p.c.batch * p.heads), dim3(p.c.dim), 0, stream, a,
+                   (!a.plan || ctx.launch("paged_merge_kernel", stream, [&] {
+                       hipLaunchKernelGGL(merge, dim3(a.p.c.batch * p.heads), dim3(THREADS), 0, stream, a,
                                           s.grid * WAVES);
-                   });
+                   }));
         };
         bool ok = false;
         auto of = [&](auto dim) {

@@ -176,3 +176,41 @@ def test_frequencies_yarn():
 def test_frequencies_refused(args):
     with pytest.raises(aigpu.AiGpuError):
         aigpu.rotary_frequencies(**args)
+
+
+def test_struct_layouts(tmp_path):
+    """the ctypes structures and the packed forms have the header's layout"""
+    import os
+    import subprocess
+    header = os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "include",
+                          "aigpu_attention.h")
+    structs = {c.__name__: c for c in (aigpu.AiGpuRotary, aigpu.AiGpuRotaryScaling, aigpu.AiGpuPagedCache,
+                                       aigpu.AiGpuPagedAppend, aigpu.AiGpuPagedDecode)}
+    lines = ["#include <stdio.h>", "#include <stddef.h>", f'#include "{header}"', "int main(void){"]
+    for name, cls in structs.items():
+        lines.append(f'printf("{name} size %zu\\n", sizeof({name}));')
+        lines += [f'printf("{name} {f} %zu\\n", offsetof({name}, {f}));' for f, _ in cls._fields_]
+    src, exe = tmp_path / "layout.c", tmp_path / "layout"
+    src.write_text("\n".join(lines + ["return 0;}"]))
+    subprocess.run(["gcc", "-o", str(exe), str(src)], check=True)
+    for line in subprocess.run([str(exe)], capture_output=True, text=True, check=True).stdout.splitlines():
+        name, field, value = line.split()
+        cls = structs[name]
+        assert (C.sizeof(cls) if field == "size" else getattr(cls, field).offset) == int(value), (name, field)
+    for name, cls in (("aigpu_rotary", aigpu.AiGpuRotary), ("aigpu_paged_append", aigpu.AiGpuPagedAppend),
+                      ("aigpu_paged_decode", aigpu.AiGpuPagedDecode)):
+        packed = aigpu._PACK[name]
+        assert packed.size == C.sizeof(cls)
+        # each value lands in the field of its place
+        flat = [f for f, t in cls._fields_ if f != "cache"]
+        if cls is not aigpu.AiGpuRotary:
+            flat = [f for f, _ in aigpu.AiGpuPagedCache._fields_] + flat
+        a = cls.from_buffer_copy(packed.pack(*range(1, len(flat) + 1)))
+        for i, f in enumerate(flat):
+            assert getattr(a if hasattr(a, f) else a.cache, f) == i + 1, f
+
+
+def test_values_out_of_range_are_refused_not_wrapped():
+    for bad in (-1, 2 ** 32):
+        with pytest.raises(ValueError):
+            aigpu._packed("aigpu_paged_decode", *([0] * 24 + [bad] + [0] * 10))
