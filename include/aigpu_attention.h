@@ -595,7 +595,7 @@ typedef struct AiGpuPagedCache {
    rounded to bf16. Without `starts` there is one token a sequence (count =
    batch). With it, rows starts[b] .. starts[b + 1] - 1 of k and v are the last
    starts[b + 1] - starts[b] positions of sequence b, and rows before starts[0]
-   or from starts[batch] on are not read. A token whose position is negative
+   or from starts[batch] on are left out. A token whose position is negative
    (a length below its new tokens), beyond the table or in a page outside the
    pool is not written; a decode over such a length answers NaN. No two
    tokens may share a row: a page shared by sequences is copied before either

@@ -31,6 +31,14 @@ __device__ __forceinline__ uint16_t float_to_bf16_bits(float x) {
     return uint16_t(u >> 16);
 }
 
+/* two fp32 values as bf16 bits, a in the low half: round to nearest even, NaN
+   stays NaN (one v_cvt_pk_bf16_f32) */
+__device__ __forceinline__ uint32_t pack_bf16(float a, float b) {
+    typedef float float2v __attribute__((ext_vector_type(2)));
+    typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
+    return __builtin_bit_cast(uint32_t, __builtin_convertvector(float2v{a, b}, bf16x2));
+}
+
 /* element i of a tensor tagged F32 (0) or BF16 (1) */
 __device__ __forceinline__ float load_elem(const void* base, size_t i, int type) {
     if (type == 0) return static_cast<const float*>(base)[i];

@@ -25,17 +25,20 @@ __device__ __forceinline__ uint64_t row_offset(const PagedCache& c, uint32_t b, 
 }
 
 /*
-    Appending. A workgroup takes `tokens` tokens; a wave works out each one's
-    sequence (the count of starts at or before it: one round of loads, where a
-    binary search would take one a step), its position and its page, and the
-    workgroup their cosines and sines, once for all kv heads. Then D / 8 lanes
-    take a row of k or v, 8 elements each. HBM bounds it: rows are read once and
-    written once, 16 bytes a lane.
+    Appending. A workgroup takes a few tokens; D / 8 lanes take a row of k or v, 8
+    elements each, up to PASSES rows a lane. Their loads go out first. Meanwhile
+    a wave works out each token's sequence (the count of starts at or before it:
+    one round of loads, where a binary search would take one a step), its position
+    and its page, and the workgroup the tokens' cosines and sines, once for all kv
+    heads. Then k's rows are normed and turned, and all rows rounded and stored.
+    HBM bounds it: rows are read once and written once, 16 bytes a lane.
 */
+constexpr int PASSES = 4;
+constexpr uint32_t MAX_TOKENS = 16;
 struct AppendArgs {
     PagedAppendParams p;
-    uint32_t tokens;
-    int wide;                   // k and v rows can be read 16 bytes at a time
+    uint32_t tokens;                // of a workgroup, at most MAX_TOKENS
+    int wide;                       // k and v rows can be read 16 bytes at a time
 };
 
 /* sum over the LPR lanes of a row: a power of two times 1 or 3 */
@@ -53,37 +56,86 @@ __device__ __forceinline__ float row_sum(float x, int lane) {
     }
 }
 
-template <int D>
+template <int D, bool BF>
 __global__ __launch_bounds__(THREADS) void paged_append_kernel(AppendArgs a) {
     constexpr int LPR = D / 8, RPW = WAVE / LPR;     // lanes of a row, rows of a wave
-    extern __shared__ float2 turns[];                // [tokens][rot / 2]
-    __shared__ float rows[THREADS / WAVE][RPW][D];
-    __shared__ uint64_t base[32];                    // of head 0, ~0: not written
-    __shared__ uint32_t place[32];
+    constexpr int NW = THREADS / WAVE, DEEP = NW * RPW, RAW = BF ? 1 : 2;
+    extern __shared__ __attribute__((aligned(16))) float2 turns[];   // [tokens][rot / 2]
+    __shared__ __attribute__((aligned(16))) float rows[NW][RPW][D];
+    __shared__ uint64_t base[MAX_TOKENS];            // of kv head 0, ~0: not written
+    __shared__ uint32_t place[MAX_TOKENS];
     const PagedAppendParams& p = a.p;
     const PagedCache& c = p.c;
     const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
     const uint64_t t0 = uint64_t(blockIdx.x) * a.tokens;
     const uint32_t nt = p.count - t0 < a.tokens ? uint32_t(p.count - t0) : a.tokens;
-    for (uint32_t i = w; i < nt; i += THREADS / WAVE) {
-        const uint64_t t = t0 + i;
-        uint32_t b = uint32_t(t);
-        uint64_t back = 1;      // t is the sequence's back-th newest token
-        bool live = true;
-        if (p.starts) {
-            uint32_t before = 0;
-            for (uint32_t k = lane; k <= c.batch; k += WAVE) before += p.starts[k] <= t ? 1u : 0u;
+    const uint32_t keys = nt * c.kvHeads, total = 2 * keys;      // k's rows, then v's
+    const int sub = lane / LPR, d0 = (lane % LPR) * 8;
+    const uint32_t r0 = w * RPW + sub;               // of the lanes that have a row (sub < RPW)
+
+    u32x4 raw[PASSES][RAW];
+    uint32_t which[PASSES];                          // token << 16 | kv head; NOWHERE: no row
+    auto load = [&](uint32_t first) {
 #pragma unroll
-            for (int o = 32; o > 0; o >>= 1) before += __shfl_xor(before, o, WAVE);
-            live = before > 0 && before <= c.batch;
-            b = live ? before - 1 : 0;
-            const uint64_t end = p.starts[b + 1];
-            live = live && end > t;
-            back = live ? end - t : 1;
+        for (int k = 0; k < PASSES; ++k) {
+            const uint32_t r = first + k * DEEP;
+            which[k] = NOWHERE;
+            if (sub >= RPW || r >= total) continue;
+            const bool isKey = r < keys;
+            const uint32_t rest = isKey ? r : r - keys, t = rest / c.kvHeads, h = rest - t * c.kvHeads;
+            which[k] = t << 16 | h;
+            const char* src = static_cast<const char*>(isKey ? p.k : p.v) +
+                              ((t0 + t) * (isKey ? p.kStride : p.vStride) + size_t(h) * D + d0) * (BF ? 2 : 4);
+            if (a.wide) {
+#pragma unroll
+                for (int i = 0; i < RAW; ++i) raw[k][i] = reinterpret_cast<const u32x4*>(src)[i];
+            } else if constexpr (BF) {
+                const uint16_t* e = reinterpret_cast<const uint16_t*>(src);
+#pragma unroll
+                for (int i = 0; i < 4; ++i) raw[k][0][i] = e[2 * i] | uint32_t(e[2 * i + 1]) << 16;
+            } else {
+                const uint32_t* e = reinterpret_cast<const uint32_t*>(src);
+#pragma unroll
+                for (int i = 0; i < 8; ++i) raw[k][i / 4][i % 4] = e[i];
+            }
         }
-        if (lane == 0) {
-            const uint64_t len = c.lengths[b];
-            const uint64_t pos = len - back;
+    };
+    load(r0);
+    float gamma[8];
+    if (p.gamma) {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) gamma[e] = sub < RPW ? p.gamma[d0 + e] + p.offset : 0.0f;
+    }
+
+    // ---- each token's sequence, position and page: a wave takes every NW-th ----
+    {
+        constexpr int MINE = MAX_TOKENS / NW;
+        uint32_t before[MINE] = {};
+        if (p.starts) {
+            for (uint32_t k = 0; k <= c.batch; k += WAVE) {
+                const bool in = k + lane <= c.batch;
+                const uint32_t start = in ? p.starts[k + lane] : 0u;
+#pragma unroll
+                for (int i = 0; i < MINE; ++i) before[i] += __popcll(__ballot(in && start <= t0 + w + i * NW));
+            }
+        }
+        uint32_t mine = 0;
+#pragma unroll
+        for (int i = 0; i < MINE; ++i) mine = lane == i ? before[i] : mine;
+        const uint32_t i = w + lane * NW;            // lane's token
+        if (lane < MINE && i < nt) {
+            const uint64_t t = t0 + i;
+            uint32_t b = uint32_t(t);
+            uint64_t back = 1;                       // it is the sequence's back-th newest
+            bool live = true;
+            if (p.starts) {
+                live = mine > 0 && mine <= c.batch;
+                b = live ? mine - 1 : 0;
+                const uint64_t end = p.starts[b + 1];
+                live = live && end > t;
+                back = live ? end - t : 1;
+            }
+            const uint64_t len = c.lengths[b], pos = len - back;
             place[i] = uint32_t(pos);
             base[i] = live && len >= back ? row_offset(c, b, pos, 0) : ~uint64_t(0);
         }
@@ -96,86 +148,95 @@ __global__ __launch_bounds__(THREADS) void paged_append_kernel(AppendArgs a) {
         turns[i] = float2{cs * p.amplitude, sn * p.amplitude};
     }
     __syncthreads();
-    const int r = lane / LPR, d0 = (lane % LPR) * 8;
-    const uint32_t total = nt * c.kvHeads * 2;      // k's rows of a token, then v's
+
+    float* row = rows[w][sub < RPW ? sub : 0];
     // every lane of a wave stays in the loop: the row sums shuffle over all of it
-    for (uint32_t first = w * RPW; first < total; first += THREADS / WAVE * RPW) {
-        const uint32_t i = first + r;
-        const bool in = r < RPW && i < total;
-        const uint32_t t = in ? i / (2 * c.kvHeads) : 0, rest = in ? i % (2 * c.kvHeads) : 0;
-        const bool isKey = rest < c.kvHeads;
-        const uint32_t h = isKey ? rest : rest - c.kvHeads;
-        const uint64_t to = base[t];
-        const bool live = in && to != ~uint64_t(0);
-        float x[8] = {};
-        if (live) {
-            const void* src = isKey ? p.k : p.v;
-            const size_t at = (t0 + t) * (isKey ? p.kStride : p.vStride) + size_t(h) * D + d0;
-            if (!a.wide) {
+#pragma unroll 1
+    for (uint32_t first = r0, wave = w * RPW; wave < total; first += PASSES * DEEP, wave += PASSES * DEEP) {
+        if (first != r0) load(first);
 #pragma unroll
-                for (int e = 0; e < 8; ++e) x[e] = load_elem(src, at + e, p.inType);
-            } else if (p.inType == 1) {
-                const u32x4 raw = *reinterpret_cast<const u32x4*>(static_cast<const uint16_t*>(src) + at);
-#pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                    x[2 * e] = bf16_bits_to_float(raw[e] & 0xFFFFu);
-                    x[2 * e + 1] = __uint_as_float(raw[e] & 0xFFFF0000u);
-                }
-            } else {
-                const floatx4* f = reinterpret_cast<const floatx4*>(static_cast<const float*>(src) + at);
-                const floatx4 lo = f[0], hi = f[1];
-#pragma unroll
-                for (int e = 0; e < 4; ++e) x[e] = lo[e], x[4 + e] = hi[e];
-            }
-        }
-        if (p.gamma) {
-            float ss = 0.0f;
-#pragma unroll
-            for (int e = 0; e < 8; ++e) ss += x[e] * x[e];
-            const float inv = 1.0f / sqrtf(row_sum<LPR>(ss, lane) / float(D) + p.eps);
-            if (live && isKey) {
-#pragma unroll
-                for (int e = 0; e < 8; ++e) x[e] = x[e] * inv * (p.gamma[d0 + e] + p.offset);
-            }
-        }
-        if (half) {
-            // a half-layout partner sits in another lane: through LDS
-            float* row = rows[w][r < RPW ? r : 0];
-            if (!p.interleaved && live && isKey) {
-#pragma unroll
-                for (int e = 0; e < 8; ++e) row[d0 + e] = x[e];
-            }
-            wave_sync();
-            if (live && isKey) {
-                const float2* turn = turns + t * half;
-                float y[8];
+        for (int k = 0; k < PASSES; ++k) {
+            const uint32_t r = first + k * DEEP;
+            if (wave + k * DEEP >= total) break;     // no row of this wave's is left
+            const bool in = which[k] != NOWHERE, isKey = r < keys;
+            const uint32_t t = in ? which[k] >> 16 : 0, h = which[k] & 0xFFFFu;
+            const uint64_t to = base[t];
+            const bool live = in && to != ~uint64_t(0);
+            u32x4 bits = raw[k][0];
+            if (!BF || wave + k * DEEP < keys) {     // not only bf16 values, which are stored as they are
+                float x[8];
 #pragma unroll
                 for (int e = 0; e < 8; ++e) {
-                    const uint32_t d = d0 + e;
-                    y[e] = x[e];
-                    if (d < 2 * half) {
-                        if (p.interleaved) {
-                            const float2 cs = turn[d / 2];
-                            y[e] = d & 1 ? x[e] * cs.x + x[e ^ 1] * cs.y : x[e] * cs.x - x[e ^ 1] * cs.y;
-                        } else {
-                            const bool late = d >= half;
-                            const float2 cs = turn[late ? d - half : d];
-                            const float other = row[late ? d - half : d + half];
-                            y[e] = late ? x[e] * cs.x + other * cs.y : x[e] * cs.x - other * cs.y;
-                        }
+                    if constexpr (BF) x[e] = __uint_as_float(e & 1 ? raw[k][0][e / 2] & 0xFFFF0000u : raw[k][0][e / 2] << 16);
+                    else x[e] = __uint_as_float(raw[k][e / 4][e % 4]);
+                }
+                if (p.gamma) {
+                    float ss = 0.0f;
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) ss += x[e] * x[e];
+                    const float inv = 1.0f / sqrtf(row_sum<LPR>(ss, lane) / float(D) + p.eps);
+                    if (live && isKey) {
+#pragma unroll
+                        for (int e = 0; e < 8; ++e) x[e] = x[e] * inv * gamma[e];
                     }
                 }
+                if (half && p.interleaved) {
+                    if (live && isKey) {
 #pragma unroll
-                for (int e = 0; e < 8; ++e) x[e] = y[e];
+                        for (int e = 0; e < 8; e += 2) {
+                            if (uint32_t(d0 + e) >= 2 * half) break;
+                            const float2 cs = turns[t * half + (d0 + e) / 2];
+                            const float u = x[e], v = x[e + 1];
+                            x[e] = u * cs.x - v * cs.y;
+                            x[e + 1] = v * cs.x + u * cs.y;
+                        }
+                    }
+                } else if (half) {
+                    // a half-layout partner sits in another lane: through LDS
+                    if (live && isKey) {
+                        *reinterpret_cast<floatx4*>(row + d0) = floatx4{x[0], x[1], x[2], x[3]};
+                        *reinterpret_cast<floatx4*>(row + d0 + 4) = floatx4{x[4], x[5], x[6], x[7]};
+                    }
+                    wave_sync();
+                    if (live && isKey && uint32_t(d0) < 2 * half) {
+                        if (half % 8 == 0) {         // all eight partners in one lane
+                            const bool late = uint32_t(d0) >= half;
+                            const uint32_t o = late ? d0 - half : d0 + half;
+                            const floatx4* cs = reinterpret_cast<const floatx4*>(turns + t * half + (late ? o : d0));
+                            const float sign = late ? 1.0f : -1.0f;
+#pragma unroll
+                            for (int i = 0; i < 2; ++i) {
+                                const floatx4 y = *reinterpret_cast<const floatx4*>(row + o + 4 * i);
+                                const floatx4 c0 = cs[2 * i], c1 = cs[2 * i + 1];
+                                x[4 * i] = x[4 * i] * c0[0] + sign * y[0] * c0[1];
+                                x[4 * i + 1] = x[4 * i + 1] * c0[2] + sign * y[1] * c0[3];
+                                x[4 * i + 2] = x[4 * i + 2] * c1[0] + sign * y[2] * c1[1];
+                                x[4 * i + 3] = x[4 * i + 3] * c1[2] + sign * y[3] * c1[3];
+                            }
+                        } else {
+#pragma unroll
+                            for (int e = 0; e < 8; ++e) {
+                                const uint32_t d = d0 + e;
+                                if (d >= 2 * half) break;
+                                const bool late = d >= half;
+                                const uint32_t o = late ? d - half : d + half;
+                                const float2 cs = turns[t * half + (late ? o : d)];
+                                x[e] = x[e] * cs.x + (late ? row[o] : -row[o]) * cs.y;
+                            }
+                        }
+                    }
+                    wave_sync();
+                }
+                if (!BF || isKey) {
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) bits[e] = pack_bf16(x[2 * e], x[2 * e + 1]);
+                }
             }
-            wave_sync();
-        }
-        if (live) {
-            u32x4 raw;
-#pragma unroll
-            for (int e = 0; e < 4; ++e)
-                raw[e] = float_to_bf16_bits(x[2 * e]) | uint32_t(float_to_bf16_bits(x[2 * e + 1])) << 16;
-            *reinterpret_cast<u32x4*>((isKey ? c.keys : c.values) + to + h * c.headStride + d0) = raw;
+            // nontemporal: who reads the pages next is rarely on this XCD, whose L2
+            // they would fill (33 MB of prompts: 21.8 us stored plainly, 20.4 so)
+            if (live)
+                __builtin_nontemporal_store(
+                    bits, reinterpret_cast<u32x4*>((isKey ? c.keys : c.values) + to + h * c.headStride + d0));
         }
     }
 }
@@ -1117,20 +1178,28 @@ bool launch_paged_append(const PagedAppendParams& p, hipStream_t stream) {
     AppendArgs a{};
     a.p = p;
     a.wide = (at & 15) == 0 && (p.count == 1 || (p.kStride | p.vStride) % (16 / es) == 0);
-    // one round of the workgroup's rows, but no more tokens than a wave a token
-    const uint32_t rows = THREADS / WAVE * (WAVE / (p.c.dim / 8));
-    a.tokens = rows / (2 * p.c.kvHeads);
-    a.tokens = a.tokens < 1 ? 1 : (a.tokens > 16 ? 16 : a.tokens);
+    // as many tokens as the lanes hold rows of at once, fewer where workgroups
+    // would be less than two a CU: the index chain is what small calls wait for
+    const uint32_t rows = THREADS / WAVE * (WAVE / (p.c.dim / 8)) * PASSES;
+    const uint64_t spread = p.count / 512;
+    uint32_t tokens = rows / (2 * p.c.kvHeads);
+    if (tokens > spread) tokens = uint32_t(spread);
+    a.tokens = tokens < 1 ? 1 : (tokens > MAX_TOKENS ? MAX_TOKENS : tokens);
     const unsigned grid = unsigned((p.count + a.tokens - 1) / a.tokens);
     const size_t lds = p.freqs ? size_t(a.tokens) * (p.rot / 2) * sizeof(float2) : 0;
     return ctx.launch("paged_append_kernel", stream, [&] {
         auto go = [&](auto kernel) { hipLaunchKernelGGL(kernel, dim3(grid), dim3(THREADS), lds, stream, a); };
+        auto of = [&](auto dim) {
+            constexpr int D = decltype(dim)::value;
+            if (p.inType == 1) go(paged_append_kernel<D, true>);
+            else go(paged_append_kernel<D, false>);
+        };
         switch (p.c.dim) {
-            case 64: go(paged_append_kernel<64>); break;
-            case 96: go(paged_append_kernel<96>); break;
-            case 128: go(paged_append_kernel<128>); break;
-            case 192: go(paged_append_kernel<192>); break;
-            default: go(paged_append_kernel<256>); break;
+            case 64: of(std::integral_constant<int, 64>{}); break;
+            case 96: of(std::integral_constant<int, 96>{}); break;
+            case 128: of(std::integral_constant<int, 128>{}); break;
+            case 192: of(std::integral_constant<int, 192>{}); break;
+            default: of(std::integral_constant<int, 256>{}); break;
         }
     });
 }

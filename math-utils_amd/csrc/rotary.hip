@@ -3,12 +3,13 @@
 //
 // One pass over the data: 2 bytes moved per byte of x and 3 flops an element,
 // so HBM bounds it, or the launch where x is small. A workgroup takes a tile of
-// tokens and heads. Its tokens' cosines and sines go to LDS first, one
-// evaluation a (token, pair) for all the heads of the tile: the 64-bit angle
-// and the two functions cost about 60 instructions, as much as rotating 20
-// heads' pairs. Then each thread turns units of 16 bytes (half layout: the two
-// 16-byte pieces whose elements pair up; interleaved: one piece, its pairs
-// within) and copies the pieces that stay as they are.
+// tokens and heads. A thread owns a unit of every row it takes: 16 bytes that
+// turn within themselves (interleaved), the two 16-byte pieces whose elements
+// pair up (half layout), or a piece to copy. Its first rows' loads go out, then
+// the tokens' cosines and sines are formed into LDS, one evaluation a (token,
+// pair) for all heads of the tile (the 64-bit angle and the two functions take
+// about 100 instructions, as many as rotating 15 heads' pairs), then the rows
+// are turned and stored.
 #include <cmath>
 
 #include "context.hpp"
@@ -20,63 +21,113 @@ namespace aigpu {
 namespace {
 
 constexpr uint32_t THREADS = 256;
-constexpr uint32_t TILE_UNITS = 1024;   // units a workgroup aims at: four a thread
-constexpr uint32_t MAX_TOKENS = 32;     // tokens of a tile: at most this, and a 32 KB table
+constexpr uint32_t PIECES = 4;          // pieces a thread has in flight
+constexpr uint32_t TABLE_BYTES = 32 << 10;
 
 struct RotaryArgs {
     RotaryParams p;
     uint32_t tokens, headsTile;         // of one tile
-    uint32_t units, turned;             // units of one head, and how many of them turn
+    uint32_t units, turned;             // units of one row, and how many of them turn
+    uint32_t across;                    // threads side by side over a row's units
 };
 
-/* V elements (16 bytes, or one) as fp32 */
+/* V elements: 16 bytes, or one */
+template <int V>
+struct Piece {
+    u32x4 bits;
+};
+template <>
+struct Piece<1> {
+    uint32_t bits;
+};
+
 template <int V, bool BF>
-__device__ __forceinline__ void load_piece(const void* base, size_t at, float (&x)[V]) {
+__device__ __forceinline__ void load_piece(const void* base, size_t at, Piece<V>& x) {
+    if constexpr (V > 1) x.bits = *reinterpret_cast<const u32x4*>(static_cast<const char*>(base) + at * (BF ? 2 : 4));
+    else if constexpr (BF) x.bits = uint32_t(static_cast<const uint16_t*>(base)[at]) << 16;
+    else x.bits = static_cast<const uint32_t*>(base)[at];
+}
+
+template <int V, bool BF>
+__device__ __forceinline__ void store_piece(void* base, size_t at, const Piece<V>& x) {
+    if constexpr (V > 1) *reinterpret_cast<u32x4*>(static_cast<char*>(base) + at * (BF ? 2 : 4)) = x.bits;
+    else if constexpr (BF) static_cast<uint16_t*>(base)[at] = uint16_t(x.bits >> 16);
+    else static_cast<uint32_t*>(base)[at] = x.bits;
+}
+
+template <int V, bool BF>
+__device__ __forceinline__ void widen(const Piece<V>& x, float (&y)[V]) {
     if constexpr (V == 1) {
-        x[0] = load_elem(base, at, BF ? 1 : 0);
+        y[0] = __uint_as_float(x.bits);
     } else {
-        const u32x4 raw = *reinterpret_cast<const u32x4*>(static_cast<const char*>(base) + at * (BF ? 2 : 4));
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
             if constexpr (BF) {
-                x[2 * i] = bf16_bits_to_float(raw[i] & 0xFFFFu);
-                x[2 * i + 1] = __uint_as_float(raw[i] & 0xFFFF0000u);
+                y[2 * i] = bf16_bits_to_float(x.bits[i] & 0xFFFFu);
+                y[2 * i + 1] = __uint_as_float(x.bits[i] & 0xFFFF0000u);
             } else {
-                x[i] = __uint_as_float(raw[i]);
+                y[i] = __uint_as_float(x.bits[i]);
             }
         }
     }
 }
 
 template <int V, bool BF>
-__device__ __forceinline__ void store_piece(void* base, size_t at, const float (&x)[V]) {
+__device__ __forceinline__ void narrow(const float (&y)[V], Piece<V>& x) {
     if constexpr (V == 1) {
-        if constexpr (BF) static_cast<uint16_t*>(base)[at] = float_to_bf16_bits(x[0]);
-        else static_cast<float*>(base)[at] = x[0];
+        x.bits = BF ? pack_bf16(0.0f, y[0]) : __float_as_uint(y[0]);
     } else {
-        u32x4 raw;
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-            if constexpr (BF)
-                raw[i] = float_to_bf16_bits(x[2 * i]) | uint32_t(float_to_bf16_bits(x[2 * i + 1])) << 16;
-            else
-                raw[i] = __float_as_uint(x[i]);
+            if constexpr (BF) x.bits[i] = pack_bf16(y[2 * i], y[2 * i + 1]);
+            else x.bits[i] = __float_as_uint(y[i]);
         }
-        *reinterpret_cast<u32x4*>(static_cast<char*>(base) + at * (BF ? 2 : 4)) = raw;
     }
 }
 
 /* V: elements of a piece (16 bytes of BF ? bf16 : fp32, or 1); IL: interleaved
-   pairs, where a piece of one element comes with its partner */
+   pairs. A unit is two pieces, but for interleaved ones of 16 bytes, whose pairs
+   lie within one. */
 template <int V, bool BF, bool IL>
 __global__ __launch_bounds__(THREADS) void rotary_kernel(RotaryArgs a) {
-    extern __shared__ float2 turns[];   // [tokens][rot / 2]: cos, sin times the amplitude
+    constexpr bool TWO = !IL || V == 1;
+    constexpr uint32_t ROWS = TWO ? PIECES / 2 : PIECES;
+    // [tokens][rot / 2]: cos, sin times the amplitude
+    extern __shared__ __attribute__((aligned(16))) float2 turns[];
     const RotaryParams& p = a.p;
-    const uint32_t half = p.rot / 2;
+    const uint32_t half = p.rot / 2, dim = uint32_t(p.dim);
     const uint64_t t0 = uint64_t(blockIdx.x) * a.tokens;
     const uint32_t h0 = blockIdx.y * a.headsTile;
     const uint32_t nt = p.count - t0 < a.tokens ? uint32_t(p.count - t0) : a.tokens;
     const uint32_t nh = uint32_t(p.heads) - h0 < a.headsTile ? uint32_t(p.heads) - h0 : a.headsTile;
+    const uint32_t deep = THREADS / a.across, rows = nt * nh;      // rows of one pass over the threads
+    const uint32_t u0 = threadIdx.x % a.across, r0 = threadIdx.x / a.across;
+    const uint32_t stepT = deep / nh, stepH = deep % nh;
+
+    struct At {
+        uint32_t t, h;
+    };
+    Piece<V> x[ROWS], y[ROWS];
+    // the elements of unit u: piece one at d, piece two at d2 (kept out of rows of odd length)
+    auto first = [&](uint32_t u) { return IL ? u * (V == 1 ? 2 : V) : (u < a.turned ? u * V : p.rot + (u - a.turned) * V); };
+    auto second = [&](uint32_t u) { return IL ? u * 2 + 1 : u * V + half; };
+    auto paired = [&](uint32_t u) { return IL ? u * 2 + 1 < dim : u < a.turned; };
+    auto load = [&](uint32_t u, uint32_t r, At at) {
+#pragma unroll
+        for (uint32_t k = 0; k < ROWS; ++k) {
+            if (r + k * deep < rows && u < a.units) {
+                const size_t from = (t0 + at.t) * p.tokenStride + (h0 + at.h) * p.headStride;
+                load_piece<V, BF>(p.x, from + first(u), x[k]);
+                if (TWO && paired(u)) load_piece<V, BF>(p.x, from + second(u), y[k]);
+            }
+            at.t += stepT;
+            at.h += stepH;
+            if (at.h >= nh) at.h -= nh, ++at.t;
+        }
+    };
+    At at{r0 / nh, r0 % nh};
+    if (r0 < deep) load(u0, r0, at);
+
     for (uint32_t i = threadIdx.x; i < nt * half; i += THREADS) {
         const uint32_t t = i / half, j = i % half;
         const uint32_t pos = p.positions ? p.positions[t0 + t] : uint32_t(p.start + t0 + t);
@@ -85,59 +136,59 @@ __global__ __launch_bounds__(THREADS) void rotary_kernel(RotaryArgs a) {
         turns[i] = float2{cs * p.amplitude, (p.transpose ? -sn : sn) * p.amplitude};
     }
     __syncthreads();
-    const uint32_t total = nt * nh * a.units;
-    for (uint32_t i = threadIdx.x; i < total; i += THREADS) {
-        const uint32_t u = i % a.units, th = i / a.units, h = th % nh, t = th / nh;
-        const size_t from = (t0 + t) * p.tokenStride + (h0 + h) * p.headStride;
-        const size_t to = (t0 + t) * p.outTokenStride + (h0 + h) * p.outHeadStride;
-        const float2* turn = turns + t * half;
-        if constexpr (IL) {
-            constexpr int W = V == 1 ? 2 : V;
-            const uint32_t d = u * W;
-            float x[W];
-            if constexpr (V == 1) {
-                float one[1];
-                load_piece<1, BF>(p.x, from + d, one), x[0] = one[0];
-                if (d + 1 < p.dim) load_piece<1, BF>(p.x, from + d + 1, one);
-                x[1] = one[0];
-            } else {
-                load_piece<V, BF>(p.x, from + d, x);
-            }
-            if (u < a.turned) {
+    if (r0 >= deep) return;             // threads beyond the last whole row
+    for (uint32_t u = u0; u < a.units; u += a.across) {
+        At here = At{r0 / nh, r0 % nh};
+        for (uint32_t r = r0; r < rows; r += ROWS * deep) {
+            if (u != u0 || r != r0) load(u, r, here);
 #pragma unroll
-                for (int i2 = 0; i2 < W; i2 += 2) {
-                    const float2 cs = turn[d / 2 + i2 / 2];
-                    const float b = x[i2], c = x[i2 + 1];
-                    x[i2] = b * cs.x - c * cs.y;
-                    x[i2 + 1] = c * cs.x + b * cs.y;
-                }
-            }
-            if constexpr (V == 1) {
-                store_piece<1, BF>(p.out, to + d, {x[0]});
-                if (d + 1 < p.dim) store_piece<1, BF>(p.out, to + d + 1, {x[1]});
-            } else {
-                store_piece<V, BF>(p.out, to + d, x);
-            }
-        } else {
-            if (u < a.turned) {
-                const uint32_t d = u * V;
-                float x[V], y[V];
-                load_piece<V, BF>(p.x, from + d, x);
-                load_piece<V, BF>(p.x, from + d + half, y);
+            for (uint32_t k = 0; k < ROWS; ++k) {
+                if (r + k * deep < rows) {
+                    if (u < a.turned) {
+                        // (a unit's turns start on 16 bytes: its pairs are a piece's, or half of one's)
+                        constexpr int PAIRS = TWO ? V : V / 2;
+                        float2 turn[PAIRS];
+                        const float2* cells = turns + here.t * half + (IL ? first(u) / 2 : first(u));
+                        if constexpr (PAIRS == 1) {
+                            turn[0] = cells[0];
+                        } else {
 #pragma unroll
-                for (int e = 0; e < V; ++e) {
-                    const float2 cs = turn[d + e];
-                    const float b = x[e], c = y[e];
-                    x[e] = b * cs.x - c * cs.y;
-                    y[e] = c * cs.x + b * cs.y;
+                            for (int i = 0; i < PAIRS; i += 2) {
+                                const floatx4 two = *reinterpret_cast<const floatx4*>(cells + i);
+                                turn[i] = float2{two[0], two[1]};
+                                turn[i + 1] = float2{two[2], two[3]};
+                            }
+                        }
+                        float b[V], c[V];
+                        widen<V, BF>(x[k], b);
+                        if constexpr (TWO) {
+                            widen<V, BF>(y[k], c);
+#pragma unroll
+                            for (int e = 0; e < V; ++e) {
+                                const float2 cs = turn[e];
+                                const float v = b[e];
+                                b[e] = v * cs.x - c[e] * cs.y;
+                                c[e] = c[e] * cs.x + v * cs.y;
+                            }
+                            narrow<V, BF>(c, y[k]);
+                        } else {
+#pragma unroll
+                            for (int e = 0; e < V; e += 2) {
+                                const float2 cs = turn[e / 2];
+                                const float v = b[e];
+                                b[e] = v * cs.x - b[e + 1] * cs.y;
+                                b[e + 1] = b[e + 1] * cs.x + v * cs.y;
+                            }
+                        }
+                        narrow<V, BF>(b, x[k]);
+                    }
+                    const size_t to = (t0 + here.t) * p.outTokenStride + (h0 + here.h) * p.outHeadStride;
+                    store_piece<V, BF>(p.out, to + first(u), x[k]);
+                    if (TWO && paired(u)) store_piece<V, BF>(p.out, to + second(u), y[k]);
                 }
-                store_piece<V, BF>(p.out, to + d, x);
-                store_piece<V, BF>(p.out, to + d + half, y);
-            } else {
-                const uint32_t d = p.rot + (u - a.turned) * V;
-                float x[V];
-                load_piece<V, BF>(p.x, from + d, x);
-                store_piece<V, BF>(p.out, to + d, x);
+                here.t += stepT;
+                here.h += stepH;
+                if (here.h >= nh) here.h -= nh, ++here.t;
             }
         }
     }
@@ -219,13 +270,14 @@ bool launch_rotary(const RotaryParams& p, hipStream_t stream) {
         a.units = a.turned + uint32_t((p.dim - p.rot) / V);
     }
     if (inPlace) a.units = a.turned;   // the rest is where it belongs
-    const uint32_t heads = uint32_t(p.heads);
-    a.headsTile = TILE_UNITS / a.units;
-    a.headsTile = a.headsTile < 1 ? 1 : (a.headsTile > heads ? heads : a.headsTile);
-    a.tokens = TILE_UNITS / (a.headsTile * a.units);
-    const uint32_t table = (32u << 10) / (p.rot / 2 * 8);
-    const uint32_t most = table < 1 ? 1 : (table < MAX_TOKENS ? table : MAX_TOKENS);
-    a.tokens = a.tokens < 1 ? 1 : (a.tokens > most ? most : a.tokens);
+    // a tile of as many rows as the threads hold at once, of whole tokens if
+    // that is more than one token's heads
+    a.across = a.units < THREADS ? a.units : THREADS;
+    const uint32_t heads = uint32_t(p.heads), rows = THREADS / a.across * (p.interleaved && V > 1 ? PIECES : PIECES / 2);
+    a.headsTile = heads < rows ? heads : rows;
+    const uint32_t most = TABLE_BYTES / (p.rot / 2 * uint32_t(sizeof(float2)));
+    a.tokens = rows / a.headsTile;
+    a.tokens = a.tokens > most ? most : a.tokens;
     if (a.tokens > p.count) a.tokens = uint32_t(p.count);
     const dim3 grid(unsigned((p.count + a.tokens - 1) / a.tokens), (heads + a.headsTile - 1) / a.headsTile);
     const size_t lds = size_t(a.tokens) * (p.rot / 2) * sizeof(float2);
