@@ -648,7 +648,11 @@ AIGPU_ABI int aigpu_paged_decode(const AiGpuPagedDecode* args);
    (as aigpu_allocate leaves it); every call leaves the part that matters zero
    again, so calls of any sizes may follow one another in it, but calls that may
    run at once need one each. A call captured into a graph has to bring one
-   where this is not 0: the backend's scratch may move. */
+   where this is not 0: the backend's scratch may move. That scratch is a
+   stream's own for the first eight streams that decode, so their calls are not
+   ordered among one another (destroy such a stream only when its decodes have
+   ended: its scratch goes with the handle); the calls of later streams share
+   one, in turn. */
 AIGPU_ABI uint64_t aigpu_paged_decode_workspace(const AiGpuPagedDecode* args);
 
 /* ------------------------------------------------------------------------ */

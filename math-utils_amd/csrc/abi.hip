@@ -159,6 +159,45 @@ void* Context::growZeroed(ScratchSlot slot, size_t bytes) {
     return p;
 }
 
+bool Context::scratchOf(hipStream_t stream, size_t bytes, void** at) {
+    *at = nullptr;
+    if (stream == hipStreamPerThread) return true;
+    StreamScratch* own = nullptr;
+    for (StreamScratch& s : streamScratches)
+        if (s.stream == stream) own = &s;
+    if (own && own->bytes >= bytes) {
+        *at = own->at;
+        return true;
+    }
+    if (!own) {
+        if (streamScratches.size() >= STREAM_SCRATCHES) return true;
+        streamScratches.push_back({stream, nullptr, 0});
+        own = &streamScratches.back();
+    }
+    if (own->at) {
+        (void)hipDeviceSynchronize();   // queued work may still use the smaller one
+        (void)hipFree(own->at);
+        allocated -= own->bytes;
+        own->at = nullptr;
+        own->bytes = 0;
+    }
+    void* fresh = nullptr;
+    if (hipMalloc(&fresh, bytes) != hipSuccess) {
+        (void)hipGetLastError();
+        return fail("hipMalloc failed for " + std::to_string(bytes) + " scratch bytes");
+    }
+    // waited for: the stream need not follow the one of the memset
+    if (hipMemset(fresh, 0, bytes) != hipSuccess || hipDeviceSynchronize() != hipSuccess) {
+        (void)hipGetLastError();
+        (void)hipFree(fresh);
+        return fail("hipMemset of scratch failed");
+    }
+    own->at = *at = fresh;
+    own->bytes = bytes;
+    allocated += bytes;
+    return true;
+}
+
 hipEvent_t Context::takeEvent() {
     if (!spareEvents.empty()) {
         hipEvent_t e = spareEvents.back();
@@ -1220,8 +1259,11 @@ AIGPU_ABI int aigpu_paged_decode(const AiGpuPagedDecode* args) {
         return ctx.fail("paged decode: a captured call needs a workspace of its own (" + std::to_string(need) +
                         " bytes)"),
                0;
+    void* work = nullptr;
+    if (!ctx.scratchOf(stream, need, &work)) return 0;
+    if (work) return aigpu::launch_paged_decode(p, work, stream) ? 1 : 0;
     const StreamOrder order(ctx, stream);
-    void* work = ctx.growZeroed(aigpu::SLOT_PAGED, need);
+    work = ctx.growZeroed(aigpu::SLOT_PAGED, need);
     return work && aigpu::launch_paged_decode(p, work, stream) ? 1 : 0;
 }
 

@@ -123,6 +123,17 @@ struct Context {
         return true;
     }
 
+    // a zero-filled scratch that belongs to one stream's calls, which stream
+    // order keeps apart (kernels that use it leave what matters zero): unlike
+    // the slots it needs no handoff event, which costs a call 3 us. Null for
+    // the streams past STREAM_SCRATCHES and for the per-thread default stream,
+    // whose handle stands for many; those share a slot
+    static constexpr size_t STREAM_SCRATCHES = 8;
+    struct StreamScratch { hipStream_t stream; void* at; size_t bytes; };
+    std::vector<StreamScratch> streamScratches;
+    // false on failure (error set); *at null where the stream gets none
+    bool scratchOf(hipStream_t stream, size_t bytes, void** at);
+
     hipEvent_t takeEvent();
     void resolveProfile();
 

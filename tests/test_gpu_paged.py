@@ -413,19 +413,22 @@ def test_two_graphs_with_a_workspace_each_replay_together(gpu):
             assert np.array_equal(host(m[0]), m[1])
 
 
-def test_calls_on_two_streams_share_the_scratch_in_turn(gpu):
+def test_calls_on_many_streams_at_once(gpu):
     import torch
     cases = [_graph_case(gpu, lengths, 70 + i) for i, lengths in enumerate(([5000, 300], [4000, 9, 2000]))]
     want = [_decode(gpu, c[0], c[2], "bf16", c[1]) for c in cases]
-    sides = [torch.cuda.Stream(), torch.cuda.Stream()]
-    outs = [torch.full((len(c[0].lengths), 16, 128), 7.0, device="cuda") for c in cases]
+    # more streams than have a scratch of their own
+    sides = [torch.cuda.Stream() for _ in range(12)]
+    outs = [[torch.full((len(c[0].lengths), 16, 128), 7.0, device="cuda") for c in cases] for _ in sides]
     torch.cuda.synchronize()
     for _ in range(8):
-        for c, out, side in zip(cases, outs, sides):
-            gpu.paged_decode(c[3], out, *c[4], q_norm=c[5], freqs=c[6], stream=side.cuda_stream)
+        for side, row in zip(sides, outs):
+            for c, out in zip(cases, row):
+                gpu.paged_decode(c[3], out, *c[4], q_norm=c[5], freqs=c[6], stream=side.cuda_stream)
     torch.cuda.synchronize()
-    for out, w in zip(outs, want):
-        assert np.array_equal(host(out), w)
+    for row in outs:
+        for out, w in zip(row, want):
+            assert np.array_equal(host(out), w)
 
 
 def test_gpu_refusals(gpu):
