@@ -425,116 +425,105 @@ __device__ __forceinline__ float gated(const PagedDecodeParams& p, uint32_t b, u
 
 /*
     Joins rows `row0` .. of a pair's records into the output of query heads
-    `head` .. of sequence b, by TEAM threads: a workgroup or a wave, with the same
-    sums in the same order. A thread takes four columns of a row and adds the
-    parts up, a tile of them (one trip to memory) at a time; or, where that takes
+    `head` .. of sequence b, by a whole workgroup or, with `alone`, by a wave: the
+    same sums in the same order. A thread takes four columns of a row and adds the
+    parts up, TILE of them (one trip to memory) at a time; or, where that takes
     fewer trips, the parts are dealt to WAVES shares, a wave of the workgroup each
     (a wave alone takes them one after the other), that meet in `room`.
 */
 constexpr int JOIN_FLOATS = 6;
-constexpr uint32_t FEW = 8, MANY = 16;   // parts of a tile: of all of them, of a share
-template <int D, int TEAM>
+template <int D, uint32_t TILE>
 __device__ __forceinline__ void join_parts(const DecodeArgs& a, const Parts& parts, uint32_t b, uint32_t head,
-                                           uint32_t row0, uint32_t rows, float* room) {
+                                           uint32_t row0, uint32_t rows, bool alone, float* room) {
     const PagedDecodeParams& p = a.p;
     const uint32_t size = record_floats(a.perGroup, D), skip = record_heads(a.perGroup), units = rows * (D / 4);
     const auto records = buffer_of(a.records);
-    float top, sum;
-    floatx4 x;
-    auto clear = [&] {
-        top = -INFINITY;
-        sum = 0.0f;
-        x = floatx4{0.0f, 0.0f, 0.0f, 0.0f};
-    };
     auto word = [&](uint32_t at) {
         return __uint_as_float(__builtin_amdgcn_raw_buffer_load_b32(records, at * 4, 0, PAST_L2));
     };
-    // parts k0, k0 + step, ... `count` of them, of columns `unit`
-    auto add = [&](auto count, uint32_t unit, uint32_t k0, uint32_t step) {
-        constexpr uint32_t N = decltype(count)::value;
-        const uint32_t row = row0 + unit / (D / 4), d = unit % (D / 4) * 4;
-        float mk[N], lk[N];
-        u32x4 xk[N];
-#pragma unroll
-        for (uint32_t i = 0; i < N; ++i) {
-            const uint32_t k = k0 + i * step, at = parts.slot(k < parts.total ? k : k0) * size;
-            mk[i] = word(at + row);
-            lk[i] = word(at + a.perGroup + row);
-            xk[i] = __builtin_amdgcn_raw_buffer_load_b128(records, (at + skip + row * D + d) * 4, 0, PAST_L2);
-        }
-        float next = top;
-#pragma unroll
-        for (uint32_t i = 0; i < N; ++i)
-            if (k0 + i * step < parts.total) next = fmaxf(next, mk[i]);
-        const float base = next == -INFINITY ? 0.0f : next, keep = exp2f(top - base);
-        sum *= keep;
-        x *= keep;
-#pragma unroll
-        for (uint32_t i = 0; i < N; ++i) {
-            if (k0 + i * step >= parts.total) break;
-            const float f = exp2f(mk[i] - base);
-            sum += lk[i] * f;
-            x += __builtin_bit_cast(floatx4, xk[i]) * f;
-        }
-        top = next;
-    };
-    auto write = [&](uint32_t unit) {
-        const uint32_t h = head + unit / (D / 4), d = unit % (D / 4) * 4;
-        const float by = 1.0f / sum;
-#pragma unroll
-        for (int i = 0; i < 4; ++i)
-            p.out[(size_t(b) * p.heads + h) * D + d + i] = gated(p, b, h, d + i, x[i] * by);
-    };
-    const uint32_t trips = (units + THREADS - 1) / THREADS * ((parts.total + FEW - 1) / FEW);
-    const uint32_t shared = (units + WAVE - 1) / WAVE * ((parts.total + WAVES * MANY - 1) / (WAVES * MANY));
-    if (trips <= shared) {
+    const uint32_t lane = threadIdx.x % WAVE, wave = alone ? 0 : uniform(threadIdx.x / WAVE);
+    const uint32_t waves = alone ? 1 : WAVES;
+    const uint32_t trips = (units + THREADS - 1) / THREADS * ((parts.total + TILE - 1) / TILE);
+    const uint32_t shared = (units + WAVE - 1) / WAVE * ((parts.total + WAVES * TILE - 1) / (WAVES * TILE));
+    const uint32_t shares = trips <= shared ? 1 : WAVES;
+    // without shares the waves take the columns in turn, with them the shares
+    const uint32_t stepU = shares == 1 ? waves * WAVE : WAVE;
 #pragma unroll 1
-        for (uint32_t unit = threadIdx.x % TEAM; unit < units; unit += TEAM) {
-            clear();
-#pragma unroll 1
-            for (uint32_t k0 = 0; k0 < parts.total; k0 += FEW)
-                add(std::integral_constant<uint32_t, FEW>{}, unit, k0, 1);
-            write(unit);
-        }
-        return;
-    }
-    auto meet = [] {
-        if constexpr (TEAM == WAVE) wave_sync();
-        else __syncthreads();
-    };
-    const uint32_t lane = threadIdx.x % WAVE, wave = TEAM == WAVE ? 0 : uniform(threadIdx.x / WAVE);
-#pragma unroll 1
-    for (uint32_t u0 = 0; u0 < units; u0 += WAVE) {
+    for (uint32_t u0 = shares == 1 ? wave * WAVE : 0; u0 < units; u0 += stepU) {
         const uint32_t unit = u0 + lane;
+        const bool live = unit < units;
+        const uint32_t row = row0 + unit / (D / 4), d = unit % (D / 4) * 4;
+        float top = -INFINITY, sum = 0.0f;
+        floatx4 x = floatx4{0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll 1
-        for (uint32_t q = wave; q < WAVES; q += TEAM / WAVE) {
-            if (unit >= units) continue;
-            clear();
+        for (uint32_t q = shares == 1 ? 0 : wave; q < shares; q += waves) {
+            top = -INFINITY;
+            sum = 0.0f;
+            x = floatx4{0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll 1
-            for (uint32_t k0 = q; k0 < parts.total; k0 += WAVES * MANY)
-                add(std::integral_constant<uint32_t, MANY>{}, unit, k0, WAVES);
+            for (uint32_t k0 = q; k0 < parts.total && live; k0 += shares * TILE) {
+                float mk[TILE], lk[TILE];
+                u32x4 xk[TILE];
+#pragma unroll
+                for (uint32_t i = 0; i < TILE; ++i) {
+                    const uint32_t k = k0 + i * shares, at = parts.slot(k < parts.total ? k : k0) * size;
+                    mk[i] = word(at + row);
+                    lk[i] = word(at + a.perGroup + row);
+                    xk[i] = __builtin_amdgcn_raw_buffer_load_b128(records, (at + skip + row * D + d) * 4, 0, PAST_L2);
+                }
+                float next = top;
+#pragma unroll
+                for (uint32_t i = 0; i < TILE; ++i)
+                    if (k0 + i * shares < parts.total) next = fmaxf(next, mk[i]);
+                const float base = next == -INFINITY ? 0.0f : next, keep = exp2f(top - base);
+                sum *= keep;
+                x *= keep;
+#pragma unroll
+                for (uint32_t i = 0; i < TILE; ++i) {
+                    if (k0 + i * shares >= parts.total) break;
+                    const float f = exp2f(mk[i] - base);
+                    sum += lk[i] * f;
+                    x += __builtin_bit_cast(floatx4, xk[i]) * f;
+                }
+                top = next;
+            }
+            if (shares == 1) break;
             float* mine = room + (q * WAVE + lane) * JOIN_FLOATS;
             mine[0] = top;
             mine[1] = sum;
 #pragma unroll
             for (int i = 0; i < 4; ++i) mine[2 + i] = x[i];
         }
-        meet();
-        if (wave == 0 && unit < units) {
-            clear();
+        if (shares > 1) {
+            if (alone) wave_sync();
+            else __syncthreads();
+            if (wave == 0) {
+                top = -INFINITY;
+                sum = 0.0f;
+                x = floatx4{0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll 1
+                for (uint32_t o = 0; o < WAVES; ++o) {
+                    const float* theirs = room + (o * WAVE + lane) * JOIN_FLOATS;
+                    const float next = fmaxf(top, theirs[0]), base = next == -INFINITY ? 0.0f : next;
+                    const float keep = exp2f(top - base), f = exp2f(theirs[0] - base);
+                    sum = sum * keep + theirs[1] * f;
 #pragma unroll
-            for (uint32_t o = 0; o < WAVES; ++o) {
-                const float* theirs = room + (o * WAVE + lane) * JOIN_FLOATS;
-                const float next = fmaxf(top, theirs[0]), base = next == -INFINITY ? 0.0f : next;
-                const float keep = exp2f(top - base), f = exp2f(theirs[0] - base);
-                sum = sum * keep + theirs[1] * f;
-#pragma unroll
-                for (int i = 0; i < 4; ++i) x[i] = x[i] * keep + theirs[2 + i] * f;
-                top = next;
+                    for (int i = 0; i < 4; ++i) x[i] = x[i] * keep + theirs[2 + i] * f;
+                    top = next;
+                }
             }
-            write(unit);
         }
-        meet();
+        if (live && (shares == 1 || wave == 0)) {
+            const uint32_t h = head + row - row0;
+            const float by = 1.0f / sum;
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+                p.out[(size_t(b) * p.heads + h) * D + d + i] = gated(p, b, h, d + i, x[i] * by);
+        }
+        if (shares > 1) {            // the room is free again
+            if (alone) wave_sync();
+            else __syncthreads();
+        }
     }
 }
 
@@ -1110,10 +1099,8 @@ __global__ __launch_bounds__(THREADS, occupancy(D)) void paged_attention_kernel(
     for (int k = apart ? w : 0; k < 2 * WAVES; k += apart ? WAVES : 1) {
         if (uniform(joins[k].total) == 0) continue;
         const Piece& piece = pieces[k];
-        if (apart)
-            join_parts<D, WAVE>(a, joins[k], piece.b, piece.head, 0, piece.rows, reinterpret_cast<float*>(vbuf[w]));
-        else
-            join_parts<D, THREADS>(a, joins[k], piece.b, piece.head, 0, piece.rows, reinterpret_cast<float*>(vbuf[0]));
+        join_parts<D, 8>(a, joins[k], piece.b, piece.head, 0, piece.rows, apart,
+                      reinterpret_cast<float*>(vbuf[apart ? w : 0]));
     }
 }
 
@@ -1128,7 +1115,7 @@ __global__ __launch_bounds__(THREADS) void paged_merge_kernel(DecodeArgs a, uint
     if (units == 0) return;
     const uint32_t begin = before + pair * units;
     const Parts parts(Cut(a.plan[p.c.batch], runs), begin, begin + units);
-    if (parts.total > 1) join_parts<D, THREADS>(a, parts, b, head, head % G % a.perGroup, 1, room);
+    if (parts.total > 1) join_parts<D, 16>(a, parts, b, head, head % G % a.perGroup, 1, false, room);
 }
 
 bool rotation_ok(Context& ctx, const char* who, const float* freqs, int rot, uint32_t dim, float amplitude) {
