@@ -14,16 +14,6 @@ namespace {
 constexpr uint32_t THREADS = 256;
 constexpr uint32_t NOWHERE = 0xFFFFFFFFu;
 
-/* element offset of (page, row) for kv head h, or ~0 where the sequence's table
-   does not lead to a page of the pool */
-__device__ __forceinline__ uint64_t row_offset(const PagedCache& c, uint32_t b, uint64_t pos, uint32_t h) {
-    const uint64_t slot = pos / c.pageSize;
-    if (slot >= c.tableWidth) return ~uint64_t(0);
-    const uint32_t page = c.table[b * c.tableStride + slot];
-    if (page >= c.pages) return ~uint64_t(0);
-    return page * c.pageStride + h * c.headStride + (pos - slot * c.pageSize) * c.rowStride;
-}
-
 /*
     Appending. A workgroup takes a few tokens; D / 8 lanes take a row of k or v, 8
     elements each, up to PASSES rows a lane. Their loads go out first. Meanwhile
@@ -107,38 +97,40 @@ __global__ __launch_bounds__(THREADS) void paged_append_kernel(AppendArgs a) {
         for (int e = 0; e < 8; ++e) gamma[e] = sub < RPW ? p.gamma[d0 + e] + p.offset : 0.0f;
     }
 
-    // ---- each token's sequence, position and page: a wave takes every NW-th ----
-    {
-        constexpr int MINE = MAX_TOKENS / NW;
-        uint32_t before[MINE] = {};
+    // ---- each token's sequence, position and page: a wave takes every NW-th,
+    //      lane l < MINE its l-th; the page id is on its way during the angles ----
+    constexpr int MINE = MAX_TOKENS / NW;
+    uint32_t before[MINE] = {};
+    if (p.starts) {
+        for (uint32_t k = 0; k <= c.batch; k += WAVE) {
+            const bool in = k + lane <= c.batch;
+            const uint32_t start = in ? p.starts[k + lane] : 0u;
+#pragma unroll
+            for (int i = 0; i < MINE; ++i) before[i] += __popcll(__ballot(in && start <= t0 + w + i * NW));
+        }
+    }
+    uint32_t mine = 0, page = NOWHERE, at = 0;
+#pragma unroll
+    for (int i = 0; i < MINE; ++i) mine = lane == i ? before[i] : mine;
+    const uint32_t own = w + lane * NW;
+    const bool finds = lane < MINE && own < nt;
+    if (finds) {
+        const uint64_t t = t0 + own;
+        uint32_t b = uint32_t(t);
+        uint64_t back = 1;                           // it is the sequence's back-th newest
+        bool live = true;
         if (p.starts) {
-            for (uint32_t k = 0; k <= c.batch; k += WAVE) {
-                const bool in = k + lane <= c.batch;
-                const uint32_t start = in ? p.starts[k + lane] : 0u;
-#pragma unroll
-                for (int i = 0; i < MINE; ++i) before[i] += __popcll(__ballot(in && start <= t0 + w + i * NW));
-            }
+            live = mine > 0 && mine <= c.batch;
+            b = live ? mine - 1 : 0;
+            const uint64_t end = p.starts[b + 1];
+            live = live && end > t;
+            back = live ? end - t : 1;
         }
-        uint32_t mine = 0;
-#pragma unroll
-        for (int i = 0; i < MINE; ++i) mine = lane == i ? before[i] : mine;
-        const uint32_t i = w + lane * NW;            // lane's token
-        if (lane < MINE && i < nt) {
-            const uint64_t t = t0 + i;
-            uint32_t b = uint32_t(t);
-            uint64_t back = 1;                       // it is the sequence's back-th newest
-            bool live = true;
-            if (p.starts) {
-                live = mine > 0 && mine <= c.batch;
-                b = live ? mine - 1 : 0;
-                const uint64_t end = p.starts[b + 1];
-                live = live && end > t;
-                back = live ? end - t : 1;
-            }
-            const uint64_t len = c.lengths[b], pos = len - back;
-            place[i] = uint32_t(pos);
-            base[i] = live && len >= back ? row_offset(c, b, pos, 0) : ~uint64_t(0);
-        }
+        const uint64_t len = c.lengths[b];
+        const uint32_t pos = uint32_t(len - back), slot = pos / c.pageSize;
+        place[own] = pos;
+        at = pos - slot * c.pageSize;
+        if (live && len >= back && slot < c.tableWidth) page = c.table[b * c.tableStride + slot];
     }
     __syncthreads();
     const uint32_t half = p.freqs ? p.rot / 2 : 0;
@@ -147,6 +139,7 @@ __global__ __launch_bounds__(THREADS) void paged_append_kernel(AppendArgs a) {
         rotation_at(place[i / half], p.freqs[i % half], cs, sn);
         turns[i] = float2{cs * p.amplitude, sn * p.amplitude};
     }
+    if (finds) base[own] = page < c.pages ? page * c.pageStride + at * c.rowStride : ~uint64_t(0);
     __syncthreads();
 
     float* row = rows[w][sub < RPW ? sub : 0];
