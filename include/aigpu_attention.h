@@ -532,7 +532,7 @@ AIGPU_ABI int aigpu_select_keys(const AiGpuSelectKeys* args);
 typedef struct AiGpuRotary {
     const void* x;            /* element (token, head, d) at token*tokenStride + head*headStride + d, type */
     void* out;                /* the same with the out strides, type */
-    const uint32_t* positions;/* [count], or NULL: start, start + 1, ... */
+    const uint32_t* positions;/* [count], unsigned, or NULL: start, start + 1, ... */
     const float* frequencies; /* [rotaryDims/2] */
     float amplitude;          /* of cos and sin (scaled long contexts); 0 means 1 */
     uint32_t rotaryDims;      /* even, 2 .. dim */
@@ -627,14 +627,14 @@ AIGPU_ABI int aigpu_paged_append(const AiGpuPagedAppend* args);
 typedef struct AiGpuPagedDecode {
     AiGpuPagedCache cache;
     const void* q;            /* [batch][heads][qStride], inType; sequence b at b*qTokenStride */
-    float* out;               /* [batch][heads][dim] fp32 */
+    float* out;               /* [batch][heads][dim] fp32, apart from q */
     const float* qNorm;
     const float* rotaryFrequencies;
     float epsilon, normOffset, amplitude;
     float scale;              /* of the scores; 0 means 1/sqrt(dim) */
     uint32_t rotaryDims, interleaved, inType;
     uint32_t outputGate;      /* as AiGpuPrefill::outputGate */
-    uint32_t maxLength;       /* >= every lengths[b]; sizes the launch */
+    uint32_t maxLength;       /* >= every lengths[b], at most 2^31; sizes the launch */
     uint32_t reserved;
     uint64_t heads, qStride, qTokenStride;  /* qStride 0 means dim, qTokenStride 0 heads*qStride */
     uint64_t window;          /* the last `window` positions only; 0 = all */

@@ -876,6 +876,17 @@ _PACK = {"aigpu_rotary": _struct.Struct("4Pf5I8QP"),
          "aigpu_paged_append": _struct.Struct(_CACHE + "5P3f3I3QP"),
          "aigpu_paged_decode": _struct.Struct(_CACHE + "4P4f6I4QPQP")}
 _entries = {}
+_torch = None
+
+
+def _with_torch():
+    """torch, imported by the first call that takes tensors (an import statement in each helper would cost 2 us a
+    call)"""
+    global _torch
+    if _torch is None:
+        import torch
+        _torch = torch
+    return _torch
 
 
 def _entry(name):
@@ -912,19 +923,18 @@ def _own_stream(stream):
     """the stream given, or torch's current one of the backend's device"""
     if stream is not None:
         return stream
-    import torch
-    raw = getattr(torch._C, "_cuda_getCurrentRawStream", None)   # without a Stream object built round it
-    return raw(0) if raw else torch.cuda.current_stream(0).cuda_stream
+    raw = getattr(_torch._C, "_cuda_getCurrentRawStream", None)   # without a Stream object built round it
+    return raw(0) if raw else _torch.cuda.current_stream(0).cuda_stream
 
 
 def _kind(t):
     """the type tag of a float32 or bfloat16 tensor"""
-    import torch
-    if t.dtype is torch.bfloat16:
+    dtype = t.dtype
+    if dtype is _torch.bfloat16:
         return BF16
-    if t.dtype is torch.float32:
+    if dtype is _torch.float32:
         return F32
-    raise TypeError(f"unsupported dtype {t.dtype}: float32 or bfloat16")
+    raise TypeError(f"unsupported dtype {dtype}: float32 or bfloat16")
 
 
 def _vector(t, name, least, exact=False):
@@ -942,12 +952,12 @@ def _vector(t, name, least, exact=False):
 
 def _indices(t, name, dims, entries=None):
     """the address of an int32 (or uint32) tensor of `dims` dimensions with unit stride in the last"""
-    import torch
-    at = _at(t, name)
-    if t.dtype not in (torch.int32, torch.uint32) or t.dim() != dims or (t.stride(-1) != 1 and t.shape[-1] > 1):
+    at, shape, dtype = _at(t, name), t.shape, t.dtype
+    if (dtype is not _torch.int32 and dtype is not _torch.uint32) or len(shape) != dims \
+            or (t.stride(-1) != 1 and shape[-1] > 1):
         raise TypeError(f"{name} must be an int32 tensor of {dims} dimensions with unit stride")
-    if entries is not None and t.shape[0] != entries:
-        raise ValueError(f"{name} has {t.shape[0]} entries, {entries} are needed")
+    if entries is not None and shape[0] != entries:
+        raise ValueError(f"{name} has {shape[0]} entries, {entries} are needed")
     return at
 
 
@@ -975,6 +985,7 @@ def rotary(x, out, freqs, positions=None, start=0, rotary_dims=None, interleaved
     freqs[j], halves paired or neighbours (interleaved); the rest is copied.
     positions [tokens] int32, or start, start + 1, ... backward=True gives x's
     gradient from out's (the transposed rotation). Asynchronous."""
+    _with_torch()
     of, to = _at(x, "x"), _at(out, "out")
     if x.dim() != 3 or out.shape != x.shape or out.dtype != x.dtype:
         raise ValueError("x must be [tokens][heads][dim], and out of its shape and type")
@@ -994,6 +1005,7 @@ def rotary(x, out, freqs, positions=None, start=0, rotary_dims=None, interleaved
 
 def _paged_cache(keys, values, table, lengths):
     """AiGpuPagedCache's fields"""
+    _with_torch()
     at = _at(keys, "key_pages"), _at(values, "value_pages"), _indices(table, "table", 2), _indices(lengths, "lengths", 1)
     if _kind(keys) != BF16 or _kind(values) != BF16:
         raise TypeError("the pages must be bfloat16")
@@ -1055,7 +1067,7 @@ def _paged_decode(q, out, key_pages, value_pages, table, lengths, max_length, q_
             raise ValueError("workspace must be contiguous")
         room, nbytes = _at(workspace, "workspace"), workspace.numel() * workspace.element_size()
     if max_length is None:
-        max_length = min(cache[9] * cache[6], 0xFFFFFFFF)
+        max_length = min(cache[9] * cache[6], 1 << 31)
     return _packed("aigpu_paged_decode", *cache, of_q, to, _vector(q_norm, "q_norm", dim, True),
                    _vector(freqs, "freqs", rot // 2), eps, norm_offset, amplitude, scale, rot,
                    1 if interleaved else 0, _kind(q), 1 if output_gate else 0, max_length, 0, heads, hs, ts, window,
@@ -1082,8 +1094,7 @@ def paged_decode(q, out, key_pages, value_pages, table, lengths, max_length=None
 def paged_decode_workspace(q, out, key_pages, value_pages, table, lengths, max_length=None):
     """a workspace (zero-filled uint8 tensor) for paged_decode calls of these
     sizes or smaller ones of the same heads and dim, whatever the lengths hold"""
-    import torch
     args = _paged_decode(q, out, key_pages, value_pages, table, lengths, max_length, None, 1e-6, 0.0, None, None,
                          False, 1.0, 0.0, 0, False, None, None)
     need = lib().aigpu_paged_decode_workspace(C.cast(C.c_char_p(args), C.POINTER(AiGpuPagedDecode)))
-    return torch.zeros(int(need), dtype=torch.uint8, device=q.device)
+    return _torch.zeros(int(need), dtype=_torch.uint8, device=q.device)

@@ -1237,6 +1237,14 @@ bool check_paged_decode(const PagedDecodeParams& p) {
     if (p.qStride < p.c.dim) return ctx.fail("paged decode: qStride < dim");
     if (p.outputGate && p.qStride < 2 * uint64_t(p.c.dim))
         return ctx.fail("paged decode: the output gate needs qStride >= 2 dim");
+    if (p.c.batch) {
+        const uintptr_t q = reinterpret_cast<uintptr_t>(p.q), out = reinterpret_cast<uintptr_t>(p.out);
+        const uint64_t row = (p.outputGate ? 2 : 1) * uint64_t(p.c.dim);
+        const uint64_t last = (p.c.batch - 1) * p.qTokenStride + (p.heads - 1) * p.qStride + row;
+        const uint64_t outBytes = uint64_t(p.c.batch) * p.heads * p.c.dim * sizeof(float);
+        if (q < out + outBytes && out < q + last * (p.inType == 1 ? 2 : 4))
+            return ctx.fail("paged decode: out overlaps q");
+    }
     if (!(p.scale > 0.0f) || !std::isfinite(p.scale))
         return ctx.fail("paged decode: the scale must be positive and finite");
     if (p.maxLength > uint64_t(p.c.tableWidth) * p.c.pageSize)

@@ -96,10 +96,43 @@ def test_decode_scale_norm_offset_and_strided_queries(gpu):
     _check_decode(got, cache, rows[:, 8:16], opt, scale=0.03)
 
 
-def test_decode_output_gate(gpu):
+@pytest.mark.parametrize("dtype", ["bf16", "f32"])
+def test_rows_off_16_bytes(gpu, dtype):
+    """queries, keys and values that start on no 16-byte boundary"""
+    import torch
+    opt = _options(96, 90, True, 40)
+    cache = Cache([77, 640, 1], 3, 16, 96, 91)
+    flat = rounded(O.fill_normal((3 * 6 * 96 + 1,), 92, "q"), dtype)
+    off = _dev(flat, dtype)[1:].view(3, 6, 96)
+    assert off.data_ptr() % 16
+    q = flat[1:].reshape(3, 6, 96)
+    device = cache.device()
+    _check_decode(_decode(gpu, cache, off, dtype, opt, device=device), cache, q, opt)
+    k, v = off[:, :3], _dev(flat, dtype)[:-1].view(3, 6, 96)[:, 3:]
+    gpu.paged_append(k, v, *device)
+    keys, values = host(device[0]), host_bits(device[1])
+    for b, n in enumerate(cache.lengths):
+        at = cache.table[b][(n - 1) // 16], slice(None), (n - 1) % 16
+        assert np.array_equal(keys[at], rounded(q[b, :3], "bf16"))
+        assert np.array_equal(values[at], O.pack_bf16(flat[:-1].reshape(3, 6, 96)[b, 3:]).reshape(3, 96))
+
+
+def test_decode_repeats_to_the_bit(gpu):
+    """whichever workgroup joins a sequence's parts"""
+    opt = _options(128, 93, True, 128)
+    cache = Cache([12000, 3, 700, 5000, 64, 1, 8191, 0, 2500], 4, 16, 128, 94)
+    q = rounded(O.fill_normal((9, 32, 128), 95, "q"), "bf16")
+    device = cache.device()
+    first = _decode(gpu, cache, q, "bf16", opt, device=device)
+    for _ in range(30):
+        assert np.array_equal(_decode(gpu, cache, q, "bf16", opt, device=device), first)
+
+
+@pytest.mark.parametrize("heads", [8, 40])
+def test_decode_output_gate(gpu, heads):
     opt = _options(128, 14, True, 128)
     cache = Cache([50, 3000, 0], 2, 16, 128, 15)
-    q = rounded(O.fill_normal((3, 8, 256), 16, "q"), "bf16")
+    q = rounded(O.fill_normal((3, heads, 256), 16, "q"), "bf16")
     got = _decode(gpu, cache, q, "bf16", opt, output_gate=True)
     for b, n in enumerate(cache.lengths):
         if n == 0:
@@ -456,7 +489,7 @@ def test_gpu_refusals(gpu):
            decode(lens=lens.long()), decode(table=table.long()), decode(table=table.t()), decode(lens=lens[:1]),
            decode(keys=keys.float(), values=values.float()), decode(values=values[:-1]), decode(keys=odd, values=odd),
            decode(keys=off, values=off), decode(q=q[..., :80], out=out[..., :80].contiguous(), keys=tiny, values=tiny),
-           decode(q_norm=g[:64]), decode(q_norm=g.double()), decode(freqs=f, rotary_dims=63),
+           decode(out=q), decode(q_norm=g[:64]), decode(q_norm=g.double()), decode(freqs=f, rotary_dims=63),
            decode(freqs=f, rotary_dims=130), decode(freqs=f[:10], rotary_dims=64),
            append(k=kv[:1], v=kv[:1]), append(k=kv[:, :1], v=kv[:, :1]), append(v=kv.bfloat16()),
            append(starts=lens), append(starts=torch.zeros(3, device="cuda")), append(k_norm=g[:64]),

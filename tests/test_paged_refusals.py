@@ -37,7 +37,7 @@ def _append(cache=None, **kw):
 
 
 def _decode(cache=None, **kw):
-    base = dict(cache=cache or _cache(), q=PTR, out=PTR, rotaryFrequencies=PTR, rotaryDims=128, maxLength=80, heads=4)
+    base = dict(cache=cache or _cache(), q=PTR, out=2 * PTR, rotaryFrequencies=PTR, rotaryDims=128, maxLength=80, heads=4)
     return aigpu.AiGpuPagedDecode(**{**base, **kw})
 
 
@@ -87,7 +87,8 @@ def test_append_refuses(change, why):
     (dict(heads=5), "heads"), (dict(heads=2 ** 17), "heads"), (dict(qStride=64), "qStride"),
     (dict(outputGate=1), "gate"), (dict(scale=-1.0), "scale"), (dict(scale=math.nan), "scale"),
     (dict(maxLength=81), "maxLength"), (dict(rotaryDims=130), "rotaryDims"), (dict(amplitude=math.inf), "amplitude"),
-    (dict(qTokenStride=2 ** 41), "range"), (dict(q=PTR + 2), "aligned"),
+    (dict(qTokenStride=2 ** 41), "range"), (dict(q=PTR + 2), "aligned"), (dict(out=PTR), "overlaps"),
+    (dict(out=PTR + 4 * 128 * 11), "overlaps"), (dict(maxLength=2 ** 31 + 1), "maxLength"),
     (dict(workspace=PTR + 64, workspaceBytes=1 << 40), "aligned"),
 ])
 def test_decode_refuses(change, why):
