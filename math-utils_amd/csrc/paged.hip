@@ -1212,9 +1212,13 @@ DecodeShape decode_shape(const PagedDecodeParams& p) {
     return s;
 }
 
-// a pair's records that one workgroup joins within the attention's launch; past
-// it, a workgroup a query head of a second launch
-constexpr uint64_t JOIN_BYTES = 256 << 10;
+// A pair's records that one workgroup joins within the attention's launch; past
+// it, a workgroup a query head of a second launch. At 133 KB (131072 positions,
+// 8 x 4 heads of 128) joining within takes 113 us in all, the second launch 109;
+// at 33 KB (4096 positions, 8 x 2 heads) both 16; with few records of many pairs
+// (256 sequences of 1 to 700, 4 KB) 78 against 92, most of whose workgroups find
+// nothing to join.
+constexpr uint64_t JOIN_BYTES = 64 << 10;
 bool joins_in_kernel(const PagedDecodeParams& p, const DecodeShape& s, uint32_t batch) {
     const uint64_t parts = s.grid / (uint64_t(batch) * p.c.kvHeads * s.groups) + 1;
     return parts * s.perGroup * p.c.dim * sizeof(float) <= JOIN_BYTES;
