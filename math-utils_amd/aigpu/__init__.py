@@ -919,6 +919,12 @@ def _at(t, name):
     return t.data_ptr()
 
 
+def _all_here(*pairs):
+    """raises for the first of (tensor or None, name) that is not on the backend's device"""
+    for t, name in pairs:
+        _at(t, name)
+
+
 def _own_stream(stream):
     """the stream given, or torch's current one of the backend's device"""
     if stream is not None:
@@ -941,10 +947,10 @@ def _vector(t, name, least, exact=False):
     """the address of an fp32 vector of at least (or exactly) `least` elements, or 0 for None"""
     if t is None:
         return 0
-    at = _at(t, name)
-    if _kind(t) != F32 or t.dim() != 1 or not t.is_contiguous():
+    at, shape = _at(t, name), t.shape
+    if t.dtype is not _torch.float32 or len(shape) != 1 or not t.is_contiguous():
         raise TypeError(f"{name} must be a contiguous float32 vector")
-    n = t.shape[0]
+    n = shape[0]
     if n < least or (exact and n != least):
         raise ValueError(f"{name} has {n} elements, {least} are needed")
     return at
@@ -1006,8 +1012,19 @@ def rotary(x, out, freqs, positions=None, start=0, rotary_dims=None, interleaved
 def _paged_cache(keys, values, table, lengths):
     """AiGpuPagedCache's fields"""
     _with_torch()
-    at = _at(keys, "key_pages"), _at(values, "value_pages"), _indices(table, "table", 2), _indices(lengths, "lengths", 1)
-    if _kind(keys) != BF16 or _kind(values) != BF16:
+    try:
+        away = keys.get_device() | values.get_device() | table.get_device() | lengths.get_device()
+    except AttributeError:
+        away = -1
+    if away:
+        _all_here((keys, "key_pages"), (values, "value_pages"), (table, "table"), (lengths, "lengths"))
+    i32, u32, bf16 = _torch.int32, _torch.uint32, _torch.bfloat16
+    if (table.dtype is not i32 and table.dtype is not u32) or table.dim() != 2 \
+            or (table.stride(1) != 1 and table.shape[1] > 1):
+        raise TypeError("table must be an int32 tensor of two dimensions with unit stride")
+    if (lengths.dtype is not i32 and lengths.dtype is not u32) or not lengths.dim() == 1 or not lengths.is_contiguous():
+        raise TypeError("lengths must be a contiguous int32 vector")
+    if keys.dtype is not bf16 or values.dtype is not bf16:
         raise TypeError("the pages must be bfloat16")
     strides = keys.stride()
     if len(strides) != 4 or values.shape != keys.shape or values.stride() != strides:
@@ -1020,8 +1037,9 @@ def _paged_cache(keys, values, table, lengths):
     batch, (rows, width) = lengths.shape[0], table.shape
     if rows != batch:
         raise ValueError(f"table has {rows} entries, {batch} are needed")
-    return at + (batch, pages, size, kv_heads, dim, width, table.stride(0) if batch > 1 else width,
-                 ps if pages > 1 else dim, hs if kv_heads > 1 else dim, rs if size > 1 else dim)
+    return (keys.data_ptr(), values.data_ptr(), table.data_ptr(), lengths.data_ptr(), batch, pages, size, kv_heads,
+            dim, width, table.stride(0) if batch > 1 else width, ps if pages > 1 else dim,
+            hs if kv_heads > 1 else dim, rs if size > 1 else dim)
 
 
 def paged_append(k, v, key_pages, value_pages, table, lengths, starts=None, k_norm=None, eps=1e-6, norm_offset=0.0,
@@ -1042,9 +1060,13 @@ def paged_append(k, v, key_pages, value_pages, table, lengths, starts=None, k_no
     turns, gamma = _vector(freqs, "freqs", rot // 2), _vector(k_norm, "k_norm", dim, True)
     if shape[0] == 0:
         return
-    (ks, kh), (vs, vh) = _strides(k, "k"), _strides(v, "v")
-    if kh != dim or vh != dim:
+    (ks, kh, k1), (vs, vh, v1) = k.stride(), v.stride()
+    if k1 != 1 or v1 != 1 or (kv_heads > 1 and (kh != dim or vh != dim)):
         raise ValueError("the heads of a token's k and v must lie one after the other")
+    if shape[0] == 1:                # any stride stands for one token
+        ks = vs = kv_heads * dim
+    if ks <= 0 or vs <= 0:
+        raise ValueError("k and v must not be broadcast views")
     args = _packed("aigpu_paged_append", *cache, of_k, of_v, begins, gamma, turns, eps, norm_offset, amplitude, rot,
                    1 if interleaved else 0, _kind(k), shape[0], ks, vs, _own_stream(stream))
     _check(_entry("aigpu_paged_append")(args))
