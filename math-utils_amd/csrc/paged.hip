@@ -21,7 +21,10 @@ constexpr uint32_t NOWHERE = 0xFFFFFFFFu;
     one round of loads, where a binary search would take one a step), its position
     and its page, and the workgroup the tokens' cosines and sines, once for all kv
     heads. Then k's rows are normed and turned, and all rows rounded and stored.
-    HBM bounds it: rows are read once and written once, 16 bytes a lane.
+    Rows are read once and written once, 16 bytes a lane, which HBM would bound;
+    what does is a workgroup's chain of starts, lengths, table and angles beside
+    the four workgroups that a CU's registers hold: 8199 bf16 tokens of 8 heads of
+    128 (67 MB) take 18.2 us, 3.7 TB/s; 32 tokens 4.1 us.
 */
 constexpr int PASSES = 4;
 constexpr uint32_t MAX_TOKENS = 16;
@@ -260,6 +263,11 @@ __global__ __launch_bounds__(THREADS) void paged_append_kernel(AppendArgs a) {
     itself the last of the pair's (a counter that it sets back to zero), or, where
     a pair's records are more than one workgroup should read, by
     paged_merge_kernel.
+
+    32 sequences of 1k to 32k under 32/4 heads of 128 (1.11 GB): 190 us, 5.8 TB/s
+    of the 6.1 that a large copy reaches. Small calls are a chain of about 15 us:
+    dispatch, lengths and list 4, page ids and queries 2, a first slab 3, its
+    weights 1, the joins 5 (one sequence of 4096 under 16/8 heads, 16.8 MB: 15).
 */
 constexpr int SLAB = 32;
 constexpr int WAVES = 4;
