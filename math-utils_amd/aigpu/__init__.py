@@ -1037,9 +1037,11 @@ def _paged_cache(keys, values, table, lengths):
     batch, (rows, width) = lengths.shape[0], table.shape
     if rows != batch:
         raise ValueError(f"table has {rows} entries, {batch} are needed")
+    step = table.stride(0) if batch > 1 else width
+    if (step == 0 and width) or (rs == 0 and size > 1):      # 0 means the dense stride to the entries
+        raise ValueError("the table and the rows of the pages must not be broadcast views")
     return (keys.data_ptr(), values.data_ptr(), table.data_ptr(), lengths.data_ptr(), batch, pages, size, kv_heads,
-            dim, width, table.stride(0) if batch > 1 else width, ps if pages > 1 else dim,
-            hs if kv_heads > 1 else dim, rs if size > 1 else dim)
+            dim, width, step, ps if pages > 1 else dim, hs if kv_heads > 1 else dim, rs if size > 1 else dim)
 
 
 def paged_append(k, v, key_pages, value_pages, table, lengths, starts=None, k_norm=None, eps=1e-6, norm_offset=0.0,
@@ -1117,6 +1119,7 @@ def paged_decode_workspace(q, out, key_pages, value_pages, table, lengths, max_l
     """a workspace (zero-filled uint8 tensor) for paged_decode calls of these
     sizes or smaller ones of the same heads and dim, whatever the lengths hold"""
     args = _paged_decode(q, out, key_pages, value_pages, table, lengths, max_length, None, 1e-6, 0.0, None, None,
-                         False, 1.0, 0.0, 0, False, None, None)
+                         False, 1.0, 0.0, 0, False, None, 0)
     need = lib().aigpu_paged_decode_workspace(C.cast(C.c_char_p(args), C.POINTER(AiGpuPagedDecode)))
+    _check(need or q.shape[0] == 0)
     return _torch.zeros(int(need), dtype=_torch.uint8, device=q.device)

@@ -127,6 +127,48 @@ def test_wrappers_refuse_host_tensors():
         aigpu.rotary(np.zeros((2, 2, 64)), x, x)
 
 
+def _here(t):
+    """t, saying that it lies on the backend's device"""
+    import torch
+
+    class Here(torch.Tensor):
+        def get_device(self):
+            return 0
+    return t.as_subclass(Here)
+
+
+def test_wrappers_refuse_broadcast_tables_and_pages():
+    """a row stride of 0 means the dense one to the entries, which lies past what a broadcast view holds"""
+    import torch
+    if aigpu.available():
+        pytest.skip("the tensors are the host's: no call is made beside a device")
+    aigpu._with_torch()
+    pages = _here(torch.zeros((4, 2, 16, 64), dtype=torch.bfloat16))
+    row = _here(torch.zeros((4, 2, 16, 1), dtype=torch.bfloat16)[:1, :1, :1].expand(1, 1, 1, 64))
+    one = _here(torch.zeros(64, dtype=torch.bfloat16).expand(4, 2, 16, 64))
+    table, lengths = _here(torch.zeros((3, 5), dtype=torch.int32)), _here(torch.zeros(3, dtype=torch.int32))
+    shared = _here(torch.zeros((1, 5), dtype=torch.int32).expand(3, 5))
+    with pytest.raises(ValueError, match="broadcast"):
+        aigpu._paged_cache(pages, pages, shared, lengths)
+    with pytest.raises(ValueError, match="broadcast"):
+        aigpu._paged_cache(one, one, table, lengths)
+    with pytest.raises(ValueError, match="unit stride"):
+        aigpu._paged_cache(row, row, table, lengths)
+    assert aigpu._paged_cache(pages, pages, table, lengths)[-4:] == (5, 2048, 1024, 64)
+
+
+def test_a_workspace_for_a_refused_call_is_refused():
+    import torch
+    if aigpu.available():
+        pytest.skip("the tensors are the host's: no call is made beside a device")
+    pages = _here(torch.zeros((4, 2, 16, 64), dtype=torch.bfloat16))
+    table, lengths = _here(torch.zeros((3, 5), dtype=torch.int32)), _here(torch.zeros(3, dtype=torch.int32))
+    q, out = _here(torch.zeros((3, 4, 64))), _here(torch.zeros((3, 4, 64)))
+    aigpu._with_torch()
+    with pytest.raises(aigpu.AiGpuError, match="maxLength"):
+        aigpu.paged_decode_workspace(q, out, pages, pages, table, lengths, max_length=81)
+
+
 # ----------------------------------------------------------------- frequency tables
 def test_frequencies_of_the_shared_kinds():
     """the oracle forms them in fp32: a power (2 ulp), a division, and for llama3 the wave's (4 roundings through a
