@@ -599,7 +599,8 @@ typedef struct AiGpuPagedCache {
    (a length below its new tokens), beyond the table or in a page outside the
    pool is not written; a decode over such a length answers NaN. No two
    tokens may share a row: a page shared by sequences is copied before either
-   writes to it. Asynchronous; needs no scratch, so calls on different streams
+   writes to it, and strides that let rows of the pool overlap are refused
+   (a decode reads such a pool). Asynchronous; needs no scratch, so calls on different streams
    are not ordered by the backend. */
 typedef struct AiGpuPagedAppend {
     AiGpuPagedCache cache;

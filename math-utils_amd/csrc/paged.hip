@@ -1,5 +1,6 @@
 // paged.hip - a paged KV cache: appending the newest tokens, and one token's
 // attention over each sequence's pages.
+#include <algorithm>
 #include <cmath>
 #include <type_traits>
 
@@ -1151,6 +1152,16 @@ bool check_paged_append(const PagedAppendParams& p) {
     if (!p.starts && p.count != p.c.batch)
         return ctx.fail("paged append: without starts there is one token a sequence");
     if (p.count >= (uint64_t(1) << 31)) return ctx.fail("paged append: too many tokens");
+    // the pool's rows are written, so no two may meet: each stride spans what the shorter ones do
+    struct Axis { uint64_t stride, size; };
+    Axis axes[3] = {{p.c.rowStride, p.c.pageSize}, {p.c.headStride, p.c.kvHeads}, {p.c.pageStride, p.c.pages}};
+    std::sort(axes, axes + 3, [](const Axis& a, const Axis& b) { return a.stride < b.stride; });
+    uint64_t extent = p.c.dim;
+    for (const Axis& a : axes) {
+        if (a.size == 1) continue;
+        if (a.stride < extent) return ctx.fail("paged append: the rows of the pages overlap");
+        extent += (a.size - 1) * a.stride;
+    }
     if (p.kStride < uint64_t(p.c.kvHeads) * p.c.dim || p.vStride < uint64_t(p.c.kvHeads) * p.c.dim)
         return ctx.fail("paged append: the rows of k or v overlap");
     const uintptr_t at = reinterpret_cast<uintptr_t>(p.k) | reinterpret_cast<uintptr_t>(p.v);

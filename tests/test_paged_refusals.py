@@ -82,6 +82,18 @@ def test_append_refuses(change, why):
     _refused("aigpu_paged_append", _append(**change), why)
 
 
+def test_append_needs_rows_of_their_own():
+    """pages that share rows are read by a decode, but two tokens would be written to one place"""
+    for shared in (dict(pageStride=0, headStride=2048, rowStride=128), dict(pageStride=2048, headStride=0, rowStride=128),
+                   dict(pageStride=4096, headStride=1024, rowStride=128),
+                   dict(pageStride=2048, headStride=2048, rowStride=128)):
+        _refused("aigpu_paged_append", _append(_cache(**shared)), "overlap")
+        _refused("aigpu_paged_decode", _decode(_cache(**shared)), "no usable gfx950 device")
+    for apart in (dict(pageStride=4096, headStride=128, rowStride=256), dict(pageStride=8192, headStride=4096, rowStride=256),
+                  dict(pageStride=128, headStride=1280, rowStride=2560), dict(pageStride=16, headStride=0, rowStride=128, pages=1, kvHeads=1)):
+        _refused("aigpu_paged_append", _append(_cache(**apart)), "no usable gfx950 device")
+
+
 @pytest.mark.parametrize("change,why", [
     (dict(q=None), "null"), (dict(out=None), "null"), (dict(inType=7), "type"), (dict(heads=0), "heads"),
     (dict(heads=5), "heads"), (dict(heads=2 ** 17), "heads"), (dict(qStride=64), "qStride"),
