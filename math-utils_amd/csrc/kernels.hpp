@@ -263,6 +263,17 @@ struct GdnGatedNormParams {
 };
 bool launch_gdn_gated_norm(const GdnGatedNormParams& p, hipStream_t stream);
 
+// Tiles laid over two dimensions of a grid: one of them holds less than 2^32
+// threads, so 2^24 workgroups of 256. The last side may have places past the end.
+struct Tiles {
+    uint32_t side, sides;
+    explicit Tiles(uint64_t n) {
+        constexpr uint64_t MOST = uint64_t(1) << 23;
+        side = uint32_t(n < MOST ? n : MOST);
+        sides = uint32_t((n + side - 1) / side);
+    }
+};
+
 // ---- rotary positions ----
 struct RotaryParams {
     const void* x;

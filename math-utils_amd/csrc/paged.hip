@@ -61,7 +61,8 @@ __global__ __launch_bounds__(THREADS) void paged_append_kernel(AppendArgs a) {
     const PagedAppendParams& p = a.p;
     const PagedCache& c = p.c;
     const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
-    const uint64_t t0 = uint64_t(blockIdx.x) * a.tokens;
+    const uint64_t t0 = (uint64_t(blockIdx.y) * gridDim.x + blockIdx.x) * a.tokens;
+    if (t0 >= p.count) return;
     const uint32_t nt = p.count - t0 < a.tokens ? uint32_t(p.count - t0) : a.tokens;
     const uint32_t keys = nt * c.kvHeads, total = 2 * keys;      // k's rows, then v's
     const int sub = lane / LPR, d0 = (lane % LPR) * 8;
@@ -1184,10 +1185,10 @@ bool launch_paged_append(const PagedAppendParams& p, hipStream_t stream) {
     uint32_t tokens = rows / (2 * p.c.kvHeads);
     if (tokens > spread) tokens = uint32_t(spread);
     a.tokens = tokens < 1 ? 1 : (tokens > MAX_TOKENS ? MAX_TOKENS : tokens);
-    const unsigned grid = unsigned((p.count + a.tokens - 1) / a.tokens);
+    const Tiles tiles((p.count + a.tokens - 1) / a.tokens);
     const size_t lds = p.freqs ? size_t(a.tokens) * (p.rot / 2) * sizeof(float2) : 0;
     return ctx.launch("paged_append_kernel", stream, [&] {
-        auto go = [&](auto kernel) { hipLaunchKernelGGL(kernel, dim3(grid), dim3(THREADS), lds, stream, a); };
+        auto go = [&](auto kernel) { hipLaunchKernelGGL(kernel, dim3(tiles.side, tiles.sides), dim3(THREADS), lds, stream, a); };
         auto of = [&](auto dim) {
             constexpr int D = decltype(dim)::value;
             if (p.inType == 1) go(paged_append_kernel<D, true>);

@@ -102,7 +102,8 @@ __global__ __launch_bounds__(THREADS) void rotary_kernel(RotaryArgs a) {
     extern __shared__ __attribute__((aligned(16))) float2 turns[];
     const RotaryParams& p = a.p;
     const uint32_t half = p.rot / 2, dim = uint32_t(p.dim);
-    const uint64_t t0 = uint64_t(blockIdx.x) * a.tokens;
+    const uint64_t t0 = (uint64_t(blockIdx.z) * gridDim.x + blockIdx.x) * a.tokens;
+    if (t0 >= p.count) return;
     const uint32_t h0 = blockIdx.y * a.headsTile;
     const uint32_t nt = p.count - t0 < a.tokens ? uint32_t(p.count - t0) : a.tokens;
     const uint32_t nh = uint32_t(p.heads) - h0 < a.headsTile ? uint32_t(p.heads) - h0 : a.headsTile;
@@ -285,7 +286,8 @@ bool launch_rotary(const RotaryParams& p, hipStream_t stream) {
     a.tokens = rows / a.headsTile;
     a.tokens = a.tokens > most ? most : a.tokens;
     if (a.tokens > p.count) a.tokens = uint32_t(p.count);
-    const dim3 grid(unsigned((p.count + a.tokens - 1) / a.tokens), (heads + a.headsTile - 1) / a.headsTile);
+    const Tiles tiles((p.count + a.tokens - 1) / a.tokens);
+    const dim3 grid(tiles.side, (heads + a.headsTile - 1) / a.headsTile, tiles.sides);
     const size_t lds = size_t(a.tokens) * (p.rot / 2) * sizeof(float2);
     const int which = (V > 1 ? 4 : 0) | (p.type == 1 ? 2 : 0) | (p.interleaved ? 1 : 0);
     return ctx.launch("rotary_kernel", stream, [&] {

@@ -56,6 +56,21 @@ def test_many_tokens_and_heads(gpu):
         _check(_run(gpu, x, None, freqs, "bf16", start=17), x, 17 + np.arange(tokens), freqs, False, 1.0, "bf16")
 
 
+def test_more_tiles_than_one_side_of_a_grid(gpu):
+    """2^24 + 7 tokens that take a tile each: 2^32 threads and more, 17 GB of output over rows of x one element apart"""
+    import torch
+    n, heads, dim, freqs = 2 ** 24 + 7, 2, 257, np.ones(1, np.float32)
+    x = O.fill_normal((n + heads * dim,), 6, "x")
+    flat = torch.from_numpy(x).cuda()
+    out = torch.empty((n, heads, dim), dtype=torch.bfloat16, device="cuda")
+    picked = np.array([0, 1, 2 ** 23 - 1, 2 ** 23, 2 ** 23 + 1, 2 ** 24 - 1, 2 ** 24, 2 ** 24 + 6])
+    out[picked] = float("nan")
+    say("rotary", n, heads, dim)
+    gpu.rotary(flat.bfloat16().as_strided((n, heads, dim), (1, dim, 1)), out, dev_f32(freqs), start=5)
+    rows = rounded(x, "bf16")[picked[:, None] + np.arange(heads * dim)].reshape(len(picked), heads, dim)
+    _check(host(out[torch.from_numpy(picked).cuda()]), rows, 5 + picked, freqs, False, 1.0, "bf16")
+
+
 @pytest.mark.parametrize("position", [0, 1, 131071, 2 ** 24 + 1, 2 ** 31, 2 ** 32 - 1])
 def test_far_positions(gpu, position):
     """float64 holds the angle of position 2^32 to 2^-53 2^32 radians, within TURN_STEPS"""
