@@ -622,8 +622,8 @@ AIGPU_ABI int aigpu_paged_append(const AiGpuPagedAppend* args);
    lengths[b] - 1 on load. fp32 throughout but for the cache's bf16: q and the
    softmax's weights enter the products in three bf16 terms each. A sequence of
    length 0 gets zeros; one whose length exceeds maxLength, or that needs a page
-   outside the pool, gets NaN. Attended rows have to be finite (a value that is
-   not makes the heads that read it NaN); rows that no position covers may hold
+   outside the pool, gets NaN. Attended rows have to be finite (one that is not
+   makes the heads that read it NaN or infinite); rows that no position covers may hold
    anything. */
 typedef struct AiGpuPagedDecode {
     AiGpuPagedCache cache;

@@ -315,10 +315,6 @@ __device__ __forceinline__ int fresh_lane(int x) {
     asm volatile("" : "+v"(x));
     return x;
 }
-__device__ __forceinline__ uint32_t fresh_uniform(uint32_t x) {
-    asm volatile("" : "+s"(x));
-    return x;
-}
 
 /* the eight rows of 32 bytes that 32 lanes read transposed lie in distinct
    banks (64 of 4 bytes): block x of 16 bytes of row r sits at x ^ this */
