@@ -15,6 +15,15 @@ namespace {
 constexpr uint32_t THREADS = 256;
 constexpr uint32_t NOWHERE = 0xFFFFFFFFu;
 
+/* x, hidden from the compiler: what is derived from it is formed where it is
+   used. Unrolled loops would otherwise hold every address and mask of their
+   rare parts in registers: a hundred of the decode's, spilled, and twenty of
+   append's, which cost it two of its six workgroups a CU. */
+__device__ __forceinline__ int fresh_lane(int x) {
+    asm volatile("" : "+v"(x));
+    return x;
+}
+
 /*
     Appending. A workgroup takes a few tokens; D / 8 lanes take a row of k or v, 8
     elements each, up to PASSES rows a lane. Their loads go out first. Meanwhile
@@ -23,9 +32,10 @@ constexpr uint32_t NOWHERE = 0xFFFFFFFFu;
     and its page, and the workgroup the tokens' cosines and sines, once for all kv
     heads. Then k's rows are normed and turned, and all rows rounded and stored.
     Rows are read once and written once, 16 bytes a lane, which HBM would bound;
-    what does is a workgroup's chain of starts, lengths, table and angles beside
-    the four workgroups that a CU's registers hold: 8199 bf16 tokens of 8 heads of
-    128 (67 MB) take 18.2 us, 3.7 TB/s; 32 tokens 4.1 us.
+    what does is a workgroup's chain of starts, lengths, table and angles, of
+    which as many run at once as a CU's registers hold (74 a thread: six; at 106,
+    four, it took 19.2 us): 8199 bf16 tokens of 8 heads of 128 (67 MB) take 17.2
+    us, 3.9 TB/s; 32 tokens 4.0 us.
 */
 constexpr int PASSES = 4;
 constexpr uint32_t MAX_TOKENS = 16;
@@ -56,6 +66,7 @@ __global__ __launch_bounds__(THREADS) void paged_append_kernel(AppendArgs a) {
     constexpr int NW = THREADS / WAVE, DEEP = NW * RPW, RAW = BF ? 1 : 2;
     extern __shared__ __attribute__((aligned(16))) float2 turns[];   // [tokens][rot / 2]
     __shared__ __attribute__((aligned(16))) float rows[NW][RPW][D];
+    __shared__ __attribute__((aligned(16))) float gammas[D];
     __shared__ uint64_t base[MAX_TOKENS];            // of kv head 0, ~0: not written
     __shared__ uint32_t place[MAX_TOKENS];
     const PagedAppendParams& p = a.p;
@@ -96,11 +107,7 @@ __global__ __launch_bounds__(THREADS) void paged_append_kernel(AppendArgs a) {
         }
     };
     load(r0);
-    float gamma[8];
-    if (p.gamma) {
-#pragma unroll
-        for (int e = 0; e < 8; ++e) gamma[e] = sub < RPW ? p.gamma[d0 + e] + p.offset : 0.0f;
-    }
+    if (p.gamma && threadIdx.x < D) gammas[threadIdx.x] = p.gamma[threadIdx.x] + p.offset;
 
     // ---- each token's sequence, position and page: a wave takes every NW-th,
     //      lane l < MINE its l-th; the page id is on its way during the angles ----
@@ -154,6 +161,7 @@ __global__ __launch_bounds__(THREADS) void paged_append_kernel(AppendArgs a) {
         if (first != r0) load(first);
 #pragma unroll
         for (int k = 0; k < PASSES; ++k) {
+            const int d0 = fresh_lane((lane % LPR) * 8);
             const uint32_t r = first + k * DEEP;
             if (wave + k * DEEP >= total) break;     // no row of this wave's is left
             const bool in = which[k] != NOWHERE, isKey = r < keys;
@@ -174,8 +182,10 @@ __global__ __launch_bounds__(THREADS) void paged_append_kernel(AppendArgs a) {
                     for (int e = 0; e < 8; ++e) ss += x[e] * x[e];
                     const float inv = 1.0f / sqrtf(row_sum<LPR>(ss, lane) / float(D) + p.eps);
                     if (live && isKey) {
+                        const floatx4 ga = *reinterpret_cast<const floatx4*>(gammas + d0);
+                        const floatx4 gb = *reinterpret_cast<const floatx4*>(gammas + d0 + 4);
 #pragma unroll
-                        for (int e = 0; e < 8; ++e) x[e] = x[e] * inv * gamma[e];
+                        for (int e = 0; e < 8; ++e) x[e] = x[e] * inv * (e < 4 ? ga[e] : gb[e - 4]);
                     }
                 }
                 if (half && p.interleaved) {
@@ -196,8 +206,8 @@ __global__ __launch_bounds__(THREADS) void paged_append_kernel(AppendArgs a) {
                         *reinterpret_cast<floatx4*>(row + d0 + 4) = floatx4{x[4], x[5], x[6], x[7]};
                     }
                     wave_sync();
-                    if (live && isKey && uint32_t(d0) < 2 * half) {
-                        if (half % 8 == 0) {         // all eight partners in one lane
+                    if (half % 8 == 0) {             // all eight partners in one lane
+                        if (live && isKey && uint32_t(d0) < 2 * half) {
                             const bool late = uint32_t(d0) >= half;
                             const uint32_t o = late ? d0 - half : d0 + half;
                             const floatx4* cs = reinterpret_cast<const floatx4*>(turns + t * half + (late ? o : d0));
@@ -211,16 +221,21 @@ __global__ __launch_bounds__(THREADS) void paged_append_kernel(AppendArgs a) {
                                 x[4 * i + 2] = x[4 * i + 2] * c1[0] + sign * y[2] * c1[1];
                                 x[4 * i + 3] = x[4 * i + 3] * c1[2] + sign * y[3] * c1[3];
                             }
-                        } else {
-#pragma unroll
-                            for (int e = 0; e < 8; ++e) {
-                                const uint32_t d = d0 + e;
-                                if (d >= 2 * half) break;
-                                const bool late = d >= half;
-                                const uint32_t o = late ? d - half : d + half;
-                                const float2 cs = turns[t * half + (late ? o : d)];
-                                x[e] = x[e] * cs.x + (late ? row[o] : -row[o]) * cs.y;
+                        }
+                    } else {                         // the row's pairs, dealt to its lanes
+                        if (live && isKey) {
+#pragma unroll 1
+                            for (uint32_t j = d0 / 8; j < half; j += LPR) {
+                                const float2 cs = turns[t * half + j];
+                                const float u = row[j], v = row[j + half];
+                                row[j] = u * cs.x - v * cs.y;
+                                row[j + half] = v * cs.x + u * cs.y;
                             }
+                        }
+                        wave_sync();
+                        if (live && isKey) {
+#pragma unroll
+                            for (int e = 0; e < 8; ++e) x[e] = row[d0 + e];
                         }
                     }
                     wave_sync();
@@ -308,13 +323,6 @@ __device__ __forceinline__ void wait_loads() {
 
 __device__ __forceinline__ uint32_t uniform(uint32_t x) { return __builtin_amdgcn_readfirstlane(x); }
 
-/* x, hidden from the compiler: what is derived from it is formed where it is
-   used. The pipeline's loop would otherwise hold every address and mask of its
-   rare parts in registers (a hundred of them, spilled). */
-__device__ __forceinline__ int fresh_lane(int x) {
-    asm volatile("" : "+v"(x));
-    return x;
-}
 
 /* the eight rows of 32 bytes that 32 lanes read transposed lie in distinct
    banks (64 of 4 bytes): block x of 16 bytes of row r sits at x ^ this */

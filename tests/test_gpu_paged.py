@@ -233,7 +233,9 @@ def test_decode_offsets_past_32_bits(gpu):
                           (96, 1, "bf16", 96, False, True), (192, 3, "f32", 64, False, True),
                           (256, 2, "bf16", 256, True, True), (128, 8, "f32", 14, False, False),
                           (64, 33, "bf16", 0, False, True), (128, 1, "bf16", 0, False, False),
-                          (96, 2, "f32", 10, True, True)])
+                          (96, 2, "f32", 10, True, True),
+                          (96, 2, "bf16", 12, False, True), (192, 1, "f32", 190, False, False),
+                          (256, 2, "bf16", 250, False, True)])
 @pytest.mark.parametrize("kind", ["head", "position"])
 @pytest.mark.parametrize("new", [None, [3, 0, 40, 1, 17, 0]])
 def test_append(gpu, dim, kv, dtype, rot, interleaved, norm, kind, new):
