@@ -34,8 +34,8 @@ __device__ __forceinline__ int fresh_lane(int x) {
     Rows are read once and written once, 16 bytes a lane, which HBM would bound;
     what does is a workgroup's chain of starts, lengths, table and angles, of
     which as many run at once as a CU's registers hold (74 a thread: six; at 106,
-    four, it took 19.2 us): 8199 bf16 tokens of 8 heads of 128 (67 MB) take 17.2
-    us, 3.9 TB/s; 32 tokens 4.0 us.
+    four, 19.2 us in place of 17.2 there): 8199 bf16 tokens of 8 heads of 128 (67
+    MB) take 16.5 us, 4.1 TB/s; 32 tokens 4.1 us.
 */
 constexpr int PASSES = 4;
 constexpr uint32_t MAX_TOKENS = 16;
@@ -246,7 +246,7 @@ __global__ __launch_bounds__(THREADS) void paged_append_kernel(AppendArgs a) {
                 }
             }
             // nontemporal: who reads the pages next is rarely on this XCD, whose L2
-            // they would fill (33 MB of prompts: 21.8 us stored plainly, 20.4 so)
+            // they would fill (33 MB of prompts: 18.9 us stored plainly, 17.2 so)
             if (live)
                 __builtin_nontemporal_store(
                     bits, reinterpret_cast<u32x4*>((isKey ? c.keys : c.values) + to + h * c.headStride + d0));
