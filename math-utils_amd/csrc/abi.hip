@@ -238,7 +238,8 @@ hipStream_t as_stream(void* s) { return static_cast<hipStream_t>(s); }
    the event recorded after the previous call's launches, and this call's own
    launches are followed by the event in turn. A stream being captured into a
    graph is left alone (the caller orders captured work); so is the case of
-   one stream, where stream order already holds. */
+   one stream, where stream order already holds. The per-thread default stream
+   is another stream in every thread, under one handle: it always waits. */
 struct StreamOrder {
     Context& ctx;
     hipStream_t stream;
@@ -253,7 +254,8 @@ struct StreamOrder {
             active = false;
             return;
         }
-        if (ctx.handoffValid && ctx.handoffStream != s && hipStreamWaitEvent(s, ctx.handoff, 0) != hipSuccess)
+        if (ctx.handoffValid && (ctx.handoffStream != s || s == hipStreamPerThread) &&
+            hipStreamWaitEvent(s, ctx.handoff, 0) != hipSuccess)
             (void)hipGetLastError();
     }
     ~StreamOrder() {

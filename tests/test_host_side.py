@@ -1,0 +1,88 @@
+"""The host side of the paged entries without a GPU: what they allocate, free,
+order and launch, read from the log of a HIP runtime that does nothing else
+(fake_hip.cpp). Each test runs in a process of its own that loads that runtime
+ahead of the backend and never imports torch."""
+import os
+import subprocess
+import sys
+import textwrap
+
+import pytest
+
+import aigpu
+
+HERE = os.path.dirname(os.path.abspath(__file__))
+PACKAGE = os.path.dirname(os.path.dirname(os.path.abspath(aigpu.__file__)))
+ROCM = os.environ.get("ROCM_PATH", "/opt/rocm")
+
+PRELUDE = """
+import ctypes as C, sys, threading
+sys.modules["torch"] = None
+fake = C.CDLL({fake!r}, mode=C.RTLD_GLOBAL)
+fake.fake_log.restype = C.c_char_p
+sys.path.insert(0, {package!r})
+import aigpu
+assert aigpu.available(), aigpu.last_error()
+PTR, PER_THREAD = 1 << 20, 2
+
+def log():
+    return fake.fake_log().decode().splitlines()
+
+def names(lines):
+    return [line.split()[0] for line in lines]
+
+def decode(batch=1, heads=16, kv=8, dim=128, length=4096, stream=0, gate=0, ok=1):
+    cache = aigpu.AiGpuPagedCache(keys=PTR, values=PTR, table=PTR, lengths=PTR, batch=batch, pages=1 << 20, pageSize=16,
+                                  kvHeads=kv, dim=dim, tableWidth=1 << 16)
+    args = aigpu.AiGpuPagedDecode(cache=cache, q=PTR, out=1 << 28, maxLength=length, heads=heads, outputGate=gate,
+                                  stream=stream)
+    got = aigpu.lib().aigpu_paged_decode(C.byref(args))
+    assert got == ok, aigpu.last_error()
+
+log()
+"""
+
+
+@pytest.fixture(scope="module")
+def fake(tmp_path_factory):
+    path = str(tmp_path_factory.mktemp("fake") / "libfake_hip.so")
+    subprocess.run(["g++", "-std=c++17", "-O1", "-w", "-shared", "-fPIC", "-D__HIP_PLATFORM_AMD__",
+                    f"-I{ROCM}/include", os.path.join(HERE, "fake_hip.cpp"), "-o", path], check=True)
+    return path
+
+
+def _run(fake, body):
+    code = PRELUDE.format(fake=fake, package=PACKAGE) + textwrap.dedent(body)
+    r = subprocess.run([sys.executable, "-c", code], capture_output=True, text=True, timeout=120)
+    assert r.returncode == 0, r.stdout + r.stderr
+
+
+def test_one_launch_one_scratch_a_stream(fake):
+    """the log itself: a stream's first call allocates and clears, the next one only launches"""
+    _run(fake, """
+        decode(stream=64)
+        first = log()
+        assert names(first) == ["hipMalloc", "hipMemset", "hipDeviceSynchronize", "launch"], first
+        assert "paged_attention_kernel" in first[-1] and first[-1].split()[1] == "64"
+        decode(stream=64)
+        assert names(log()) == ["launch"]
+    """)
+
+
+def test_calls_on_the_per_thread_stream_are_ordered(fake):
+    """its handle names another stream in every thread, so equal handles say nothing: each call waits for the one
+    before it, from whichever thread that came, and is recorded for the next"""
+    _run(fake, """
+        for _ in range(3):
+            t = threading.Thread(target=lambda: decode(stream=PER_THREAD))
+            t.start()
+            t.join()
+        calls = [n for n in names(log()) if n in ("wait", "launch", "record")]
+        assert calls == ["launch", "record", "wait", "launch", "record", "wait", "launch", "record"], calls
+        # streams of one meaning wait where the handle changes only
+        for s in range(64, 73):
+            decode(stream=s)
+        log()
+        decode(stream=72)
+        assert names(log()) == ["launch", "record"]
+    """)
