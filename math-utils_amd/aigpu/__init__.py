@@ -1078,8 +1078,8 @@ def _paged_decode(q, out, key_pages, value_pages, table, lengths, max_length, q_
                   rotary_dims, interleaved, amplitude, scale, window, output_gate, workspace, stream):
     cache = _paged_cache(key_pages, value_pages, table, lengths)
     of_q, to, batch, dim = _at(q, "q"), _at(out, "out"), cache[4], cache[8]
-    if q.dim() != 3 or q.shape[0] != batch or q.shape[2] < dim:
-        raise ValueError("q must be [batch][heads][at least dim]")
+    if q.dim() != 3 or q.shape[0] != batch or q.shape[2] < (2 * dim if output_gate else dim):
+        raise ValueError("q must be [batch][heads][at least dim, 2 dim with output_gate]")
     heads = q.shape[1]
     if _kind(out) != F32 or tuple(out.shape) != (batch, heads, dim) or not out.is_contiguous():
         raise ValueError("out must be a contiguous float32 [batch][heads][dim]")
