@@ -125,11 +125,19 @@ Context::~Context() {
     // process teardown: the runtime reclaims device memory itself
 }
 
+bool Context::idle() {
+    const hipError_t e = hipDeviceSynchronize();
+    if (e == hipSuccess) return true;
+    (void)hipGetLastError();
+    return fail(std::string("a scratch in use cannot be replaced by a larger one: ") + hipGetErrorString(e));
+}
+
 void* Context::grow(ScratchSlot slot, size_t bytes) {
     if (bytes == 0) bytes = 256;
     if (scratchBytes[slot] >= bytes) return scratch[slot];
     if (scratch[slot]) {
-        (void)hipDeviceSynchronize();   // the old buffer may still be in use by queued work
+        // the old buffer may still be in use by queued work
+        if (!idle()) return nullptr;
         (void)hipFree(scratch[slot]);
         allocated -= scratchBytes[slot];
         scratch[slot] = nullptr;
@@ -175,7 +183,7 @@ bool Context::scratchOf(hipStream_t stream, size_t bytes, void** at) {
         own = &streamScratches.back();
     }
     if (own->at) {
-        (void)hipDeviceSynchronize();   // queued work may still use the smaller one
+        if (!idle()) return false;      // queued work may still use the smaller one
         (void)hipFree(own->at);
         allocated -= own->bytes;
         own->at = nullptr;

@@ -91,6 +91,9 @@ struct Context {
 
     static Context& instance();
 
+    // waits for all queued work; false (and error set) where that is refused,
+    // as while another thread captures: nothing may be freed then
+    bool idle();
     // a scratch slot of at least `bytes`; nullptr (and error set) on failure
     void* grow(ScratchSlot slot, size_t bytes);
     // the same, zero-filled whenever it is (re)allocated; kernels that use it

@@ -86,3 +86,27 @@ def test_calls_on_the_per_thread_stream_are_ordered(fake):
         decode(stream=72)
         assert names(log()) == ["launch", "record"]
     """)
+
+
+def test_scratch_in_use_is_kept_when_the_wait_for_it_is_refused(fake):
+    """a scratch too small for a call is freed only after the work that may use it has been waited for: where that
+    is refused (another thread captures), the call fails, the scratch stays, and a later call grows it"""
+    _run(fake, """
+        for own in (True, False):       # a stream's own scratch, and the one that later streams share
+            stream = 64 if own else 99
+            if not own:
+                for s in range(65, 74):
+                    decode(stream=s)
+            decode(stream=stream)
+            log()
+            fake.fake_fail(b"hipDeviceSynchronize", 1)
+            decode(stream=stream, dim=256, batch=64, ok=0)
+            assert "scratch" in aigpu.last_error(), aigpu.last_error()
+            lines = log()
+            assert "hipFree" not in names(lines) and "launch" not in names(lines), lines
+            decode(stream=stream)       # with what it has
+            assert "hipMalloc" not in names(log())
+            decode(stream=stream, dim=256, batch=64)
+            lines = names(log())
+            assert lines.index("hipDeviceSynchronize") < lines.index("hipFree") < lines.index("launch"), lines
+    """)
