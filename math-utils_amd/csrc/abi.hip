@@ -1269,11 +1269,12 @@ AIGPU_ABI int aigpu_paged_decode(const AiGpuPagedDecode* args) {
         return ctx.fail("paged decode: a captured call needs a workspace of its own (" + std::to_string(need) +
                         " bytes)"),
                0;
+    const size_t room = aigpu::paged_decode_scratch(p);
     void* work = nullptr;
-    if (!ctx.scratchOf(stream, need, &work)) return 0;
+    if (!ctx.scratchOf(stream, room, &work)) return 0;
     if (work) return aigpu::launch_paged_decode(p, work, stream) ? 1 : 0;
     const StreamOrder order(ctx, stream);
-    work = ctx.growZeroed(aigpu::SLOT_PAGED, need);
+    work = ctx.growZeroed(aigpu::SLOT_PAGED, room);
     return work && aigpu::launch_paged_decode(p, work, stream) ? 1 : 0;
 }
 

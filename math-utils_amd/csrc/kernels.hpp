@@ -327,6 +327,10 @@ struct PagedDecodeParams {
 };
 bool check_paged_decode(const PagedDecodeParams& p);
 size_t paged_decode_workspace(const PagedDecodeParams& p);
+// what the calls of these heads and dim need at most, whatever their batch and
+// lengths: the backend's own scratch is of this size, as one that grew with a
+// conversation would be replaced, and the device waited for, every few tokens
+size_t paged_decode_scratch(const PagedDecodeParams& p);
 // work: paged_decode_workspace(p) bytes, or null where that is 0
 bool launch_paged_decode(const PagedDecodeParams& p, void* work, hipStream_t stream);
 

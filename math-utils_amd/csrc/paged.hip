@@ -1217,6 +1217,12 @@ struct DecodeShape {
     uint32_t grid;
 };
 
+/* the workgroups that the chip holds at once */
+uint32_t full_grid(uint32_t dim) {
+    const int cus = Context::instance().cus ? Context::instance().cus : 256;
+    return std::min(uint32_t(cus) * occupancy(int(dim)), MAX_RUNS / WAVES);
+}
+
 DecodeShape decode_shape(const PagedDecodeParams& p) {
     DecodeShape s{};
     const uint32_t G = p.heads / p.c.kvHeads;
@@ -1228,11 +1234,8 @@ DecodeShape decode_shape(const PagedDecodeParams& p) {
     uint64_t slice = p.c.batch < MAXB ? p.c.batch : MAXB;
     if (each && slice > most / each) slice = most / each;
     s.slice = uint32_t(slice);
-    const int cus = Context::instance().cus ? Context::instance().cus : 256;
-    uint64_t most_grid = uint64_t(cus) * occupancy(int(p.c.dim));
-    if (most_grid > MAX_RUNS / WAVES) most_grid = MAX_RUNS / WAVES;
-    const uint64_t want = (slice * each + WAVES - 1) / WAVES;
-    s.grid = uint32_t(want < most_grid ? (want ? want : 1) : most_grid);
+    const uint64_t want = (slice * each + WAVES - 1) / WAVES, fills = full_grid(p.c.dim);
+    s.grid = uint32_t(want < fills ? (want ? want : 1) : fills);
     return s;
 }
 
@@ -1250,6 +1253,9 @@ bool joins_in_kernel(const PagedDecodeParams& p, const DecodeShape& s, uint32_t 
 
 // workspace: a place for arrivals that no call's records overlap, the plan, the records
 constexpr size_t ARRIVED_BYTES = MAX_RUNS * 4, PLAN_BYTES = (MAXB + 1) * 4 + 252 & ~size_t(255);
+size_t workspace_of(uint32_t grid, uint32_t perGroup, uint32_t dim) {
+    return ARRIVED_BYTES + PLAN_BYTES + size_t(grid) * WAVES * 2 * record_floats(perGroup, dim) * sizeof(float);
+}
 
 } // namespace
 
@@ -1285,8 +1291,11 @@ bool check_paged_decode(const PagedDecodeParams& p) {
 size_t paged_decode_workspace(const PagedDecodeParams& p) {
     if (p.c.batch == 0) return 0;
     const DecodeShape s = decode_shape(p);
-    return ARRIVED_BYTES + PLAN_BYTES +
-           size_t(s.grid) * WAVES * 2 * record_floats(s.perGroup, p.c.dim) * sizeof(float);
+    return workspace_of(s.grid, s.perGroup, p.c.dim);
+}
+
+size_t paged_decode_scratch(const PagedDecodeParams& p) {
+    return workspace_of(full_grid(p.c.dim), decode_shape(p).perGroup, p.c.dim);
 }
 
 bool launch_paged_decode(const PagedDecodeParams& p, void* work, hipStream_t stream) {

@@ -100,13 +100,48 @@ def test_scratch_in_use_is_kept_when_the_wait_for_it_is_refused(fake):
             decode(stream=stream)
             log()
             fake.fake_fail(b"hipDeviceSynchronize", 1)
-            decode(stream=stream, dim=256, batch=64, ok=0)
+            decode(stream=stream, kv=1, dim=256, ok=0)
             assert "scratch" in aigpu.last_error(), aigpu.last_error()
             lines = log()
             assert "hipFree" not in names(lines) and "launch" not in names(lines), lines
             decode(stream=stream)       # with what it has
             assert "hipMalloc" not in names(log())
-            decode(stream=stream, dim=256, batch=64)
+            decode(stream=stream, kv=1, dim=256)
             lines = names(log())
             assert lines.index("hipDeviceSynchronize") < lines.index("hipFree") < lines.index("launch"), lines
+    """)
+
+
+@pytest.mark.parametrize("heads,kv,dim,batch", [(16, 8, 128, 1), (32, 4, 128, 1), (16, 1, 256, 3), (12, 12, 64, 2)])
+def test_a_growing_conversation_allocates_once(fake, heads, kv, dim, batch):
+    """max_length follows the longest sequence, step by step: only the first call allocates or waits for the device,
+    on a stream with a scratch of its own and on those that share one"""
+    _run(fake, f"""
+        def steps(stream):
+            first = log()
+            for length in range(1, 20000, 7):
+                decode(heads={heads}, kv={kv}, dim={dim}, batch={batch}, length=length, stream=stream)
+                if length == 1:
+                    first = names(log())
+            assert first.count("hipMalloc") == 1, first
+            rest = set(names(log()))
+            assert rest <= {{"launch", "record"}}, rest
+
+        steps(64)
+        for s in range(65, 72):
+            decode(heads={heads}, kv={kv}, dim={dim}, stream=s)
+        log()
+        steps(99)
+    """)
+
+
+def test_one_scratch_serves_every_batch_of_a_model(fake):
+    """other batches, lengths and windows of the same heads and dim fit the first call's scratch"""
+    _run(fake, """
+        decode(batch=1, length=1)
+        log()
+        for batch in (1, 2, 7, 31, 200, 1000):
+            for length in (1, 31, 33, 700, 9000, 131072):
+                decode(batch=batch, length=length)
+        assert set(names(log())) == {"launch"}
     """)
