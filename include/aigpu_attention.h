@@ -522,10 +522,11 @@ AIGPU_ABI int aigpu_select_keys(const AiGpuSelectKeys* args);
 /*      (u, w) -> amplitude (u cos a - w sin a, w cos a + u sin a)           */
 /*    and elements from rotaryDims on copied. transpose = 1 turns by -a (the */
 /*    amplitude still multiplies): the gradient of x from the gradient of    */
-/*    out. The angle is formed in 64 bits, so far positions keep their       */
-/*    fp32-exact cosine (the reference, and the entries above, round it to   */
-/*    fp32 first: 3e-3 radians at position 100000); the rotation itself is   */
-/*    fp32, rounded once to `type`. out may be x (same strides); other       */
+/*    out. The angle is formed and reduced in 64 bits (the reference, and    */
+/*    the entries above, round it to fp32 first: 3e-3 radians at position    */
+/*    100000), and its cosine and sine are within 3 units of fp32's last     */
+/*    place, small ones too; the amplitude and the rotation round in fp32,   */
+/*    the result once to `type`. out may be x (same strides); other          */
 /*    overlaps are refused. Asynchronous; needs no scratch, so calls on      */
 /*    different streams are not ordered by the backend.                      */
 /* ------------------------------------------------------------------------ */

@@ -118,10 +118,18 @@ __device__ __forceinline__ void norm_rope_row(float* x, int dim, const float* ga
 
 /* cos and sin of pos * freq radians. The product and its reduction to a turn
    are in 64 bits (in fp32 the angle of position 100000 is already 3e-3 radians
-   off), the functions in fp32 of the remaining half turn. */
+   off), the functions in fp32 of the remaining half turns as a sum of two
+   terms: what the first leaves out, up to 9e-8 radians, turns their result by
+   its first order (the second is below 1e-14), so that a small cosine or sine
+   keeps its bits too. Left: the functions' own rounding and one addition's. */
 __device__ __forceinline__ void rotation_at(uint32_t pos, float freq, float& cs, float& sn) {
     const double turns = double(pos) * double(freq) * 0.15915494309189535;   // 1 / (2 pi)
-    sincospif(2.0f * float(turns - rint(turns)), &sn, &cs);
+    const double halves = 2.0 * (turns - rint(turns));
+    const float first = float(halves), rest = float(halves - double(first)) * 3.14159265f;
+    float s, c;
+    sincospif(first, &s, &c);
+    cs = fmaf(-s, rest, c);
+    sn = fmaf(c, rest, s);
 }
 
 /* fp16 of a finite fp32 value, noting in `bad` when it does not fit fp16's
