@@ -12,7 +12,9 @@
 // are turned and stored. 8192 tokens of 32 bf16 heads of 128 (134 MB): 23.7 us,
 // 5.7 TB/s, where a plain copy of as much takes 24; 1999 tokens of 40 fp32 heads
 // of 192 (123 MB): 22.7 us, 5.4 TB/s; one token: 2.1 us, the launch.
+#include <algorithm>
 #include <cmath>
+#include <cstdlib>
 
 #include "context.hpp"
 #include "device.hpp"
@@ -211,6 +213,22 @@ bool in_place(const RotaryParams& p) {
            (p.heads == 1 || p.headStride == p.outHeadStride);
 }
 
+/* whether a row of x and one of out share an element, where out has x's strides and starts `apart` elements on */
+bool rows_meet(const RotaryParams& p, int64_t apart) {
+    const int64_t dim = int64_t(p.dim), ts = int64_t(p.tokenStride), mostT = int64_t(p.count) - 1,
+                  mostH = int64_t(p.heads) - 1;
+    for (int64_t dh = -mostH; dh <= mostH; ++dh) {
+        const int64_t from = apart + dh * int64_t(p.headStride);    // between rows of one token
+        // the token distance that brings them nearest, from either side
+        const int64_t near = mostT ? -from / ts : 0;
+        for (int64_t dt : {near - 1, near, near + 1}) {
+            dt = std::max(-mostT, std::min(mostT, dt));
+            if (std::abs(from + dt * ts) < dim) return true;
+        }
+    }
+    return false;
+}
+
 } // namespace
 
 bool check_rotary(const RotaryParams& p) {
@@ -242,7 +260,10 @@ bool check_rotary(const RotaryParams& p) {
         const uint64_t row = p.tokenStride * es;
         const uint64_t xr = ((p.heads - 1) * p.headStride + p.dim) * es, orow = ((p.heads - 1) * ohs + p.dim) * es;
         const uint64_t gap = row ? (ob >= xb ? (ob - xb) % row : (row - (xb - ob) % row) % row) : 0;
-        if (p.tokenStride != ots || !row || gap < xr || row - gap < orow)
+        const bool sideBySide = p.tokenStride == ots && row && gap >= xr && row - gap >= orow;
+        // nor do equal lattices of rows that lie between one another (the halves of wider heads)
+        const bool equal = (p.count == 1 || p.tokenStride == ots) && (p.heads == 1 || p.headStride == ohs);
+        if (!sideBySide && (!equal || rows_meet(p, (int64_t(ob) - int64_t(xb)) / int64_t(es))))
             return ctx.fail("rotary: out overlaps x without being x");
     }
 
