@@ -350,7 +350,8 @@ bool rotary_frequencies(const AiGpuRotaryScaling& s, float* out, float* amplitud
         };
         first = std::fmax(std::floor(pair_of(s.high)), 0.0);
         last = std::fmin(std::ceil(pair_of(s.low)), s.dims - 1.0);
-        if (!(last - first >= 0.001)) last = first + 0.001;
+        // no pair between: those from `last` on (all, where none makes `low` turns) are divided
+        if (!(last - first >= 0.001)) first = last - 1.0;
     }
     for (uint32_t j = 0; j < n; ++j) {
         double f = std::pow(base, -2.0 * j / s.dims);
