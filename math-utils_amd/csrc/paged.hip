@@ -801,8 +801,8 @@ __global__ __launch_bounds__(THREADS, occupancy(D)) void paged_attention_kernel(
                 wave_sync();
 #pragma unroll 8
                 for (uint32_t j = g; j < half; j += 4) {      // the row's pairs, a quarter a lane
-                    float* u = row + ((p.interleaved ? 2 * j : j) ^ sw);
-                    float* v = row + ((p.interleaved ? 2 * j + 1 : j + half) ^ sw);
+                    float* u = row + (j ^ sw);
+                    float* v = row + ((j + half) ^ sw);
                     const float2 cs = turns[w][j];
                     const float xu = *u, xv = *v;
                     *u = xu * cs.x - xv * cs.y;
