@@ -524,11 +524,11 @@ AIGPU_ABI int aigpu_select_keys(const AiGpuSelectKeys* args);
 /*    amplitude still multiplies): the gradient of x from the gradient of    */
 /*    out. The angle is formed and reduced in 64 bits (the reference, and    */
 /*    the entries above, round it to fp32 first: 3e-3 radians at position    */
-/*    100000), and its cosine and sine are within 3 units of fp32's last     */
-/*    place, small ones too; the amplitude and the rotation round in fp32,   */
-/*    the result once to `type`. out may be x (same strides); other          */
-/*    overlaps are refused. Asynchronous; needs no scratch, so calls on      */
-/*    different streams are not ordered by the backend.                      */
+/*    100000), good to 2^-51 of itself, and its cosine and sine, small ones  */
+/*    too, to 3 units of fp32's last place; the amplitude and the rotation   */
+/*    round in fp32, the result once to `type`. out may be x (same strides)  */
+/*    or share no element with it. Asynchronous; needs no scratch, so calls  */
+/*    on different streams are not ordered by the backend.                   */
 /* ------------------------------------------------------------------------ */
 typedef struct AiGpuRotary {
     const void* x;            /* element (token, head, d) at token*tokenStride + head*headStride + d, type */
@@ -599,10 +599,10 @@ typedef struct AiGpuPagedCache {
    or from starts[batch] on are left out. A token whose position is negative
    (a length below its new tokens), beyond the table or in a page outside the
    pool is not written; a decode over such a length answers NaN. No two
-   tokens may share a row: a page shared by sequences is copied before either
-   writes to it, and strides that let rows of the pool overlap are refused
-   (a decode reads such a pool). Asynchronous; needs no scratch, so calls on different streams
-   are not ordered by the backend. */
+   tokens may share a row, nor a key one with a value: a page shared by
+   sequences is copied before either writes to it, and strides that let rows of
+   the pool overlap are refused (a decode reads such a pool). Asynchronous; needs
+   no scratch, so calls on different streams are not ordered by the backend. */
 typedef struct AiGpuPagedAppend {
     AiGpuPagedCache cache;
     const void* k;            /* [count][kvHeads][dim], inType; token t at t*kStride */
@@ -650,11 +650,12 @@ AIGPU_ABI int aigpu_paged_decode(const AiGpuPagedDecode* args);
    (as aigpu_allocate leaves it); every call leaves the part that matters zero
    again, so calls of any sizes may follow one another in it, but calls that may
    run at once need one each. A call captured into a graph has to bring one
-   where this is not 0: the backend's scratch may move. That scratch is a
-   stream's own for the first eight streams that decode, so their calls are not
-   ordered among one another (destroy such a stream only when its decodes have
-   ended: its scratch goes with the handle); the calls of later streams share
-   one, in turn. */
+   where this is not 0: the backend's scratch may move. That scratch, of one
+   size for calls of the same heads and dim (34 MB at most), is a stream's own
+   for the first eight streams that decode, so their calls are not ordered among
+   one another (destroy such a stream only when its decodes have ended: its
+   scratch goes with the handle); the calls of later streams, and of the
+   per-thread default stream, share one, in turn. */
 AIGPU_ABI uint64_t aigpu_paged_decode_workspace(const AiGpuPagedDecode* args);
 
 /* ------------------------------------------------------------------------ */

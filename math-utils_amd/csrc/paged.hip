@@ -34,8 +34,8 @@ __device__ __forceinline__ int fresh_lane(int x) {
     Rows are read once and written once, 16 bytes a lane, which HBM would bound;
     what does is a workgroup's chain of starts, lengths, table and angles, of
     which as many run at once as a CU's registers hold (74 a thread: six; at 106,
-    four, 19.2 us in place of 17.2 there): 8199 bf16 tokens of 8 heads of 128 (67
-    MB) take 16.5 us, 4.1 TB/s; 32 tokens 4.1 us.
+    four, 12% slower): 8199 bf16 tokens of 8 heads of 128 (67 MB) take 16.8 us,
+    4.0 TB/s; 32 tokens 4.1 us.
 */
 constexpr int PASSES = 4;
 constexpr uint32_t MAX_TOKENS = 16;
@@ -246,7 +246,7 @@ __global__ __launch_bounds__(THREADS) void paged_append_kernel(AppendArgs a) {
                 }
             }
             // nontemporal: who reads the pages next is rarely on this XCD, whose L2
-            // they would fill (33 MB of prompts: 18.9 us stored plainly, 17.2 so)
+            // they would fill (8199 tokens stored plainly take 10% longer)
             if (live)
                 __builtin_nontemporal_store(
                     bits, reinterpret_cast<u32x4*>((isKey ? c.keys : c.values) + to + h * c.headStride + d0));
@@ -278,11 +278,11 @@ __global__ __launch_bounds__(THREADS) void paged_append_kernel(AppendArgs a) {
     (max, sum, weighted values) records, two a wave at most, that are joined in
     their order, so results do not depend on timing: by the workgroup that finds
     itself the last of the pair's (a counter that it sets back to zero), or, where
-    a pair's records are more than one workgroup should read, by
-    paged_merge_kernel.
+    sequences of one length would leave a pair more records than one workgroup
+    should read, by paged_merge_kernel.
 
-    32 sequences of 1k to 32k under 32/4 heads of 128 (1.11 GB): 190 us, 5.8 TB/s
-    of the 6.1 that a large copy reaches. Small calls are a chain of about 15 us:
+    32 sequences of 1k to 32k under 32/4 heads of 128 (1.11 GB): 190 us, 5.8 TB/s,
+    where a copy of 256 or 512 MB moves 5.9. Small calls are a chain of about 15 us:
     dispatch, lengths and list 4, page ids and queries 2, a first slab 3, its
     weights 1, the joins 5 (one sequence of 4096 under 16/8 heads, 16.8 MB: 15).
 */
@@ -1244,7 +1244,11 @@ DecodeShape decode_shape(const PagedDecodeParams& p) {
 // 8 x 4 heads of 128) joining within takes 113 us in all, the second launch 109;
 // at 33 KB (4096 positions, 8 x 2 heads) both 16; with few records of many pairs
 // (256 sequences of 1 to 700, 4 KB) 78 against 92, most of whose workgroups find
-// nothing to join.
+// nothing to join. The host does not know the lengths, so the records are counted
+// as if all places held as many positions. One long sequence among short or empty
+// places leaves more than that, which one workgroup then reads alone: 131072
+// positions under 16/1 heads of 256 take 197 us among 127 empty places and 44 by
+// themselves, under 32/4 heads of 128 among 15 places 73 and 59.
 constexpr uint64_t JOIN_BYTES = 64 << 10;
 bool joins_in_kernel(const PagedDecodeParams& p, const DecodeShape& s, uint32_t batch) {
     const uint64_t parts = s.grid / (uint64_t(batch) * p.c.kvHeads * s.groups) + 1;

@@ -11,7 +11,7 @@
 // about 100 instructions, as many as rotating 15 heads' pairs), then the rows
 // are turned and stored. 8192 tokens of 32 bf16 heads of 128 (134 MB): 23.7 us,
 // 5.7 TB/s, where a plain copy of as much takes 24; 1999 tokens of 40 fp32 heads
-// of 192 (123 MB): 22.7 us, 5.4 TB/s; one token: 2.1 us, the launch.
+// of 192 (123 MB): 23.1 us, 5.3 TB/s; one token: 2.2 us, the launch.
 #include <algorithm>
 #include <cmath>
 #include <cstdlib>
