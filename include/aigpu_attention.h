@@ -654,8 +654,9 @@ AIGPU_ABI int aigpu_paged_decode(const AiGpuPagedDecode* args);
    size for calls of the same heads and dim (34 MB at most), is a stream's own
    for the first eight streams that decode, so their calls are not ordered among
    one another (destroy such a stream only when its decodes have ended: its
-   scratch goes with the handle); the calls of later streams, and of the
-   per-thread default stream, share one, in turn. */
+   scratch goes with the handle); the calls of later streams share one, in turn,
+   and so do those of the per-thread default stream, which return when their
+   work is done. */
 AIGPU_ABI uint64_t aigpu_paged_decode_workspace(const AiGpuPagedDecode* args);
 
 /* ------------------------------------------------------------------------ */

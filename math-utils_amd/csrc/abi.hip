@@ -247,7 +247,9 @@ hipStream_t as_stream(void* s) { return static_cast<hipStream_t>(s); }
    launches are followed by the event in turn. A stream being captured into a
    graph is left alone (the caller orders captured work); so is the case of
    one stream, where stream order already holds. The per-thread default stream
-   is another stream in every thread, under one handle: it always waits. */
+   is another stream in every thread, under one handle, and goes with its thread
+   and whatever was recorded on it: its calls wait on the host, for the call
+   before them and then for their own work, and leave nothing to wait for. */
 struct StreamOrder {
     Context& ctx;
     hipStream_t stream;
@@ -262,12 +264,18 @@ struct StreamOrder {
             active = false;
             return;
         }
-        if (ctx.handoffValid && (ctx.handoffStream != s || s == hipStreamPerThread) &&
-            hipStreamWaitEvent(s, ctx.handoff, 0) != hipSuccess)
-            (void)hipGetLastError();
+        if (!ctx.handoffValid || (ctx.handoffStream == s && s != hipStreamPerThread)) return;
+        const hipError_t e =
+            s == hipStreamPerThread ? hipEventSynchronize(ctx.handoff) : hipStreamWaitEvent(s, ctx.handoff, 0);
+        if (e != hipSuccess) (void)hipGetLastError();
     }
     ~StreamOrder() {
         if (!active) return;
+        if (stream == hipStreamPerThread) {
+            ctx.handoffValid = false;
+            if (hipStreamSynchronize(stream) == hipSuccess) return;
+            (void)hipGetLastError();
+        }
         if (hipEventRecord(ctx.handoff, stream) == hipSuccess) {
             ctx.handoffStream = stream;
             ctx.handoffValid = true;

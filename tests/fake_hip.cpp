@@ -88,4 +88,6 @@ FAKE hipError_t hipStreamIsCapturing(hipStream_t, hipStreamCaptureStatus* s) {
 FAKE hipError_t hipEventCreate(hipEvent_t* e) { *e = nullptr; return hipSuccess; }
 FAKE hipError_t hipEventCreateWithFlags(hipEvent_t* e, unsigned) { *e = nullptr; return hipSuccess; }
 FAKE hipError_t hipEventRecord(hipEvent_t, hipStream_t s) { return called("record", text(s)); }
+FAKE hipError_t hipEventSynchronize(hipEvent_t) { return called("finish"); }
+FAKE hipError_t hipStreamSynchronize(hipStream_t s) { return called("finish", text(s)); }
 FAKE hipError_t hipStreamWaitEvent(hipStream_t s, hipEvent_t, unsigned) { return called("wait", text(s)); }

@@ -181,11 +181,11 @@ def test_many_streams_of_either_join(gpu, join):
 
 @pytest.mark.parametrize("join", JOINS)
 def test_threads_on_their_per_thread_streams(gpu, join):
-    """one handle, a stream in each thread, one scratch between them"""
+    """one handle, a stream in each thread that goes with it, one scratch between them"""
     import torch
     per_thread = 2
     cases = [_case(gpu, lengths, 180 + i, join) for i, lengths in enumerate(([5000, 300], [4000, 9, 2000]))]
-    outs = [[torch.full_like(c["out"], 7.0) for _ in range(20)] for c in cases]
+    outs = [[torch.full_like(c["out"], 7.0) for _ in range(100)] for c in cases]
     torch.cuda.synchronize()
     failures = []
 
@@ -196,11 +196,12 @@ def test_threads_on_their_per_thread_streams(gpu, join):
         except Exception as e:
             failures.append(e)
 
-    threads = [threading.Thread(target=work, args=pair) for pair in zip(cases, outs)]
-    for t in threads:
-        t.start()
-    for t in threads:
-        t.join()
+    for at in range(0, 100, 10):     # threads that end with their last call's work just queued
+        threads = [threading.Thread(target=work, args=(c, row[at:at + 10])) for c, row in zip(cases, outs)]
+        for t in threads:
+            t.start()
+        for t in threads:
+            t.join()
     torch.cuda.synchronize()
     assert not failures
     for c, row in zip(cases, outs):

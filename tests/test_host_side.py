@@ -70,20 +70,33 @@ def test_one_launch_one_scratch_a_stream(fake):
 
 
 def test_calls_on_the_per_thread_stream_are_ordered(fake):
-    """its handle names another stream in every thread, so equal handles say nothing: each call waits for the one
-    before it, from whichever thread that came, and is recorded for the next"""
+    """its handle names another stream in every thread, and the stream goes with its thread: a call waits for the one
+    before it, and for its own work, on the host, so that none of it is left when the next one takes the scratch"""
     _run(fake, """
         for _ in range(3):
             t = threading.Thread(target=lambda: decode(stream=PER_THREAD))
             t.start()
             t.join()
-        calls = [n for n in names(log()) if n in ("wait", "launch", "record")]
-        assert calls == ["launch", "record", "wait", "launch", "record", "wait", "launch", "record"], calls
-        # streams of one meaning wait where the handle changes only
-        for s in range(64, 73):
+        calls = [n for n in log() if n.split()[0] in ("wait", "launch", "record", "finish")]
+        assert names(calls) == ["launch", "finish"] * 3 and calls[1::2] == [f"finish {PER_THREAD}"] * 3, calls
+        # behind a call of another stream, and one of another stream behind it
+        for s in range(128, 137):
             decode(stream=s)
         log()
-        decode(stream=72)
+        decode(stream=PER_THREAD)
+        decode(stream=136)
+        calls = [" ".join(n.split()[:2]) for n in log()]
+        assert calls == ["finish", "launch 2", "finish 2", "launch 136", "record 136"], calls
+        # where its wait is refused the event is left, for whichever call comes next
+        fake.fake_fail(b"finish", 2)
+        decode(stream=PER_THREAD)
+        log()
+        decode(stream=PER_THREAD)
+        decode(stream=136)
+        calls = [" ".join(n.split()[:2]) for n in log()]
+        assert calls == ["finish", "launch 2", "finish 2", "launch 136", "record 136"], calls
+        # streams of one meaning wait where the handle changes only
+        decode(stream=136)
         assert names(log()) == ["launch", "record"]
     """)
 
