@@ -254,6 +254,7 @@ struct StreamOrder {
     Context& ctx;
     hipStream_t stream;
     bool active = true;
+    bool waited = true;              // nothing before this call is left to wait for
     StreamOrder(Context& c, hipStream_t s) : ctx(c), stream(s) {
         hipStreamCaptureStatus capture = hipStreamCaptureStatusNone;
         if (hipStreamIsCapturing(s, &capture) != hipSuccess) {
@@ -267,13 +268,16 @@ struct StreamOrder {
         if (!ctx.handoffValid || (ctx.handoffStream == s && s != hipStreamPerThread)) return;
         const hipError_t e =
             s == hipStreamPerThread ? hipEventSynchronize(ctx.handoff) : hipStreamWaitEvent(s, ctx.handoff, 0);
-        if (e != hipSuccess) (void)hipGetLastError();
+        waited = e == hipSuccess;
+        if (!waited) (void)hipGetLastError();
     }
     ~StreamOrder() {
         if (!active) return;
         if (stream == hipStreamPerThread) {
-            ctx.handoffValid = false;
-            if (hipStreamSynchronize(stream) == hipSuccess) return;
+            if (hipStreamSynchronize(stream) == hipSuccess) {
+                if (waited) ctx.handoffValid = false;
+                return;
+            }
             (void)hipGetLastError();
         }
         if (hipEventRecord(ctx.handoff, stream) == hipSuccess) {

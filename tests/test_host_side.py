@@ -98,6 +98,12 @@ def test_calls_on_the_per_thread_stream_are_ordered(fake):
         # streams of one meaning wait where the handle changes only
         decode(stream=136)
         assert names(log()) == ["launch", "record"]
+        # where the wait for the call before is refused, that call is still to be waited for
+        fake.fake_fail(b"finish", 1)
+        decode(stream=PER_THREAD)
+        log()
+        decode(stream=135)
+        assert [" ".join(n.split()[:2]) for n in log()] == ["wait 135", "launch 135", "record 135"]
     """)
 
 
