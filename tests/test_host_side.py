@@ -102,8 +102,8 @@ def test_calls_on_the_per_thread_stream_are_ordered(fake):
         fake.fake_fail(b"finish", 1)
         decode(stream=PER_THREAD)
         log()
-        decode(stream=135)
-        assert [" ".join(n.split()[:2]) for n in log()] == ["wait 135", "launch 135", "record 135"]
+        decode(stream=137)
+        assert [" ".join(n.split()[:2]) for n in log()] == ["wait 137", "launch 137", "record 137"]
     """)
 
 
