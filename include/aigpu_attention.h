@@ -659,6 +659,100 @@ AIGPU_ABI int aigpu_paged_decode(const AiGpuPagedDecode* args);
    work is done. */
 AIGPU_ABI uint64_t aigpu_paged_decode_workspace(const AiGpuPagedDecode* args);
 
+/* aigpu_paged_decode with its scores capped or biased: with s the scaled product of a
+   query of head h and the key `apart` positions before it,
+     cap > 0   s = cap tanh(s / cap)
+     slopes    s -= slopes[h] apart      (after the cap)
+   before the softmax; cap 0 and slopes NULL leave them out. The workspace is
+   aigpu_paged_decode_workspace's. */
+typedef struct AiGpuScores {
+    const float* slopes;      /* [heads] or NULL */
+    float cap;                /* finite, not negative */
+    uint32_t reserved;
+} AiGpuScores;
+AIGPU_ABI int aigpu_paged_decode_scored(const AiGpuPagedDecode* args, const AiGpuScores* scores);
+
+/* ------------------------------------------------------------------------ */
+/* 13. A paged cache held in 4 bits: the tables, lengths and rules of 12, a   */
+/*    row being dim codes of 4 bits and a scale for every 32 of them, at      */
+/*      row r = page*pageStride + head*headStride + row*rowStride             */
+/*    (strides in rows) of the codes [r][dim / 2] bytes, element d in byte    */
+/*    d / 2, the even one in the low half, and of the scales [r][dim / 32]    */
+/*    fp16. An element's value is scale * (code - 8). An append makes the     */
+/*    scale s of a block the least fp16 number of at most 8 significant bits  */
+/*    with 7 s >= its largest magnitude, at most 2720, and a code             */
+/*    floor(x / s + 1/2) + 8 within 1 .. 15: an element is off by s / 2 at    */
+/*    most, or, past 7 * 2720 = 19040, becomes that. A block with an element  */
+/*    that is not finite reads as NaN. Keys are normed and rotated in 64      */
+/*    bits, so that their codes are those of the exact rows. The scales of a  */
+/*    cache of other origin may be any fp16 numbers of at most 8 significant  */
+/*    bits up to 2720, and its codes 0 .. 15: then every value is exact in    */
+/*    fp16, which the decode's products take.                                 */
+/* ------------------------------------------------------------------------ */
+typedef struct AiGpuPagedCacheQ4 {
+    void* keyCodes;           /* 16-byte aligned, as the other three */
+    void* valueCodes;
+    void* keyScales;
+    void* valueScales;
+    const uint32_t* table;    /* [batch][tableStride], the first tableWidth of each row */
+    const uint32_t* lengths;  /* [batch] */
+    uint64_t batch, pages, pageSize, kvHeads, dim;  /* dim 64, 96, 128, 192 or 256 */
+    uint64_t tableWidth, tableStride;               /* tableStride 0 means tableWidth */
+    uint64_t pageStride, headStride, rowStride;     /* in rows; all 0: [pages][kvHeads][pageSize] */
+} AiGpuPagedCacheQ4;
+
+/* as AiGpuPagedAppend, into 4-bit pages */
+typedef struct AiGpuPagedAppendQ4 {
+    AiGpuPagedCacheQ4 cache;
+    const void* k;
+    const void* v;
+    const uint32_t* starts;
+    const float* kNorm;
+    const float* rotaryFrequencies;
+    float epsilon, normOffset, amplitude;
+    uint32_t rotaryDims, interleaved, inType;
+    uint64_t count, kStride, vStride;
+    void* stream;
+} AiGpuPagedAppendQ4;
+AIGPU_ABI int aigpu_paged_append_q4(const AiGpuPagedAppendQ4* args);
+
+/* The rows of the newest tokens (which ones, `starts` says as an append's) read back:
+   the values that their codes stand for, rounded once to outType. Rows of k and v
+   before starts[0] or from starts[batch] on stay as they were; a token without a
+   place in the pool reads as NaN. With the lengths summed up as starts this is every
+   sequence whole, as aigpu_packed_attention takes the keys of a chunk's documents.
+   Asynchronous, without scratch. */
+typedef struct AiGpuPagedReadQ4 {
+    AiGpuPagedCacheQ4 cache;
+    void* k;                  /* [count][kvHeads][dim], outType; token t at t*kStride */
+    void* v;                  /* the same at t*vStride */
+    const uint32_t* starts;   /* [batch + 1], not decreasing, or NULL: one token a sequence */
+    uint32_t outType, reserved;
+    uint64_t count, kStride, vStride; /* strides 0 mean kvHeads*dim */
+    void* stream;
+} AiGpuPagedReadQ4;
+AIGPU_ABI int aigpu_paged_read_q4(const AiGpuPagedReadQ4* args);
+
+/* As aigpu_paged_decode_scored, over 4-bit pages: fp32 throughout, the products taking
+   q and the weights in two fp16 terms each (22 bits) and the pages' values exactly. */
+typedef struct AiGpuPagedDecodeQ4 {
+    AiGpuPagedCacheQ4 cache;
+    const void* q;
+    float* out;
+    const float* qNorm;
+    const float* rotaryFrequencies;
+    const float* slopes;      /* as AiGpuScores */
+    float epsilon, normOffset, amplitude, scale, cap;
+    uint32_t rotaryDims, interleaved, inType, outputGate, maxLength;
+    uint64_t heads, qStride, qTokenStride;
+    uint64_t window;
+    void* workspace;
+    uint64_t workspaceBytes;
+    void* stream;
+} AiGpuPagedDecodeQ4;
+AIGPU_ABI int aigpu_paged_decode_q4(const AiGpuPagedDecodeQ4* args);
+AIGPU_ABI uint64_t aigpu_paged_decode_q4_workspace(const AiGpuPagedDecodeQ4* args);
+
 /* ------------------------------------------------------------------------ */
 /* Per-kernel timing. With profiling on, every launch is bracketed by a pair */
 /* of hipEvents on the stream it runs on; aigpu_profile_read synchronises    */

@@ -846,7 +846,38 @@ class AiGpuPagedDecode(C.Structure):
                 ("workspace", _vp), ("workspaceBytes", _u64), ("stream", _vp)]
 
 
+class AiGpuScores(C.Structure):
+    _fields_ = [("slopes", _vp), ("cap", _f32), ("reserved", _u32)]
+
+
+class AiGpuPagedCacheQ4(C.Structure):
+    _fields_ = [("keyCodes", _vp), ("valueCodes", _vp), ("keyScales", _vp), ("valueScales", _vp)] + \
+        AiGpuPagedCache._fields_[2:]
+
+
+class AiGpuPagedAppendQ4(C.Structure):
+    _fields_ = [("cache", AiGpuPagedCacheQ4)] + AiGpuPagedAppend._fields_[1:]
+
+
+class AiGpuPagedReadQ4(C.Structure):
+    _fields_ = [("cache", AiGpuPagedCacheQ4), ("k", _vp), ("v", _vp), ("starts", _vp), ("outType", _u32),
+                ("reserved", _u32), ("count", _u64), ("kStride", _u64), ("vStride", _u64), ("stream", _vp)]
+
+
+class AiGpuPagedDecodeQ4(C.Structure):
+    _fields_ = [("cache", AiGpuPagedCacheQ4), ("q", _vp), ("out", _vp), ("qNorm", _vp), ("rotaryFrequencies", _vp),
+                ("slopes", _vp), ("epsilon", _f32), ("normOffset", _f32), ("amplitude", _f32), ("scale", _f32),
+                ("cap", _f32), ("rotaryDims", _u32), ("interleaved", _u32), ("inType", _u32), ("outputGate", _u32),
+                ("maxLength", _u32), ("heads", _u64), ("qStride", _u64), ("qTokenStride", _u64), ("window", _u64),
+                ("workspace", _vp), ("workspaceBytes", _u64), ("stream", _vp)]
+
+
 SIGNATURES.update({
+    "aigpu_paged_decode_scored": (C.c_int, [C.POINTER(AiGpuPagedDecode), C.POINTER(AiGpuScores)]),
+    "aigpu_paged_append_q4": (C.c_int, [C.POINTER(AiGpuPagedAppendQ4)]),
+    "aigpu_paged_read_q4": (C.c_int, [C.POINTER(AiGpuPagedReadQ4)]),
+    "aigpu_paged_decode_q4": (C.c_int, [C.POINTER(AiGpuPagedDecodeQ4)]),
+    "aigpu_paged_decode_q4_workspace": (_u64, [C.POINTER(AiGpuPagedDecodeQ4)]),
     "aigpu_rotary": (C.c_int, [C.POINTER(AiGpuRotary)]),
     "aigpu_rotary_frequencies": (C.c_int, [C.POINTER(AiGpuRotaryScaling), _vp, C.POINTER(_f32)]),
     "aigpu_paged_append": (C.c_int, [C.POINTER(AiGpuPagedAppend)]),
@@ -874,7 +905,11 @@ def rotary_frequencies(rotary_dims, theta, scaling=None, factor=1.0, original=0.
 _CACHE = "4P10Q"
 _PACK = {"aigpu_rotary": _struct.Struct("4Pf5I8QP"),
          "aigpu_paged_append": _struct.Struct(_CACHE + "5P3f3I3QP"),
-         "aigpu_paged_decode": _struct.Struct(_CACHE + "4P4f6I4QPQP")}
+         "aigpu_paged_decode": _struct.Struct(_CACHE + "4P4f6I4QPQP"),
+         "aigpu_paged_append_q4": _struct.Struct("2P" + _CACHE + "5P3f3I3QP"),
+         "aigpu_paged_read_q4": _struct.Struct("2P" + _CACHE + "3P2I3QP"),
+         "aigpu_paged_decode_q4": _struct.Struct("2P" + _CACHE + "5P5f5I4QPQP"),
+         "scores": _struct.Struct("PfI")}
 _entries = {}
 _torch = None
 
@@ -894,7 +929,7 @@ def _entry(name):
     fn = _entries.get(name)
     if fn is None:
         fn = lib()[name]         # a function object of its own beside the one that SIGNATURES declares
-        fn.restype, fn.argtypes = C.c_int, [C.c_char_p]
+        fn.restype, fn.argtypes = C.c_int, [C.c_char_p] * len(SIGNATURES[name][1])
         _entries[name] = fn
     return fn
 
@@ -1044,6 +1079,38 @@ def _paged_cache(keys, values, table, lengths):
             dim, width, step, ps if pages > 1 else dim, hs if kv_heads > 1 else dim, rs if size > 1 else dim)
 
 
+def _token_rows(k, v, cache, at, starts):
+    """(k, v, starts, tokens, kStride, vStride) as the entries take them; cache[at] is the batch; no tokens: None"""
+    of_k, of_v, batch, kv_heads, dim = _at(k, "k"), _at(v, "v"), cache[at], cache[at + 3], cache[at + 4]
+    shape = k.shape
+    if len(shape) != 3 or shape[1] != kv_heads or shape[2] != dim or v.shape != shape or v.dtype != k.dtype:
+        raise ValueError("k and v must be [tokens][kv_heads][dim] of one type, as the pages have them")
+    begins = 0 if starts is None else _indices(starts, "starts", 1, batch + 1)
+    if shape[0] == 0:
+        return None
+    (ks, kh, k1), (vs, vh, v1) = k.stride(), v.stride()
+    if k1 != 1 or v1 != 1 or (kv_heads > 1 and (kh != dim or vh != dim)):
+        raise ValueError("the heads of a token's k and v must lie one after the other")
+    if shape[0] == 1:                # any stride stands for one token
+        ks = vs = kv_heads * dim
+    if ks <= 0 or vs <= 0:
+        raise ValueError("k and v must not be broadcast views")
+    return of_k, of_v, begins, shape[0], ks, vs
+
+
+def _append(entry, cache, at, k, v, starts, k_norm, eps, norm_offset, freqs, rotary_dims, interleaved, amplitude,
+            stream):
+    rows = _token_rows(k, v, cache, at, starts)
+    rot = 0 if freqs is None else (2 * freqs.shape[0] if rotary_dims is None else rotary_dims)
+    turns, gamma = _vector(freqs, "freqs", rot // 2), _vector(k_norm, "k_norm", cache[at + 4], True)
+    if rows is None:
+        return
+    of_k, of_v, begins, count, ks, vs = rows
+    args = _packed(entry, *cache, of_k, of_v, begins, gamma, turns, eps, norm_offset, amplitude, rot,
+                   1 if interleaved else 0, _kind(k), count, ks, vs, _own_stream(stream))
+    _check(_entry(entry)(args))
+
+
 def paged_append(k, v, key_pages, value_pages, table, lengths, starts=None, k_norm=None, eps=1e-6, norm_offset=0.0,
                  freqs=None, rotary_dims=None, interleaved=False, amplitude=1.0, stream=None):
     """The newest tokens' k (normed, rotated) and v [tokens][kv_heads][dim]
@@ -1053,31 +1120,14 @@ def paged_append(k, v, key_pages, value_pages, table, lengths, starts=None, k_no
     included) say; starts [batch + 1] where a sequence has other than one.
     Asynchronous."""
     cache = _paged_cache(key_pages, value_pages, table, lengths)
-    of_k, of_v, batch, kv_heads, dim = _at(k, "k"), _at(v, "v"), cache[4], cache[7], cache[8]
-    shape = k.shape
-    if len(shape) != 3 or shape[1] != kv_heads or shape[2] != dim or v.shape != shape or v.dtype != k.dtype:
-        raise ValueError("k and v must be [tokens][kv_heads][dim] of one type, as the pages have them")
-    begins = 0 if starts is None else _indices(starts, "starts", 1, batch + 1)
-    rot = 0 if freqs is None else (2 * freqs.shape[0] if rotary_dims is None else rotary_dims)
-    turns, gamma = _vector(freqs, "freqs", rot // 2), _vector(k_norm, "k_norm", dim, True)
-    if shape[0] == 0:
-        return
-    (ks, kh, k1), (vs, vh, v1) = k.stride(), v.stride()
-    if k1 != 1 or v1 != 1 or (kv_heads > 1 and (kh != dim or vh != dim)):
-        raise ValueError("the heads of a token's k and v must lie one after the other")
-    if shape[0] == 1:                # any stride stands for one token
-        ks = vs = kv_heads * dim
-    if ks <= 0 or vs <= 0:
-        raise ValueError("k and v must not be broadcast views")
-    args = _packed("aigpu_paged_append", *cache, of_k, of_v, begins, gamma, turns, eps, norm_offset, amplitude, rot,
-                   1 if interleaved else 0, _kind(k), shape[0], ks, vs, _own_stream(stream))
-    _check(_entry("aigpu_paged_append")(args))
+    _append("aigpu_paged_append", cache, 4, k, v, starts, k_norm, eps, norm_offset, freqs, rotary_dims, interleaved,
+            amplitude, stream)
 
 
-def _paged_decode(q, out, key_pages, value_pages, table, lengths, max_length, q_norm, eps, norm_offset, freqs,
-                  rotary_dims, interleaved, amplitude, scale, window, output_gate, workspace, stream):
-    cache = _paged_cache(key_pages, value_pages, table, lengths)
-    of_q, to, batch, dim = _at(q, "q"), _at(out, "out"), cache[4], cache[8]
+def _decode_args(entry, cache, at, q, out, max_length, q_norm, eps, norm_offset, freqs, rotary_dims, interleaved,
+                 amplitude, scale, window, output_gate, workspace, stream, scores=None):
+    """a decode's structure; scores: (slopes, cap) where the structure has them"""
+    of_q, to, batch, dim = _at(q, "q"), _at(out, "out"), cache[at], cache[at + 4]
     if q.dim() != 3 or q.shape[0] != batch or q.shape[2] < (2 * dim if output_gate else dim):
         raise ValueError("q must be [batch][heads][at least dim, 2 dim with output_gate]")
     heads = q.shape[1]
@@ -1091,26 +1141,36 @@ def _paged_decode(q, out, key_pages, value_pages, table, lengths, max_length, q_
             raise ValueError("workspace must be contiguous")
         room, nbytes = _at(workspace, "workspace"), workspace.numel() * workspace.element_size()
     if max_length is None:
-        max_length = min(cache[9] * cache[6], 1 << 31)
-    return _packed("aigpu_paged_decode", *cache, of_q, to, _vector(q_norm, "q_norm", dim, True),
-                   _vector(freqs, "freqs", rot // 2), eps, norm_offset, amplitude, scale, rot,
-                   1 if interleaved else 0, _kind(q), 1 if output_gate else 0, max_length, 0, heads, hs, ts, window,
-                   room, nbytes, _own_stream(stream))
+        max_length = min(cache[at + 5] * cache[at + 2], 1 << 31)
+    gamma, turns = _vector(q_norm, "q_norm", dim, True), _vector(freqs, "freqs", rot // 2)
+    tail = (heads, hs, ts, window, room, nbytes, _own_stream(stream))
+    flags = (rot, 1 if interleaved else 0, _kind(q), 1 if output_gate else 0, max_length)
+    if scores is None:
+        return _packed(entry, *cache, of_q, to, gamma, turns, eps, norm_offset, amplitude, scale, *flags, 0, *tail)
+    return _packed(entry, *cache, of_q, to, gamma, turns, _vector(scores[0], "slopes", heads, True), eps, norm_offset,
+                   amplitude, scale, scores[1], *flags, *tail)
 
 
 def paged_decode(q, out, key_pages, value_pages, table, lengths, max_length=None, q_norm=None, eps=1e-6,
                  norm_offset=0.0, freqs=None, rotary_dims=None, interleaved=False, amplitude=1.0, scale=0.0, window=0,
-                 output_gate=False, workspace=None, stream=None):
+                 output_gate=False, workspace=None, stream=None, cap=0.0, slopes=None):
     """Attention of each sequence's newest token over its cached positions:
     q [batch][heads][dim] (fp32 or bf16; 2 dim wide with output_gate), normed
     and rotated at lengths[b] - 1 on load; out [batch][heads][dim] fp32; the
     pages, table and lengths as paged_append left them. max_length (default:
-    what the table can hold) is at least every length. A call captured into a
-    graph brings a workspace (paged_decode_workspace), its own where calls may
-    run at once. Asynchronous."""
-    args = _paged_decode(q, out, key_pages, value_pages, table, lengths, max_length, q_norm, eps, norm_offset, freqs,
-                         rotary_dims, interleaved, amplitude, scale, window, output_gate, workspace, stream)
-    if q.shape[0]:
+    what the table can hold) is at least every length. cap > 0 caps the scores
+    (cap tanh(s / cap)), then slopes [heads] take slope times the distance from
+    them. A call captured into a graph brings a workspace
+    (paged_decode_workspace), its own where calls may run at once.
+    Asynchronous."""
+    cache = _paged_cache(key_pages, value_pages, table, lengths)
+    args = _decode_args("aigpu_paged_decode", cache, 4, q, out, max_length, q_norm, eps, norm_offset, freqs,
+                        rotary_dims, interleaved, amplitude, scale, window, output_gate, workspace, stream)
+    if cap or slopes is not None:
+        scores = _packed("scores", _vector(slopes, "slopes", q.shape[1], True), cap, 0)
+        if q.shape[0]:
+            _check(_entry("aigpu_paged_decode_scored")(args, scores))
+    elif q.shape[0]:
         _check(_entry("aigpu_paged_decode")(args))
     return out
 
@@ -1118,8 +1178,100 @@ def paged_decode(q, out, key_pages, value_pages, table, lengths, max_length=None
 def paged_decode_workspace(q, out, key_pages, value_pages, table, lengths, max_length=None):
     """a workspace (zero-filled uint8 tensor) for paged_decode calls of these
     sizes or smaller ones of the same heads and dim, whatever the lengths hold"""
-    args = _paged_decode(q, out, key_pages, value_pages, table, lengths, max_length, None, 1e-6, 0.0, None, None,
-                         False, 1.0, 0.0, 0, False, None, 0)
+    cache = _paged_cache(key_pages, value_pages, table, lengths)
+    args = _decode_args("aigpu_paged_decode", cache, 4, q, out, max_length, None, 1e-6, 0.0, None, None, False, 1.0,
+                        0.0, 0, False, None, 0)
     need = lib().aigpu_paged_decode_workspace(C.cast(C.c_char_p(args), C.POINTER(AiGpuPagedDecode)))
+    _check(need or q.shape[0] == 0)
+    return _torch.zeros(int(need), dtype=_torch.uint8, device=q.device)
+
+
+def _paged_cache_q4(key_codes, key_scales, value_codes, value_scales, table, lengths):
+    """AiGpuPagedCacheQ4's fields"""
+    _with_torch()
+    names = ("key_codes", "value_codes", "key_scales", "value_scales")
+    tensors = (key_codes, value_codes, key_scales, value_scales)
+    at = [_at(t, name) for t, name in zip(tensors, names)]
+    of_table, of_lengths = _indices(table, "table", 2), _indices(lengths, "lengths", 1)
+    if not lengths.is_contiguous():
+        raise TypeError("lengths must be a contiguous int32 vector")
+    if key_codes.dtype is not _torch.uint8 or value_codes.dtype is not _torch.uint8:
+        raise TypeError("the codes must be uint8")
+    if key_scales.dtype is not _torch.float16 or value_scales.dtype is not _torch.float16:
+        raise TypeError("the scales must be float16")
+    shape, blocks = tuple(key_codes.shape), tuple(key_scales.shape)
+    if len(shape) != 4 or tuple(value_codes.shape) != shape or tuple(value_scales.shape) != blocks \
+            or len(blocks) != 4 or blocks[:3] != shape[:3] or 16 * blocks[3] != shape[3]:
+        raise ValueError("codes must be [pages][kv_heads][page_size][dim / 2], "
+                         "scales [pages][kv_heads][page_size][dim / 32]")
+    pages, kv_heads, size, half = shape
+    steps = None
+    for t, row in ((key_codes, half), (value_codes, half), (key_scales, half // 16), (value_scales, half // 16)):
+        strides = t.stride()
+        if (strides[3] != 1 and row > 1) or any(s % row for s, n in zip(strides, shape[:3]) if n > 1):
+            raise ValueError("the rows of the pages must be dense")
+        # a dimension of one may carry any stride
+        own = tuple(s // row if n > 1 else 1 for s, n in zip(strides, shape[:3]))
+        if steps is not None and own != steps:
+            raise ValueError("codes and scales must have the same strides, counted in rows")
+        steps = own
+    batch, (rows, width) = lengths.shape[0], table.shape
+    if rows != batch:
+        raise ValueError(f"table has {rows} entries, {batch} are needed")
+    step = table.stride(0) if batch > 1 else width
+    if (step == 0 and width) or steps[2] == 0:       # 0 means the dense stride to the entries
+        raise ValueError("the table and the rows of the pages must not be broadcast views")
+    return (*at, of_table, of_lengths, batch, pages, size, kv_heads, 2 * half, width, step, *steps)
+
+
+def paged_append_q4(k, v, key_codes, key_scales, value_codes, value_scales, table, lengths, starts=None, k_norm=None,
+                    eps=1e-6, norm_offset=0.0, freqs=None, rotary_dims=None, interleaved=False, amplitude=1.0,
+                    stream=None):
+    """paged_append into pages of 4-bit codes: codes uint8
+    [pages][kv_heads][page_size][dim / 2] and scales float16
+    [pages][kv_heads][page_size][dim / 32] (or views whose strides agree,
+    counted in rows). Asynchronous."""
+    cache = _paged_cache_q4(key_codes, key_scales, value_codes, value_scales, table, lengths)
+    _append("aigpu_paged_append_q4", cache, 6, k, v, starts, k_norm, eps, norm_offset, freqs, rotary_dims,
+            interleaved, amplitude, stream)
+
+
+def paged_read_q4(k, v, key_codes, key_scales, value_codes, value_scales, table, lengths, starts=None, stream=None):
+    """The newest tokens' rows of 4-bit pages into k and v
+    [tokens][kv_heads][dim] (fp32 or bf16, any token stride): one a sequence, or
+    the last starts[b + 1] - starts[b] of sequence b (the lengths summed up:
+    every sequence whole). Asynchronous."""
+    cache = _paged_cache_q4(key_codes, key_scales, value_codes, value_scales, table, lengths)
+    rows = _token_rows(k, v, cache, 6, starts)
+    if rows is not None:
+        of_k, of_v, begins, count, ks, vs = rows
+        args = _packed("aigpu_paged_read_q4", *cache, of_k, of_v, begins, _kind(k), 0, count, ks, vs,
+                       _own_stream(stream))
+        _check(_entry("aigpu_paged_read_q4")(args))
+    return k, v
+
+
+def paged_decode_q4(q, out, key_codes, key_scales, value_codes, value_scales, table, lengths, max_length=None,
+                    q_norm=None, eps=1e-6, norm_offset=0.0, freqs=None, rotary_dims=None, interleaved=False,
+                    amplitude=1.0, scale=0.0, window=0, output_gate=False, workspace=None, stream=None, cap=0.0,
+                    slopes=None):
+    """paged_decode over pages of 4-bit codes as paged_append_q4 left them; a
+    captured call's workspace is paged_decode_q4_workspace's. Asynchronous."""
+    cache = _paged_cache_q4(key_codes, key_scales, value_codes, value_scales, table, lengths)
+    args = _decode_args("aigpu_paged_decode_q4", cache, 6, q, out, max_length, q_norm, eps, norm_offset, freqs,
+                        rotary_dims, interleaved, amplitude, scale, window, output_gate, workspace, stream,
+                        (slopes, cap))
+    if q.shape[0]:
+        _check(_entry("aigpu_paged_decode_q4")(args))
+    return out
+
+
+def paged_decode_q4_workspace(q, out, key_codes, key_scales, value_codes, value_scales, table, lengths,
+                              max_length=None):
+    """paged_decode_workspace for paged_decode_q4"""
+    cache = _paged_cache_q4(key_codes, key_scales, value_codes, value_scales, table, lengths)
+    args = _decode_args("aigpu_paged_decode_q4", cache, 6, q, out, max_length, None, 1e-6, 0.0, None, None, False,
+                        1.0, 0.0, 0, False, None, 0, (None, 0.0))
+    need = lib().aigpu_paged_decode_q4_workspace(C.cast(C.c_char_p(args), C.POINTER(AiGpuPagedDecodeQ4)))
     _check(need or q.shape[0] == 0)
     return _torch.zeros(int(need), dtype=_torch.uint8, device=q.device)

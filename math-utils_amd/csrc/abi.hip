@@ -1119,9 +1119,10 @@ bool usable(Context& ctx, const char* who) {
     return ctx.ok || ctx.fail(std::string(who) + ": no usable gfx950 device");
 }
 
-/* the cache as the kernels take it; sizes past these limits have no use and
-   would overflow the index arithmetic */
-bool paged_cache(Context& ctx, const char* who, const AiGpuPagedCache& a, aigpu::PagedCache& c) {
+/* the cache as the kernels take it, its strides in elements of which a row has `row`;
+   sizes past these limits have no use and would overflow the index arithmetic */
+template <typename Cache>
+bool paged_sizes(Context& ctx, const char* who, const Cache& a, uint64_t row, aigpu::PagedCache& c) {
     const std::string w = std::string(who) + ": ";
     if (a.batch > (1u << 20) || a.kvHeads > 65535 || a.dim > 4096 || a.pages > 0x7FFFFFFFu)
         return ctx.fail(w + "sizes out of range");
@@ -1134,16 +1135,14 @@ bool paged_cache(Context& ctx, const char* who, const AiGpuPagedCache& a, aigpu:
     c.headStride = a.headStride;
     c.rowStride = a.rowStride;
     if (a.pageStride == 0 && a.headStride == 0 && a.rowStride == 0) {
-        c.rowStride = a.dim;
-        c.headStride = a.pageSize * a.dim;
+        c.rowStride = row;
+        c.headStride = a.pageSize * row;
         c.pageStride = a.kvHeads * c.headStride;
     }
     // the last element of the pool within 2^62
     const uint64_t top = uint64_t(1) << 60;
     if (c.rowStride > top / a.pageSize || c.headStride > top / a.kvHeads || c.pageStride > top / a.pages)
         return ctx.fail(w + "page strides out of range");
-    c.keys = static_cast<uint16_t*>(a.keys);
-    c.values = static_cast<uint16_t*>(a.values);
     c.table = a.table;
     c.lengths = a.lengths;
     c.batch = uint32_t(a.batch);
@@ -1155,7 +1154,45 @@ bool paged_cache(Context& ctx, const char* who, const AiGpuPagedCache& a, aigpu:
     return true;
 }
 
-bool paged_decode_params(Context& ctx, const AiGpuPagedDecode* args, aigpu::PagedDecodeParams& p) {
+bool paged_cache(Context& ctx, const char* who, const AiGpuPagedCache& a, aigpu::PagedCache& c) {
+    c.keys = static_cast<uint16_t*>(a.keys);
+    c.values = static_cast<uint16_t*>(a.values);
+    return paged_sizes(ctx, who, a, a.dim, c);
+}
+
+bool paged_cache(Context& ctx, const char* who, const AiGpuPagedCacheQ4& a, aigpu::PagedCache& c) {
+    c.keys = static_cast<uint16_t*>(a.keyCodes);
+    c.values = static_cast<uint16_t*>(a.valueCodes);
+    if (!paged_sizes(ctx, who, a, 1, c)) return false;
+    if (c.rowStride == 0) return ctx.fail(std::string(who) + ": the rows of a page overlap");
+    return true;
+}
+
+template <typename Append>
+bool paged_append_params(Context& ctx, const Append* args, aigpu::PagedAppendParams& p) {
+    if (!paged_cache(ctx, "paged append", args->cache, p.c)) return false;
+    const uint64_t row = args->cache.kvHeads * args->cache.dim;
+    p.k = args->k;
+    p.v = args->v;
+    p.starts = args->starts;
+    p.gamma = args->kNorm;
+    p.freqs = args->rotaryFrequencies;
+    p.eps = args->epsilon;
+    p.offset = args->normOffset;
+    p.amplitude = args->amplitude == 0.0f ? 1.0f : args->amplitude;
+    p.rot = args->rotaryDims > 4096 ? -1 : int(args->rotaryDims);
+    p.interleaved = args->interleaved ? 1 : 0;
+    p.inType = args->inType > 1 ? -1 : int(args->inType);
+    p.count = args->count;
+    p.kStride = args->kStride ? args->kStride : row;
+    p.vStride = args->vStride ? args->vStride : row;
+    if (p.kStride >= (uint64_t(1) << 40) || p.vStride >= (uint64_t(1) << 40))
+        return ctx.fail("paged append: a stride of k or v is out of range");
+    return true;
+}
+
+template <typename Decode>
+bool paged_decode_params(Context& ctx, const Decode* args, aigpu::PagedDecodeParams& p) {
     if (!paged_cache(ctx, "paged decode", args->cache, p.c)) return false;
     if (args->heads > 65535) return ctx.fail("paged decode: heads out of range");
     p.q = args->q;
@@ -1177,7 +1214,70 @@ bool paged_decode_params(Context& ctx, const AiGpuPagedDecode* args, aigpu::Page
     if (p.qStride >= (uint64_t(1) << 40) || p.qTokenStride >= (uint64_t(1) << 40))
         return ctx.fail("paged decode: a stride of q is out of range");
     p.window = args->window;
+    return true;
+}
+
+bool decode_params(Context& ctx, const AiGpuPagedDecode* args, const AiGpuScores* scores, aigpu::PagedDecodeParams& p) {
+    if (!paged_decode_params(ctx, args, p)) return false;
+    if (scores) {
+        p.form = aigpu::PAGED_SCORED;
+        p.cap = scores->cap;
+        p.slopes = scores->slopes;
+    }
     return aigpu::check_paged_decode(p);
+}
+
+bool decode_params(Context& ctx, const AiGpuPagedDecodeQ4* args, const AiGpuScores*, aigpu::PagedDecodeParams& p) {
+    if (!paged_decode_params(ctx, args, p)) return false;
+    p.form = aigpu::PAGED_CODES;
+    p.cap = args->cap;
+    p.slopes = args->slopes;
+    p.keyScales = static_cast<const uint16_t*>(args->cache.keyScales);
+    p.valueScales = static_cast<const uint16_t*>(args->cache.valueScales);
+    return aigpu::check_paged_decode(p);
+}
+
+template <typename Decode>
+int paged_decode(const Decode* args, const AiGpuScores* scores) {
+    Context& ctx = Context::instance();
+    std::lock_guard<std::recursive_mutex> lock(ctx.gate);
+    if (!args) return ctx.fail("paged decode: null arguments"), 0;
+    aigpu::PagedDecodeParams p{};
+    if (!decode_params(ctx, args, scores, p)) return 0;
+    const size_t need = aigpu::paged_decode_workspace(p);
+    if (args->workspace) {
+        if (reinterpret_cast<uintptr_t>(args->workspace) & 255)
+            return ctx.fail("paged decode: the workspace must be 256-byte aligned"), 0;
+        if (args->workspaceBytes < need)
+            return ctx.fail("paged decode: the workspace holds " + std::to_string(args->workspaceBytes) +
+                            " bytes, the call needs " + std::to_string(need)),
+                   0;
+    }
+    if (!usable(ctx, "paged decode")) return 0;
+    const OnDevice device;
+    hipStream_t stream = as_stream(args->stream);
+    if (args->workspace) return aigpu::launch_paged_decode(p, args->workspace, stream) ? 1 : 0;
+    if (need == 0) return aigpu::launch_paged_decode(p, nullptr, stream) ? 1 : 0;
+    if (aigpu::capturing(stream))
+        return ctx.fail("paged decode: a captured call needs a workspace of its own (" + std::to_string(need) +
+                        " bytes)"),
+               0;
+    const size_t room = aigpu::paged_decode_scratch(p);
+    void* work = nullptr;
+    if (!ctx.scratchOf(stream, room, &work)) return 0;
+    if (work) return aigpu::launch_paged_decode(p, work, stream) ? 1 : 0;
+    const StreamOrder order(ctx, stream);
+    work = ctx.growZeroed(aigpu::SLOT_PAGED, room);
+    return work && aigpu::launch_paged_decode(p, work, stream) ? 1 : 0;
+}
+
+template <typename Decode>
+uint64_t paged_decode_bytes(const Decode* args) {
+    Context& ctx = Context::instance();
+    std::lock_guard<std::recursive_mutex> lock(ctx.gate);
+    if (!args) return ctx.fail("paged decode: null arguments"), 0;
+    aigpu::PagedDecodeParams p{};
+    return decode_params(ctx, args, nullptr, p) ? aigpu::paged_decode_workspace(p) : 0;
 }
 
 } // namespace
@@ -1226,68 +1326,60 @@ AIGPU_ABI int aigpu_paged_append(const AiGpuPagedAppend* args) {
     std::lock_guard<std::recursive_mutex> lock(ctx.gate);
     if (!args) return ctx.fail("paged append: null arguments"), 0;
     aigpu::PagedAppendParams p{};
-    if (!paged_cache(ctx, "paged append", args->cache, p.c)) return 0;
-    const uint64_t row = args->cache.kvHeads * args->cache.dim;
-    p.k = args->k;
-    p.v = args->v;
-    p.starts = args->starts;
-    p.gamma = args->kNorm;
-    p.freqs = args->rotaryFrequencies;
-    p.eps = args->epsilon;
-    p.offset = args->normOffset;
-    p.amplitude = args->amplitude == 0.0f ? 1.0f : args->amplitude;
-    p.rot = args->rotaryDims > 4096 ? -1 : int(args->rotaryDims);
-    p.interleaved = args->interleaved ? 1 : 0;
-    p.inType = args->inType > 1 ? -1 : int(args->inType);
-    p.count = args->count;
-    p.kStride = args->kStride ? args->kStride : row;
-    p.vStride = args->vStride ? args->vStride : row;
-    if (p.kStride >= (uint64_t(1) << 40) || p.vStride >= (uint64_t(1) << 40))
-        return ctx.fail("paged append: a stride of k or v is out of range"), 0;
-    if (!aigpu::check_paged_append(p) || !usable(ctx, "paged append")) return 0;
+    if (!paged_append_params(ctx, args, p) || !aigpu::check_paged_append(p) || !usable(ctx, "paged append")) return 0;
     const OnDevice device;
     return aigpu::launch_paged_append(p, as_stream(args->stream)) ? 1 : 0;
 }
 
-AIGPU_ABI uint64_t aigpu_paged_decode_workspace(const AiGpuPagedDecode* args) {
+AIGPU_ABI int aigpu_paged_append_q4(const AiGpuPagedAppendQ4* args) {
     Context& ctx = Context::instance();
     std::lock_guard<std::recursive_mutex> lock(ctx.gate);
-    if (!args) return ctx.fail("paged decode: null arguments"), 0;
-    aigpu::PagedDecodeParams p{};
-    return paged_decode_params(ctx, args, p) ? aigpu::paged_decode_workspace(p) : 0;
+    if (!args) return ctx.fail("paged append: null arguments"), 0;
+    aigpu::PagedAppendQ4Params p{};
+    if (!paged_append_params(ctx, args, p.a)) return 0;
+    p.keyScales = static_cast<uint16_t*>(args->cache.keyScales);
+    p.valueScales = static_cast<uint16_t*>(args->cache.valueScales);
+    if (!aigpu::check_paged_append_q4(p) || !usable(ctx, "paged append")) return 0;
+    const OnDevice device;
+    return aigpu::launch_paged_append_q4(p, as_stream(args->stream)) ? 1 : 0;
 }
 
-AIGPU_ABI int aigpu_paged_decode(const AiGpuPagedDecode* args) {
+AIGPU_ABI int aigpu_paged_read_q4(const AiGpuPagedReadQ4* args) {
     Context& ctx = Context::instance();
     std::lock_guard<std::recursive_mutex> lock(ctx.gate);
-    if (!args) return ctx.fail("paged decode: null arguments"), 0;
-    aigpu::PagedDecodeParams p{};
-    if (!paged_decode_params(ctx, args, p)) return 0;
-    const size_t need = aigpu::paged_decode_workspace(p);
-    if (args->workspace) {
-        if (reinterpret_cast<uintptr_t>(args->workspace) & 255)
-            return ctx.fail("paged decode: the workspace must be 256-byte aligned"), 0;
-        if (args->workspaceBytes < need)
-            return ctx.fail("paged decode: the workspace holds " + std::to_string(args->workspaceBytes) +
-                            " bytes, the call needs " + std::to_string(need)),
-                   0;
-    }
-    if (!usable(ctx, "paged decode")) return 0;
+    if (!args) return ctx.fail("paged read: null arguments"), 0;
+    aigpu::PagedReadQ4Params p{};
+    if (!paged_cache(ctx, "paged read", args->cache, p.c)) return 0;
+    const uint64_t row = args->cache.kvHeads * args->cache.dim;
+    p.keyScales = static_cast<const uint16_t*>(args->cache.keyScales);
+    p.valueScales = static_cast<const uint16_t*>(args->cache.valueScales);
+    p.k = args->k;
+    p.v = args->v;
+    p.starts = args->starts;
+    p.outType = args->outType > 1 ? -1 : int(args->outType);
+    p.count = args->count;
+    p.kStride = args->kStride ? args->kStride : row;
+    p.vStride = args->vStride ? args->vStride : row;
+    if (p.kStride >= (uint64_t(1) << 40) || p.vStride >= (uint64_t(1) << 40))
+        return ctx.fail("paged read: a stride of k or v is out of range"), 0;
+    if (!aigpu::check_paged_read_q4(p) || !usable(ctx, "paged read")) return 0;
     const OnDevice device;
-    hipStream_t stream = as_stream(args->stream);
-    if (args->workspace) return aigpu::launch_paged_decode(p, args->workspace, stream) ? 1 : 0;
-    if (need == 0) return aigpu::launch_paged_decode(p, nullptr, stream) ? 1 : 0;
-    if (aigpu::capturing(stream))
-        return ctx.fail("paged decode: a captured call needs a workspace of its own (" + std::to_string(need) +
-                        " bytes)"),
-               0;
-    const size_t room = aigpu::paged_decode_scratch(p);
-    void* work = nullptr;
-    if (!ctx.scratchOf(stream, room, &work)) return 0;
-    if (work) return aigpu::launch_paged_decode(p, work, stream) ? 1 : 0;
-    const StreamOrder order(ctx, stream);
-    work = ctx.growZeroed(aigpu::SLOT_PAGED, room);
-    return work && aigpu::launch_paged_decode(p, work, stream) ? 1 : 0;
+    return aigpu::launch_paged_read_q4(p, as_stream(args->stream)) ? 1 : 0;
+}
+
+AIGPU_ABI uint64_t aigpu_paged_decode_workspace(const AiGpuPagedDecode* args) { return paged_decode_bytes(args); }
+
+AIGPU_ABI uint64_t aigpu_paged_decode_q4_workspace(const AiGpuPagedDecodeQ4* args) { return paged_decode_bytes(args); }
+
+AIGPU_ABI int aigpu_paged_decode(const AiGpuPagedDecode* args) { return paged_decode(args, nullptr); }
+
+AIGPU_ABI int aigpu_paged_decode_q4(const AiGpuPagedDecodeQ4* args) { return paged_decode(args, nullptr); }
+
+AIGPU_ABI int aigpu_paged_decode_scored(const AiGpuPagedDecode* args, const AiGpuScores* scores) {
+    Context& ctx = Context::instance();
+    std::lock_guard<std::recursive_mutex> lock(ctx.gate);
+    if (!scores) return ctx.fail("paged decode: null scores"), 0;
+    return paged_decode(args, scores);
 }
 
 } // extern "C"

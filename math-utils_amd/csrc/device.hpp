@@ -45,11 +45,23 @@ __device__ __forceinline__ float load_elem(const void* base, size_t i, int type)
     return bf16_bits_to_float(static_cast<const uint16_t*>(base)[i]);
 }
 
-/* wave64 butterflies */
 /* softplusOf and sigmoidOf (LocalModel.hpp:1371-1376) with the library exp */
 __device__ __forceinline__ float softplus_of(float x) { return x > 20.0f ? x : log1pf(expf(x)); }
 __device__ __forceinline__ float sigmoid_of(float x) { return 1.0f / (1.0f + expf(-x)); }
 
+/* tanh to 2 units of fp32's last place: its series below 0.625 (five terms fitted over
+   that range), 1 - 2 / (e^2x + 1) past it */
+__device__ __forceinline__ float tanh_of(float x) {
+    const float t = x * x, a = fabsf(x);
+    const float small =
+        x + x * (t * (-0.3333328068256378f +
+                      t * (0.13331381976604462f +
+                           t * (-0.05373531952500343f + t * (0.020626291632652283f - 0.005691985599696636f * t)))));
+    const float large = 1.0f - 2.0f / (exp2f(2.0f * LOG2E * a) + 1.0f);
+    return a < 0.625f ? small : copysignf(large, x);
+}
+
+/* wave64 butterflies */
 __device__ __forceinline__ float wave_sum(float x) {
 #pragma unroll
     for (int o = 32; o > 0; o >>= 1) x += __shfl_xor(x, o, WAVE);

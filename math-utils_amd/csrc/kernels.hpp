@@ -314,8 +314,10 @@ struct PagedAppendParams {
 };
 bool check_paged_append(const PagedAppendParams& p);
 bool launch_paged_append(const PagedAppendParams& p, hipStream_t stream);
+// the forms of one kernel: the scores as they are; capped or biased; over 4-bit pages
+enum PagedForm { PAGED_PLAIN = 0, PAGED_SCORED, PAGED_CODES };
 struct PagedDecodeParams {
-    PagedCache c;
+    PagedCache c;               // 4-bit pages: keys and values are the codes, strides count rows
     const void* q;
     float* out;
     const float* gamma;
@@ -324,6 +326,11 @@ struct PagedDecodeParams {
     int rot, interleaved, inType, outputGate;
     uint32_t maxLength, heads;
     uint64_t qStride, qTokenStride, window;
+    int form;
+    float cap;                  // 0: none
+    const float* slopes;        // [heads] or null
+    const uint16_t* keyScales;  // 4-bit pages: fp16 [row][dim / 32]
+    const uint16_t* valueScales;
 };
 bool check_paged_decode(const PagedDecodeParams& p);
 size_t paged_decode_workspace(const PagedDecodeParams& p);
@@ -333,6 +340,37 @@ size_t paged_decode_workspace(const PagedDecodeParams& p);
 size_t paged_decode_scratch(const PagedDecodeParams& p);
 // work: paged_decode_workspace(p) bytes, or null where that is 0
 bool launch_paged_decode(const PagedDecodeParams& p, void* work, hipStream_t stream);
+bool launch_paged_scored(const PagedDecodeParams& p, void* work, hipStream_t stream);
+bool launch_paged_codes(const PagedDecodeParams& p, void* work, hipStream_t stream);
+
+
+// ---- a paged cache of 4-bit codes ----
+// PagedCache with the codes as keys and values ([row][dim / 2] bytes), its strides in rows
+struct PagedAppendQ4Params {
+    PagedAppendParams a;
+    uint16_t* keyScales;        // fp16 [row][dim / 32]
+    uint16_t* valueScales;
+};
+bool check_paged_append_q4(const PagedAppendQ4Params& p);
+bool launch_paged_append_q4(const PagedAppendQ4Params& p, hipStream_t stream);
+struct PagedReadQ4Params {
+    PagedCache c;
+    const uint16_t* keyScales;
+    const uint16_t* valueScales;
+    void* k;
+    void* v;
+    const uint32_t* starts;
+    int outType;
+    uint64_t count, kStride, vStride;
+};
+bool check_paged_read_q4(const PagedReadQ4Params& p);
+bool launch_paged_read_q4(const PagedReadQ4Params& p, hipStream_t stream);
+// parts of the paged entries' checks
+struct Context;
+bool rotation_ok(Context& ctx, const char* who, const float* freqs, int rot, uint32_t dim, float amplitude);
+bool codes_ok(Context& ctx, const char* who, const PagedCache& c, const void* keyScales, const void* valueScales);
+// no two rows of `row` elements of the pool share one: each stride spans what the shorter ones do
+bool rows_apart(const PagedCache& c, uint64_t row);
 
 // ---- a plain streaming device copy (the bench's achievable-bandwidth line) ----
 bool launch_copy(void* dst, const void* src, uint64_t bytes, hipStream_t stream);

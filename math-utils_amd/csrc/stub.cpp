@@ -70,6 +70,11 @@ AIGPU_ABI int aigpu_rotary_frequencies(const AiGpuRotaryScaling*, float*, float*
 AIGPU_ABI int aigpu_paged_append(const AiGpuPagedAppend*) { return 0; }
 AIGPU_ABI int aigpu_paged_decode(const AiGpuPagedDecode*) { return 0; }
 AIGPU_ABI uint64_t aigpu_paged_decode_workspace(const AiGpuPagedDecode*) { return 0; }
+AIGPU_ABI int aigpu_paged_decode_scored(const AiGpuPagedDecode*, const AiGpuScores*) { return 0; }
+AIGPU_ABI int aigpu_paged_append_q4(const AiGpuPagedAppendQ4*) { return 0; }
+AIGPU_ABI int aigpu_paged_read_q4(const AiGpuPagedReadQ4*) { return 0; }
+AIGPU_ABI int aigpu_paged_decode_q4(const AiGpuPagedDecodeQ4*) { return 0; }
+AIGPU_ABI uint64_t aigpu_paged_decode_q4_workspace(const AiGpuPagedDecodeQ4*) { return 0; }
 
 AIGPU_ABI void aigpu_profile(int) {}
 AIGPU_ABI int aigpu_profile_read(const char*, double* ms, uint64_t* n) {
