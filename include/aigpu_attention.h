@@ -754,6 +754,52 @@ AIGPU_ABI int aigpu_paged_decode_q4(const AiGpuPagedDecodeQ4* args);
 AIGPU_ABI uint64_t aigpu_paged_decode_q4_workspace(const AiGpuPagedDecodeQ4* args);
 
 /* ------------------------------------------------------------------------ */
+/* 14. Attention of the tokens of many documents in one call (prompts, or the */
+/*    new tokens of conversations behind their cached keys). Document b has    */
+/*    tokens starts[b] .. starts[b + 1] - 1 of q and out and keys              */
+/*    keyStarts[b] .. keyStarts[b + 1] - 1 of k and v; its tokens are the last */
+/*    of its keys' positions, 0, 1, ... A token at position i sees the keys j  */
+/*    of its own document with                                                 */
+/*      (j <= i or j < prefix[b]) and (window = 0 or i - j < window)           */
+/*    with the scores s = scale q.k, then cap > 0: s = cap tanh(s / cap), then */
+/*    slopes: s -= slopes[head] |i - j|. A token that sees nothing gets zeros  */
+/*    (more tokens than keys: the first ones). Rows of out that no document    */
+/*    has stay as they were; a document whose starts decrease, or end past     */
+/*    count or keyCount, has no tokens or keys. Every row of a document's keys */
+/*    and values has to be finite, rows of no document may hold anything.      */
+/*    Types: q, k, v of inType, out of outType. bf16 to bf16 rounds the        */
+/*    weights to bf16 (their sum adds the rounded ones) and the result once;   */
+/*    bf16 to fp32 takes the weights in two terms, 2^-16 of each; fp32 is fp32 */
+/*    throughout. Rows of q, k and v are 16-byte aligned. No counterpart in    */
+/*    the reference, whose call is one sequence's. Asynchronous.               */
+/* ------------------------------------------------------------------------ */
+typedef struct AiGpuPackedAttention {
+    const void* q;            /* element (token, head, d) at token*qTokenStride + head*qHeadStride + d */
+    const void* k;            /* the same with heads = kvHeads */
+    const void* v;
+    void* out;                /* apart from q, k and v (slices of the same rows may be) */
+    const uint32_t* starts;   /* [documents + 1], or NULL: one document of all tokens and keys */
+    const uint32_t* keyStarts;/* [documents + 1], or NULL: starts (keyCount = count) */
+    const uint32_t* prefix;   /* [documents], or NULL: none */
+    const float* slopes;      /* [heads], or NULL: none */
+    float cap;                /* 0: none */
+    float scale;              /* 0 means 1/sqrt(dim) */
+    uint32_t inType, outType;
+    uint64_t count, keyCount, documents, heads, kvHeads, dim;   /* dim 64, 96, 128, 192 or 256 */
+    uint64_t window;          /* 0 = all */
+    uint64_t qTokenStride, qHeadStride, kTokenStride, kHeadStride;  /* 0 mean heads*headStride and dim */
+    uint64_t vTokenStride, vHeadStride, outTokenStride, outHeadStride;
+    void* workspace;          /* device, 256-byte aligned; NULL: the backend's scratch */
+    uint64_t workspaceBytes;
+    void* stream;
+} AiGpuPackedAttention;
+AIGPU_ABI int aigpu_packed_attention(const AiGpuPackedAttention* args);
+/* The workspace bytes of a call with these sizes (0: none): few tokens over many keys
+   are split over workgroups. It need not be zero-filled; calls that may run at once
+   need one each. A call captured into a graph has to bring one where this is not 0. */
+AIGPU_ABI uint64_t aigpu_packed_attention_workspace(const AiGpuPackedAttention* args);
+
+/* ------------------------------------------------------------------------ */
 /* Per-kernel timing. With profiling on, every launch is bracketed by a pair */
 /* of hipEvents on the stream it runs on; aigpu_profile_read synchronises    */
 /* and reports the summed device time and launch count of kernels whose name */

@@ -872,7 +872,18 @@ class AiGpuPagedDecodeQ4(C.Structure):
                 ("workspace", _vp), ("workspaceBytes", _u64), ("stream", _vp)]
 
 
+class AiGpuPackedAttention(C.Structure):
+    _fields_ = [(n, _vp) for n in ("q", "k", "v", "out", "starts", "keyStarts", "prefix", "slopes")] + \
+        [("cap", _f32), ("scale", _f32), ("inType", _u32), ("outType", _u32)] + \
+        [(n, _u64) for n in ("count", "keyCount", "documents", "heads", "kvHeads", "dim", "window", "qTokenStride",
+                             "qHeadStride", "kTokenStride", "kHeadStride", "vTokenStride", "vHeadStride",
+                             "outTokenStride", "outHeadStride")] + \
+        [("workspace", _vp), ("workspaceBytes", _u64), ("stream", _vp)]
+
+
 SIGNATURES.update({
+    "aigpu_packed_attention": (C.c_int, [C.POINTER(AiGpuPackedAttention)]),
+    "aigpu_packed_attention_workspace": (_u64, [C.POINTER(AiGpuPackedAttention)]),
     "aigpu_paged_decode_scored": (C.c_int, [C.POINTER(AiGpuPagedDecode), C.POINTER(AiGpuScores)]),
     "aigpu_paged_append_q4": (C.c_int, [C.POINTER(AiGpuPagedAppendQ4)]),
     "aigpu_paged_read_q4": (C.c_int, [C.POINTER(AiGpuPagedReadQ4)]),
@@ -909,6 +920,7 @@ _PACK = {"aigpu_rotary": _struct.Struct("4Pf5I8QP"),
          "aigpu_paged_append_q4": _struct.Struct("2P" + _CACHE + "5P3f3I3QP"),
          "aigpu_paged_read_q4": _struct.Struct("2P" + _CACHE + "3P2I3QP"),
          "aigpu_paged_decode_q4": _struct.Struct("2P" + _CACHE + "5P5f5I4QPQP"),
+         "aigpu_packed_attention": _struct.Struct("8P2f2I15QPQP"),
          "scores": _struct.Struct("PfI")}
 _entries = {}
 _torch = None
@@ -1275,3 +1287,54 @@ def paged_decode_q4_workspace(q, out, key_codes, key_scales, value_codes, value_
     need = lib().aigpu_paged_decode_q4_workspace(C.cast(C.c_char_p(args), C.POINTER(AiGpuPagedDecodeQ4)))
     _check(need or q.shape[0] == 0)
     return _torch.zeros(int(need), dtype=_torch.uint8, device=q.device)
+
+
+def _packed_attention(q, k, v, out, starts, key_starts, prefix, window, cap, slopes, scale, workspace, stream):
+    _with_torch()
+    of_q, of_k, of_v, to = _at(q, "q"), _at(k, "k"), _at(v, "v"), _at(out, "out")
+    if q.dim() != 3 or out.shape != q.shape or k.dim() != 3 or v.shape != k.shape or k.shape[2] != q.shape[2] \
+            or k.dtype != q.dtype or v.dtype != q.dtype:
+        raise ValueError("q and out must be [tokens][heads][dim], k and v [keys][kv_heads][dim], q, k, v of one type")
+    (count, heads, dim), (keys, kv_heads, _) = q.shape, k.shape
+    documents = 1 if starts is None else starts.shape[0] - 1
+    if documents < 0:
+        raise ValueError("starts must have an entry more than documents")
+    begins = 0 if starts is None else _indices(starts, "starts", 1)
+    key_begins = 0 if key_starts is None else _indices(key_starts, "key_starts", 1, documents + 1)
+    whole = 0 if prefix is None else _indices(prefix, "prefix", 1, documents)
+    room, nbytes = 0, 0
+    if workspace is not None:
+        if not workspace.is_contiguous():
+            raise ValueError("workspace must be contiguous")
+        room, nbytes = _at(workspace, "workspace"), workspace.numel() * workspace.element_size()
+    strides = []
+    for t, name in ((q, "q"), (k, "k"), (v, "v"), (out, "out")):
+        strides += _strides(t, name) if t.numel() else (t.shape[1] * dim, dim)
+    return _packed("aigpu_packed_attention", of_q, of_k, of_v, to, begins, key_begins, whole,
+                   _vector(slopes, "slopes", heads, True), cap, scale, _kind(q), _kind(out), count, keys, documents,
+                   heads, kv_heads, dim, window, *strides, room, nbytes, _own_stream(stream))
+
+
+def packed_attention(q, k, v, out, starts=None, key_starts=None, prefix=None, window=0, cap=0.0, slopes=None,
+                     scale=0.0, workspace=None, stream=None):
+    """Attention of the tokens of many documents: q, out [tokens][heads][dim],
+    k, v [keys][kv_heads][dim] (fp32 or bf16, any token and head strides of 16
+    bytes; out of either type). Document b has tokens starts[b] .. starts[b + 1]
+    - 1 and keys key_starts[b] .. key_starts[b + 1] - 1 (default: starts;
+    neither: one document), its tokens the last of its positions. A token sees
+    its document's keys at or before it, and the first prefix[b] whatever its
+    place, no further back than window (0: all). cap > 0 caps the scores
+    (cap tanh(s / cap)), then slopes [heads] take slope times the distance from
+    them. A call captured into a graph brings a workspace
+    (packed_attention_workspace) where its size is not 0. Asynchronous."""
+    args = _packed_attention(q, k, v, out, starts, key_starts, prefix, window, cap, slopes, scale, workspace, stream)
+    if q.shape[0]:
+        _check(_entry("aigpu_packed_attention")(args))
+    return out
+
+
+def packed_attention_workspace(q, k, v, out, starts=None, key_starts=None):
+    """a workspace (uint8 tensor, perhaps empty) for packed_attention calls of these sizes"""
+    args = _packed_attention(q, k, v, out, starts, key_starts, None, 0, 0.0, None, 0.0, None, 0)
+    need = lib().aigpu_packed_attention_workspace(C.cast(C.c_char_p(args), C.POINTER(AiGpuPackedAttention)))
+    return _torch.empty(int(need), dtype=_torch.uint8, device=q.device)

@@ -1383,3 +1383,84 @@ AIGPU_ABI int aigpu_paged_decode_scored(const AiGpuPagedDecode* args, const AiGp
 }
 
 } // extern "C"
+
+/* -------------------------------------------------------------------- 14 */
+
+namespace {
+
+bool packed_params(Context& ctx, const AiGpuPackedAttention* a, aigpu::PackedParams& p) {
+    constexpr uint64_t LIMIT = (uint64_t(1) << 31) - 1024;    // positions and a tile past them fit 31 bits
+    if (a->count >= LIMIT || a->keyCount >= LIMIT || a->documents > (1u << 24) || a->heads > 65535 ||
+        a->kvHeads > 65535 || a->dim > 4096)
+        return ctx.fail("packed attention: sizes out of range");
+    p.q = a->q;
+    p.k = a->k;
+    p.v = a->v;
+    p.out = a->out;
+    p.starts = a->starts;
+    p.keyStarts = a->keyStarts;
+    p.prefix = a->prefix;
+    p.slopes = a->slopes;
+    p.cap = a->cap;
+    p.scale = a->scale == 0.0f && a->dim ? 1.0f / sqrtf(float(a->dim)) : a->scale;
+    p.inType = a->inType > 1 ? -1 : int(a->inType);
+    p.outType = a->outType > 1 ? -1 : int(a->outType);
+    p.count = uint32_t(a->count);
+    p.keyCount = uint32_t(a->keyCount);
+    p.documents = uint32_t(a->documents);
+    p.heads = uint32_t(a->heads);
+    p.kvHeads = uint32_t(a->kvHeads);
+    p.dim = uint32_t(a->dim);
+    p.window = a->window;
+    auto strides = [&](uint64_t token, uint64_t head, uint64_t heads, uint64_t& t, uint64_t& h) {
+        h = head ? head : a->dim;
+        t = token ? token : heads * h;
+    };
+    strides(a->qTokenStride, a->qHeadStride, a->heads, p.qTokenStride, p.qHeadStride);
+    strides(a->kTokenStride, a->kHeadStride, a->kvHeads, p.kTokenStride, p.kHeadStride);
+    strides(a->vTokenStride, a->vHeadStride, a->kvHeads, p.vTokenStride, p.vHeadStride);
+    strides(a->outTokenStride, a->outHeadStride, a->heads, p.outTokenStride, p.outHeadStride);
+    return aigpu::check_packed_attention(p);
+}
+
+} // namespace
+
+extern "C" {
+
+AIGPU_ABI uint64_t aigpu_packed_attention_workspace(const AiGpuPackedAttention* args) {
+    Context& ctx = Context::instance();
+    std::lock_guard<std::recursive_mutex> lock(ctx.gate);
+    if (!args) return ctx.fail("packed attention: null arguments"), 0;
+    aigpu::PackedParams p{};
+    return packed_params(ctx, args, p) ? aigpu::packed_attention_workspace(p) : 0;
+}
+
+AIGPU_ABI int aigpu_packed_attention(const AiGpuPackedAttention* args) {
+    Context& ctx = Context::instance();
+    std::lock_guard<std::recursive_mutex> lock(ctx.gate);
+    if (!args) return ctx.fail("packed attention: null arguments"), 0;
+    aigpu::PackedParams p{};
+    if (!packed_params(ctx, args, p)) return 0;
+    const size_t need = aigpu::packed_attention_workspace(p);
+    if (args->workspace) {
+        if (reinterpret_cast<uintptr_t>(args->workspace) & 255)
+            return ctx.fail("packed attention: the workspace must be 256-byte aligned"), 0;
+        if (args->workspaceBytes < need)
+            return ctx.fail("packed attention: the workspace holds " + std::to_string(args->workspaceBytes) +
+                            " bytes, the call needs " + std::to_string(need)),
+                   0;
+    }
+    if (!usable(ctx, "packed attention")) return 0;
+    const OnDevice device;
+    hipStream_t stream = as_stream(args->stream);
+    if (args->workspace || need == 0) return aigpu::launch_packed_attention(p, args->workspace, stream) ? 1 : 0;
+    if (aigpu::capturing(stream))
+        return ctx.fail("packed attention: a captured call needs a workspace of its own (" + std::to_string(need) +
+                        " bytes)"),
+               0;
+    const StreamOrder order(ctx, stream);
+    void* work = ctx.grow(aigpu::SLOT_PACKED, need);
+    return work && aigpu::launch_packed_attention(p, work, stream) ? 1 : 0;
+}
+
+} // extern "C"

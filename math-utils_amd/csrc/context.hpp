@@ -36,6 +36,7 @@ enum ScratchSlot {
     SLOT_ATTN_PARTS,     // split records of the tiled fp32 attention
     SLOT_DELTA_SEG,      // segment maps and start states of the two-level delta-rule scan
     SLOT_PAGED,          // partial softmax records of a paged decode
+    SLOT_PACKED,         // split records of a packed attention
     SLOT_COUNT
 };
 

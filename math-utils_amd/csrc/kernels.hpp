@@ -372,6 +372,27 @@ bool codes_ok(Context& ctx, const char* who, const PagedCache& c, const void* ke
 // no two rows of `row` elements of the pool share one: each stride spans what the shorter ones do
 bool rows_apart(const PagedCache& c, uint64_t row);
 
+// ---- attention of packed documents ----
+struct PackedParams {
+    const void* q;
+    const void* k;
+    const void* v;
+    void* out;
+    const uint32_t* starts;     // [documents + 1] or null: one document
+    const uint32_t* keyStarts;  // [documents + 1] or null: starts
+    const uint32_t* prefix;     // [documents] or null
+    const float* slopes;        // [heads] or null
+    float cap, scale;
+    int inType, outType;
+    uint32_t count, keyCount, documents, heads, kvHeads, dim;
+    uint64_t window;
+    uint64_t qTokenStride, qHeadStride, kTokenStride, kHeadStride, vTokenStride, vHeadStride, outTokenStride, outHeadStride;
+};
+bool check_packed_attention(const PackedParams& p);
+// 0 where the keys are not split over workgroups
+size_t packed_attention_workspace(const PackedParams& p);
+bool launch_packed_attention(const PackedParams& p, void* work, hipStream_t stream);
+
 // ---- a plain streaming device copy (the bench's achievable-bandwidth line) ----
 bool launch_copy(void* dst, const void* src, uint64_t bytes, hipStream_t stream);
 

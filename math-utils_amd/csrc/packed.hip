@@ -1,0 +1,540 @@
+// packed.hip - attention of many documents' tokens in one call: a document mask, scores
+// capped or biased, a prefix that all of a document's tokens see, a window.
+#include <algorithm>
+#include <cmath>
+#include <type_traits>
+
+#include "context.hpp"
+#include "device.hpp"
+#include "kernels.hpp"
+
+namespace aigpu {
+
+namespace {
+
+/*
+    A row of work is a (token, query head) of one document and kv head: the G heads of a
+    token lie next to each other, so that the heads which share keys share their loads. A
+    workgroup takes ROWS_WG = 128 consecutive rows, a wave 32 of them, and walks the keys
+    that any of its rows sees in tiles of BN, two stages of LDS filled by DMA: past a tile's
+    one barrier it has landed for every wave, and every wave has left the tile before, whose
+    stage is then refilled. Per tile and 32 keys
+      S^T = K Q^T      32 x 32 MFMA, keys as rows: a lane holds 16 keys' scores of one row
+      softmax          a running maximum and sum a row, in the lane and the one 32 lanes on
+      O^T += V^T P^T   the weights as they lie in the lane, V transposed out of LDS
+    The rows of a key tile stand in LDS in the order that makes a lane's 16 scores two runs
+    of 8 keys, which is how the second product takes them.
+
+    bf16 in, bf16 out: the weights round to bf16, and the sum adds up the rounded ones.
+    bf16 in, fp32 out: the weights in two bf16 terms (2^-16 of each at most).
+    fp32 in: fp32 products (v_mfma_f32_32x32x2_f32), for which the keys' order is the plain one.
+*/
+constexpr int WAVES = 4, THREADS = 64 * WAVES, ROWS_WG = 32 * WAVES;
+enum Kind { BF16_OUT = 0, BF16_F32 = 1, FULL = 2 };
+
+struct PackedArgs {
+    PackedParams p;
+    float* records;                  // of split keys, or null: [(slot, kv head)][split] of record floats
+    uint32_t group, slots, splits;   // query heads of a kv head; 128-row slots over all documents
+    float factor;                    // the product to the scores' fractions of the cap, or to units of ln 2
+    float capLog2;
+    int wide;                        // out's rows can be written four elements at a time
+};
+
+template <int D>
+constexpr uint32_t record_floats() { return ROWS_WG * (D + 2); }
+
+__device__ __forceinline__ uint32_t scalar(uint32_t x) { return __builtin_amdgcn_readfirstlane(x); }
+
+template <int N>
+__device__ __forceinline__ void wait_vmcnt() {
+    __builtin_amdgcn_s_waitcnt((N & 15) | (7 << 4) | (15 << 8) | ((N >> 4) << 14));
+}
+
+/* row i of 32 in a key tile is this key: lane group g's 16 accumulators are keys 16 g + r */
+__device__ __forceinline__ int key_of_row(int i) { return 16 * ((i >> 2) & 1) + 4 * (i >> 3) + (i & 3); }
+
+/* LDS swizzles: block x of 16 bytes of a tile's row i sits at x ^ this. Keys are read a row a
+   lane, values (bf16) four rows of 64 bytes at once: each in distinct banks (64 of 4 bytes). */
+template <int BYTES>
+__device__ __forceinline__ int key_swizzle(int i) {
+    if constexpr (BYTES % 256 == 0) return i & 15;
+    else if constexpr (BYTES % 128 == 0) return (i >> 1) & 7;
+    else return (i >> 2) & 3;
+}
+template <int BYTES>
+__device__ __forceinline__ int value_swizzle(int i) {
+    if constexpr (BYTES % 256 == 0) return 4 * (i & 3);
+    else if constexpr (BYTES % 128 == 0) return 4 * ((i >> 1) & 1);
+    else return 0;
+}
+
+typedef __bf16 bf16v4 __attribute__((__vector_size__(4 * sizeof(__bf16))));
+__device__ __forceinline__ bf16x8 read_transposed(const uint16_t* a0, const uint16_t* a1) {
+    typedef __attribute__((address_space(3))) bf16v4 lds_bf16v4;
+    const bf16v4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4bf16((lds_bf16v4*)(a0));
+    const bf16v4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4bf16((lds_bf16v4*)(a1));
+    return __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
+}
+
+/* A workgroup's document and rows. Document b owns the slots from starts[b] G / 128 + b on
+   (rounded down), one more than its rows may need; a slot past its rows does nothing. */
+struct Work {
+    uint32_t first, tokens;          // the document's tokens: q and out rows first ..
+    uint32_t key0, keys;             // its keys
+    int32_t shift;                   // a token's position less its number in the document
+    uint32_t prefix;
+    uint64_t row0, rows;             // the workgroup's first row, the document's rows
+};
+__device__ __forceinline__ bool find_work(const PackedArgs& a, uint32_t slot, int lane, Work& x) {
+    const PackedParams& p = a.p;
+    uint32_t b = 0;
+    uint64_t slot0 = 0;
+    if (p.starts) {
+        uint32_t before = 0;         // documents whose slots start at or before this one
+        for (uint32_t k = 0; k < p.documents; k += WAVE) {
+            const bool in = k + lane < p.documents;
+            const uint64_t at = in ? uint64_t(p.starts[k + lane]) * a.group / ROWS_WG + k + lane : ~uint64_t(0);
+            before += __popcll(__ballot(at <= slot));
+        }
+        before = scalar(before);
+        if (before == 0) return false;
+        b = before - 1;
+        const uint32_t s0 = scalar(p.starts[b]), s1 = scalar(p.starts[b + 1]);
+        slot0 = uint64_t(s0) * a.group / ROWS_WG + b;
+        x.first = s0;
+        x.tokens = s1 > s0 && s1 <= p.count ? s1 - s0 : 0;
+        x.key0 = s0;
+        x.keys = x.tokens;
+    } else {
+        x.first = x.key0 = 0;
+        x.tokens = p.count;
+        x.keys = p.keyCount;
+    }
+    if (p.keyStarts) {
+        const uint32_t s0 = scalar(p.keyStarts[b]), s1 = scalar(p.keyStarts[b + 1]);
+        x.key0 = s0;
+        x.keys = s1 > s0 && s1 <= p.keyCount ? s1 - s0 : 0;
+    }
+    x.prefix = p.prefix ? scalar(p.prefix[b]) : 0;
+    x.prefix = x.prefix < x.keys ? x.prefix : x.keys;
+    x.shift = int32_t(x.keys) - int32_t(x.tokens);
+    x.rows = uint64_t(x.tokens) * a.group;
+    x.row0 = (slot - slot0) * ROWS_WG;
+    return x.row0 < x.rows;
+}
+
+/* four elements of an out row */
+__device__ __forceinline__ void put4(const PackedArgs& a, uint64_t at, const float (&x)[4]) {
+    if (a.p.outType == 1) {
+        uint16_t* out = static_cast<uint16_t*>(a.p.out) + at;
+        const u32x2 two = {pack_bf16(x[0], x[1]), pack_bf16(x[2], x[3])};
+        if (a.wide) {
+            *reinterpret_cast<u32x2*>(out) = two;
+        } else {
+#pragma unroll
+            for (int i = 0; i < 4; ++i) out[i] = uint16_t(two[i / 2] >> 16 * (i & 1));
+        }
+    } else {
+        float* out = static_cast<float*>(a.p.out) + at;
+        if (a.wide) {
+            *reinterpret_cast<floatx4*>(out) = floatx4{x[0], x[1], x[2], x[3]};
+        } else {
+#pragma unroll
+            for (int i = 0; i < 4; ++i) out[i] = x[i];
+        }
+    }
+}
+
+constexpr int tile_keys(int D, int kind) { return kind == FULL ? (D <= 96 ? 64 : 32) : (D <= 128 ? 64 : 32); }
+constexpr int workgroups(int D, int kind) { return D <= (kind == FULL ? 96 : 128) ? 2 : 1; }
+
+template <int D, int KIND>
+__global__ __launch_bounds__(THREADS, workgroups(D, KIND)) void packed_attention_kernel(PackedArgs a) {
+    typedef std::conditional_t<KIND == FULL, float, uint16_t> elem;
+    constexpr int ES = sizeof(elem), BYTES = D * ES;       // of a row
+    constexpr int BN = tile_keys(D, KIND), KB = BN / 32;   // keys of a tile, their blocks of 32
+    constexpr int DT = D / 32;                             // 32-wide tiles of the output
+    constexpr int BPR = BYTES / 16;                        // 16-byte blocks of a row
+    constexpr int BLOCKS = BN * BPR / WAVE / WAVES;        // DMA blocks (1 KB) of a wave and tile, K or V
+    constexpr int QV = KIND == FULL ? D / 8 : D / 16;      // 16-byte pieces of a lane's half query
+    static_assert(BN * BPR % (WAVE * WAVES) == 0, "a tile's blocks are the waves' alike");
+    __shared__ __attribute__((aligned(16))) elem ktile[2][BN * D], vtile[2][BN * D];
+    const PackedParams& p = a.p;
+    const int lane = threadIdx.x & 63, w = int(scalar(threadIdx.x >> 6)), g = lane >> 5, c = lane & 31;
+
+    // consecutive workgroups go round the 8 XCDs: give each XCD a run of them, so that
+    // the rows that share a kv head's keys share an L2. Late rows, which see most, go first.
+    uint32_t id = blockIdx.x;
+    if (gridDim.x % 8 == 0) id = id % 8 * (gridDim.x / 8) + id / 8;
+    const uint32_t split = id % a.splits, kvh = id / a.splits / a.slots, slot = a.slots - 1 - id / a.splits % a.slots;
+    Work x;
+    if (!find_work(a, slot, lane, x)) return;
+
+    // this lane's row
+    const uint64_t row = x.row0 + 32 * w + c;
+    const bool live = row < x.rows;
+    const uint32_t token = uint32_t((live ? row : x.rows - 1) / a.group);
+    const uint32_t head = kvh * a.group + uint32_t((live ? row : x.rows - 1) % a.group);
+    const int32_t pos = x.shift + int32_t(token);          // negative: before every key
+    const uint64_t lastRow = x.row0 + ROWS_WG - 1 < x.rows ? x.row0 + ROWS_WG - 1 : x.rows - 1;
+    const int32_t pos0 = x.shift + int32_t(x.row0 / a.group), pos1 = x.shift + int32_t(lastRow / a.group);
+
+    // the keys that any row sees: [kbeg, kend), in whole tiles from a multiple of BN on
+    uint32_t kend = pos1 < 0 ? 0 : uint32_t(pos1) + 1;
+    kend = kend > x.prefix ? kend : x.prefix;
+    uint32_t kbeg = 0;
+    if (p.window && pos0 >= 0 && uint64_t(pos0) + 1 > p.window) kbeg = uint32_t(pos0 + 1 - int64_t(p.window)) / BN * BN;
+    uint32_t tiles = kend > kbeg ? (kend - kbeg + BN - 1) / BN : 0;
+    if (a.splits > 1) {
+        const uint32_t t0 = uint32_t(uint64_t(tiles) * split / a.splits), t1 = uint32_t(uint64_t(tiles) * (split + 1) / a.splits);
+        kbeg += t0 * BN;
+        tiles = t1 - t0;
+    }
+    // a row sees keys [lo, hi)
+    int32_t hi = pos + 1;
+    hi = hi > int32_t(x.prefix) ? hi : int32_t(x.prefix);
+    const int32_t lo = p.window && pos >= 0 && uint64_t(pos) + 1 > p.window ? int32_t(pos + 1 - int64_t(p.window)) : 0;
+    // what every row of the wave sees
+    const uint64_t waveFirst = x.row0 + 32 * w < x.rows ? x.row0 + 32 * w : x.rows - 1;
+    const uint64_t waveLast = waveFirst + 31 < x.rows ? waveFirst + 31 : x.rows - 1;
+    const int32_t p0 = x.shift + int32_t(waveFirst / a.group), p1 = x.shift + int32_t(waveLast / a.group);
+    int32_t hi0 = p0 + 1;
+    hi0 = hi0 > int32_t(x.prefix) ? hi0 : int32_t(x.prefix);
+    const int32_t lo1 = p.window && p1 >= 0 && uint64_t(p1) + 1 > p.window ? int32_t(p1 + 1 - int64_t(p.window)) : 0;
+    int32_t hi1 = p1 + 1;
+    hi1 = hi1 > int32_t(x.prefix) ? hi1 : int32_t(x.prefix);
+    const int32_t lo0 = p.window && p0 >= 0 && uint64_t(p0) + 1 > p.window ? int32_t(p0 + 1 - int64_t(p.window)) : 0;
+    const bool busy = x.row0 + 32 * w < x.rows;            // the wave has rows
+
+    // the query: elements 16 db + 8 g .. of bf16, D / 2 g .. of fp32
+    u32x4 q[QV];
+    {
+        const elem* src = static_cast<const elem*>(p.q) + (uint64_t(x.first) + token) * p.qTokenStride + head * p.qHeadStride;
+#pragma unroll
+        for (int i = 0; i < QV; ++i)
+            q[i] = *reinterpret_cast<const u32x4*>(src + (KIND == FULL ? D / 2 * g + 4 * i : 16 * i + 8 * g));
+    }
+    const float slope = p.slopes ? p.slopes[head] * LOG2E : 0.0f;
+
+    const elem* keys = static_cast<const elem*>(p.k) + x.key0 * p.kTokenStride + kvh * p.kHeadStride;
+    const elem* values = static_cast<const elem*>(p.v) + x.key0 * p.vTokenStride + kvh * p.vHeadStride;
+    auto issue = [&](uint32_t k0, int stage) {
+        const uint32_t kl = scalar(lds_address(ktile[stage])), vl = scalar(lds_address(vtile[stage]));
+#pragma unroll
+        for (int n = 0; n < BLOCKS; ++n) {
+            const int i = (w * BLOCKS + n) * WAVE + lane, r = i / BPR, at = i % BPR;
+            // rows past the document's last key hold that one again
+            uint32_t key = k0 + (KIND == FULL ? r : (r & ~31) + key_of_row(r & 31));
+            key = key < x.keys ? key : x.keys - 1;
+            dma_block(keys + key * p.kTokenStride + 16 / ES * (at ^ key_swizzle<BYTES>(r)), kl + (w * BLOCKS + n) * 1024);
+        }
+#pragma unroll
+        for (int n = 0; n < BLOCKS; ++n) {
+            const int i = (w * BLOCKS + n) * WAVE + lane, r = i / BPR, at = i % BPR;
+            uint32_t key = k0 + r;
+            key = key < x.keys ? key : x.keys - 1;
+            dma_block(values + key * p.vTokenStride + 16 / ES * (KIND == FULL ? at : at ^ value_swizzle<BYTES>(r)),
+                      vl + (w * BLOCKS + n) * 1024);
+        }
+    };
+
+    floatx16 o[DT];
+#pragma unroll
+    for (int dt = 0; dt < DT; ++dt)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) o[dt][r] = 0.0f;
+    float m = -INFINITY, l = 0.0f;
+
+    if (tiles) issue(kbeg, 0);
+#pragma unroll 1
+    for (uint32_t it = 0; it < tiles; ++it) {
+        const uint32_t k0 = kbeg + it * BN;
+        const int stage = it & 1;
+        wait_vmcnt<0>();
+        lds_barrier();
+        if (it + 1 < tiles) issue(k0 + BN, stage ^ 1);
+        if (!busy || int32_t(k0) >= hi1 || int32_t(k0 + BN) <= lo0) continue;
+
+        floatx16 s[KB];
+#pragma unroll
+        for (int kb = 0; kb < KB; ++kb) {
+#pragma unroll
+            for (int r = 0; r < 16; ++r) s[kb][r] = 0.0f;
+            const elem* kr = ktile[stage] + (32 * kb + c) * D;
+#pragma unroll
+            for (int i = 0; i < QV; ++i) {
+                const int block = KIND == FULL ? QV * g + i : 2 * i + g;
+                const u32x4 k = *reinterpret_cast<const u32x4*>(kr + 16 / ES * (block ^ key_swizzle<BYTES>(c)));
+                if constexpr (KIND == FULL) {
+                    const floatx4 kf = __builtin_bit_cast(floatx4, k), qf = __builtin_bit_cast(floatx4, q[i]);
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) s[kb] = __builtin_amdgcn_mfma_f32_32x32x2f32(kf[j], qf[j], s[kb], 0, 0, 0);
+                } else {
+                    s[kb] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, k),
+                                                                    __builtin_bit_cast(bf16x8, q[i]), s[kb], 0, 0, 0);
+                }
+            }
+        }
+        // register r of block kb is key k0 + 32 kb + key(r)
+        auto key = [&](int r) { return KIND == FULL ? (r & 3) + 8 * (r >> 2) + 4 * g : 16 * g + r; };
+#pragma unroll
+        for (int kb = 0; kb < KB; ++kb)
+#pragma unroll
+            for (int r = 0; r < 16; ++r) {
+                float y = s[kb][r] * a.factor;
+                if (a.capLog2 != 0.0f) y = a.capLog2 * tanh_of(y);
+                if (p.slopes) y = fmaf(-slope, fabsf(float(pos - int32_t(k0) - 32 * kb - key(r))), y);
+                s[kb][r] = y;
+            }
+        if (int32_t(k0 + BN) > hi0 || int32_t(k0) < lo1) {
+#pragma unroll
+            for (int kb = 0; kb < KB; ++kb)
+#pragma unroll
+                for (int r = 0; r < 16; ++r) {
+                    const int32_t j = int32_t(k0) + 32 * kb + key(r);
+                    s[kb][r] = j >= lo && j < hi ? s[kb][r] : -INFINITY;
+                }
+        }
+        float top = -INFINITY;
+#pragma unroll
+        for (int kb = 0; kb < KB; ++kb)
+#pragma unroll
+            for (int r = 0; r < 16; ++r) top = fmaxf(top, s[kb][r]);
+        top = fmaxf(top, __shfl_xor(top, 32, WAVE));
+        // weights may grow to 2^8 before the maximum is taken up anew
+        const bool grow = top > m + 8.0f;
+        const float next = grow ? top : m, base = next == -INFINITY ? 0.0f : next;
+        const float keep = grow ? __builtin_amdgcn_exp2f(m - next) : 1.0f;
+        m = next;
+        if (__any(grow)) {
+            l *= keep;
+#pragma unroll
+            for (int dt = 0; dt < DT; ++dt)
+#pragma unroll
+                for (int r = 0; r < 16; ++r) o[dt][r] *= keep;
+        }
+#pragma unroll
+        for (int kb = 0; kb < KB; ++kb) {
+            if constexpr (KIND == FULL) {
+#pragma unroll
+                for (int r = 0; r < 16; ++r) {
+                    const float e = __builtin_amdgcn_exp2f(s[kb][r] - base);
+                    l += e;
+                    const float* vr = vtile[stage] + (32 * kb + key(r)) * D + c;
+#pragma unroll
+                    for (int dt = 0; dt < DT; ++dt)
+                        o[dt] = __builtin_amdgcn_mfma_f32_32x32x2f32(vr[32 * dt], e, o[dt], 0, 0, 0);
+                }
+            } else {
+#pragma unroll
+                for (int h = 0; h < 2; ++h) {
+                    u32x4 hi4, lo4;
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) {
+                        const float e0 = __builtin_amdgcn_exp2f(s[kb][8 * h + 2 * j] - base);
+                        const float e1 = __builtin_amdgcn_exp2f(s[kb][8 * h + 2 * j + 1] - base);
+                        const uint32_t both = pack_bf16(e0, e1);
+                        hi4[j] = both;
+                        const float f0 = __uint_as_float(both << 16), f1 = __uint_as_float(both & 0xFFFF0000u);
+                        if constexpr (KIND == BF16_F32) {
+                            lo4[j] = pack_bf16(e0 - f0, e1 - f1);
+                            l += e0 + e1;
+                        } else {
+                            l += f0 + f1;
+                        }
+                    }
+                    // V^T rows 32 dt + c: lane q16 of each 16 addresses row 16 g + 8 h + q16 / 4, and 4 on
+                    const int q16 = lane & 15, vr = 32 * kb + 16 * g + 8 * h + (q16 >> 2);
+#pragma unroll
+                    for (int dt = 0; dt < DT; ++dt) {
+                        const int d = 32 * dt + 16 * (lane >> 4 & 1) + 4 * (q16 & 3);
+                        const uint16_t* at = vtile[stage] + vr * D + 8 * ((d >> 3) ^ value_swizzle<BYTES>(vr)) + (d & 7);
+                        const bf16x8 v = read_transposed(at, at + 4 * D);
+                        if constexpr (KIND == BF16_F32)
+                            o[dt] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(v, __builtin_bit_cast(bf16x8, lo4), o[dt], 0, 0, 0);
+                        o[dt] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(v, __builtin_bit_cast(bf16x8, hi4), o[dt], 0, 0, 0);
+                    }
+                }
+            }
+        }
+    }
+
+    l += __shfl_xor(l, 32, WAVE);
+    if (!live) return;
+    // register r of tile dt is element 32 dt + (r & 3) + 8 (r >> 2) + 4 g
+    if (a.records) {
+        float* rec = a.records + ((uint64_t(slot) * p.kvHeads + kvh) * a.splits + split) * record_floats<D>();
+        const uint32_t at = 32 * w + c;
+        if (g == 0) {
+            rec[at] = m;
+            rec[ROWS_WG + at] = l;
+        }
+        float* to = rec + 2 * ROWS_WG + at * D + 4 * g;
+#pragma unroll
+        for (int dt = 0; dt < DT; ++dt)
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+                *reinterpret_cast<floatx4*>(to + 32 * dt + 8 * i) =
+                    floatx4{o[dt][4 * i], o[dt][4 * i + 1], o[dt][4 * i + 2], o[dt][4 * i + 3]};
+        return;
+    }
+    const float by = l == 0.0f ? 0.0f : 1.0f / l;          // nothing seen: zeros
+    const uint64_t to = (uint64_t(x.first) + token) * p.outTokenStride + head * p.outHeadStride + 4 * g;
+#pragma unroll
+    for (int dt = 0; dt < DT; ++dt)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const float y[4] = {o[dt][4 * i] * by, o[dt][4 * i + 1] * by, o[dt][4 * i + 2] * by, o[dt][4 * i + 3] * by};
+            put4(a, to + 32 * dt + 8 * i, y);
+        }
+}
+
+/* joins the records of the splits: a workgroup 128 rows of one kv head, a thread four
+   elements of a row */
+template <int D>
+__global__ __launch_bounds__(THREADS) void packed_merge_kernel(PackedArgs a) {
+    const PackedParams& p = a.p;
+    const uint32_t slot = blockIdx.x, kvh = blockIdx.y;
+    Work x;
+    if (!find_work(a, slot, threadIdx.x & 63, x)) return;
+    const float* rec = a.records + (uint64_t(slot) * p.kvHeads + kvh) * a.splits * record_floats<D>();
+    const uint32_t unit = blockIdx.z * THREADS + threadIdx.x, r = unit / (D / 4), d = unit % (D / 4) * 4;
+    if (r >= ROWS_WG || x.row0 + r >= x.rows) return;
+    float m = -INFINITY;
+    for (uint32_t i = 0; i < a.splits; ++i) m = fmaxf(m, rec[i * record_floats<D>() + r]);
+    const float base = m == -INFINITY ? 0.0f : m;
+    float l = 0.0f;
+    floatx4 o = floatx4{0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll 4
+    for (uint32_t i = 0; i < a.splits; ++i) {
+        const float* at = rec + i * record_floats<D>();
+        const float f = exp2f(at[r] - base);
+        l += at[ROWS_WG + r] * f;
+        o += *reinterpret_cast<const floatx4*>(at + 2 * ROWS_WG + r * D + d) * f;
+    }
+    const uint64_t row = x.row0 + r;
+    const uint32_t token = uint32_t(row / a.group), head = kvh * a.group + uint32_t(row % a.group);
+    const float by = l == 0.0f ? 0.0f : 1.0f / l;
+    const float y[4] = {o[0] * by, o[1] * by, o[2] * by, o[3] * by};
+    put4(a, (uint64_t(x.first) + token) * p.outTokenStride + head * p.outHeadStride + d, y);
+}
+
+struct Shape { uint64_t slots, splits; };
+
+/* Few rows over many keys leave CUs idle: their keys are split over workgroups, whose
+   records a second launch joins. */
+Shape shape_of(const PackedParams& p) {
+    const uint64_t group = p.heads / p.kvHeads;
+    Shape s{};
+    s.slots = p.starts ? uint64_t(p.count) * group / ROWS_WG + p.documents : (uint64_t(p.count) * group + ROWS_WG - 1) / ROWS_WG;
+    const uint64_t each = s.slots * p.kvHeads, want = 512;
+    s.splits = 1;
+    if (each && each * 2 <= want) {
+        const uint64_t most = p.keyCount / 512;            // keys of a split, at the least, were there one document
+        s.splits = std::min(want / each, std::max<uint64_t>(most, 1));
+    }
+    return s;
+}
+
+/* whether two tensors [tokens][heads][dim] (bytes between tokens and heads) may share an element */
+struct Extent { uintptr_t at; uint64_t tokens, token, heads, head, row; };
+bool may_meet(const Extent& a, const Extent& b) {
+    if (!a.tokens || !b.tokens) return false;
+    const uint64_t ra = (a.heads - 1) * a.head + a.row, rb = (b.heads - 1) * b.head + b.row;
+    if (a.at >= b.at + (b.tokens - 1) * b.token + rb || b.at >= a.at + (a.tokens - 1) * a.token + ra) return false;
+    // rows of one token side by side in the same wider rows
+    if (a.token != b.token || !a.token) return true;
+    const uint64_t gap = b.at >= a.at ? (b.at - a.at) % a.token : (a.token - (a.at - b.at) % a.token) % a.token;
+    return !(gap >= ra && a.token - gap >= rb);
+}
+
+} // namespace
+
+bool check_packed_attention(const PackedParams& p) {
+    Context& ctx = Context::instance();
+    if (p.dim != 64 && p.dim != 96 && p.dim != 128 && p.dim != 192 && p.dim != 256)
+        return ctx.fail("packed attention: dim must be 64, 96, 128, 192 or 256");
+    if (p.inType < 0 || p.outType < 0) return ctx.fail("packed attention: unknown element type");
+    if (p.heads == 0 || p.kvHeads == 0 || p.heads % p.kvHeads)
+        return ctx.fail("packed attention: heads must be a multiple of kvHeads");
+    if (!p.starts && p.documents != 1) return ctx.fail("packed attention: without starts there is one document");
+    if (!p.starts && p.keyStarts) return ctx.fail("packed attention: keyStarts without starts");
+    if (p.starts && !p.keyStarts && p.keyCount != p.count)
+        return ctx.fail("packed attention: without keyStarts there are as many keys as tokens");
+    if (!(p.scale > 0.0f) || !std::isfinite(p.scale))
+        return ctx.fail("packed attention: the scale must be positive and finite");
+    if (p.cap < 0.0f || !std::isfinite(p.cap))
+        return ctx.fail("packed attention: the cap must be finite and not negative");
+    for (uint64_t s : {p.qTokenStride, p.qHeadStride, p.kTokenStride, p.kHeadStride, p.vTokenStride, p.vHeadStride,
+                       p.outTokenStride, p.outHeadStride})
+        if (s >= (uint64_t(1) << 40)) return ctx.fail("packed attention: a stride is out of range");
+    if (p.count == 0 || p.documents == 0) return true;
+    if (!p.q || !p.out || (p.keyCount && (!p.k || !p.v))) return ctx.fail("packed attention: null tensor");
+    const uint64_t es = p.inType == 1 ? 2 : 4, os = p.outType == 1 ? 2 : 4;
+    const uintptr_t in = reinterpret_cast<uintptr_t>(p.q) | reinterpret_cast<uintptr_t>(p.k) | reinterpret_cast<uintptr_t>(p.v);
+    const uint64_t strides = p.qTokenStride | p.qHeadStride | p.kTokenStride | p.kHeadStride | p.vTokenStride | p.vHeadStride;
+    if ((in & 15) || strides * es % 16) return ctx.fail("packed attention: rows of q, k and v must be 16-byte aligned");
+    if (reinterpret_cast<uintptr_t>(p.out) & (os - 1)) return ctx.fail("packed attention: out must be aligned to its elements");
+    if ((reinterpret_cast<uintptr_t>(p.starts) | reinterpret_cast<uintptr_t>(p.keyStarts) |
+         reinterpret_cast<uintptr_t>(p.prefix) | reinterpret_cast<uintptr_t>(p.slopes)) & 3)
+        return ctx.fail("packed attention: the vectors must be aligned to their elements");
+    const uint64_t ot = p.outTokenStride, oh = p.outHeadStride, D = p.dim;
+    const bool tokensApart = (p.count == 1 || ot >= (p.heads - 1) * oh + D) && (p.heads == 1 || oh >= D);
+    const bool headsApart = (p.heads == 1 || oh >= (p.count - 1) * ot + D) && (p.count == 1 || ot >= D);
+    if (!tokensApart && !headsApart) return ctx.fail("packed attention: the rows of out overlap");
+    const Extent out{reinterpret_cast<uintptr_t>(p.out), p.count, ot * os, p.heads, oh * os, D * os};
+    for (const Extent& e : {Extent{reinterpret_cast<uintptr_t>(p.q), p.count, p.qTokenStride * es, p.heads, p.qHeadStride * es, D * es},
+                            Extent{reinterpret_cast<uintptr_t>(p.k), p.keyCount, p.kTokenStride * es, p.kvHeads, p.kHeadStride * es, D * es},
+                            Extent{reinterpret_cast<uintptr_t>(p.v), p.keyCount, p.vTokenStride * es, p.kvHeads, p.vHeadStride * es, D * es}})
+        if (may_meet(out, e)) return ctx.fail("packed attention: out overlaps q, k or v");
+    const Shape s = shape_of(p);
+    if (s.slots * s.splits * p.kvHeads >= (uint64_t(1) << 31)) return ctx.fail("packed attention: too many rows");
+    return true;
+}
+
+size_t packed_attention_workspace(const PackedParams& p) {
+    if (p.count == 0 || p.documents == 0) return 0;
+    const Shape s = shape_of(p);
+    return s.splits > 1 ? s.slots * p.kvHeads * s.splits * ROWS_WG * (p.dim + 2) * sizeof(float) : 0;
+}
+
+bool launch_packed_attention(const PackedParams& p, void* work, hipStream_t stream) {
+    Context& ctx = Context::instance();
+    if (p.count == 0 || p.documents == 0) return true;
+    const Shape s = shape_of(p);
+    PackedArgs a{};
+    a.p = p;
+    a.group = p.heads / p.kvHeads;
+    a.slots = uint32_t(s.slots);
+    a.splits = uint32_t(s.splits);
+    a.records = s.splits > 1 ? static_cast<float*>(work) : nullptr;
+    a.capLog2 = p.cap * LOG2E;
+    a.factor = p.cap > 0.0f ? p.scale / p.cap : p.scale * LOG2E;
+    const uint64_t piece = p.outType == 1 ? 8 : 16, os = piece / 4;
+    a.wide = (reinterpret_cast<uintptr_t>(p.out) | p.outTokenStride * os | p.outHeadStride * os) % piece == 0;
+    const uint32_t grid = a.slots * p.kvHeads * a.splits;
+    auto of = [&](auto dim) {
+        constexpr int D = decltype(dim)::value;
+        auto go = [&](auto kernel) {
+            return ctx.launch("packed_attention_kernel", stream, [&] {
+                       hipLaunchKernelGGL(kernel, dim3(grid), dim3(THREADS), 0, stream, a);
+                   }) &&
+                   (!a.records || ctx.launch("packed_merge_kernel", stream, [&] {
+                       hipLaunchKernelGGL(packed_merge_kernel<D>, dim3(a.slots, p.kvHeads, ROWS_WG * (D / 4) / THREADS),
+                                          dim3(THREADS), 0, stream, a);
+                   }));
+        };
+        if (p.inType != 1) return go(packed_attention_kernel<D, FULL>);
+        return p.outType == 1 ? go(packed_attention_kernel<D, BF16_OUT>) : go(packed_attention_kernel<D, BF16_F32>);
+    };
+    switch (p.dim) {
+        case 64: return of(std::integral_constant<int, 64>{});
+        case 96: return of(std::integral_constant<int, 96>{});
+        case 128: return of(std::integral_constant<int, 128>{});
+        case 192: return of(std::integral_constant<int, 192>{});
+        default: return of(std::integral_constant<int, 256>{});
+    }
+}
+
+} // namespace aigpu

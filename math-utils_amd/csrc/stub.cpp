@@ -70,6 +70,8 @@ AIGPU_ABI int aigpu_rotary_frequencies(const AiGpuRotaryScaling*, float*, float*
 AIGPU_ABI int aigpu_paged_append(const AiGpuPagedAppend*) { return 0; }
 AIGPU_ABI int aigpu_paged_decode(const AiGpuPagedDecode*) { return 0; }
 AIGPU_ABI uint64_t aigpu_paged_decode_workspace(const AiGpuPagedDecode*) { return 0; }
+AIGPU_ABI int aigpu_packed_attention(const AiGpuPackedAttention*) { return 0; }
+AIGPU_ABI uint64_t aigpu_packed_attention_workspace(const AiGpuPackedAttention*) { return 0; }
 AIGPU_ABI int aigpu_paged_decode_scored(const AiGpuPagedDecode*, const AiGpuScores*) { return 0; }
 AIGPU_ABI int aigpu_paged_append_q4(const AiGpuPagedAppendQ4*) { return 0; }
 AIGPU_ABI int aigpu_paged_read_q4(const AiGpuPagedReadQ4*) { return 0; }
