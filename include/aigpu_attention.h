@@ -769,7 +769,7 @@ AIGPU_ABI uint64_t aigpu_paged_decode_q4_workspace(const AiGpuPagedDecodeQ4* arg
 /*    and values has to be finite, rows of no document may hold anything.      */
 /*    Types: q, k, v of inType, out of outType. bf16 to bf16 rounds the        */
 /*    weights to bf16 (their sum adds the rounded ones) and the result once;   */
-/*    bf16 to fp32 takes the weights in two terms, 2^-16 of each; fp32 is fp32 */
+/*    bf16 to fp32 takes the weights whole, in three terms; fp32 is fp32       */
 /*    throughout. Rows of q, k and v are 16-byte aligned. No counterpart in    */
 /*    the reference, whose call is one sequence's. Asynchronous.               */
 /* ------------------------------------------------------------------------ */

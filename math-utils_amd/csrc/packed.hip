@@ -26,7 +26,7 @@ namespace {
     of 8 keys, which is how the second product takes them.
 
     bf16 in, bf16 out: the weights round to bf16, and the sum adds up the rounded ones.
-    bf16 in, fp32 out: the weights in two bf16 terms (2^-16 of each at most).
+    bf16 in, fp32 out: the weights in three bf16 terms, whose sum they are.
     fp32 in: fp32 products (v_mfma_f32_32x32x2_f32), for which the keys' order is the plain one.
 */
 constexpr int WAVES = 4, THREADS = 64 * WAVES, ROWS_WG = 32 * WAVES;
@@ -147,7 +147,7 @@ __device__ __forceinline__ void put4(const PackedArgs& a, uint64_t at, const flo
 }
 
 constexpr int tile_keys(int D, int kind) { return kind == FULL ? (D <= 96 ? 64 : 32) : (D <= 128 ? 64 : 32); }
-constexpr int workgroups(int D, int kind) { return D <= (kind == FULL ? 96 : 128) ? 2 : 1; }
+constexpr int workgroups(int D, int kind) { return D <= (kind == FULL ? 64 : 128) ? 2 : 1; }
 
 template <int D, int KIND>
 __global__ __launch_bounds__(THREADS, workgroups(D, KIND)) void packed_attention_kernel(PackedArgs a) {
@@ -329,19 +329,26 @@ __global__ __launch_bounds__(THREADS, workgroups(D, KIND)) void packed_attention
             } else {
 #pragma unroll
                 for (int h = 0; h < 2; ++h) {
-                    u32x4 hi4, lo4;
+                    constexpr int TERMS = KIND == BF16_F32 ? 3 : 1;
+                    u32x4 term[TERMS];
 #pragma unroll
                     for (int j = 0; j < 4; ++j) {
                         const float e0 = __builtin_amdgcn_exp2f(s[kb][8 * h + 2 * j] - base);
                         const float e1 = __builtin_amdgcn_exp2f(s[kb][8 * h + 2 * j + 1] - base);
-                        const uint32_t both = pack_bf16(e0, e1);
-                        hi4[j] = both;
-                        const float f0 = __uint_as_float(both << 16), f1 = __uint_as_float(both & 0xFFFF0000u);
                         if constexpr (KIND == BF16_F32) {
-                            lo4[j] = pack_bf16(e0 - f0, e1 - f1);
                             l += e0 + e1;
+                            float f0 = e0, f1 = e1;          // each term takes the next 8 bits
+#pragma unroll
+                            for (int t = 0; t < TERMS; ++t) {
+                                const uint32_t u0 = __float_as_uint(f0), u1 = __float_as_uint(f1);
+                                term[t][j] = __builtin_amdgcn_perm(u1, u0, 0x07060302);
+                                f0 -= __uint_as_float(u0 & 0xFFFF0000u);
+                                f1 -= __uint_as_float(u1 & 0xFFFF0000u);
+                            }
                         } else {
-                            l += f0 + f1;
+                            const uint32_t both = pack_bf16(e0, e1);
+                            term[0][j] = both;
+                            l += __uint_as_float(both << 16) + __uint_as_float(both & 0xFFFF0000u);
                         }
                     }
                     // V^T rows 32 dt + c: lane q16 of each 16 addresses row 16 g + 8 h + q16 / 4, and 4 on
@@ -351,9 +358,9 @@ __global__ __launch_bounds__(THREADS, workgroups(D, KIND)) void packed_attention
                         const int d = 32 * dt + 16 * (lane >> 4 & 1) + 4 * (q16 & 3);
                         const uint16_t* at = vtile[stage] + vr * D + 8 * ((d >> 3) ^ value_swizzle<BYTES>(vr)) + (d & 7);
                         const bf16x8 v = read_transposed(at, at + 4 * D);
-                        if constexpr (KIND == BF16_F32)
-                            o[dt] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(v, __builtin_bit_cast(bf16x8, lo4), o[dt], 0, 0, 0);
-                        o[dt] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(v, __builtin_bit_cast(bf16x8, hi4), o[dt], 0, 0, 0);
+#pragma unroll
+                        for (int t = TERMS - 1; t >= 0; --t)
+                            o[dt] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(v, __builtin_bit_cast(bf16x8, term[t]), o[dt], 0, 0, 0);
                     }
                 }
             }

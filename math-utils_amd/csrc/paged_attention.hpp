@@ -64,6 +64,7 @@ struct DecodeArgs {
     uint32_t* plan;                  // [MAXB + 1] units before each sequence, and in all; null: joined in the kernel
     float* records;                  // [runs][2] of record_floats
     uint32_t groups, perGroup;       // of one kv head's query heads
+    uint32_t pageMagic, pageShift;   // pos / pageSize = pos pageMagic >> pageShift (pos below 2^31)
     float scaleLog2;                 // of q: the scores in units of ln 2; with a cap, as its fractions
     float capLog2;                   // the cap in units of ln 2, 0: none
     int wideQ;                       // q rows can be read 16 bytes at a time
@@ -323,34 +324,38 @@ __device__ __forceinline__ half2v scale_of(uint16_t bits, half2v& off) {
     off = half2v{s, s} * half2v{_Float16(-24.0f), _Float16(-24.0f)};
     return half2v{s, s};
 }
-template <int I>
-__device__ __forceinline__ half2v shifted(uint32_t word) {
-    const uint32_t at = I == 0 ? word << 6 : (I == 1 ? word << 2 : (I == 2 ? word >> 2 : word >> 6));
-    return __builtin_bit_cast(half2v, (at & 0x03C003C0u) | 0x4C004C00u);
-}
+/* the unpacking's constants, in registers: an instruction takes no two literals */
+struct Unpack {
+    uint32_t mask = 0x03C003C0u, sixteen = 0x4C004C00u;
+    __device__ __forceinline__ Unpack() { asm("" : "+v"(mask), "+s"(sixteen)); }
+    __device__ __forceinline__ half2v pair(uint32_t at) const {
+        return __builtin_bit_cast(half2v, (at & mask) | sixteen);
+    }
+};
 __device__ __forceinline__ half8 joined(half2v a, half2v b, half2v c, half2v d) {
     return half8{a[0], a[1], b[0], b[1], c[0], c[1], d[0], d[1]};
 }
-__device__ __forceinline__ half8 values_of(uint32_t word, half2v by, half2v off) {
-    return joined(__builtin_elementwise_fma(shifted<0>(word), by, off), __builtin_elementwise_fma(shifted<1>(word), by, off),
-                  __builtin_elementwise_fma(shifted<2>(word), by, off), __builtin_elementwise_fma(shifted<3>(word), by, off));
+__device__ __forceinline__ half8 values_of(const Unpack& u, uint32_t word, half2v by, half2v off) {
+    return joined(__builtin_elementwise_fma(u.pair(word << 6), by, off), __builtin_elementwise_fma(u.pair(word << 2), by, off),
+                  __builtin_elementwise_fma(u.pair(word >> 2), by, off), __builtin_elementwise_fma(u.pair(word >> 6), by, off));
 }
 /* a word of eight rows' codes of one column, with their scales in pairs alike */
-__device__ __forceinline__ half8 values_of(uint32_t word, u32x4 scales) {
-    half2v by[4], off[4];
+__device__ __forceinline__ half8 values_of(const Unpack& u, uint32_t word, const half2v (&by)[4], const half2v (&off)[4]) {
+    return joined(__builtin_elementwise_fma(u.pair(word << 6), by[0], off[0]), __builtin_elementwise_fma(u.pair(word << 2), by[1], off[1]),
+                  __builtin_elementwise_fma(u.pair(word >> 2), by[2], off[2]), __builtin_elementwise_fma(u.pair(word >> 6), by[3], off[3]));
+}
+__device__ __forceinline__ void scales_of(u32x4 scales, half2v (&by)[4], half2v (&off)[4]) {
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
         const uint32_t pair = scales[i];             // (the cast of an element in place takes the first one)
         by[i] = __builtin_bit_cast(half2v, pair);
         off[i] = by[i] * half2v{_Float16(-24.0f), _Float16(-24.0f)};
     }
-    return joined(__builtin_elementwise_fma(shifted<0>(word), by[0], off[0]), __builtin_elementwise_fma(shifted<1>(word), by[1], off[1]),
-                  __builtin_elementwise_fma(shifted<2>(word), by[2], off[2]), __builtin_elementwise_fma(shifted<3>(word), by[3], off[3]));
 }
 /* two fp32 values as pairs of fp16 terms: the nearest, then what it leaves */
 __device__ __forceinline__ u32x2 split_f16(float a, float b) {
     const half2v hi = __builtin_convertvector(float2v{a, b}, half2v);
-    const half2v lo = __builtin_convertvector(float2v{a - float(hi[0]), b - float(hi[1])}, half2v);
+    const half2v lo = __builtin_convertvector(float2v{fmaf(float(hi[0]), -1.0f, a), fmaf(float(hi[1]), -1.0f, b)}, half2v);
     return u32x2{__builtin_bit_cast(uint32_t, hi), __builtin_bit_cast(uint32_t, lo)};
 }
 /* N words of a row from an address of 4 bytes' alignment */
@@ -403,6 +408,15 @@ __device__ __forceinline__ int code_swizzle(int r) {
     else if constexpr (D == 128) return r >> 4 & 3;
     else if constexpr (D == 64 || D == 192) return r >> 4 & 1;
     else return 0;
+}
+
+/* The kernel's arguments, read where they are used: kept in scalar registers over the
+   loop, those that it does not need push out (through vector lanes) those that it does. */
+__device__ __forceinline__ const DecodeArgs& arguments() {
+    typedef const __attribute__((address_space(4))) DecodeArgs constant_args;
+    constant_args* at = (constant_args*)__builtin_amdgcn_kernarg_segment_ptr();
+    asm("" : "+s"(at));
+    return *(const DecodeArgs*)at;
 }
 
 template <int D, bool BF, int FORM>
@@ -523,42 +537,55 @@ __global__ __launch_bounds__(THREADS, occupancy(D, FORM)) void paged_attention_k
         return true;
     };
 
+    auto cold = [&]() -> const DecodeArgs& {
+        if constexpr (CODES) return arguments();
+        else return a;
+    };
+
     // ---- the stages of a slab ----
     // its page ids: lane r (of SLAB) holds row r's; rows outside the attended
     // range stand at its ends, so that nothing else is read
     struct Rows { uint32_t page, row; };
     auto find = [&](const Slab& s, Rows& r) {
+        const DecodeArgs& a = cold();
+        const PagedCache& c = a.p.c;
         uint32_t pos = s.pos + (lane & (SLAB - 1));
         pos = pos < s.first ? s.first : (pos < s.len ? pos : s.len - 1);
-        const uint32_t slot = pos / c.pageSize;
+        const uint32_t slot = CODES ? uint32_t(uint64_t(pos) * a.pageMagic >> a.pageShift) : pos / c.pageSize;
         r.row = pos - slot * c.pageSize;
         r.page = c.table[s.b * c.tableStride + slot];
     };
     // its keys into registers (A operands: row lane % 16, 8 elements a lane),
     // its values into LDS; false where a page lies outside the pool (its rows
     // are then read from page 0)
+    struct Chunk {                   // the j-th 16 bytes of a lane among a slab's rows of DB each
+        uint32_t row, block;
+        __device__ __forceinline__ Chunk(uint32_t j, uint32_t lane) {
+            if constexpr (WAVE % DB == 0) row = WAVE / DB * j + lane / DB, block = lane % DB;
+            else row = (WAVE * j + lane) / DB, block = (WAVE * j + lane) % DB;
+        }
+    };
     constexpr int KRB = CODES ? 4 : 2, KRD = CODES ? (DB + 3) / 4 : DB;
     u32x4 kr[KRB][KRD];              // keys: rows 16 rb + lane % 16
     u32x4 vr[CODES ? DB : 1];        // 4-bit values: 16 bytes a lane, row after row
     uint32_t ksr[CODES ? (DB + 1) / 2 : 1], vsr[CODES ? (DB + 1) / 2 : 1];   // row `lane`'s scales
     auto issue = [&](const Slab& s, const Rows& r, int half) -> bool {
+        const DecodeArgs& a = cold();
+        const PagedDecodeParams& p = a.p;
+        const PagedCache& c = p.c;
         const int lane = fresh_lane(threadIdx.x & 63), g = lane >> 4, c16 = lane & 15;
         const bool ok = r.page < c.pages;
         const uint64_t mine = (ok ? uint64_t(r.page) * c.pageStride + uint64_t(r.row) * c.rowStride : 0) +
                               uint64_t(s.pair / a.groups) * c.headStride;
         wave_sync();
-        if (lane < SLAB) place[w][lane] = mine;
+        if (lane < SLAB) place[w][lane] = CODES ? mine * (D / 2) : mine;
         wave_sync();
         if constexpr (CODES) {
-            const char* keys = reinterpret_cast<const char*>(c.keys);
             const char* values = reinterpret_cast<const char*>(c.values);
 #pragma unroll
-            for (int rb = 0; rb < KRB; ++rb)
-                read_words<DB>(keys + place[w][16 * rb + c16] * (D / 2) + g * (D / 8), kr[rb]);
-#pragma unroll
             for (int j = 0; j < DB; ++j) {
-                const int i = j * WAVE + lane, row = i / DB, chunk = i % DB;
-                vr[j] = *reinterpret_cast<const u32x4*>(values + place[w][row] * (D / 2) + 16 * chunk);
+                const Chunk at(j, lane);
+                vr[j] = *reinterpret_cast<const u32x4*>(values + place[w][at.row] + 16 * at.block);
             }
             read_scales<DB>(p.keyScales + mine * DB, ksr);
             read_scales<DB>(p.valueScales + mine * DB, vsr);
@@ -578,19 +605,32 @@ __global__ __launch_bounds__(THREADS, occupancy(D, FORM)) void paged_attention_k
         }
         return __all(ok);
     };
+    // 4-bit rows: the keys apart, as the scores free their registers later
+    auto issue_keys = [&] {
+        const PagedCache& c = cold().p.c;
+        const int lane = fresh_lane(threadIdx.x & 63), g = lane >> 4, c16 = lane & 15;
+        const char* keys = reinterpret_cast<const char*>(c.keys) + g * (D / 8);
+#pragma unroll
+        for (int rb = 0; rb < KRB; ++rb) read_words<DB>(keys + place[w][16 * rb + c16], kr[rb]);
+    };
     // 4-bit rows: the values and both scales from the registers into LDS
     auto stage = [&] {
         if constexpr (CODES) {
-            const int lane = fresh_lane(threadIdx.x & 63);
 #pragma unroll
             for (int j = 0; j < DB; ++j) {
-                const int i = j * WAVE + lane, row = i / DB, chunk = (i % DB) ^ code_swizzle<D>(row);
-                *reinterpret_cast<u32x4*>(vbuf[w][0] + (row * DB + chunk) * 8) = vr[j];
+                const Chunk at(j, lane);
+                *reinterpret_cast<u32x4*>(vbuf[w][0] + (at.row * DB + (at.block ^ code_swizzle<D>(at.row))) * 8) = vr[j];
+            }
+            if constexpr (DB % 2 == 0) {
+#pragma unroll
+                for (int i = 0; i < DB / 2; ++i) reinterpret_cast<uint32_t*>(kscales[w] + lane * DB)[i] = ksr[i];
+            } else {
+#pragma unroll
+                for (int b = 0; b < DB; ++b) kscales[w][lane * DB + b] = uint16_t(ksr[b / 2] >> 16 * (b & 1));
             }
             uint16_t* pairs = reinterpret_cast<uint16_t*>(vscales[w]);
 #pragma unroll
             for (int b = 0; b < DB; ++b) {
-                kscales[w][lane * DB + b] = uint16_t(ksr[b / 2] >> 16 * (b & 1));
                 // rows 16 rb + 4 g + i of even and odd rb are pairs
                 pairs[((b * 2 + (lane >> 5)) * 16 + (lane & 15)) * 2 + (lane >> 4 & 1)] =
                     uint16_t(vsr[b / 2] >> 16 * (b & 1));
@@ -603,6 +643,8 @@ __global__ __launch_bounds__(THREADS, occupancy(D, FORM)) void paged_attention_k
     constexpr int RAW = BF ? 1 : 2;
     u32x4 raw[DB][RAW];
     auto ask = [&](const Slab& s) {
+        const DecodeArgs& a = cold();
+        const PagedDecodeParams& p = a.p;
         const int lane = fresh_lane(threadIdx.x & 63), g = lane >> 4, c16 = lane & 15;
         const uint32_t group = s.pair % a.groups, kvh = s.pair / a.groups;
         const uint32_t h = group * a.perGroup + c16;
@@ -643,6 +685,8 @@ __global__ __launch_bounds__(THREADS, occupancy(D, FORM)) void paged_attention_k
     // `spare` holds 16 rows in LDS, element d of row r at d ^ 4 (r % 8), so that
     // a column of them is spread over the banks
     auto prepare = [&](const Slab& s, float* spare) {
+        const DecodeArgs& a = cold();
+        const PagedDecodeParams& p = a.p;
         const int lane = fresh_lane(threadIdx.x & 63), g = lane >> 4, c16 = lane & 15;
         const uint32_t group = s.pair % a.groups;
         const bool live = uint32_t(c16) < a.perGroup && group * a.perGroup + c16 < G;
@@ -796,7 +840,9 @@ __global__ __launch_bounds__(THREADS, occupancy(D, FORM)) void paged_attention_k
     floatx4 acc[CT];                 // [tile][r]: head 4 g + r, column 16 tile + c16
     bool bad = false, begun = false;
     float sv[KRB][4];                // scores: of head c16 at positions 16 rb + 4 g + i
+    float svBy = 1.0f;
     auto score = [&](const Slab& s) {
+        const Unpack unpack;
         const int lane = fresh_lane(threadIdx.x & 63), g = lane >> 4, c16 = lane & 15;
 #pragma unroll
         for (int rb = 0; rb < KRB; ++rb) {
@@ -808,7 +854,7 @@ __global__ __launch_bounds__(THREADS, occupancy(D, FORM)) void paged_attention_k
                 for (int db = 0; db < DB; ++db) {
                     // word g DB + db of the row, of block (g DB + db) / 4
                     if (db == 0 || (DB % 4 == 0 ? db % 4 == 0 : DB != 2)) by = scale_of(scales[(g * DB + db) / 4], off);
-                    const half8 k = values_of(kr[rb][db / 4][db % 4], by, off);
+                    const half8 k = values_of(unpack, kr[rb][db / 4][db % 4], by, off);
                     sc = __builtin_amdgcn_mfma_f32_16x16x32_f16(k, qb[db][1], sc, 0, 0, 0);
                     sc = __builtin_amdgcn_mfma_f32_16x16x32_f16(k, qb[db][0], sc, 0, 0, 0);
                 }
@@ -820,46 +866,84 @@ __global__ __launch_bounds__(THREADS, occupancy(D, FORM)) void paged_attention_k
                         sc = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, kr[rb][db]), qb[db][k],
                                                                      sc, 0, 0, 0);
             }
+            if constexpr (CODES) {
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                const uint32_t pos = s.pos + 16 * rb + 4 * g + i;
-                float x = sc[i];
-                if constexpr (CODES) x *= qpow;
-                if constexpr (scored(FORM)) {
-                    if (a.capLog2 != 0.0f) x = a.capLog2 * tanh_of(x);
-                    if (p.slopes) x -= slope * float(s.len - 1 - pos);
+                for (int i = 0; i < 4; ++i) sv[rb][i] = sc[i];
+            } else {
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const uint32_t pos = s.pos + 16 * rb + 4 * g + i;
+                    float x = sc[i];
+                    if constexpr (scored(FORM)) {
+                        if (a.capLog2 != 0.0f) x = a.capLog2 * tanh_of(x);
+                        if (p.slopes) x -= slope * float(s.len - 1 - pos);
+                    }
+                    sv[rb][i] = pos >= s.first && pos < s.len ? x : -INFINITY;
                 }
-                sv[rb][i] = pos >= s.first && pos < s.len ? x : -INFINITY;
+            }
+        }
+        if constexpr (CODES) {
+            svBy = qpow;             // what takes sv to scores: left to the exponentials where nothing comes between
+            if (a.capLog2 != 0.0f || p.slopes) {
+                svBy = 1.0f;
+                const float apart = float(s.len - 1 - s.pos - 4 * g);
+                if (a.capLog2 != 0.0f) {
+#pragma unroll
+                    for (int i = 0; i < 16; ++i) sv[i >> 2][i & 3] = a.capLog2 * tanh_of(sv[i >> 2][i & 3] * qpow);
+                } else {
+#pragma unroll
+                    for (int i = 0; i < 16; ++i) sv[i >> 2][i & 3] *= qpow;
+                }
+                if (p.slopes) {
+#pragma unroll
+                    for (int i = 0; i < 16; ++i) sv[i >> 2][i & 3] -= slope * (apart - float(16 * (i >> 2) + (i & 3)));
+                }
+            }
+            if (s.pos < s.first || s.pos + SLAB > s.len) {
+#pragma unroll
+                for (int i = 0; i < 16; ++i) {
+                    const uint32_t pos = s.pos + 16 * (i >> 2) + 4 * g + (i & 3);
+                    sv[i >> 2][i & 3] = pos >= s.first && pos < s.len ? sv[i >> 2][i & 3] : -INFINITY;
+                }
             }
         }
     };
     auto weigh = [&](int bufHalf, bool nextInFlight) {
         const int lane = fresh_lane(threadIdx.x & 63), g = lane >> 4, c16 = lane & 15;
-        float top = -INFINITY;
-#pragma unroll
-        for (int i = 0; i < 4 * KRB; ++i) top = fmaxf(top, sv[i >> 2][i & 3]);
-        top = fmaxf(top, __shfl_xor(top, 16, WAVE));
-        top = fmaxf(top, __shfl_xor(top, 32, WAVE));
-        const float next = fmaxf(m, top), base = next == -INFINITY ? 0.0f : next;
-        const float keep = exp2f(m - base);
-        float pv[4 * KRB], sum = 0.0f;
-        // 4-bit rows: weights up to 2^14, as the queries (their sums carry it too)
-        const float under = CODES ? base - 14.0f : base;
-#pragma unroll
-        for (int i = 0; i < 4 * KRB; ++i) {
-            pv[i] = exp2f(sv[i >> 2][i & 3] - under);
-            sum += pv[i];
-        }
-        l = l * keep + sum;
-        m = next;
-        float rk[4];
-#pragma unroll
-        for (int r = 0; r < 4; ++r) rk[r] = __shfl(keep, 4 * g + r, WAVE);
-#pragma unroll
-        for (int t = 0; t < CT; ++t)
-#pragma unroll
-            for (int r = 0; r < 4; ++r) acc[t][r] *= rk[r];
         if constexpr (CODES) {
+            const Unpack unpack;
+            float top = sv[0][0];
+#pragma unroll
+            for (int i = 1; i < 16; ++i) top = fmaxf(top, sv[i >> 2][i & 3]);
+            top = fmaxf(top, __shfl_xor(top, 16, WAVE));
+            top = fmaxf(top, __shfl_xor(top, 32, WAVE)) * svBy;
+            // weights of 2^6, and up to 2^14 before the maximum is taken up anew (their sum
+            // carries it too): the second fp16 term of small ones stays above fp16's least
+            const bool grow = top > m + 8.0f;
+            const float next = grow ? top : m;
+            if (__any(grow)) {
+                const float keep = grow ? __builtin_amdgcn_exp2f(m - next) : 1.0f;
+                l *= keep;
+                float rk[4];
+#pragma unroll
+                for (int r = 0; r < 4; ++r) rk[r] = __shfl(keep, 4 * g + r, WAVE);
+#pragma unroll
+                for (int t = 0; t < CT; ++t)
+#pragma unroll
+                    for (int r = 0; r < 4; ++r) acc[t][r] *= rk[r];
+            }
+            // (the accumulators stay where they are on both ways here)
+#pragma unroll
+            for (int t = 0; t < CT; ++t) asm("" : "+v"(acc[t]));
+            m = next;
+            const float under = (next == -INFINITY ? 0.0f : next) - 6.0f;
+            float pv[16], sum = 0.0f;
+#pragma unroll
+            for (int i = 0; i < 16; ++i) {
+                pv[i] = __builtin_amdgcn_exp2f(fmaf(sv[i >> 2][i & 3], svBy, -under));
+                sum += pv[i];
+            }
+            l += sum;
             u32x4 hi[2], lo[2];
 #pragma unroll
             for (int h = 0; h < 2; ++h)
@@ -879,10 +963,11 @@ __global__ __launch_bounds__(THREADS, occupancy(D, FORM)) void paged_attention_k
                 for (int t = 0; t < 2; ++t) col[t] = read_codes(codes + (b ^ code_swizzle<D>(row)) * 8 + 4 * t);
 #pragma unroll
                 for (int h = 0; h < 2; ++h) {
-                    const u32x4 by = *reinterpret_cast<const u32x4*>(vscales[w] + (b * 2 + h) * 16 + 4 * g);
+                    half2v by[4], off[4];
+                    scales_of(*reinterpret_cast<const u32x4*>(vscales[w] + (b * 2 + h) * 16 + 4 * g), by, off);
 #pragma unroll
                     for (int t = 0; t < 2; ++t) {
-                        const half8 v = values_of(col[t][h], by);
+                        const half8 v = values_of(unpack, col[t][h], by, off);
                         floatx4& x = acc[2 * b + t];
                         x = __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(half8, lo[h]), v, x, 0, 0, 0);
                         x = __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(half8, hi[h]), v, x, 0, 0, 0);
@@ -890,34 +975,55 @@ __global__ __launch_bounds__(THREADS, occupancy(D, FORM)) void paged_attention_k
                 }
             }
             return;
-        } else {
-            u32x4 pa[3];
-            split3(pv, pa);
-            // this slab's values have landed: at most the next slab's loads are out
-            if (nextInFlight) wait_loads<2 * DB + VLOADS>();
-            else wait_loads<0>();
-            wave_sync();
-            // lane c16 of group g gets column 16 t + c16 of rows 4 g + 0..3, then 16 + 4 g + 0..3
-            const uint16_t* vs = vbuf[w][bufHalf];
-            const int r0 = 4 * g + (c16 >> 2), r1 = r0 + 16, x0 = (c16 >> 1) & 1, sub = 4 * (c16 & 1);
-            constexpr int BATCH = CT % 4 == 0 ? 4 : 2;       // tiles whose reads go out together
+        }
+        float top = -INFINITY;
 #pragma unroll
-            for (int t0 = 0; t0 < CT; t0 += BATCH) {
-                bf16v4 lo[BATCH], hi[BATCH];
+        for (int i = 0; i < 8; ++i) top = fmaxf(top, sv[i >> 2][i & 3]);
+        top = fmaxf(top, __shfl_xor(top, 16, WAVE));
+        top = fmaxf(top, __shfl_xor(top, 32, WAVE));
+        const float next = fmaxf(m, top), base = next == -INFINITY ? 0.0f : next;
+        const float keep = exp2f(m - base);
+        float pv[8], sum = 0.0f;
 #pragma unroll
-                for (int t = 0; t < BATCH; ++t) {
-                    const int x = 2 * (t0 + t) + x0;
-                    lo[t] = read_transposed(vs + r0 * D + 8 * (x ^ value_swizzle<D>(r0)) + sub);
-                    hi[t] = read_transposed(vs + r1 * D + 8 * (x ^ value_swizzle<D>(r1)) + sub);
-                }
+        for (int i = 0; i < 8; ++i) {
+            pv[i] = exp2f(sv[i >> 2][i & 3] - base);
+            sum += pv[i];
+        }
+        l = l * keep + sum;
+        m = next;
+        float rk[4];
 #pragma unroll
-                for (int k = 2; k >= 0; --k)
+        for (int r = 0; r < 4; ++r) rk[r] = __shfl(keep, 4 * g + r, WAVE);
 #pragma unroll
-                    for (int t = 0; t < BATCH; ++t)
-                        acc[t0 + t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(
-                            __builtin_bit_cast(bf16x8, pa[k]), __builtin_shufflevector(lo[t], hi[t], 0, 1, 2, 3, 4, 5, 6, 7),
-                            acc[t0 + t], 0, 0, 0);
+        for (int t = 0; t < CT; ++t)
+#pragma unroll
+            for (int r = 0; r < 4; ++r) acc[t][r] *= rk[r];
+        u32x4 pa[3];
+        split3(pv, pa);
+        // this slab's values have landed: at most the next slab's loads are out
+        if (nextInFlight) wait_loads<2 * DB + VLOADS>();
+        else wait_loads<0>();
+        wave_sync();
+        // lane c16 of group g gets column 16 t + c16 of rows 4 g + 0..3, then 16 + 4 g + 0..3
+        const uint16_t* vs = vbuf[w][bufHalf];
+        const int r0 = 4 * g + (c16 >> 2), r1 = r0 + 16, x0 = (c16 >> 1) & 1, sub = 4 * (c16 & 1);
+        constexpr int BATCH = CT % 4 == 0 ? 4 : 2;       // tiles whose reads go out together
+#pragma unroll
+        for (int t0 = 0; t0 < CT; t0 += BATCH) {
+            bf16v4 lo[BATCH], hi[BATCH];
+#pragma unroll
+            for (int t = 0; t < BATCH; ++t) {
+                const int x = 2 * (t0 + t) + x0;
+                lo[t] = read_transposed(vs + r0 * D + 8 * (x ^ value_swizzle<D>(r0)) + sub);
+                hi[t] = read_transposed(vs + r1 * D + 8 * (x ^ value_swizzle<D>(r1)) + sub);
             }
+#pragma unroll
+            for (int k = 2; k >= 0; --k)
+#pragma unroll
+                for (int t = 0; t < BATCH; ++t)
+                    acc[t0 + t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(
+                        __builtin_bit_cast(bf16x8, pa[k]), __builtin_shufflevector(lo[t], hi[t], 0, 1, 2, 3, 4, 5, 6, 7),
+                        acc[t0 + t], 0, 0, 0);
         }
     };
     // a pair's last slab of this run: the sum over lanes, then its output or,
@@ -925,12 +1031,16 @@ __global__ __launch_bounds__(THREADS, occupancy(D, FORM)) void paged_attention_k
     // registers, for the workgroup's join)
     const auto records = buffer_of(a.records);
     auto piece_of = [&](const Slab& s) {
+        const DecodeArgs& a = cold();
+        const PagedDecodeParams& p = a.p;
         const uint32_t h0 = s.pair % a.groups * a.perGroup, units = slabs_of<SLAB>(p, s.len) + OPENING;
         const uint32_t begin = uniform(pre[s.b]) + s.pair * units;
         return Piece{begin, begin + units, s.b, s.pair / a.groups * G + h0,
                      a.perGroup < G - h0 ? a.perGroup : G - h0};
     };
     auto finish = [&](const Slab& s, bool last) {
+        const DecodeArgs& a = cold();
+        const PagedDecodeParams& p = a.p;
         const int lane = fresh_lane(threadIdx.x & 63), g = lane >> 4, c16 = lane & 15;
         l += __shfl_xor(l, 16, WAVE);
         l += __shfl_xor(l, 32, WAVE);
@@ -940,6 +1050,7 @@ __global__ __launch_bounds__(THREADS, occupancy(D, FORM)) void paged_attention_k
         const Piece piece = piece_of(s);
         const uint32_t rows = piece.rows;
         if (!whole) {
+            const auto records = buffer_of(a.records);
             const uint32_t rec = run * 2 * record_floats(a.perGroup, D);
             auto put = [&](uint32_t at, float x) {
                 __builtin_amdgcn_raw_buffer_store_b32(__float_as_uint(x), records, (rec + at) * 4, 0, PAST_L2);
@@ -990,6 +1101,7 @@ __global__ __launch_bounds__(THREADS, occupancy(D, FORM)) void paged_attention_k
         if (more) find(s1, r1);
         ask(s0);
         ok0 = issue(s0, r0, 0);
+        if constexpr (CODES) issue_keys();
     }
     __builtin_amdgcn_sched_barrier(0);
 #pragma unroll 1
@@ -1005,14 +1117,26 @@ __global__ __launch_bounds__(THREADS, occupancy(D, FORM)) void paged_attention_k
             begun = s0.is & BEGINS;
         }
         bad |= !ok0;
-        stage();
-        score(s0);
-        __builtin_amdgcn_sched_barrier(0);
-        if (more) {
-            moreThen = list(s2);
-            if (moreThen) find(s2, r2);
-            if (s1.is & OPENS) ask(s1);
-            ok0 = issue(s1, r1, buf ^ 1);
+        auto ahead = [&] {
+            if (more) {
+                moreThen = list(s2);
+                if (moreThen) find(s2, r2);
+                if (s1.is & OPENS) ask(s1);
+                ok0 = issue(s1, r1, buf ^ 1);
+            }
+        };
+        if constexpr (CODES) {
+            stage();
+            __builtin_amdgcn_sched_barrier(0);
+            ahead();
+            __builtin_amdgcn_sched_barrier(0);
+            score(s0);
+            __builtin_amdgcn_sched_barrier(0);
+            if (more) issue_keys();
+        } else {
+            score(s0);
+            __builtin_amdgcn_sched_barrier(0);
+            ahead();
         }
         __builtin_amdgcn_sched_barrier(0);
         weigh(buf, more);
@@ -1207,6 +1331,12 @@ bool launch_decode_as(const char* name, const PagedDecodeParams& p, void* work, 
     a.perGroup = s.perGroup;
     a.capLog2 = scored(FORM) ? p.cap * LOG2E : 0.0f;
     a.scaleLog2 = a.capLog2 != 0.0f ? p.scale / p.cap : p.scale * LOG2E;
+    // division by multiplication, exact below 2^31: the least power of two that holds the
+    // page, and 2^31 times it over the page
+    uint32_t log = 0;
+    while ((uint64_t(1) << log) < p.c.pageSize) ++log;
+    a.pageShift = 31 + log;
+    a.pageMagic = uint32_t((uint64_t(1) << a.pageShift) / p.c.pageSize + 1);
     const size_t es = p.inType == 1 ? 2 : 4;
     a.wideQ = (reinterpret_cast<uintptr_t>(p.q) & 15) == 0 && (p.heads == 1 || p.qStride % (16 / es) == 0) &&
               (p.c.batch == 1 || p.qTokenStride % (16 / es) == 0);

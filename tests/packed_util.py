@@ -3,8 +3,8 @@ import numpy as np
 
 from paged_util import U
 
-# half a step of a weight, relative to it, before the sum and beyond it (the two-term weights' sum adds them whole)
-WEIGHT = {("bf16", "bf16"): 2.0 ** -8, ("bf16", "f32"): 2.0 ** -16, ("f32", "f32"): 0.0, ("f32", "bf16"): 0.0}
+# half a step of a weight, relative to it
+WEIGHT = {("bf16", "bf16"): 2.0 ** -8, ("bf16", "f32"): 0.0, ("f32", "f32"): 0.0, ("f32", "bf16"): 0.0}
 OUT = {"bf16": 2.0 ** -8, "f32": 2.0 ** -24}
 
 
@@ -13,8 +13,7 @@ def document64(q, k, v, dtype, out, prefix=0, window=0, cap=0.0, slopes=None, sc
 
     A score's products are exact or round once, and add as a random walk (eight deviations); the cap, the bias, the
     weights' exponential and the weighted sum add their roundings as scored64 says. A rounded weight moves the result
-    by its half step of the value's distance from the result, as the sum adds what was rounded (two terms: of the
-    value, as it does not)."""
+    by its half step of the value's distance from the result, as the sum adds what was rounded."""
     n, heads, dim = q.shape
     m, kv, _ = k.shape
     scale = scale or 1.0 / np.sqrt(dim)
@@ -50,10 +49,8 @@ def document64(q, k, v, dtype, out, prefix=0, window=0, cap=0.0, slopes=None, sc
         a = np.abs(vh)
         bound[:, h] = ((w * e) @ a + (w * e).sum(1, keepdims=True) * (w @ a) + (8 * np.sqrt(2.0 * m) + 64) * (w @ a)) * U
         step = WEIGHT[dtype, out]
-        if (dtype, out) == ("bf16", "bf16"):
+        if step:
             off = np.abs(vh[None] - res[:, h][:, None])
             bound[:, h] += 1.02 * step * np.einsum("ij,ijd->id", w, off)
-        else:
-            bound[:, h] += step * (w @ a)
         bound[:, h] += OUT[out] * np.abs(res[:, h])
     return res, bound
