@@ -38,6 +38,9 @@ struct PackedArgs {
     uint32_t group, slots, splits;   // query heads of a kv head; 128-row slots over all documents
     float factor;                    // the product to the scores' fractions of the cap, or to units of ln 2
     float capLog2;
+    float series[6];                 // capped scores in units of ln 2: s (series[0] + s^2 (series[1] + ...)) ...
+    float within;                    // ... for products s up to this
+    uint32_t fits;                   // tiles' rows lie within 31 bits of their first
     int wide;                        // out's rows can be written four elements at a time
 };
 
@@ -75,6 +78,19 @@ __device__ __forceinline__ bf16x8 read_transposed(const uint16_t* a0, const uint
     const bf16v4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4bf16((lds_bf16v4*)(a0));
     const bf16v4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4bf16((lds_bf16v4*)(a1));
     return __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
+}
+
+/* The cap's tanh as x (c0 + c1 x^2 + ...) up to 0.7, fitted for least relative error: 5e-6
+   where weights round to bf16, 1.4e-8 elsewhere. */
+constexpr int series_terms(int kind) { return kind == BF16_OUT ? 4 : 6; }
+constexpr float series_limit(int) { return 0.7f; }
+constexpr double SERIES4[4] = {0.999993310856002, -0.3328904637288124, 0.1286421024681964, -0.037290488627409184};
+constexpr double SERIES6[6] = {0.9999999863006178, -0.33333130413688367, 0.13328414724231763, -0.053526006423195875, 0.02002445111525679, -0.005088330528203937};
+
+/* acc plus both halves of a pair of bf16 values */
+__device__ __forceinline__ float add_pair(uint32_t pair, float acc) {
+    typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
+    return __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(bf16x2, pair), __builtin_bit_cast(bf16x2, 0x3F803F80u), acc, false);
 }
 
 /* A workgroup's document and rows. Document b owns the slots from starts[b] G / 128 + b on
@@ -219,23 +235,40 @@ __global__ __launch_bounds__(THREADS, workgroups(D, KIND)) void packed_attention
 
     const elem* keys = static_cast<const elem*>(p.k) + x.key0 * p.kTokenStride + kvh * p.kHeadStride;
     const elem* values = static_cast<const elem*>(p.v) + x.key0 * p.vTokenStride + kvh * p.vHeadStride;
+    // byte offsets of this lane's blocks from a tile's first row
+    uint32_t koff[BLOCKS], voff[BLOCKS];
+#pragma unroll
+    for (int n = 0; n < BLOCKS; ++n) {
+        const uint32_t i = (w * BLOCKS + n) * WAVE + lane, r = i / BPR, at = i % BPR;
+        const uint32_t kr = KIND == FULL ? r : (r & ~31u) + key_of_row(r & 31);
+        koff[n] = uint32_t(kr * p.kTokenStride * ES) + 16 * (at ^ key_swizzle<BYTES>(r));
+        voff[n] = uint32_t(r * p.vTokenStride * ES) + 16 * (KIND == FULL ? at : at ^ value_swizzle<BYTES>(r));
+    }
     auto issue = [&](uint32_t k0, int stage) {
-        const uint32_t kl = scalar(lds_address(ktile[stage])), vl = scalar(lds_address(vtile[stage]));
+        const uint32_t kl = scalar(lds_address(ktile[stage])) + w * BLOCKS * 1024, vl = scalar(lds_address(vtile[stage])) + w * BLOCKS * 1024;
+        if (a.fits && k0 + BN <= x.keys) {
+            const elem* kt = keys + k0 * p.kTokenStride;
+            const elem* vt = values + k0 * p.vTokenStride;
+#pragma unroll
+            for (int n = 0; n < BLOCKS; ++n) dma_block(kt, koff[n], kl + n * 1024);
+#pragma unroll
+            for (int n = 0; n < BLOCKS; ++n) dma_block(vt, voff[n], vl + n * 1024);
+            return;
+        }
+        // rows past the document's last key hold that one again
 #pragma unroll
         for (int n = 0; n < BLOCKS; ++n) {
-            const int i = (w * BLOCKS + n) * WAVE + lane, r = i / BPR, at = i % BPR;
-            // rows past the document's last key hold that one again
-            uint32_t key = k0 + (KIND == FULL ? r : (r & ~31) + key_of_row(r & 31));
+            const uint32_t i = (w * BLOCKS + n) * WAVE + lane, r = i / BPR, at = i % BPR;
+            uint32_t key = k0 + (KIND == FULL ? r : (r & ~31u) + key_of_row(r & 31));
             key = key < x.keys ? key : x.keys - 1;
-            dma_block(keys + key * p.kTokenStride + 16 / ES * (at ^ key_swizzle<BYTES>(r)), kl + (w * BLOCKS + n) * 1024);
+            dma_block(keys + key * p.kTokenStride + 16 / ES * (at ^ key_swizzle<BYTES>(r)), kl + n * 1024);
         }
 #pragma unroll
         for (int n = 0; n < BLOCKS; ++n) {
-            const int i = (w * BLOCKS + n) * WAVE + lane, r = i / BPR, at = i % BPR;
+            const uint32_t i = (w * BLOCKS + n) * WAVE + lane, r = i / BPR, at = i % BPR;
             uint32_t key = k0 + r;
             key = key < x.keys ? key : x.keys - 1;
-            dma_block(values + key * p.vTokenStride + 16 / ES * (KIND == FULL ? at : at ^ value_swizzle<BYTES>(r)),
-                      vl + (w * BLOCKS + n) * 1024);
+            dma_block(values + key * p.vTokenStride + 16 / ES * (KIND == FULL ? at : at ^ value_swizzle<BYTES>(r)), vl + n * 1024);
         }
     };
 
@@ -258,14 +291,15 @@ __global__ __launch_bounds__(THREADS, workgroups(D, KIND)) void packed_attention
 
         floatx16 s[KB];
 #pragma unroll
-        for (int kb = 0; kb < KB; ++kb) {
+        for (int kb = 0; kb < KB; ++kb)
 #pragma unroll
             for (int r = 0; r < 16; ++r) s[kb][r] = 0.0f;
-            const elem* kr = ktile[stage] + (32 * kb + c) * D;
 #pragma unroll
-            for (int i = 0; i < QV; ++i) {
+        for (int i = 0; i < QV; ++i)
+#pragma unroll
+            for (int kb = 0; kb < KB; ++kb) {
                 const int block = KIND == FULL ? QV * g + i : 2 * i + g;
-                const u32x4 k = *reinterpret_cast<const u32x4*>(kr + 16 / ES * (block ^ key_swizzle<BYTES>(c)));
+                const u32x4 k = *reinterpret_cast<const u32x4*>(ktile[stage] + (32 * kb + c) * D + 16 / ES * (block ^ key_swizzle<BYTES>(c)));
                 if constexpr (KIND == FULL) {
                     const floatx4 kf = __builtin_bit_cast(floatx4, k), qf = __builtin_bit_cast(floatx4, q[i]);
 #pragma unroll
@@ -275,33 +309,68 @@ __global__ __launch_bounds__(THREADS, workgroups(D, KIND)) void packed_attention
                                                                     __builtin_bit_cast(bf16x8, q[i]), s[kb], 0, 0, 0);
                 }
             }
-        }
         // register r of block kb is key k0 + 32 kb + key(r)
         auto key = [&](int r) { return KIND == FULL ? (r & 3) + 8 * (r >> 2) + 4 * g : 16 * g + r; };
+        // what takes s to units of ln 2: left to the exponentials where nothing comes between
+        float by = a.factor;
+        if (a.capLog2 != 0.0f) {
+            float most = 0.0f;
 #pragma unroll
-        for (int kb = 0; kb < KB; ++kb)
+            for (int kb = 0; kb < KB; ++kb)
 #pragma unroll
-            for (int r = 0; r < 16; ++r) {
-                float y = s[kb][r] * a.factor;
-                if (a.capLog2 != 0.0f) y = a.capLog2 * tanh_of(y);
-                if (p.slopes) y = fmaf(-slope, fabsf(float(pos - int32_t(k0) - 32 * kb - key(r))), y);
-                s[kb][r] = y;
+                for (int r = 0; r < 16; ++r) most = fmaxf(most, fabsf(s[kb][r]));
+            if (__all(most <= a.within)) {
+#pragma unroll
+                for (int kb = 0; kb < KB; ++kb)
+#pragma unroll
+                    for (int r = 0; r < 16; ++r) {
+                        const float y = s[kb][r], t = y * y;
+                        float f = a.series[series_terms(KIND) - 1];
+#pragma unroll
+                        for (int i = series_terms(KIND) - 2; i >= 0; --i) f = fmaf(f, t, a.series[i]);
+                        s[kb][r] = y * f;
+                    }
+            } else {
+#pragma unroll
+                for (int kb = 0; kb < KB; ++kb)
+#pragma unroll
+                    for (int r = 0; r < 16; ++r) {
+                        const float y = s[kb][r] * a.factor;
+                        if constexpr (KIND == BF16_OUT)
+                            s[kb][r] = a.capLog2 * (1.0f - 2.0f * __builtin_amdgcn_rcpf(__builtin_amdgcn_exp2f(2.0f * LOG2E * y) + 1.0f));
+                        else s[kb][r] = a.capLog2 * tanh_of(y);
+                    }
             }
+            by = 1.0f;
+        }
+        if (p.slopes) {
+            const float apart = float(pos - int32_t(k0) - key(0));
+#pragma unroll
+            for (int kb = 0; kb < KB; ++kb)
+#pragma unroll
+                for (int r = 0; r < 16; ++r)
+                    s[kb][r] = fmaf(-slope, fabsf(apart - float(32 * kb + key(r) - key(0))), s[kb][r] * by);
+            by = 1.0f;
+        }
         if (int32_t(k0 + BN) > hi0 || int32_t(k0) < lo1) {
+            const int32_t from = lo - int32_t(k0) - key(0), to = hi - int32_t(k0) - key(0);
 #pragma unroll
             for (int kb = 0; kb < KB; ++kb)
 #pragma unroll
                 for (int r = 0; r < 16; ++r) {
-                    const int32_t j = int32_t(k0) + 32 * kb + key(r);
-                    s[kb][r] = j >= lo && j < hi ? s[kb][r] : -INFINITY;
+                    const int32_t j = 32 * kb + key(r) - key(0);
+                    s[kb][r] = j >= from && j < to ? s[kb][r] : -INFINITY;
                 }
         }
-        float top = -INFINITY;
+        float top = s[0][0];
 #pragma unroll
         for (int kb = 0; kb < KB; ++kb)
 #pragma unroll
             for (int r = 0; r < 16; ++r) top = fmaxf(top, s[kb][r]);
-        top = fmaxf(top, __shfl_xor(top, 32, WAVE));
+        {
+            const auto both = __builtin_amdgcn_permlane32_swap(__float_as_uint(top), __float_as_uint(top), false, false);
+            top = fmaxf(__uint_as_float(both[0]), __uint_as_float(both[1])) * by;
+        }
         // weights may grow to 2^8 before the maximum is taken up anew
         const bool grow = top > m + 8.0f;
         const float next = grow ? top : m, base = next == -INFINITY ? 0.0f : next;
@@ -314,12 +383,15 @@ __global__ __launch_bounds__(THREADS, workgroups(D, KIND)) void packed_attention
 #pragma unroll
                 for (int r = 0; r < 16; ++r) o[dt][r] *= keep;
         }
+        // (the accumulators stay where they are on both ways here)
+#pragma unroll
+        for (int dt = 0; dt < DT; ++dt) asm("" : "+v"(o[dt]));
 #pragma unroll
         for (int kb = 0; kb < KB; ++kb) {
             if constexpr (KIND == FULL) {
 #pragma unroll
                 for (int r = 0; r < 16; ++r) {
-                    const float e = __builtin_amdgcn_exp2f(s[kb][r] - base);
+                    const float e = __builtin_amdgcn_exp2f(fmaf(s[kb][r], by, -base));
                     l += e;
                     const float* vr = vtile[stage] + (32 * kb + key(r)) * D + c;
 #pragma unroll
@@ -333,8 +405,8 @@ __global__ __launch_bounds__(THREADS, workgroups(D, KIND)) void packed_attention
                     u32x4 term[TERMS];
 #pragma unroll
                     for (int j = 0; j < 4; ++j) {
-                        const float e0 = __builtin_amdgcn_exp2f(s[kb][8 * h + 2 * j] - base);
-                        const float e1 = __builtin_amdgcn_exp2f(s[kb][8 * h + 2 * j + 1] - base);
+                        const float e0 = __builtin_amdgcn_exp2f(fmaf(s[kb][8 * h + 2 * j], by, -base));
+                        const float e1 = __builtin_amdgcn_exp2f(fmaf(s[kb][8 * h + 2 * j + 1], by, -base));
                         if constexpr (KIND == BF16_F32) {
                             l += e0 + e1;
                             float f0 = e0, f1 = e1;          // each term takes the next 8 bits
@@ -348,7 +420,7 @@ __global__ __launch_bounds__(THREADS, workgroups(D, KIND)) void packed_attention
                         } else {
                             const uint32_t both = pack_bf16(e0, e1);
                             term[0][j] = both;
-                            l += __uint_as_float(both << 16) + __uint_as_float(both & 0xFFFF0000u);
+                            l = add_pair(both, l);
                         }
                     }
                     // V^T rows 32 dt + c: lane q16 of each 16 addresses row 16 g + 8 h + q16 / 4, and 4 on
@@ -518,6 +590,15 @@ bool launch_packed_attention(const PackedParams& p, void* work, hipStream_t stre
     a.records = s.splits > 1 ? static_cast<float*>(work) : nullptr;
     a.capLog2 = p.cap * LOG2E;
     a.factor = p.cap > 0.0f ? p.scale / p.cap : p.scale * LOG2E;
+    const int kind = p.inType != 1 ? FULL : (p.outType == 1 ? BF16_OUT : BF16_F32);
+    if (p.cap > 0.0f) {
+        double power = double(p.cap) * 1.4426950408889634 * a.factor;
+        for (int i = 0; i < series_terms(kind); ++i, power *= double(a.factor) * a.factor)
+            a.series[i] = float((kind == BF16_OUT ? SERIES4[i] : SERIES6[i]) * power);
+        a.within = series_limit(kind) / a.factor;
+    }
+    const uint64_t es = p.inType == 1 ? 2 : 4;
+    a.fits = (uint64_t(64) * (p.kTokenStride > p.vTokenStride ? p.kTokenStride : p.vTokenStride) + p.dim) * es < (uint64_t(1) << 31);
     const uint64_t piece = p.outType == 1 ? 8 : 16, os = piece / 4;
     a.wide = (reinterpret_cast<uintptr_t>(p.out) | p.outTokenStride * os | p.outHeadStride * os) % piece == 0;
     const uint32_t grid = a.slots * p.kvHeads * a.splits;
