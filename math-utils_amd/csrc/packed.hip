@@ -163,7 +163,7 @@ __device__ __forceinline__ void put4(const PackedArgs& a, uint64_t at, const flo
 }
 
 constexpr int tile_keys(int D, int kind) { return kind == FULL ? (D <= 96 ? 64 : 32) : (D <= 128 ? 64 : 32); }
-constexpr int workgroups(int D, int kind) { return D <= (kind == FULL ? 64 : 128) ? 2 : 1; }
+constexpr int workgroups(int D, int kind) { return D <= (kind == FULL ? 64 : 256) ? 2 : 1; }
 
 template <int D, int KIND>
 __global__ __launch_bounds__(THREADS, workgroups(D, KIND)) void packed_attention_kernel(PackedArgs a) {
@@ -175,6 +175,9 @@ __global__ __launch_bounds__(THREADS, workgroups(D, KIND)) void packed_attention
     constexpr int BLOCKS = BN * BPR / WAVE / WAVES;        // DMA blocks (1 KB) of a wave and tile, K or V
     constexpr int QV = KIND == FULL ? D / 8 : D / 16;      // 16-byte pieces of a lane's half query
     static_assert(BN * BPR % (WAVE * WAVES) == 0, "a tile's blocks are the waves' alike");
+    // the queries of 256 do not all stay in registers: what the scores read back must not wait
+    // for a tile that was asked for before it
+    constexpr bool LATE = D == 256 && KIND != FULL;
     __shared__ __attribute__((aligned(16))) elem ktile[2][BN * D], vtile[2][BN * D];
     const PackedParams& p = a.p;
     const int lane = threadIdx.x & 63, w = int(scalar(threadIdx.x >> 6)), g = lane >> 5, c = lane & 31;
@@ -286,8 +289,9 @@ __global__ __launch_bounds__(THREADS, workgroups(D, KIND)) void packed_attention
         const int stage = it & 1;
         wait_vmcnt<0>();
         lds_barrier();
-        if (it + 1 < tiles) issue(k0 + BN, stage ^ 1);
-        if (!busy || int32_t(k0) >= hi1 || int32_t(k0 + BN) <= lo0) continue;
+        const bool idle = !busy || int32_t(k0) >= hi1 || int32_t(k0 + BN) <= lo0;
+        if ((!LATE || idle) && it + 1 < tiles) issue(k0 + BN, stage ^ 1);
+        if (idle) continue;
 
         floatx16 s[KB];
 #pragma unroll
@@ -309,6 +313,11 @@ __global__ __launch_bounds__(THREADS, workgroups(D, KIND)) void packed_attention
                                                                     __builtin_bit_cast(bf16x8, q[i]), s[kb], 0, 0, 0);
                 }
             }
+        if (LATE && it + 1 < tiles) {
+            __builtin_amdgcn_sched_barrier(0);
+            issue(k0 + BN, stage ^ 1);
+            __builtin_amdgcn_sched_barrier(0);
+        }
         // register r of block kb is key k0 + 32 kb + key(r)
         auto key = [&](int r) { return KIND == FULL ? (r & 3) + 8 * (r >> 2) + 4 * g : 16 * g + r; };
         // what takes s to units of ln 2: left to the exponentials where nothing comes between
