@@ -36,6 +36,7 @@ struct PackedArgs {
     PackedParams p;
     float* records;                  // of split keys, or null: [(slot, kv head)][split] of record floats
     uint32_t group, slots, splits;   // query heads of a kv head; 128-row slots over all documents
+    uint32_t groupMagic, groupShift; // row / group = row groupMagic >> groupShift (rows below 2^31)
     float factor;                    // the product to the scores' fractions of the cap, or to units of ln 2
     float capLog2;
     float series[6];                 // capped scores in units of ln 2: s (series[0] + s^2 (series[1] + ...)) ...
@@ -100,8 +101,11 @@ struct Work {
     uint32_t key0, keys;             // its keys
     int32_t shift;                   // a token's position less its number in the document
     uint32_t prefix;
-    uint64_t row0, rows;             // the workgroup's first row, the document's rows
+    uint32_t row0, rows;             // the workgroup's first row, the document's rows
 };
+__device__ __forceinline__ uint32_t token_of(const PackedArgs& a, uint32_t row) {
+    return uint32_t(uint64_t(row) * a.groupMagic >> a.groupShift);
+}
 __device__ __forceinline__ bool find_work(const PackedArgs& a, uint32_t slot, int lane, Work& x) {
     const PackedParams& p = a.p;
     uint32_t b = 0;
@@ -135,9 +139,9 @@ __device__ __forceinline__ bool find_work(const PackedArgs& a, uint32_t slot, in
     x.prefix = p.prefix ? scalar(p.prefix[b]) : 0;
     x.prefix = x.prefix < x.keys ? x.prefix : x.keys;
     x.shift = int32_t(x.keys) - int32_t(x.tokens);
-    x.rows = uint64_t(x.tokens) * a.group;
-    x.row0 = (slot - slot0) * ROWS_WG;
-    return x.row0 < x.rows;
+    x.rows = x.tokens * a.group;
+    x.row0 = uint32_t(slot - slot0) * ROWS_WG;
+    return slot - slot0 < (x.rows + ROWS_WG - 1) / ROWS_WG;
 }
 
 /* four elements of an out row */
@@ -191,13 +195,13 @@ __global__ __launch_bounds__(THREADS, workgroups(D, KIND)) void packed_attention
     if (!find_work(a, slot, lane, x)) return;
 
     // this lane's row
-    const uint64_t row = x.row0 + 32 * w + c;
+    const uint32_t row = x.row0 + 32 * w + c;
     const bool live = row < x.rows;
-    const uint32_t token = uint32_t((live ? row : x.rows - 1) / a.group);
-    const uint32_t head = kvh * a.group + uint32_t((live ? row : x.rows - 1) % a.group);
+    const uint32_t token = token_of(a, live ? row : x.rows - 1);
+    const uint32_t head = kvh * a.group + (live ? row : x.rows - 1) - token * a.group;
     const int32_t pos = x.shift + int32_t(token);          // negative: before every key
-    const uint64_t lastRow = x.row0 + ROWS_WG - 1 < x.rows ? x.row0 + ROWS_WG - 1 : x.rows - 1;
-    const int32_t pos0 = x.shift + int32_t(x.row0 / a.group), pos1 = x.shift + int32_t(lastRow / a.group);
+    const uint32_t lastRow = x.row0 + ROWS_WG - 1 < x.rows ? x.row0 + ROWS_WG - 1 : x.rows - 1;
+    const int32_t pos0 = x.shift + int32_t(token_of(a, x.row0)), pos1 = x.shift + int32_t(token_of(a, lastRow));
 
     // the keys that any row sees: [kbeg, kend), in whole tiles from a multiple of BN on
     uint32_t kend = pos1 < 0 ? 0 : uint32_t(pos1) + 1;
@@ -215,9 +219,9 @@ __global__ __launch_bounds__(THREADS, workgroups(D, KIND)) void packed_attention
     hi = hi > int32_t(x.prefix) ? hi : int32_t(x.prefix);
     const int32_t lo = p.window && pos >= 0 && uint64_t(pos) + 1 > p.window ? int32_t(pos + 1 - int64_t(p.window)) : 0;
     // what every row of the wave sees
-    const uint64_t waveFirst = x.row0 + 32 * w < x.rows ? x.row0 + 32 * w : x.rows - 1;
-    const uint64_t waveLast = waveFirst + 31 < x.rows ? waveFirst + 31 : x.rows - 1;
-    const int32_t p0 = x.shift + int32_t(waveFirst / a.group), p1 = x.shift + int32_t(waveLast / a.group);
+    const uint32_t waveFirst = x.row0 + 32 * w < x.rows ? x.row0 + 32 * w : x.rows - 1;
+    const uint32_t waveLast = waveFirst + 31 < x.rows ? waveFirst + 31 : x.rows - 1;
+    const int32_t p0 = x.shift + int32_t(token_of(a, waveFirst)), p1 = x.shift + int32_t(token_of(a, waveLast));
     int32_t hi0 = p0 + 1;
     hi0 = hi0 > int32_t(x.prefix) ? hi0 : int32_t(x.prefix);
     const int32_t lo1 = p.window && p1 >= 0 && uint64_t(p1) + 1 > p.window ? int32_t(p1 + 1 - int64_t(p.window)) : 0;
@@ -501,8 +505,7 @@ __global__ __launch_bounds__(THREADS) void packed_merge_kernel(PackedArgs a) {
         l += at[ROWS_WG + r] * f;
         o += *reinterpret_cast<const floatx4*>(at + 2 * ROWS_WG + r * D + d) * f;
     }
-    const uint64_t row = x.row0 + r;
-    const uint32_t token = uint32_t(row / a.group), head = kvh * a.group + uint32_t(row % a.group);
+    const uint32_t row = x.row0 + r, token = token_of(a, row), head = kvh * a.group + row - token * a.group;
     const float by = l == 0.0f ? 0.0f : 1.0f / l;
     const float y[4] = {o[0] * by, o[1] * by, o[2] * by, o[3] * by};
     put4(a, (uint64_t(x.first) + token) * p.outTokenStride + head * p.outHeadStride + d, y);
@@ -510,18 +513,17 @@ __global__ __launch_bounds__(THREADS) void packed_merge_kernel(PackedArgs a) {
 
 struct Shape { uint64_t slots, splits; };
 
-/* Few rows over many keys leave CUs idle: their keys are split over workgroups, whose
-   records a second launch joins. */
+/* Few rows over many keys leave CUs idle: their keys are split over workgroups, two a CU,
+   whose records a second launch joins. How the rows lie in slots only the device knows: a
+   document has one at least. */
 Shape shape_of(const PackedParams& p) {
-    const uint64_t group = p.heads / p.kvHeads;
+    const uint64_t group = p.heads / p.kvHeads, full = (uint64_t(p.count) * group + ROWS_WG - 1) / ROWS_WG;
     Shape s{};
-    s.slots = p.starts ? uint64_t(p.count) * group / ROWS_WG + p.documents : (uint64_t(p.count) * group + ROWS_WG - 1) / ROWS_WG;
-    const uint64_t each = s.slots * p.kvHeads, want = 512;
+    s.slots = p.starts ? uint64_t(p.count) * group / ROWS_WG + p.documents : full;
+    const uint64_t busy = std::max<uint64_t>(full, std::min(p.documents, p.count)) * p.kvHeads, want = 512;
     s.splits = 1;
-    if (each && each * 2 <= want) {
-        const uint64_t most = p.keyCount / 512;            // keys of a split, at the least, were there one document
-        s.splits = std::min(want / each, std::max<uint64_t>(most, 1));
-    }
+    // a split of 256 keys at the least, were the documents alike
+    if (busy && busy * 2 <= want) s.splits = std::max<uint64_t>(std::min<uint64_t>(want / busy, p.keyCount / p.documents / 256), 1);
     return s;
 }
 
@@ -577,7 +579,9 @@ bool check_packed_attention(const PackedParams& p) {
                             Extent{reinterpret_cast<uintptr_t>(p.v), p.keyCount, p.vTokenStride * es, p.kvHeads, p.vHeadStride * es, D * es}})
         if (may_meet(out, e)) return ctx.fail("packed attention: out overlaps q, k or v");
     const Shape s = shape_of(p);
-    if (s.slots * s.splits * p.kvHeads >= (uint64_t(1) << 31)) return ctx.fail("packed attention: too many rows");
+    if (uint64_t(p.count) * (p.heads / p.kvHeads) >= (uint64_t(1) << 31) - ROWS_WG ||
+        s.slots * s.splits * p.kvHeads >= (uint64_t(1) << 31))
+        return ctx.fail("packed attention: too many rows");
     return true;
 }
 
@@ -594,6 +598,10 @@ bool launch_packed_attention(const PackedParams& p, void* work, hipStream_t stre
     PackedArgs a{};
     a.p = p;
     a.group = p.heads / p.kvHeads;
+    uint32_t log = 0;
+    while ((1u << log) < a.group) ++log;
+    a.groupShift = 31 + log;
+    a.groupMagic = uint32_t((uint64_t(1) << a.groupShift) / a.group + 1);
     a.slots = uint32_t(s.slots);
     a.splits = uint32_t(s.splits);
     a.records = s.splits > 1 ? static_cast<float*>(work) : nullptr;
