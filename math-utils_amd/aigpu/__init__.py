@@ -1198,42 +1198,61 @@ def paged_decode_workspace(q, out, key_pages, value_pages, table, lengths, max_l
     return _torch.zeros(int(need), dtype=_torch.uint8, device=q.device)
 
 
+def _row_strides(t, name):
+    """(page, head, row) strides of codes or scales, counted in rows; a dimension of one has 1"""
+    *strides, one = t.stride()
+    row = t.shape[3]
+    if (one != 1 and row > 1) or any(s % row for s, n in zip(strides, t.shape) if n > 1):
+        raise ValueError(f"the rows of {name} must be dense")
+    return tuple(s // row if n > 1 else 1 for s, n in zip(strides, t.shape))
+
+
 def _paged_cache_q4(key_codes, key_scales, value_codes, value_scales, table, lengths):
     """AiGpuPagedCacheQ4's fields"""
     _with_torch()
-    names = ("key_codes", "value_codes", "key_scales", "value_scales")
-    tensors = (key_codes, value_codes, key_scales, value_scales)
-    at = [_at(t, name) for t, name in zip(tensors, names)]
-    of_table, of_lengths = _indices(table, "table", 2), _indices(lengths, "lengths", 1)
-    if not lengths.is_contiguous():
+    try:
+        away = key_codes.get_device() | key_scales.get_device() | value_codes.get_device() | \
+            value_scales.get_device() | table.get_device() | lengths.get_device()
+    except AttributeError:
+        away = -1
+    if away:
+        _all_here((key_codes, "key_codes"), (key_scales, "key_scales"), (value_codes, "value_codes"),
+                  (value_scales, "value_scales"), (table, "table"), (lengths, "lengths"))
+    i32, u32, u8, f16 = _torch.int32, _torch.uint32, _torch.uint8, _torch.float16
+    if (table.dtype is not i32 and table.dtype is not u32) or table.dim() != 2 \
+            or (table.stride(1) != 1 and table.shape[1] > 1):
+        raise TypeError("table must be an int32 tensor of two dimensions with unit stride")
+    if (lengths.dtype is not i32 and lengths.dtype is not u32) or not lengths.dim() == 1 or not lengths.is_contiguous():
         raise TypeError("lengths must be a contiguous int32 vector")
-    if key_codes.dtype is not _torch.uint8 or value_codes.dtype is not _torch.uint8:
+    if key_codes.dtype is not u8 or value_codes.dtype is not u8:
         raise TypeError("the codes must be uint8")
-    if key_scales.dtype is not _torch.float16 or value_scales.dtype is not _torch.float16:
+    if key_scales.dtype is not f16 or value_scales.dtype is not f16:
         raise TypeError("the scales must be float16")
-    shape, blocks = tuple(key_codes.shape), tuple(key_scales.shape)
-    if len(shape) != 4 or tuple(value_codes.shape) != shape or tuple(value_scales.shape) != blocks \
-            or len(blocks) != 4 or blocks[:3] != shape[:3] or 16 * blocks[3] != shape[3]:
+    shape, blocks = key_codes.shape, key_scales.shape
+    if len(shape) != 4 or len(blocks) != 4 or value_codes.shape != shape or value_scales.shape != blocks \
+            or blocks[:3] != shape[:3] or 16 * blocks[3] != shape[3] or not blocks[3]:
         raise ValueError("codes must be [pages][kv_heads][page_size][dim / 2], "
                          "scales [pages][kv_heads][page_size][dim / 32]")
     pages, kv_heads, size, half = shape
-    steps = None
-    for t, row in ((key_codes, half), (value_codes, half), (key_scales, half // 16), (value_scales, half // 16)):
-        strides = t.stride()
-        if (strides[3] != 1 and row > 1) or any(s % row for s, n in zip(strides, shape[:3]) if n > 1):
-            raise ValueError("the rows of the pages must be dense")
-        # a dimension of one may carry any stride
-        own = tuple(s // row if n > 1 else 1 for s, n in zip(strides, shape[:3]))
-        if steps is not None and own != steps:
+    strides, small = key_codes.stride(), key_scales.stride()
+    ps, hs, rs, one = strides
+    if value_codes.stride() != strides or value_scales.stride() != small or one != 1 or rs != half or hs % half \
+            or ps % half or small != (ps // 16, hs // 16, rs // 16, 1):
+        # other than dense rows next to each other, or a dimension of one whose stride may be any
+        steps = {_row_strides(t, name) for t, name in ((key_codes, "key_codes"), (value_codes, "value_codes"),
+                                                       (key_scales, "key_scales"), (value_scales, "value_scales"))}
+        if len(steps) != 1:
             raise ValueError("codes and scales must have the same strides, counted in rows")
-        steps = own
+        ps, hs, rs = (s * half for s in steps.pop())
     batch, (rows, width) = lengths.shape[0], table.shape
     if rows != batch:
         raise ValueError(f"table has {rows} entries, {batch} are needed")
     step = table.stride(0) if batch > 1 else width
-    if (step == 0 and width) or steps[2] == 0:       # 0 means the dense stride to the entries
+    if (step == 0 and width) or rs == 0:             # 0 means the dense stride to the entries
         raise ValueError("the table and the rows of the pages must not be broadcast views")
-    return (*at, of_table, of_lengths, batch, pages, size, kv_heads, 2 * half, width, step, *steps)
+    return (key_codes.data_ptr(), value_codes.data_ptr(), key_scales.data_ptr(), value_scales.data_ptr(),
+            table.data_ptr(), lengths.data_ptr(), batch, pages, size, kv_heads, 2 * half, width, step,
+            ps // half if pages > 1 else 1, hs // half if kv_heads > 1 else 1, rs // half if size > 1 else 1)
 
 
 def paged_append_q4(k, v, key_codes, key_scales, value_codes, value_scales, table, lengths, starts=None, k_norm=None,

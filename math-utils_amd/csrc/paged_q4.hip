@@ -22,47 +22,86 @@ constexpr int BLOCK_LANES = 4;       // of 8 elements each
 constexpr float MOST_SCALE = 2720.0f;
 constexpr uint16_t NAN_SCALE = 0x7E00;
 
-/* A lane's 8 elements to codes 4 bits each, element j at 4 j; `scale` gets the fp16 bits.
-   The lanes of a block call it together. */
-template <typename T>
+/* x of the lane one or two on, within fours */
+template <int OFF>
+__device__ __forceinline__ uint32_t neighbour(uint32_t x) {
+    return __builtin_amdgcn_mov_dpp(x, OFF == 1 ? 0xB1 : 0x4E, 0xF, 0xF, true);
+}
+template <int OFF>
+__device__ __forceinline__ double neighbour(double x) {
+    const u32x2 b = __builtin_bit_cast(u32x2, x);
+    const uint32_t lo = b[0], hi = b[1];
+    return __builtin_bit_cast(double, u32x2{neighbour<OFF>(lo), neighbour<OFF>(hi)});
+}
+
+/* What the elements x of a lane are, for their codes: T double or float, and whether they
+   are bf16 values. `encode` gives the codes 4 bits each, element j at 4 j, and the scale's
+   fp16 bits. The lanes of a block call it together. */
+template <typename T, bool BF>
 __device__ __forceinline__ uint32_t encode(const T (&x)[8], uint16_t& scale) {
+    float f[8];
     T top = T(0);
+    uint32_t bits = 0;               // the largest magnitude's: not finite from 0x7F800000 on
 #pragma unroll
     for (int j = 0; j < 8; ++j) {
-        const T a = x[j] < T(0) ? -x[j] : x[j];
-        top = a > top ? a : top;
-        if (!(a < T(INFINITY))) top = T(INFINITY);
+        f[j] = float(x[j]);
+        bits = max(bits, __float_as_uint(f[j]) & 0x7FFFFFFFu);
+        if constexpr (sizeof(T) == 8) top = fmax(top, fabs(x[j]));
     }
-#pragma unroll
-    for (int o = 1; o < BLOCK_LANES; o <<= 1) {
-        const T other = __shfl_xor(top, o, WAVE);
-        top = other > top ? other : top;
+    bits = max(bits, neighbour<1>(bits));
+    bits = max(bits, neighbour<2>(bits));
+    if constexpr (sizeof(T) == 8) {
+        top = fmax(top, neighbour<1>(top));
+        top = fmax(top, neighbour<2>(top));
+    } else {
+        top = __uint_as_float(bits);
     }
-    if (!(top < T(INFINITY))) {
-        scale = NAN_SCALE;
-        return 0x88888888u;
+    // A seventh of it less 2^-22 of itself, so that the next number of 8 bits (a bf16) is the
+    // scale or the one before, which the exact product tells. Below 2^-17 fp16's least is the unit.
+    const float about = __uint_as_float(bits) * (0.14285714f * (1.0f - 0x1p-22f));
+    const uint32_t up = (__float_as_uint(about) + 0xFFFFu) & 0xFFFF0000u;
+    float s = __uint_as_float(T(7.0f * __uint_as_float(up)) < top ? up + 0x10000u : up);
+    if (__any(about < 0x1p-17f)) {
+        float small = ceilf(about * 0x1p24f) * 0x1p-24f;
+        if (T(7.0f * small) < top) small += 0x1p-24f;
+        s = about < 0x1p-17f ? small : s;
     }
-    // the unit of the eighth bit of about top / 7 (no finer than fp16's least), then the
-    // whole number of units: fp32 may be one low, which the exact product shows
-    const float about = float(top) / 7.0f;
-    int power = int(__float_as_uint(about) >> 23) - 127 - 7;
-    power = power < -24 ? -24 : (power > 8 ? 8 : power);
-    const float unit = ldexpf(1.0f, power);
-    float s = floorf(fminf(ldexpf(about, -power), 512.0f)) * unit;
-    if (T(7.0f * s) < top) s += unit;
     s = fminf(s, MOST_SCALE);
-    scale = __builtin_bit_cast(uint16_t, _Float16(s));
-    const float by = s > 0.0f ? 1.0f / s : 0.0f;
-    uint32_t word = 0;
+    scale = bits >= 0x7F800000u ? NAN_SCALE : __builtin_bit_cast(uint16_t, _Float16(s));
+    const float by = __builtin_amdgcn_rcpf(s);
+    float c[8];
+    if constexpr (BF) {
+        // x / s, of two numbers of 8 bits, is a border or 2^-10 away from it at least
 #pragma unroll
-    for (int j = 0; j < 8; ++j) {
-        float c = floorf(fminf(fmaxf(float(x[j]) * by, -8.0f), 8.0f) + 0.5f);
-        if (T((c + 0.5f) * s) <= x[j]) c += 1.0f;
-        else if (T((c - 0.5f) * s) > x[j]) c -= 1.0f;
-        c = s > 0.0f ? fminf(fmaxf(c, -7.0f), 7.0f) : 0.0f;
-        word |= uint32_t(int(c) + 8) << (4 * j);
+        for (int j = 0; j < 8; ++j) c[j] = floorf(fmaf(f[j], by, 0.5f + 0x1p-12f));
+    } else {
+        float edge = 0.0f;           // how far from the middle between two borders, at most
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+            const float t = fmaf(f[j], by, 0.5f);
+            c[j] = floorf(t);
+            edge = fmaxf(edge, fabsf(t - c[j] - 0.5f));
+        }
+        // t (at most 8) is off by 8 (2^-23 + 2 2^-24): nearer borders are decided by the exact ones
+        if (__any(edge > 0.5f - 4e-6f)) {
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+                if (T((c[j] + 0.5f) * s) <= x[j]) c[j] += 1.0f;
+                else if (T((c[j] - 0.5f) * s) > x[j]) c[j] -= 1.0f;
+            }
+        }
     }
-    return word;
+    // four codes, and the eights, in a sum of fp32
+    uint32_t word[2];
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+        float sum = 34952.0f;        // 0x8888
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+            sum = fmaf(__builtin_amdgcn_fmed3f(c[4 * h + j], -7.0f, 7.0f), float(1 << 4 * j), sum);
+        word[h] = uint32_t(sum);
+    }
+    return bits == 0 || bits >= 0x7F800000u ? 0x88888888u : word[0] | word[1] << 16;
 }
 
 /* cos and sin of a = pos * freq radians in 64 bits: a less a whole number of quarter
@@ -87,6 +126,18 @@ __device__ __forceinline__ void rotation64_at(uint32_t pos, float freq, double& 
     sn = turn == 0 ? s : (turn == 1 ? c : (turn == 2 ? -s : -c));
 }
 
+/* 1 / sqrt(x) in 64 bits: the instruction's 26 bits or so, twice improved */
+__device__ __forceinline__ double inverse_root(double x) {
+    double y = __builtin_amdgcn_rsq(x);
+#pragma unroll
+    for (int i = 0; i < 2; ++i) y = fma(y * 0.5, fma(-x * y, y, 1.0), y);
+    return y;
+}
+
+/* where a token's turn j stands: those that neighbouring lanes read together, together */
+__host__ __device__ constexpr uint32_t turnsOf(uint32_t half) { return (half + 7) / 8 * 8; }
+__device__ __forceinline__ uint32_t turn_slot(uint32_t j, uint32_t half) { return j % 8 * ((half + 7) / 8) + j / 8; }
+
 /* sum over the LPR lanes of a row, in 64 bits */
 template <int LPR>
 __device__ __forceinline__ double row_sum64(double x, int lane) {
@@ -105,15 +156,16 @@ __device__ __forceinline__ double row_sum64(double x, int lane) {
 */
 struct AppendQ4Args {
     PagedAppendQ4Params p;
+    uint32_t headMagic, headShift;   // n / kvHeads = n headMagic >> headShift
     uint32_t tokens;                 // of a workgroup, at most MAX_TOKENS
     int wide;                        // k and v rows can be read 16 bytes at a time
 };
 
 template <int D, bool BF>
-__global__ __launch_bounds__(THREADS) void paged_append_q4_kernel(AppendQ4Args a) {
+__global__ __launch_bounds__(THREADS, 4) void paged_append_q4_kernel(AppendQ4Args a) {
     constexpr int LPR = D / 8, RPW = WAVE / LPR, NW = THREADS / WAVE, RAW = BF ? 1 : 2;
     extern __shared__ __attribute__((aligned(16))) double2 turns64[];   // [tokens][rot / 2]
-    __shared__ double rows[NW][RPW][D];
+    __shared__ double rows[NW][8][WAVE];             // element e of each lane's eight
     __shared__ uint64_t base[MAX_TOKENS];            // row of kv head 0, ~0: not written
     __shared__ uint32_t place[MAX_TOKENS];
     const PagedAppendParams& p = a.p.a;
@@ -123,6 +175,32 @@ __global__ __launch_bounds__(THREADS) void paged_append_q4_kernel(AppendQ4Args a
     if (t0 >= p.count) return;
     const uint32_t nt = p.count - t0 < a.tokens ? uint32_t(p.count - t0) : a.tokens;
     const uint32_t keys = nt * c.kvHeads, total = 2 * keys;             // k's rows, then v's
+    const int sub = lane / LPR, d0 = (lane % LPR) * 8;
+    // row r of the workgroup: its token and kv head, and its elements of this lane
+    struct Place { uint32_t t, h; } here{};
+    u32x4 raw[RAW] = {};
+    auto load = [&](uint32_t r) {
+        const bool isKey = r < keys;
+        if (sub >= RPW || r >= total) return;
+        const uint32_t rest = isKey ? r : r - keys;
+        here.t = uint32_t(uint64_t(rest) * a.headMagic >> a.headShift);
+        here.h = rest - here.t * c.kvHeads;
+        const char* src = static_cast<const char*>(isKey ? p.k : p.v) +
+                          ((t0 + here.t) * (isKey ? p.kStride : p.vStride) + size_t(here.h) * D + d0) * (BF ? 2 : 4);
+        if (a.wide) {
+#pragma unroll
+            for (int i = 0; i < RAW; ++i) raw[i] = reinterpret_cast<const u32x4*>(src)[i];
+        } else if constexpr (BF) {
+            const uint16_t* e = reinterpret_cast<const uint16_t*>(src);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) raw[0][i] = e[2 * i] | uint32_t(e[2 * i + 1]) << 16;
+        } else {
+            const uint32_t* e = reinterpret_cast<const uint32_t*>(src);
+#pragma unroll
+            for (int i = 0; i < 8; ++i) raw[i / 4][i % 4] = e[i];
+        }
+    };
+    load(w * RPW + sub);             // the first row is on its way while its place is found
     const Token mine = find_token<NW>(c, p.starts, t0, nt, w, lane);
     if (mine.finds) {
         place[mine.own] = mine.pos;
@@ -133,43 +211,31 @@ __global__ __launch_bounds__(THREADS) void paged_append_q4_kernel(AppendQ4Args a
     for (uint32_t i = threadIdx.x; i < nt * half; i += THREADS) {
         double cs, sn;
         rotation64_at(place[i / half], p.freqs[i % half], cs, sn);
-        turns64[i] = double2{cs * double(p.amplitude), sn * double(p.amplitude)};
+        turns64[i / half * turnsOf(half) + turn_slot(i % half, half)] = double2{cs * double(p.amplitude), sn * double(p.amplitude)};
     }
     __syncthreads();
 
-    const int sub = lane / LPR, d0 = (lane % LPR) * 8;
-    double* row = rows[w][sub < RPW ? sub : 0];
+    double gamma[8] = {};
+    if (p.gamma) {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) gamma[e] = double(p.gamma[d0 + e]) + double(p.offset);
+    }
     // every lane of a wave stays in the loop: the sums and blocks shuffle over all of it
 #pragma unroll 1
     for (uint32_t wave = w * RPW; wave < total; wave += NW * RPW) {
         const uint32_t r = wave + sub;
         const bool in = sub < RPW && r < total, isKey = r < keys;
-        const uint32_t rest = !in ? 0 : (isKey ? r : r - keys), t = rest / c.kvHeads, h = rest - t * c.kvHeads;
+        const uint32_t t = here.t, h = here.h;
         const uint64_t to = base[t];
         const bool live = in && to != ~uint64_t(0);
-        float x[8] = {};
-        if (live) {
-            const char* src = static_cast<const char*>(isKey ? p.k : p.v) +
-                              ((t0 + t) * (isKey ? p.kStride : p.vStride) + size_t(h) * D + d0) * (BF ? 2 : 4);
-            u32x4 raw[RAW];
-            if (a.wide) {
+        float x[8];
 #pragma unroll
-                for (int i = 0; i < RAW; ++i) raw[i] = reinterpret_cast<const u32x4*>(src)[i];
-            } else if constexpr (BF) {
-                const uint16_t* e = reinterpret_cast<const uint16_t*>(src);
-#pragma unroll
-                for (int i = 0; i < 4; ++i) raw[0][i] = e[2 * i] | uint32_t(e[2 * i + 1]) << 16;
-            } else {
-                const uint32_t* e = reinterpret_cast<const uint32_t*>(src);
-#pragma unroll
-                for (int i = 0; i < 8; ++i) raw[i / 4][i % 4] = e[i];
-            }
-#pragma unroll
-            for (int e = 0; e < 8; ++e) {
-                if constexpr (BF) x[e] = __uint_as_float(e & 1 ? raw[0][e / 2] & 0xFFFF0000u : raw[0][e / 2] << 16);
-                else x[e] = __uint_as_float(raw[e / 4][e % 4]);
-            }
+        for (int e = 0; e < 8; ++e) {
+            if constexpr (BF) x[e] = __uint_as_float(e & 1 ? raw[0][e / 2] & 0xFFFF0000u : raw[0][e / 2] << 16);
+            else x[e] = __uint_as_float(raw[e / 4][e % 4]);
+            if (!live) x[e] = 0.0f;
         }
+        load(r + NW * RPW);          // the next row's, on its way meanwhile
         uint32_t word;
         uint16_t scale;
         if (wave < keys && (p.gamma || half)) {      // keys among the wave's rows
@@ -180,35 +246,57 @@ __global__ __launch_bounds__(THREADS) void paged_append_q4_kernel(AppendQ4Args a
                 double ss = 0.0;
 #pragma unroll
                 for (int e = 0; e < 8; ++e) ss += y[e] * y[e];
-                const double inv = 1.0 / sqrt(row_sum64<LPR>(ss, lane) / double(D) + double(p.eps));
+                const double inv = inverse_root(row_sum64<LPR>(ss, lane) * (1.0 / D) + double(p.eps));
                 if (live && isKey) {
 #pragma unroll
-                    for (int e = 0; e < 8; ++e) y[e] = y[e] * inv * (double(p.gamma[d0 + e]) + double(p.offset));
+                    for (int e = 0; e < 8; ++e) y[e] = y[e] * inv * gamma[e];
                 }
             }
             if (half) {
-                if (live && isKey) {
 #pragma unroll
-                    for (int e = 0; e < 8; ++e) row[d0 + e] = y[e];
-                }
+                for (int e = 0; e < 8; ++e) rows[w][e][lane] = y[e];
                 wave_sync();
+                const double2* cs = turns64 + t * turnsOf(half);
                 if (live && isKey) {
+                    if (p.interleaved) {
 #pragma unroll
-                    for (int e = 0; e < 8; ++e) {
-                        const uint32_t d = d0 + e;
-                        if (d >= 2 * half) break;
-                        const bool late = p.interleaved ? d & 1 : d >= half;
-                        const uint32_t j = p.interleaved ? d / 2 : (late ? d - half : d);
-                        const double other = row[p.interleaved ? d ^ 1 : (late ? j : j + half)];
-                        const double2 cs = turns64[t * half + j];
-                        y[e] = y[e] * cs.x + (late ? other : -other) * cs.y;
+                        for (int e = 0; e < 8; e += 2) {
+                            if (uint32_t(d0 + e) >= 2 * half) break;
+                            const double2 by = cs[turn_slot((d0 + e) / 2, half)];
+                            const double u = y[e], v = y[e + 1];
+                            y[e] = u * by.x - v * by.y;
+                            y[e + 1] = v * by.x + u * by.y;
+                        }
+                    } else if (half % 8 == 0) {          // all eight partners in one lane
+                        if (uint32_t(d0) < 2 * half) {
+                            const bool late = uint32_t(d0) >= half;
+                            const int other = late ? lane - int(half / 8) : lane + int(half / 8);
+                            const uint32_t j0 = late ? d0 - half : d0;
+#pragma unroll
+                            for (int e = 0; e < 8; ++e) {
+                                const double2 by = cs[turn_slot(j0 + e, half)];
+                                const double v = rows[w][e][other];
+                                y[e] = y[e] * by.x + (late ? v : -v) * by.y;
+                            }
+                        }
+                    } else {
+#pragma unroll
+                        for (int e = 0; e < 8; ++e) {
+                            const uint32_t d = d0 + e;
+                            if (d >= 2 * half) break;
+                            const bool late = d >= half;
+                            const uint32_t o = late ? d - half : d + half;
+                            const double2 by = cs[turn_slot(late ? o : d, half)];
+                            const double v = rows[w][o % 8][lane - lane % LPR + o / 8];
+                            y[e] = y[e] * by.x + (late ? v : -v) * by.y;
+                        }
                     }
                 }
                 wave_sync();
             }
-            word = encode(y, scale);
+            word = encode<double, false>(y, scale);
         } else {
-            word = encode(x, scale);
+            word = encode<float, BF>(x, scale);
         }
         if (live) {
             const uint64_t at = to + h * c.headStride;
@@ -225,6 +313,7 @@ __global__ __launch_bounds__(THREADS) void paged_append_q4_kernel(AppendQ4Args a
 */
 struct ReadQ4Args {
     PagedReadQ4Params p;
+    uint32_t headMagic, headShift;
     uint32_t tokens;
     int wide;                        // k and v rows can be written 16 bytes at a time
 };
@@ -252,15 +341,18 @@ __global__ __launch_bounds__(THREADS) void paged_read_q4_kernel(ReadQ4Args a) {
 #pragma unroll 4
     for (uint32_t r = w * RPW + sub; r < total; r += NW * RPW) {
         const bool isKey = r < keys;
-        const uint32_t rest = isKey ? r : r - keys, t = rest / c.kvHeads, h = rest - t * c.kvHeads;
+        const uint32_t rest = isKey ? r : r - keys, t = uint32_t(uint64_t(rest) * a.headMagic >> a.headShift),
+                       h = rest - t * c.kvHeads;
         if (state[t] == 0) continue;
         const uint64_t at = base[t] + h * c.headStride;
         const uint32_t word = reinterpret_cast<const uint32_t*>(isKey ? c.keys : c.values)[at * LPR + lane % LPR];
         const uint16_t bits = (isKey ? p.keyScales : p.valueScales)[at * (D / 32) + lane % LPR / BLOCK_LANES];
         const float s = state[t] == 2 ? float(__builtin_bit_cast(_Float16, bits)) : __builtin_nanf("");
+        const uint32_t even = word & 0x0F0F0F0Fu, odd = word >> 4 & 0x0F0F0F0Fu;
         float x[8];
 #pragma unroll
-        for (int e = 0; e < 8; ++e) x[e] = s * float(int(word >> (4 * e) & 15u) - 8);
+        for (int e = 0; e < 8; ++e)      // s (c - 8), exact
+            x[e] = fmaf(float((e & 1 ? odd : even) >> 8 * (e / 2) & 255u), s, -8.0f * s);
         const size_t to = (t0 + t) * (isKey ? p.kStride : p.vStride) + size_t(h) * D + d0;
         if constexpr (BF) {
             uint16_t* out = static_cast<uint16_t*>(isKey ? p.k : p.v) + to;
@@ -291,6 +383,14 @@ uint32_t tokens_of(uint64_t count, uint32_t kvHeads, uint32_t dim, uint32_t pass
     uint32_t tokens = rows / (2 * kvHeads);
     if (tokens > spread) tokens = uint32_t(spread);
     return tokens < 1 ? 1 : (tokens > MAX_TOKENS ? MAX_TOKENS : tokens);
+}
+
+/* division by multiplication, exact below 2^31 */
+void divide_by(uint32_t d, uint32_t& magic, uint32_t& shift) {
+    uint32_t log = 0;
+    while ((1u << log) < d) ++log;
+    shift = 31 + log;
+    magic = uint32_t((uint64_t(1) << shift) / d + 1);
 }
 
 template <typename Of>
@@ -350,8 +450,9 @@ bool launch_paged_append_q4(const PagedAppendQ4Params& q, hipStream_t stream) {
     a.p = q;
     a.wide = (at & 15) == 0 && (p.count == 1 || (p.kStride | p.vStride) % (16 / es) == 0);
     a.tokens = tokens_of(p.count, p.c.kvHeads, p.c.dim, 4);
+    divide_by(p.c.kvHeads, a.headMagic, a.headShift);
     // 16 tokens of 128 turns are 32 KB
-    const size_t each = p.freqs ? size_t(p.rot / 2) * sizeof(double2) : 0;
+    const size_t each = p.freqs ? size_t(turnsOf(p.rot / 2)) * sizeof(double2) : 0;
     const Tiles tiles((p.count + a.tokens - 1) / a.tokens);
     return ctx.launch("paged_append_q4_kernel", stream, [&] {
         by_dim(p.c.dim, [&](auto dim) {
@@ -380,6 +481,7 @@ bool launch_paged_read_q4(const PagedReadQ4Params& p, hipStream_t stream) {
     a.p = p;
     a.wide = (at & 15) == 0 && (p.count == 1 || (p.kStride | p.vStride) % (16 / es) == 0);
     a.tokens = tokens_of(p.count, p.c.kvHeads, p.c.dim, 4);
+    divide_by(p.c.kvHeads, a.headMagic, a.headShift);
     const Tiles tiles((p.count + a.tokens - 1) / a.tokens);
     return ctx.launch("paged_read_q4_kernel", stream, [&] {
         by_dim(p.c.dim, [&](auto dim) {
