@@ -81,12 +81,7 @@ __device__ __forceinline__ bf16x8 read_transposed(const uint16_t* a0, const uint
     return __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
 }
 
-/* The cap's tanh as x (c0 + c1 x^2 + ...) up to 0.7, fitted for least relative error: 5e-6
-   where weights round to bf16, 1.4e-8 elsewhere. */
 constexpr int series_terms(int kind) { return kind == BF16_OUT ? 4 : 6; }
-constexpr float series_limit(int) { return 0.7f; }
-constexpr double SERIES4[4] = {0.999993310856002, -0.3328904637288124, 0.1286421024681964, -0.037290488627409184};
-constexpr double SERIES6[6] = {0.9999999863006178, -0.33333130413688367, 0.13328414724231763, -0.053526006423195875, 0.02002445111525679, -0.005088330528203937};
 
 /* acc plus both halves of a pair of bf16 values */
 __device__ __forceinline__ float add_pair(uint32_t pair, float acc) {
@@ -338,10 +333,7 @@ __global__ __launch_bounds__(THREADS, workgroups(D, KIND)) void packed_attention
 #pragma unroll
                     for (int r = 0; r < 16; ++r) {
                         const float y = s[kb][r], t = y * y;
-                        float f = a.series[series_terms(KIND) - 1];
-#pragma unroll
-                        for (int i = series_terms(KIND) - 2; i >= 0; --i) f = fmaf(f, t, a.series[i]);
-                        s[kb][r] = y * f;
+                        s[kb][r] = y * tanh_series<series_terms(KIND)>(t, a.series);
                     }
             } else {
 #pragma unroll
@@ -611,8 +603,8 @@ bool launch_packed_attention(const PackedParams& p, void* work, hipStream_t stre
     if (p.cap > 0.0f) {
         double power = double(p.cap) * 1.4426950408889634 * a.factor;
         for (int i = 0; i < series_terms(kind); ++i, power *= double(a.factor) * a.factor)
-            a.series[i] = float((kind == BF16_OUT ? SERIES4[i] : SERIES6[i]) * power);
-        a.within = series_limit(kind) / a.factor;
+            a.series[i] = float((kind == BF16_OUT ? TANH4[i] : TANH6[i]) * power);
+        a.within = TANH_WITHIN / a.factor;
     }
     const uint64_t es = p.inType == 1 ? 2 : 4;
     a.fits = (uint64_t(64) * (p.kTokenStride > p.vTokenStride ? p.kTokenStride : p.vTokenStride) + p.dim) * es < (uint64_t(1) << 31);

@@ -67,6 +67,7 @@ struct DecodeArgs {
     uint32_t pageMagic, pageShift;   // pos / pageSize = pos pageMagic >> pageShift (pos below 2^31)
     float scaleLog2;                 // of q: the scores in units of ln 2; with a cap, as its fractions
     float capLog2;                   // the cap in units of ln 2, 0: none
+    float series[6];                 // of the cap's tanh, times that
     int wideQ;                       // q rows can be read 16 bytes at a time
 };
 
@@ -887,12 +888,22 @@ __global__ __launch_bounds__(THREADS, occupancy(D, FORM)) void paged_attention_k
             if (a.capLog2 != 0.0f || p.slopes) {
                 svBy = 1.0f;
                 const float apart = float(s.len - 1 - s.pos - 4 * g);
+#pragma unroll
+                for (int i = 0; i < 16; ++i) sv[i >> 2][i & 3] *= qpow;
                 if (a.capLog2 != 0.0f) {
+                    float most = 0.0f;
 #pragma unroll
-                    for (int i = 0; i < 16; ++i) sv[i >> 2][i & 3] = a.capLog2 * tanh_of(sv[i >> 2][i & 3] * qpow);
-                } else {
+                    for (int i = 0; i < 16; ++i) most = fmaxf(most, fabsf(sv[i >> 2][i & 3]));
+                    if (__all(most <= TANH_WITHIN)) {
 #pragma unroll
-                    for (int i = 0; i < 16; ++i) sv[i >> 2][i & 3] *= qpow;
+                        for (int i = 0; i < 16; ++i) {
+                            const float x = sv[i >> 2][i & 3];
+                            sv[i >> 2][i & 3] = x * tanh_series<6>(x * x, a.series);
+                        }
+                    } else {
+#pragma unroll
+                        for (int i = 0; i < 16; ++i) sv[i >> 2][i & 3] = a.capLog2 * tanh_of(sv[i >> 2][i & 3]);
+                    }
                 }
                 if (p.slopes) {
 #pragma unroll
@@ -1331,6 +1342,7 @@ bool launch_decode_as(const char* name, const PagedDecodeParams& p, void* work, 
     a.perGroup = s.perGroup;
     a.capLog2 = scored(FORM) ? p.cap * LOG2E : 0.0f;
     a.scaleLog2 = a.capLog2 != 0.0f ? p.scale / p.cap : p.scale * LOG2E;
+    for (int i = 0; i < 6; ++i) a.series[i] = float(TANH6[i] * a.capLog2);
     // division by multiplication, exact below 2^31: the least power of two that holds the
     // page, and 2^31 times it over the page
     uint32_t log = 0;
