@@ -667,7 +667,7 @@ AIGPU_ABI uint64_t aigpu_paged_decode_workspace(const AiGpuPagedDecode* args);
    aigpu_paged_decode_workspace's. */
 typedef struct AiGpuScores {
     const float* slopes;      /* [heads] or NULL */
-    float cap;                /* finite, not negative */
+    float cap;                /* 0: none; otherwise 1e-6 .. 1e6 */
     uint32_t reserved;
 } AiGpuScores;
 AIGPU_ABI int aigpu_paged_decode_scored(const AiGpuPagedDecode* args, const AiGpuScores* scores);
@@ -721,7 +721,8 @@ AIGPU_ABI int aigpu_paged_append_q4(const AiGpuPagedAppendQ4* args);
    before starts[0] or from starts[batch] on stay as they were; a token without a
    place in the pool reads as NaN. With the lengths summed up as starts this is every
    sequence whole, as aigpu_packed_attention takes the keys of a chunk's documents.
-   Asynchronous, without scratch. */
+   k and v share no element (slices of the same rows do not). Asynchronous, without
+   scratch. */
 typedef struct AiGpuPagedReadQ4 {
     AiGpuPagedCacheQ4 cache;
     void* k;                  /* [count][kvHeads][dim], outType; token t at t*kStride */
@@ -764,9 +765,10 @@ AIGPU_ABI uint64_t aigpu_paged_decode_q4_workspace(const AiGpuPagedDecodeQ4* arg
 /*    with the scores s = scale q.k, then cap > 0: s = cap tanh(s / cap), then */
 /*    slopes: s -= slopes[head] |i - j|. A token that sees nothing gets zeros  */
 /*    (more tokens than keys: the first ones). Rows of out that no document    */
-/*    has stay as they were; a document whose starts decrease, or end past     */
-/*    count or keyCount, has no tokens or keys. Every row of a document's keys */
-/*    and values has to be finite, rows of no document may hold anything.      */
+/*    has stay as they were. The starts do not decrease, nor pass count and    */
+/*    keyCount (nothing outside is touched where they do, but documents may be */
+/*    left out). Every row of a document's keys and values has to be finite,   */
+/*    rows of no document may hold anything.                                   */
 /*    Types: q, k, v of inType, out of outType. bf16 to bf16 rounds the        */
 /*    weights to bf16 (their sum adds the rounded ones) and the result once;   */
 /*    bf16 to fp32 takes the weights whole, in three terms; fp32 is fp32       */
@@ -782,7 +784,7 @@ typedef struct AiGpuPackedAttention {
     const uint32_t* keyStarts;/* [documents + 1], or NULL: starts (keyCount = count) */
     const uint32_t* prefix;   /* [documents], or NULL: none */
     const float* slopes;      /* [heads], or NULL: none */
-    float cap;                /* 0: none */
+    float cap;                /* 0: none; otherwise 1e-6 .. 1e6 */
     float scale;              /* 0 means 1/sqrt(dim) */
     uint32_t inType, outType;
     uint64_t count, keyCount, documents, heads, kvHeads, dim;   /* dim 64, 96, 128, 192 or 256 */
@@ -794,8 +796,8 @@ typedef struct AiGpuPackedAttention {
     void* stream;
 } AiGpuPackedAttention;
 AIGPU_ABI int aigpu_packed_attention(const AiGpuPackedAttention* args);
-/* The workspace bytes of a call with these sizes (0: none): few tokens over many keys
-   are split over workgroups. It need not be zero-filled; calls that may run at once
+/* The workspace bytes of a call with these sizes (0: none; UINT64_MAX: refused, as the
+   call would be): few tokens over many keys are split over workgroups. It need not be zero-filled; calls that may run at once
    need one each. A call captured into a graph has to bring one where this is not 0. */
 AIGPU_ABI uint64_t aigpu_packed_attention_workspace(const AiGpuPackedAttention* args);
 

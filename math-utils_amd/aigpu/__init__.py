@@ -1356,4 +1356,5 @@ def packed_attention_workspace(q, k, v, out, starts=None, key_starts=None):
     """a workspace (uint8 tensor, perhaps empty) for packed_attention calls of these sizes"""
     args = _packed_attention(q, k, v, out, starts, key_starts, None, 0, 0.0, None, 0.0, None, 0)
     need = lib().aigpu_packed_attention_workspace(C.cast(C.c_char_p(args), C.POINTER(AiGpuPackedAttention)))
+    _check(need != 2 ** 64 - 1)
     return _torch.empty(int(need), dtype=_torch.uint8, device=q.device)

@@ -1430,9 +1430,9 @@ extern "C" {
 AIGPU_ABI uint64_t aigpu_packed_attention_workspace(const AiGpuPackedAttention* args) {
     Context& ctx = Context::instance();
     std::lock_guard<std::recursive_mutex> lock(ctx.gate);
-    if (!args) return ctx.fail("packed attention: null arguments"), 0;
+    if (!args) return ctx.fail("packed attention: null arguments"), UINT64_MAX;
     aigpu::PackedParams p{};
-    return packed_params(ctx, args, p) ? aigpu::packed_attention_workspace(p) : 0;
+    return packed_params(ctx, args, p) ? aigpu::packed_attention_workspace(p) : UINT64_MAX;
 }
 
 AIGPU_ABI int aigpu_packed_attention(const AiGpuPackedAttention* args) {

@@ -372,6 +372,21 @@ bool codes_ok(Context& ctx, const char* who, const PagedCache& c, const void* ke
 // no two rows of `row` elements of the pool share one: each stride spans what the shorter ones do
 bool rows_apart(const PagedCache& c, uint64_t row);
 
+// ---- parts of the checks ----
+/* whether two tensors [tokens][heads][dim] (bytes between tokens and heads) may share an element */
+struct Extent { uintptr_t at; uint64_t tokens, token, heads, head, row; };
+inline bool may_meet(const Extent& a, const Extent& b) {
+    if (!a.tokens || !b.tokens) return false;
+    const uint64_t ra = (a.heads - 1) * a.head + a.row, rb = (b.heads - 1) * b.head + b.row;
+    if (a.at >= b.at + (b.tokens - 1) * b.token + rb || b.at >= a.at + (a.tokens - 1) * a.token + ra) return false;
+    // rows of one token side by side in the same wider rows
+    if (a.token != b.token || !a.token) return true;
+    const uint64_t gap = b.at >= a.at ? (b.at - a.at) % a.token : (a.token - (a.at - b.at) % a.token) % a.token;
+    return !(gap >= ra && a.token - gap >= rb);
+}
+// caps for which the scores' fractions and their multiples stay within fp32
+inline bool cap_ok(float cap) { return cap == 0.0f || (cap >= 1e-6f && cap <= 1e6f); }
+
 // ---- attention of packed documents ----
 struct PackedParams {
     const void* q;

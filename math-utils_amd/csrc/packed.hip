@@ -519,18 +519,6 @@ Shape shape_of(const PackedParams& p) {
     return s;
 }
 
-/* whether two tensors [tokens][heads][dim] (bytes between tokens and heads) may share an element */
-struct Extent { uintptr_t at; uint64_t tokens, token, heads, head, row; };
-bool may_meet(const Extent& a, const Extent& b) {
-    if (!a.tokens || !b.tokens) return false;
-    const uint64_t ra = (a.heads - 1) * a.head + a.row, rb = (b.heads - 1) * b.head + b.row;
-    if (a.at >= b.at + (b.tokens - 1) * b.token + rb || b.at >= a.at + (a.tokens - 1) * a.token + ra) return false;
-    // rows of one token side by side in the same wider rows
-    if (a.token != b.token || !a.token) return true;
-    const uint64_t gap = b.at >= a.at ? (b.at - a.at) % a.token : (a.token - (a.at - b.at) % a.token) % a.token;
-    return !(gap >= ra && a.token - gap >= rb);
-}
-
 } // namespace
 
 bool check_packed_attention(const PackedParams& p) {
@@ -546,8 +534,7 @@ bool check_packed_attention(const PackedParams& p) {
         return ctx.fail("packed attention: without keyStarts there are as many keys as tokens");
     if (!(p.scale > 0.0f) || !std::isfinite(p.scale))
         return ctx.fail("packed attention: the scale must be positive and finite");
-    if (p.cap < 0.0f || !std::isfinite(p.cap))
-        return ctx.fail("packed attention: the cap must be finite and not negative");
+    if (!cap_ok(p.cap)) return ctx.fail("packed attention: the cap must be 0, or 1e-6 .. 1e6");
     for (uint64_t s : {p.qTokenStride, p.qHeadStride, p.kTokenStride, p.kHeadStride, p.vTokenStride, p.vHeadStride,
                        p.outTokenStride, p.outHeadStride})
         if (s >= (uint64_t(1) << 40)) return ctx.fail("packed attention: a stride is out of range");

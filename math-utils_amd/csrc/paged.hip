@@ -285,7 +285,7 @@ bool check_paged_decode(const PagedDecodeParams& p) {
     if (p.form == PAGED_CODES ? !codes_ok(ctx, "paged decode", p.c, p.keyScales, p.valueScales)
                               : !cache_ok(ctx, "paged decode", p.c))
         return false;
-    if (p.cap < 0.0f || !std::isfinite(p.cap)) return ctx.fail("paged decode: the cap must be finite and not negative");
+    if (!cap_ok(p.cap)) return ctx.fail("paged decode: the cap must be 0, or 1e-6 .. 1e6");
     if (reinterpret_cast<uintptr_t>(p.slopes) & 3)
         return ctx.fail("paged decode: the slopes must be aligned to their elements");
     if (!rotation_ok(ctx, "paged decode", p.freqs, p.rot, p.c.dim, p.amplitude)) return false;

@@ -468,8 +468,14 @@ bool launch_paged_append_q4(const PagedAppendQ4Params& q, hipStream_t stream) {
 
 bool check_paged_read_q4(const PagedReadQ4Params& p) {
     Context& ctx = Context::instance();
-    return codes_ok(ctx, "paged read", p.c, p.keyScales, p.valueScales) &&
-           tokens_ok(ctx, "paged read", p.c, p.k, p.v, p.outType, p.starts, p.count, p.kStride, p.vStride);
+    if (!codes_ok(ctx, "paged read", p.c, p.keyScales, p.valueScales) ||
+        !tokens_ok(ctx, "paged read", p.c, p.k, p.v, p.outType, p.starts, p.count, p.kStride, p.vStride))
+        return false;
+    const uint64_t es = p.outType == 1 ? 2 : 4, row = uint64_t(p.c.kvHeads) * p.c.dim * es;
+    const Extent k{reinterpret_cast<uintptr_t>(p.k), p.count, p.kStride * es, 1, row, row};
+    const Extent v{reinterpret_cast<uintptr_t>(p.v), p.count, p.vStride * es, 1, row, row};
+    if (may_meet(k, v)) return ctx.fail("paged read: k and v overlap");
+    return true;
 }
 
 bool launch_paged_read_q4(const PagedReadQ4Params& p, hipStream_t stream) {
