@@ -353,6 +353,14 @@ __device__ __forceinline__ void scales_of(u32x4 scales, half2v (&by)[4], half2v 
         off[i] = by[i] * half2v{_Float16(-24.0f), _Float16(-24.0f)};
     }
 }
+/* the largest of lanes c, c + 16, c + 32 and c + 48, by swaps of lanes that need no LDS */
+__device__ __forceinline__ float over_groups(float x) {
+    const auto a = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+    const uint32_t y = __float_as_uint(fmaxf(__uint_as_float(a[0]), __uint_as_float(a[1])));
+    const auto b = __builtin_amdgcn_permlane32_swap(y, y, false, false);
+    return fmaxf(__uint_as_float(b[0]), __uint_as_float(b[1]));
+}
+
 /* two fp32 values as pairs of fp16 terms: the nearest, then what it leaves */
 __device__ __forceinline__ u32x2 split_f16(float a, float b) {
     const half2v hi = __builtin_convertvector(float2v{a, b}, half2v);
@@ -570,14 +578,14 @@ __global__ __launch_bounds__(THREADS, occupancy(D, FORM)) void paged_attention_k
     u32x4 kr[KRB][KRD];              // keys: rows 16 rb + lane % 16
     u32x4 vr[CODES ? DB : 1];        // 4-bit values: 16 bytes a lane, row after row
     uint32_t ksr[CODES ? (DB + 1) / 2 : 1], vsr[CODES ? (DB + 1) / 2 : 1];   // row `lane`'s scales
-    auto issue = [&](const Slab& s, const Rows& r, int half) -> bool {
+    auto issue = [&](uint32_t pair, Rows r, int half) -> bool {
         const DecodeArgs& a = cold();
         const PagedDecodeParams& p = a.p;
         const PagedCache& c = p.c;
         const int lane = fresh_lane(threadIdx.x & 63), g = lane >> 4, c16 = lane & 15;
         const bool ok = r.page < c.pages;
         const uint64_t mine = (ok ? uint64_t(r.page) * c.pageStride + uint64_t(r.row) * c.rowStride : 0) +
-                              uint64_t(s.pair / a.groups) * c.headStride;
+                              uint64_t(pair / a.groups) * c.headStride;
         wave_sync();
         if (lane < SLAB) place[w][lane] = CODES ? mine * (D / 2) : mine;
         wave_sync();
@@ -926,8 +934,7 @@ __global__ __launch_bounds__(THREADS, occupancy(D, FORM)) void paged_attention_k
             float top = sv[0][0];
 #pragma unroll
             for (int i = 1; i < 16; ++i) top = fmaxf(top, sv[i >> 2][i & 3]);
-            top = fmaxf(top, __shfl_xor(top, 16, WAVE));
-            top = fmaxf(top, __shfl_xor(top, 32, WAVE)) * svBy;
+            top = over_groups(top) * svBy;
             // weights of 2^6, and up to 2^14 before the maximum is taken up anew (their sum
             // carries it too): the second fp16 term of small ones stays above fp16's least
             const bool grow = top > m + 8.0f;
@@ -1101,17 +1108,16 @@ __global__ __launch_bounds__(THREADS, occupancy(D, FORM)) void paged_attention_k
 
     // ---- the pipeline ----
     Slab s0{}, s1{}, s2{};           // computed, in flight, its pages asked for
-    Rows r1{}, r2{};
+    Rows r0{}, r1{}, r2{};
     bool ok0 = true;
     const bool any = list(s0);
     bool more = false, moreThen = false;
     if (any) {
-        Rows r0;
         find(s0, r0);
         more = list(s1);
         if (more) find(s1, r1);
         ask(s0);
-        ok0 = issue(s0, r0, 0);
+        ok0 = issue(s0.pair, r0, 0);
         if constexpr (CODES) issue_keys();
     }
     __builtin_amdgcn_sched_barrier(0);
@@ -1133,7 +1139,14 @@ __global__ __launch_bounds__(THREADS, occupancy(D, FORM)) void paged_attention_k
                 moreThen = list(s2);
                 if (moreThen) find(s2, r2);
                 if (s1.is & OPENS) ask(s1);
-                ok0 = issue(s1, r1, buf ^ 1);
+                if constexpr (!CODES) ok0 = issue(s1.pair, r1, buf ^ 1);
+            }
+            // after the last slab this one's rows are asked for again: were there a way on which
+            // nothing is asked for, the wait for the keys, counted for all ways, would be one for
+            // the next slab's values too
+            if constexpr (CODES) {
+                const uint32_t pair = more ? s1.pair : s0.pair;
+                ok0 = issue(pair, Rows{more ? r1.page : r0.page, more ? r1.row : r0.row}, 0);
             }
         };
         if constexpr (CODES) {
@@ -1143,7 +1156,7 @@ __global__ __launch_bounds__(THREADS, occupancy(D, FORM)) void paged_attention_k
             __builtin_amdgcn_sched_barrier(0);
             score(s0);
             __builtin_amdgcn_sched_barrier(0);
-            if (more) issue_keys();
+            issue_keys();
         } else {
             score(s0);
             __builtin_amdgcn_sched_barrier(0);
@@ -1155,6 +1168,7 @@ __global__ __launch_bounds__(THREADS, occupancy(D, FORM)) void paged_attention_k
         if (!more) break;
         s0 = s1;
         s1 = s2;
+        if constexpr (CODES) r0 = r1;
         r1 = r2;
         more = moreThen;
     }
