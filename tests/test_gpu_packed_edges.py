@@ -157,3 +157,49 @@ def test_long_documents(gpu, dim, dtype, out):
         ref = dict(how, prefix=how["prefix"][0]) if "prefix" in how else how
         want, bound = document64(q, k, v, dtype, out, slopes=slopes, **ref)
         assert (np.abs(host(res) - want) <= bound).all()
+
+
+@pytest.mark.parametrize("dim", [64, 96, 128, 192, 256])
+@pytest.mark.parametrize("dtype,out", [("bf16", "bf16"), ("bf16", "f32"), ("f32", "f32")])
+@pytest.mark.parametrize("new,past,how", [
+    (200, 0, {}), (200, 0, dict(window=45)), (200, 0, dict(prefix=90)), (150, 0, dict(prefix=150, window=20)),
+    (21, 1500, {}), (21, 1500, dict(window=700)),
+])
+def test_rows_that_are_not_finite_reach_those_that_see_them(gpu, dim, dtype, out, new, past, how):
+    """a key or value with NaN or an infinity: NaN (or infinite) for the tokens and heads that
+    see it; the others' results are those of finite rows, to the bit"""
+    import torch
+    n, H, KV = new + past, 4, 2
+    q, k, v = (dev(rounded(O.fill_normal((m, h, dim), 21, s), dtype), dtype)
+               for m, h, s in ((new, H, "q"), (n, KV, "k"), (n, KV, "v")))
+    window, prefix = how.get("window", 0), how.get("prefix", 0)
+    args = dict(starts=vector([0, new]), key_starts=vector([0, n]), window=window)
+    if prefix:
+        args["prefix"] = vector([prefix])
+    plain, got = (torch.zeros((new, H, dim), device="cuda", dtype=torch.bfloat16 if out == "bf16" else torch.float32) for _ in "ab")
+    say("packed wild", dim, dtype, out, new, past, how)
+    gpu.packed_attention(q, k, v, plain, **args)
+    i, j = np.arange(past, n)[:, None], np.arange(n)[None]
+    sees = ((j <= i) | (j < prefix)) & ((window == 0) | (i - j < window))
+    for where, at, bad in (("v", n - 1, np.nan), ("v", n - 17, np.inf), ("k", n - 9, np.nan), ("v", past + 3, -np.inf), ("v", n // 2, np.nan)):
+        kk, vv = k.clone(), v.clone()
+        (kk if where == "k" else vv)[at, 1, dim // 2 + 5] = bad
+        gpu.packed_attention(q, kk, vv, got, **args)
+        a, b = host(plain), host(got)
+        np.testing.assert_array_equal(a[:, :2], b[:, :2])
+        np.testing.assert_array_equal(a[~sees[:, at], 2:], b[~sees[:, at], 2:])
+        assert not np.isfinite(b[sees[:, at], 2:]).all(-1).any()
+
+
+def test_capped_scores_beside_rows_that_are_not_finite(gpu):
+    import torch
+    n, H, dim = 130, 4, 128
+    q, k, v = (rounded(O.fill_normal((n, h, dim), 22, s), "bf16") for h, s in ((H, "q"), (1, "k"), (1, "v")))
+    slopes = np.array([0.3, 0.01, 0.0, 1.0], np.float32)
+    kk, vv = dev(k, "bf16"), dev(v, "bf16")
+    kk[100, 0, 7], vv[101, 0, 0] = np.inf, np.nan
+    out = torch.empty((n, H, dim), device="cuda", dtype=torch.bfloat16)
+    say("packed wild, capped")
+    gpu.packed_attention(dev(q, "bf16"), kk, vv, out, cap=20.0, slopes=dev_f32(slopes))
+    want, bound = document64(q[:100], k[:100], v[:100], "bf16", "bf16", slopes=slopes, cap=20.0)
+    assert (np.abs(host(out)[:100] - want) <= bound).all()
