@@ -601,8 +601,12 @@ Shape shape_of(const PackedParams& p) {
     s.slots = p.starts ? uint64_t(p.count) * group / ROWS_WG + p.documents : full;
     const uint64_t busy = std::max<uint64_t>(full, std::min(p.documents, p.count)) * p.kvHeads, want = 512;
     s.splits = 1;
-    // a split of 256 keys at the least, were the documents alike
-    if (busy && busy * 2 <= want) s.splits = std::max<uint64_t>(std::min<uint64_t>(want / busy, p.keyCount / p.documents / 256), 1);
+    // A split of 512 keys at the least, were the documents alike. Us with splits and without,
+    // 32/8 heads of 128, bf16 to fp32: four documents of 5 to 27 tokens behind 30011 keys 115 and
+    // 865, 8 of 64 behind 2000 47 and 69, 512 behind 8000 141 and 252; 1000 alone 41.7 and 38, 512
+    // alone 28 and 21, as the second launch costs what 500 keys do. Half or twice as many workgroups
+    // take 148 and 122 for the first.
+    if (busy && busy * 2 <= want) s.splits = std::max<uint64_t>(std::min<uint64_t>(want / busy, p.keyCount / p.documents / 512), 1);
     return s;
 }
 

@@ -152,7 +152,14 @@ __device__ __forceinline__ double row_sum64(double x, int lane) {
 /*
     Appending. A workgroup takes a few tokens, D / 8 lanes a row of k or v, 8 elements
     each: read, normed and turned (keys), encoded and stored, a word and a quarter of a
-    scale a lane.
+    scale a lane. A row's loads go out while the one before it is encoded.
+
+    8199 tokens of 8 heads of 128, bf16, normed and turned (34 MB in, 9 MB out): 26 us,
+    1.6 TB/s; without norm and rotation, whose 64 bits the keys take, 20. What bounds it is
+    a workgroup's chain (starts, lengths, page ids, angles, then four rows a lane one after
+    the other), which its registers let four workgroups a CU run at once: five and six spill
+    (36 thousand tokens and their reading back 137 and 146 us against 130). The norm's
+    weights wait in LDS, as in registers they spilled (141). 32 tokens: 5 us, that chain once.
 */
 struct AppendQ4Args {
     PagedAppendQ4Params p;
@@ -168,6 +175,7 @@ __global__ __launch_bounds__(THREADS, 4) void paged_append_q4_kernel(AppendQ4Arg
     __shared__ double rows[NW][8][WAVE];             // element e of each lane's eight
     __shared__ uint64_t base[MAX_TOKENS];            // row of kv head 0, ~0: not written
     __shared__ uint32_t place[MAX_TOKENS];
+    __shared__ double gammas[8][LPR];                // element 8 l + e at [e][l]
     const PagedAppendParams& p = a.p.a;
     const PagedCache& c = p.c;
     const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
@@ -207,6 +215,7 @@ __global__ __launch_bounds__(THREADS, 4) void paged_append_q4_kernel(AppendQ4Arg
         base[mine.own] = mine.page < c.pages ? mine.page * c.pageStride + mine.at * c.rowStride : ~uint64_t(0);
     }
     __syncthreads();
+    if (p.gamma && threadIdx.x < D) gammas[threadIdx.x % 8][threadIdx.x / 8] = double(p.gamma[threadIdx.x]) + double(p.offset);
     const uint32_t half = p.freqs ? p.rot / 2 : 0;
     for (uint32_t i = threadIdx.x; i < nt * half; i += THREADS) {
         double cs, sn;
@@ -215,11 +224,6 @@ __global__ __launch_bounds__(THREADS, 4) void paged_append_q4_kernel(AppendQ4Arg
     }
     __syncthreads();
 
-    double gamma[8] = {};
-    if (p.gamma) {
-#pragma unroll
-        for (int e = 0; e < 8; ++e) gamma[e] = double(p.gamma[d0 + e]) + double(p.offset);
-    }
     // every lane of a wave stays in the loop: the sums and blocks shuffle over all of it
 #pragma unroll 1
     for (uint32_t wave = w * RPW; wave < total; wave += NW * RPW) {
@@ -249,7 +253,7 @@ __global__ __launch_bounds__(THREADS, 4) void paged_append_q4_kernel(AppendQ4Arg
                 const double inv = inverse_root(row_sum64<LPR>(ss, lane) * (1.0 / D) + double(p.eps));
                 if (live && isKey) {
 #pragma unroll
-                    for (int e = 0; e < 8; ++e) y[e] = y[e] * inv * gamma[e];
+                    for (int e = 0; e < 8; ++e) y[e] = y[e] * inv * gammas[e][lane % LPR];
                 }
             }
             if (half) {
@@ -309,7 +313,9 @@ __global__ __launch_bounds__(THREADS, 4) void paged_append_q4_kernel(AppendQ4Arg
 
 /*
     Reading back: the rows that the tokens of a ragged batch have in the pages, as the
-    values that their codes stand for. The workgroups and lanes are append's.
+    values that their codes stand for. The workgroups and lanes are append's; rows are
+    independent, four of them in flight a lane. 8199 tokens of 8 heads of 128 to bf16
+    (9 MB in, 34 MB out): 11 us, 3.9 TB/s, the search of the tokens' sequences included.
 */
 struct ReadQ4Args {
     PagedReadQ4Params p;
@@ -376,11 +382,14 @@ __global__ __launch_bounds__(THREADS) void paged_read_q4_kernel(ReadQ4Args a) {
     }
 }
 
-/* as many tokens as the lanes hold `passes` rows of, fewer where that leaves CUs idle */
-uint32_t tokens_of(uint64_t count, uint32_t kvHeads, uint32_t dim, uint32_t passes) {
-    const uint32_t rows = THREADS / WAVE * (WAVE / (dim / 8)) * passes;
+/* As many tokens as the lanes take four rows of, eight where the workgroups are many (16
+   rounds of them: 36 thousand tokens of 8 heads of 128 121 us against 130, 8 thousand 39
+   against 38), fewer where that leaves CUs idle. */
+uint32_t tokens_of(uint64_t count, uint32_t kvHeads, uint32_t dim) {
+    const uint32_t rows = THREADS / WAVE * (WAVE / (dim / 8)) * 4;
     const uint64_t spread = count / 512;
     uint32_t tokens = rows / (2 * kvHeads);
+    if (tokens && count / tokens > 4096) tokens *= 2;
     if (tokens > spread) tokens = uint32_t(spread);
     return tokens < 1 ? 1 : (tokens > MAX_TOKENS ? MAX_TOKENS : tokens);
 }
@@ -449,7 +458,7 @@ bool launch_paged_append_q4(const PagedAppendQ4Params& q, hipStream_t stream) {
     AppendQ4Args a{};
     a.p = q;
     a.wide = (at & 15) == 0 && (p.count == 1 || (p.kStride | p.vStride) % (16 / es) == 0);
-    a.tokens = tokens_of(p.count, p.c.kvHeads, p.c.dim, 4);
+    a.tokens = tokens_of(p.count, p.c.kvHeads, p.c.dim);
     divide_by(p.c.kvHeads, a.headMagic, a.headShift);
     // 16 tokens of 128 turns are 32 KB
     const size_t each = p.freqs ? size_t(turnsOf(p.rot / 2)) * sizeof(double2) : 0;
@@ -486,7 +495,7 @@ bool launch_paged_read_q4(const PagedReadQ4Params& p, hipStream_t stream) {
     ReadQ4Args a{};
     a.p = p;
     a.wide = (at & 15) == 0 && (p.count == 1 || (p.kStride | p.vStride) % (16 / es) == 0);
-    a.tokens = tokens_of(p.count, p.c.kvHeads, p.c.dim, 4);
+    a.tokens = tokens_of(p.count, p.c.kvHeads, p.c.dim);
     divide_by(p.c.kvHeads, a.headMagic, a.headShift);
     const Tiles tiles((p.count + a.tokens - 1) / a.tokens);
     return ctx.launch("paged_read_q4_kernel", stream, [&] {
