@@ -26,8 +26,17 @@ namespace {
     of 8 keys, which is how the second product takes them.
 
     bf16 in, bf16 out: the weights round to bf16, and the sum adds up the rounded ones.
-    bf16 in, fp32 out: the weights in three bf16 terms, whose sum they are.
+    bf16 in, fp32 out: the weights in three bf16 terms, whose sum they are (two
+    leave 2^-16 of a weight, more than fp32's own roundings).
     fp32 in: fp32 products (v_mfma_f32_32x32x2_f32), for which the keys' order is the plain one.
+
+    Bounded by the matrix cores and the softmax's vector instructions, which take turns in a
+    wave and overlap between the two workgroups of a CU. A causal prompt of 8192 under 32/8
+    heads, bf16: heads of 64 345 us (800 TFLOP/s), 96 450 (915), 128 550 to 565 (970 to 1000),
+    192 775 (1065), 256 1170 (940, at 256 registers with some in scratch); capped 640 (865),
+    biased 625; to fp32 865 (635; its products are double). fp32 of 2048: 64 196 us (88), 128 326
+    (105 of 154).
+    With tanh by exponential and reciprocal the capped one took 955.
 */
 constexpr int WAVES = 4, THREADS = 64 * WAVES, ROWS_WG = 32 * WAVES;
 enum Kind { BF16_OUT = 0, BF16_F32 = 1, FULL = 2 };
@@ -168,6 +177,9 @@ __device__ __forceinline__ void put4(const PackedArgs& a, uint64_t at, const flo
     }
 }
 
+/* Keys of a tile and workgroups a CU: the most that LDS and registers hold for two:
+   256-wide heads at one took 247 us for seven prompts of up to 3001, at two 232, and 172 once
+   the tiles were asked for behind the scores */
 constexpr int tile_keys(int D, int kind) { return kind == FULL ? (D <= 96 ? 64 : 32) : (D <= 128 ? 64 : 32); }
 constexpr int workgroups(int D, int kind) { return D <= (kind == FULL ? 64 : 256) ? 2 : 1; }
 
@@ -181,12 +193,15 @@ __global__ __launch_bounds__(THREADS, workgroups(D, KIND)) void packed_attention
     constexpr int BLOCKS = BN * BPR / WAVE / WAVES;        // DMA blocks (1 KB) of a wave and tile, K or V
     constexpr int QV = KIND == FULL ? D / 8 : D / 16;      // 16-byte pieces of a lane's half query
     static_assert(BN * BPR % (WAVE * WAVES) == 0 && BLOCKS * WAVE % BPR == 0, "whole rows of a tile are the waves' alike");
-    // the queries of 256 do not all stay in registers: what the scores read back must not wait
-    // for a tile that was asked for before it
+    // The queries of 256 do not all stay in registers: three pieces wait in what LDS is left,
+    // and what the scores read back from scratch must not wait for a tile that was asked for
+    // before it.
     constexpr bool LATE = D == 256 && KIND != FULL;
     typedef std::conditional_t<BN == 64, uint16_t, uint8_t> flags;  // a bit each of the BN / WAVES rows of a wave's blocks
     __shared__ __attribute__((aligned(16))) elem ktile[2][BN * D], vtile[2][BN * D];
     __shared__ __attribute__((aligned(8))) flags wild[2][WAVES];
+    constexpr int HELD = LATE ? 3 : 0;                     // pieces of the queries that wait in LDS
+    __shared__ u32x4 held[HELD ? HELD : 1][HELD ? THREADS : 1];
     const PackedParams& p = a.p;
     const int lane = threadIdx.x & 63, w = int(scalar(threadIdx.x >> 6)), g = lane >> 5, c = lane & 31;
 
@@ -244,32 +259,27 @@ __global__ __launch_bounds__(THREADS, workgroups(D, KIND)) void packed_attention
     const int32_t loAll = p.window && pos1 >= 0 && uint64_t(pos1) + 1 > p.window ? int32_t(pos1 + 1 - int64_t(p.window)) : 0;
 
     // the query: elements 16 db + 8 g .. of bf16, D / 2 g .. of fp32
-    u32x4 q[QV];
+    u32x4 q[QV - HELD];
     {
         const elem* src = static_cast<const elem*>(p.q) + (uint64_t(x.first) + token) * p.qTokenStride + head * p.qHeadStride;
 #pragma unroll
-        for (int i = 0; i < QV; ++i)
-            q[i] = *reinterpret_cast<const u32x4*>(src + (KIND == FULL ? D / 2 * g + 4 * i : 16 * i + 8 * g));
+        for (int i = 0; i < QV; ++i) {
+            const u32x4 piece = *reinterpret_cast<const u32x4*>(src + (KIND == FULL ? D / 2 * g + 4 * i : 16 * i + 8 * g));
+            if (i < QV - HELD) q[i] = piece;
+            else held[i - (QV - HELD)][threadIdx.x] = piece;
+        }
     }
     const float slope = p.slopes ? p.slopes[head] * LOG2E : 0.0f;
 
     const elem* keys = static_cast<const elem*>(p.k) + x.key0 * p.kTokenStride + kvh * p.kHeadStride;
     const elem* values = static_cast<const elem*>(p.v) + x.key0 * p.vTokenStride + kvh * p.vHeadStride;
     // Byte offsets of this lane's blocks from a tile's first row. Of 256 channels a block is two
-    // rows, 2 n and 2 n + 1 of the wave's eight: its place is block 0's up to whole rows and a
-    // bit of the swizzle, which spares registers (offsets kept in scratch are read back
-    // between the tile's blocks, and each waits for those before: 1.98 instead of 1.17 ms
-    // at 8192 tokens of 32/8 heads).
-    constexpr int KEPT = LATE ? 1 : BLOCKS;
-    static_assert(!LATE || (BLOCKS == 4 && BPR == 32 && BN == 32), "as the offsets are found from block 0's");
-    uint32_t koff[KEPT], voff[KEPT], kat = 0, vat = 0;
-    if constexpr (LATE) {
-        const uint32_t r = 8 * w + (lane >> 5), at = lane & 31;
-        koff[0] = uint32_t(key_of_row(r) * p.kTokenStride * ES);
-        voff[0] = uint32_t(r * p.vTokenStride * ES);
-        kat = 16 * (at ^ key_swizzle<BYTES>(r));
-        vat = 16 * (at ^ value_swizzle<BYTES>(r));
-    } else {
+    // rows, 2 n and 2 n + 1 of the wave's eight, and its place is found anew each time, which
+    // spares registers (offsets kept in scratch are read back between the tile's blocks, and
+    // each waits for those before: 1.98 ms at 8192 tokens of 32/8 heads in place of 1.17).
+    static_assert(!LATE || (BLOCKS == 4 && BPR == 32 && BN == 32), "as the offsets are found");
+    uint32_t koff[LATE ? 1 : BLOCKS], voff[LATE ? 1 : BLOCKS];
+    if constexpr (!LATE) {
 #pragma unroll
         for (int n = 0; n < BLOCKS; ++n) {
             const uint32_t i = (w * BLOCKS + n) * WAVE + lane, r = i / BPR, at = i % BPR;
@@ -284,14 +294,19 @@ __global__ __launch_bounds__(THREADS, workgroups(D, KIND)) void packed_attention
             const elem* kt = keys + k0 * p.kTokenStride;
             const elem* vt = values + k0 * p.vTokenStride;
             if constexpr (LATE) {
-                uint32_t ka = kat, va = vat;
-                asm volatile("" : "+v"(ka), "+v"(va));     // (each time anew)
+                uint32_t at = threadIdx.x & 63;
+                asm volatile("" : "+v"(at));
+                const uint32_t late = at >> 5;           // of the two rows
+                at = 16 * (at & 31);
+                // row 8 w + 2 n + late of keys is key 4 w + 16 (n >> 1) + 2 (n & 1) + late
+                const uint32_t ka = at ^ 16 * (8 * (w & 1) + late), kl0 = late * uint32_t(p.kTokenStride * ES);
+                const uint32_t va = at ^ 64 * late, vl0 = late * uint32_t(p.vTokenStride * ES);
 #pragma unroll
                 for (int n = 0; n < BLOCKS; ++n)
-                    dma_block(kt + (16 * (n >> 1) + 2 * (n & 1)) * p.kTokenStride, (ka ^ 32 * n) + koff[0], kl + n * 1024);
+                    dma_block(kt + (4 * w + 16 * (n >> 1) + 2 * (n & 1)) * p.kTokenStride, (ka ^ 32 * n) + kl0, kl + n * 1024);
 #pragma unroll
                 for (int n = 0; n < BLOCKS; ++n)
-                    dma_block(vt + 2 * n * p.vTokenStride, (va ^ 128 * (n & 1)) + voff[0], vl + n * 1024);
+                    dma_block(vt + (8 * w + 2 * n) * p.vTokenStride, (va ^ 128 * (n & 1)) + vl0, vl + n * 1024);
             } else {
 #pragma unroll
                 for (int n = 0; n < BLOCKS; ++n) dma_block(kt, koff[n], kl + n * 1024);
@@ -386,13 +401,14 @@ __global__ __launch_bounds__(THREADS, workgroups(D, KIND)) void packed_attention
             for (int kb = 0; kb < KB; ++kb) {
                 const int block = KIND == FULL ? QV * g + i : 2 * i + g;
                 const u32x4 k = *reinterpret_cast<const u32x4*>(ktile[stage] + (32 * kb + c) * D + 16 / ES * (block ^ key_swizzle<BYTES>(c)));
+                const u32x4 qi = i < QV - HELD ? q[i] : held[i - (QV - HELD)][threadIdx.x];
                 if constexpr (KIND == FULL) {
-                    const floatx4 kf = __builtin_bit_cast(floatx4, k), qf = __builtin_bit_cast(floatx4, q[i]);
+                    const floatx4 kf = __builtin_bit_cast(floatx4, k), qf = __builtin_bit_cast(floatx4, qi);
 #pragma unroll
                     for (int j = 0; j < 4; ++j) s[kb] = __builtin_amdgcn_mfma_f32_32x32x2f32(kf[j], qf[j], s[kb], 0, 0, 0);
                 } else {
                     s[kb] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, k),
-                                                                    __builtin_bit_cast(bf16x8, q[i]), s[kb], 0, 0, 0);
+                                                                    __builtin_bit_cast(bf16x8, qi), s[kb], 0, 0, 0);
                 }
             }
         if (LATE && it + 1 < tiles) {
@@ -419,14 +435,25 @@ __global__ __launch_bounds__(THREADS, workgroups(D, KIND)) void packed_attention
                         s[kb][r] = y * tanh_series<series_terms(KIND)>(t, a.series);
                     }
             } else {
+                float C[6];
+#pragma unroll
+                for (int i = 0; i < 6; ++i) {
+                    C[i] = float(TANH6[i]);
+                    if constexpr (LATE) asm volatile("" : "+v"(C[i]));     // (not kept over the loop)
+                }
 #pragma unroll
                 for (int kb = 0; kb < KB; ++kb)
 #pragma unroll
                     for (int r = 0; r < 16; ++r) {
                         const float y = s[kb][r] * a.factor;
-                        if constexpr (KIND == BF16_OUT)
-                            s[kb][r] = a.capLog2 * (1.0f - 2.0f * __builtin_amdgcn_rcpf(__builtin_amdgcn_exp2f(2.0f * LOG2E * y) + 1.0f));
-                        else s[kb][r] = a.capLog2 * tanh_of(y);
+                        if constexpr (KIND == BF16_OUT) {
+                            // both ways without a branch, which would take registers
+                            const float large = 1.0f - 2.0f * __builtin_amdgcn_rcpf(__builtin_amdgcn_exp2f(2.0f * LOG2E * fabsf(y)) + 1.0f);
+                            s[kb][r] = a.capLog2 * (fabsf(y) <= TANH_WITHIN ? y * tanh_series<6>(y * y, C) : copysignf(large, y));
+                        } else {
+                            s[kb][r] = a.capLog2 * tanh_of(y);
+                        }
+                        if constexpr (LATE) __builtin_amdgcn_sched_barrier(0);   // (one after the other, for the registers)
                     }
             }
             by = 1.0f;
@@ -626,6 +653,7 @@ bool check_packed_attention(const PackedParams& p) {
     if (!(p.scale > 0.0f) || !std::isfinite(p.scale))
         return ctx.fail("packed attention: the scale must be positive and finite");
     if (!cap_ok(p.cap)) return ctx.fail("packed attention: the cap must be 0, or 1e-6 .. 1e6");
+    if (p.cap > 0.0f && !std::isnormal(p.scale / p.cap)) return ctx.fail("packed attention: the scale does not suit the cap");
     for (uint64_t s : {p.qTokenStride, p.qHeadStride, p.kTokenStride, p.kHeadStride, p.vTokenStride, p.vHeadStride,
                        p.outTokenStride, p.outHeadStride})
         if (s >= (uint64_t(1) << 40)) return ctx.fail("packed attention: a stride is out of range");
@@ -682,7 +710,13 @@ bool launch_packed_attention(const PackedParams& p, void* work, hipStream_t stre
         double power = double(p.cap) * 1.4426950408889634 * a.factor;
         for (int i = 0; i < series_terms(kind); ++i, power *= double(a.factor) * a.factor)
             a.series[i] = float((kind == BF16_OUT ? TANH4[i] : TANH6[i]) * power);
-        a.within = TANH_WITHIN / a.factor;
+        float within = TANH_WITHIN;
+        // four terms are off by 7e-6 of a score: kept below 2^-10, as a weight's rounding to bf16 is
+        if (kind == BF16_OUT) within = std::min(within, 0x1p-10f / 7e-6f / p.cap);
+        a.within = within / a.factor;
+        // a cap far from 1 may leave terms that fp32 does not hold: then none are used
+        for (int i = 0; i < series_terms(kind); ++i)
+            if (!std::isnormal(a.series[i])) a.within = -1.0f;
     }
     const uint64_t es = p.inType == 1 ? 2 : 4;
     a.fits = (uint64_t(64) * (p.kTokenStride > p.vTokenStride ? p.kTokenStride : p.vTokenStride) + p.dim) * es < (uint64_t(1) << 31);

@@ -307,6 +307,7 @@ bool check_paged_decode(const PagedDecodeParams& p) {
     }
     if (!(p.scale > 0.0f) || !std::isfinite(p.scale))
         return ctx.fail("paged decode: the scale must be positive and finite");
+    if (p.cap > 0.0f && !std::isnormal(p.scale / p.cap)) return ctx.fail("paged decode: the scale does not suit the cap");
     if (p.maxLength > uint64_t(p.c.tableWidth) * p.c.pageSize)
         return ctx.fail("paged decode: maxLength exceeds the positions of the table");
     if (p.maxLength > (1u << 31)) return ctx.fail("paged decode: maxLength must be at most 2^31");

@@ -46,6 +46,22 @@ namespace {
     where a copy of 256 or 512 MB moves 5.9. Small calls are a chain of about 15 us:
     dispatch, lengths and list 4, page ids and queries 2, a first slab 3, its
     weights 1, the joins 5 (one sequence of 4096 under 16/8 heads, 16.8 MB: 15).
+
+    The forms are kernels of their own, so that the plain one keeps its registers: scored
+    (a cap's tanh, a bias by distance), and codes, the scored one over 4-bit pages:
+      slabs    64 positions (9.2 KB of 128 channels), as 16 rows of a group are read
+               transposed at once (ds_read_b64_tr_b4) and four groups read together
+      keys     codes to registers, unpacked there into exact fp16; a lane takes a quarter
+               of a row, so its scales are two at most
+      values   codes through registers into LDS, read back transposed, unpacked per column
+      products v_mfma_f32_16x16x32_f16: the pages' values exactly, q and the weights in two
+               fp16 terms (22 bits), brought to a power of two where both hold
+    32 sequences of 1k to 32k under 32/4 heads of 128 (312 MB): 87 to 93 us, 3.3 to 3.6 TB/s;
+    11 us with a position or two each, 4.4 us a slab of each wave on top. A slab is some 650
+    vector instructions of a wave (420 of them unpack), 2.6 of those 4.4 us for a SIMD's two
+    waves, and 64 matrix ones: what is left is loads that two waves of one slab each do not
+    cover. One workgroup a CU takes 114 us, three (128 channels) spill and take twice the
+    time; of 64 channels three fit.
 */
 constexpr bool scored(int form) { return form != PAGED_PLAIN; }
 // positions of a slab: 4-bit rows are read 64 at a time, as their values are transposed in LDS
@@ -307,6 +323,7 @@ __device__ __forceinline__ void join_parts(const DecodeArgs& a, const Parts& par
     }
 }
 
+/* workgroups a CU: what registers and LDS hold without spilling */
 constexpr int occupancy(int D, int form) { return form == PAGED_CODES && D == 64 ? 3 : (D <= 128 ? 2 : 1); }
 
 /*

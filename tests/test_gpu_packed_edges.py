@@ -203,3 +203,36 @@ def test_capped_scores_beside_rows_that_are_not_finite(gpu):
     gpu.packed_attention(dev(q, "bf16"), kk, vv, out, cap=20.0, slopes=dev_f32(slopes))
     want, bound = document64(q[:100], k[:100], v[:100], "bf16", "bf16", slopes=slopes, cap=20.0)
     assert (np.abs(host(out)[:100] - want) <= bound).all()
+
+
+@pytest.mark.parametrize("dtype,out", [("bf16", "bf16"), ("bf16", "f32"), ("f32", "f32")])
+@pytest.mark.parametrize("cap", [1e-6, 1e-3, 1.0, 300.0, 2e4, 1e6])
+def test_caps_of_any_size(gpu, dtype, out, cap):
+    """scores of 0, far below the cap, about it and past it, whatever the cap"""
+    import torch
+    n, H, dim = 200, 4, 128
+    q, k, v = (O.fill_normal((n, h, dim), 23, s) for h, s in ((H, "q"), (1, "k"), (1, "v")))
+    q[::5] *= 1e-4
+    q[1::5] *= 30.0
+    q[2::5] *= min(cap, 1e3)
+    q[7] = 0.0
+    q, k, v = (rounded(x, dtype) for x in (q, k, v))
+    res = torch.empty((n, H, dim), device="cuda", dtype=torch.bfloat16 if out == "bf16" else torch.float32)
+    say("packed cap", cap, dtype, out)
+    gpu.packed_attention(dev(q, dtype), dev(k, dtype), dev(v, dtype), res, cap=cap)
+    want, bound = document64(q, k, v, dtype, out, cap=cap)
+    assert (np.abs(host(res) - want) <= bound).all()
+
+
+@pytest.mark.parametrize("cap", [1e-6, 1e-3, 300.0, 1e6])
+def test_decode_caps_of_any_size(gpu, cap):
+    import torch
+    cache = CacheQ4([300, 64, 1], 1, 16, 128, 24)
+    q, out = O.fill_normal((3, 4, 128), 24, "q"), torch.empty((3, 4, 128), device="cuda")
+    q[:, 0] = 0.0
+    q[:, 1] *= min(cap, 30.0)
+    say("q4 cap", cap)
+    gpu.paged_decode_q4(dev_f32(q), out, *cache.device(), cap=cap)
+    for b, n in enumerate(cache.lengths):
+        want, bound = scored64(q[b], *cache.rows(b), n - 1, cap=cap, terms=2, product=4.0)
+        assert (np.abs(host(out)[b] - want) <= bound).all(), b

@@ -150,6 +150,12 @@ def test_packed_attention_refuses(change, why):
     _refused("aigpu_packed_attention", why, _packed(**change))
 
 
+def test_a_scale_that_leaves_no_number_over_the_cap():
+    for scale, cap in ((1e33, 1e-6), (1e-38, 1e6)):
+        _refused("aigpu_packed_attention", "suit", _packed(scale=scale, cap=cap))
+        _refused("aigpu_paged_decode_scored", "suit", _decode(scale=scale), aigpu.AiGpuScores(cap=cap))
+
+
 def test_sound_calls_miss_only_the_device():
     lattice = dict(qTokenStride=12 * 128, kTokenStride=12 * 128, vTokenStride=12 * 128, outTokenStride=12 * 128)
     row = 2 * 128
