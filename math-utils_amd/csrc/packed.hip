@@ -678,7 +678,7 @@ bool check_packed_attention(const PackedParams& p) {
         if (may_meet(out, e)) return ctx.fail("packed attention: out overlaps q, k or v");
     const Shape s = shape_of(p);
     if (uint64_t(p.count) * (p.heads / p.kvHeads) >= (uint64_t(1) << 31) - ROWS_WG ||
-        s.slots * s.splits * p.kvHeads >= (uint64_t(1) << 31))
+        s.slots * s.splits * p.kvHeads >= (uint64_t(1) << 32) / THREADS)     // a launch's threads
         return ctx.fail("packed attention: too many rows");
     return true;
 }

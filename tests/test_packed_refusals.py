@@ -156,6 +156,11 @@ def test_a_scale_that_leaves_no_number_over_the_cap():
         _refused("aigpu_paged_decode_scored", "suit", _decode(scale=scale), aigpu.AiGpuScores(cap=cap))
 
 
+def test_more_workgroups_than_a_launch_has():
+    _refused("aigpu_packed_attention", "many", _packed(documents=2 ** 24))
+    _refused("aigpu_packed_attention", "no usable gfx950 device", _packed(documents=2 ** 20))
+
+
 def test_sound_calls_miss_only_the_device():
     lattice = dict(qTokenStride=12 * 128, kTokenStride=12 * 128, vTokenStride=12 * 128, outTokenStride=12 * 128)
     row = 2 * 128
