@@ -34,8 +34,8 @@ namespace {
     wave and overlap between the two workgroups of a CU. A causal prompt of 8192 under 32/8
     heads, bf16: heads of 64 345 us (800 TFLOP/s), 96 450 (915), 128 550 to 565 (970 to 1000),
     192 775 (1065), 256 1170 (940, three pieces of the queries in scratch); capped 625 to
-    650 (865), 980 where every tile has scores past the series; biased 620; to fp32 865 (635; its products are double). fp32 of 2048: 64 196 us (88), 128 326
-    (105 of 154).
+    650 (865), 980 where every tile has scores past the series; biased 620; to fp32 865 (635;
+    its products are double). fp32 of 2048: 64 196 us (88), 128 326 (105 of 154).
 */
 constexpr int WAVES = 4, THREADS = 64 * WAVES, ROWS_WG = 32 * WAVES;
 enum Kind { BF16_OUT = 0, BF16_F32 = 1, FULL = 2 };
