@@ -767,9 +767,10 @@ AIGPU_ABI uint64_t aigpu_paged_decode_q4_workspace(const AiGpuPagedDecodeQ4* arg
 /*    (more tokens than keys: the first ones). Rows of out that no document    */
 /*    has stay as they were. The starts do not decrease, nor pass count and    */
 /*    keyCount (nothing outside is touched where they do, but documents may be */
-/*    left out). A row of keys or values that is not finite makes NaN or       */
-/*    infinities of the tokens that see it, not of others; rows of no document */
-/*    may hold anything.                                                       */
+/*    left out). A value that is not finite makes NaN or an infinity of its    */
+/*    channel of the tokens that see it, and of nothing else; a key that makes */
+/*    a score NaN or +infinity makes NaN of the tokens that see it. Rows of no */
+/*    document may hold anything.                                              */
 /*    Types: q, k, v of inType, out of outType. bf16 to bf16 rounds the        */
 /*    weights to bf16 (their sum adds the rounded ones) and the result once;   */
 /*    bf16 to fp32 takes the weights whole, in three terms; fp32 is fp32       */

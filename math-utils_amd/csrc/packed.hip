@@ -154,6 +154,24 @@ __device__ __forceinline__ uint32_t unbounded(uint32_t x) {
     return ((x & EXPONENT) + ONE) & (BF ? 0x80008000u : 0x80000000u);
 }
 
+/* the same bits with zeros for the values that are not finite */
+template <bool BF>
+__device__ __forceinline__ uint32_t bounded(uint32_t x) {
+    return x & ~((unbounded<BF>(x) >> (BF ? 15 : 31)) * (BF ? 0xFFFFu : 0xFFFFFFFFu));
+}
+
+/* four elements of a row of values */
+__device__ __forceinline__ void get4(const uint16_t* at, float (&x)[4]) {
+    const u32x2 two = *reinterpret_cast<const u32x2*>(at);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) x[i] = __uint_as_float(i & 1 ? two[i / 2] & 0xFFFF0000u : two[i / 2] << 16);
+}
+__device__ __forceinline__ void get4(const float* at, float (&x)[4]) {
+    const floatx4 four = *reinterpret_cast<const floatx4*>(at);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) x[i] = four[i];
+}
+
 /* four elements of an out row */
 __device__ __forceinline__ void put4(const PackedArgs& a, uint64_t at, const float (&x)[4]) {
     if (a.p.outType == 1) {
@@ -334,9 +352,10 @@ __global__ __launch_bounds__(THREADS, workgroups(D, KIND)) void packed_attention
     };
 
     // A weight of 0 does not take a value that is not finite out of the product. In a tile that
-    // some row does not see whole, a row of values with one becomes zeros, each wave its own
-    // blocks', and the rows that see it get NaN (1% of the time of 8192 tokens, 2% of 32
-    // documents of 1000, whose tiles are cut more often).
+    // some row does not see whole, each wave makes zeros of such elements among its own blocks',
+    // notes their rows, and the rows that see them get them back by themselves: their own channels
+    // alone, as in a tile that all see (1% of the time of 8192 tokens, 2% of 32 documents of
+    // 1000, whose tiles are cut more often).
     auto tame = [&](int stage) {
         uint32_t at = lane;              // (its own, so that nothing of this is kept over the loop)
         asm volatile("" : "+v"(at)::"memory");
@@ -356,7 +375,12 @@ __global__ __launch_bounds__(THREADS, workgroups(D, KIND)) void packed_attention
             found = all;
 #pragma unroll 1
             for (int n = 0; n < BLOCKS; ++n)
-                if (found >> ((n * WAVE + at) / BPR) & 1) blocks[n * WAVE] = u32x4{0, 0, 0, 0};
+                if (found >> ((n * WAVE + at) / BPR) & 1) {
+                    u32x4 x = blocks[n * WAVE];
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) x[i] = bounded<KIND != FULL>(x[i]);
+                    blocks[n * WAVE] = x;
+                }
         }
         if (at == 0) wild[stage][w] = flags(found);
     };
@@ -380,15 +404,6 @@ __global__ __launch_bounds__(THREADS, workgroups(D, KIND)) void packed_attention
         const bool idle = !busy || int32_t(k0) >= hi1 || int32_t(k0 + BN) <= lo0;
         if ((!LATE || idle) && it + 1 < tiles) issue(k0 + BN, stage ^ 1);
         if (idle) continue;
-        if (partial) {
-            typedef std::conditional_t<BN == 64, uint64_t, uint32_t> bits;
-            const bits rows = *reinterpret_cast<const bits*>(wild[stage]);
-            if (__any(rows != 0)) {
-                const int32_t from = lo > int32_t(k0) ? lo - int32_t(k0) : 0, to = hi < int32_t(k0 + BN) ? hi - int32_t(k0) : BN;
-                if (to > from && rows >> from << (BN - to + from)) l = NAN;
-            }
-        }
-
         floatx16 s[KB];
 #pragma unroll
         for (int kb = 0; kb < KB; ++kb)
@@ -548,6 +563,31 @@ __global__ __launch_bounds__(THREADS, workgroups(D, KIND)) void packed_attention
                         for (int t = TERMS - 1; t >= 0; --t)
                             o[dt] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(v, __builtin_bit_cast(bf16x8, term[t]), o[dt], 0, 0, 0);
                     }
+                }
+            }
+        }
+        if (partial) {
+            typedef std::conditional_t<BN == 64, uint64_t, uint32_t> bits;
+            bits rows = *reinterpret_cast<const bits*>(wild[stage]);
+            if (__any(rows != 0)) {
+                int half = threadIdx.x >> 5 & 1;                 // g (its own, so that nothing of this is kept over the loop)
+                asm volatile("" : "+v"(half));
+#pragma unroll 1
+                for (; rows; rows &= rows - 1) {
+                    const int32_t at = int32_t(k0) + (BN == 64 ? __builtin_ctzll(rows) : __builtin_ctz(uint32_t(rows)));
+                    if (at < lo || at >= hi) continue;
+                    const elem* row = values + uint32_t(at) * p.vTokenStride + 4 * half;
+#pragma unroll
+                    for (int dt = 0; dt < DT; ++dt)
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) {
+                            float y[4];
+                            get4(row + 32 * dt + 8 * i, y);
+#pragma unroll
+                            for (int e = 0; e < 4; ++e)
+                                if (unbounded<false>(__float_as_uint(y[e]))) o[dt][4 * i + e] += y[e];
+                            __builtin_amdgcn_sched_barrier(0);   // (one after the other, for the registers)
+                        }
                 }
             }
         }
