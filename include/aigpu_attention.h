@@ -769,7 +769,8 @@ AIGPU_ABI uint64_t aigpu_paged_decode_q4_workspace(const AiGpuPagedDecodeQ4* arg
 /*    keyCount (nothing outside is touched where they do, but documents may be */
 /*    left out). A value that is not finite makes NaN or an infinity of its    */
 /*    channel of the tokens that see it, and of nothing else; a key that makes */
-/*    a score NaN or +infinity makes NaN of the tokens that see it. Rows of no */
+/*    a score NaN or +infinity makes NaN of the tokens that see it, and so do  */
+/*    scores that are all -infinity (as in 12's and 13's decode). Rows of no   */
 /*    document may hold anything.                                              */
 /*    Types: q, k, v of inType, out of outType. bf16 to bf16 rounds the        */
 /*    weights to bf16 (their sum adds the rounded ones) and the result once;   */

@@ -147,6 +147,14 @@ __device__ __forceinline__ bool find_work(const PackedArgs& a, uint32_t slot, in
     return slot - slot0 < (x.rows + ROWS_WG - 1) / ROWS_WG;
 }
 
+/* What a row's weighted values are multiplied by for its weights' sum l. A token sees its own
+   position, if that is not before its keys, and the prefix: zeros where that is nothing. Scores
+   that are all -infinity leave no weights: NaN, as in the paged decode. */
+__device__ __forceinline__ float share_of(const Work& x, uint32_t token, float l) {
+    if (x.shift + int32_t(token) < 0 && x.prefix == 0) return 0.0f;
+    return l == 0.0f ? NAN : 1.0f / l;
+}
+
 /* whether a value's bits (two bf16 or one fp32) are not all finite: an exponent of ones */
 template <bool BF>
 __device__ __forceinline__ uint32_t unbounded(uint32_t x) {
@@ -616,7 +624,7 @@ __global__ __launch_bounds__(THREADS, workgroups(D, KIND)) void packed_attention
                     floatx4{o[dt][4 * i], o[dt][4 * i + 1], o[dt][4 * i + 2], o[dt][4 * i + 3]};
         return;
     }
-    const float by = l == 0.0f ? 0.0f : 1.0f / l;          // nothing seen: zeros
+    const float by = share_of(x, r0.token, l);
     const uint64_t to = (uint64_t(x.first) + r0.token) * p.outTokenStride + r0.head * p.outHeadStride + 4 * g;
 #pragma unroll
     for (int dt = 0; dt < DT; ++dt)
@@ -651,7 +659,7 @@ __global__ __launch_bounds__(THREADS) void packed_merge_kernel(PackedArgs a) {
         o += *reinterpret_cast<const floatx4*>(at + 2 * ROWS_WG + r * D + d) * f;
     }
     const uint32_t row = x.row0 + r, token = token_of(a, row), head = kvh * a.group + row - token * a.group;
-    const float by = l == 0.0f ? 0.0f : 1.0f / l;
+    const float by = share_of(x, token, l);
     const float y[4] = {o[0] * by, o[1] * by, o[2] * by, o[3] * by};
     put4(a, (uint64_t(x.first) + token) * p.outTokenStride + head * p.outHeadStride + d, y);
 }

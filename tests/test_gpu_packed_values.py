@@ -5,6 +5,7 @@ import pytest
 
 from gpu_util import host, say
 from oracle import oracle as O
+from packed_util import document64
 from paged_util import rounded
 from test_gpu_packed import dev, vector
 
@@ -61,3 +62,41 @@ def test_an_infinity_keeps_its_sign(gpu, dtype, out):
     assert (got[:, 9] == -np.inf).all()
     assert np.isfinite(got[:7, 70]).all() and (got[7:11, 70] == np.inf).all() and np.isnan(got[11:, 70]).all()
     assert np.isfinite(np.delete(got, [9, 70], 1)).all()
+
+
+@pytest.mark.parametrize("dim", [64, 128, 256])
+@pytest.mark.parametrize("dtype,out", [("bf16", "bf16"), ("bf16", "f32"), ("f32", "f32")])
+def test_scores_that_are_all_minus_infinity(gpu, dim, dtype, out):
+    """no weight is left: NaN, in one call's documents, behind split keys and in the decode alike; a key whose score
+    is -infinity leaves the weights to the others; a token that sees nothing gets zeros"""
+    import torch
+    new, sizes, kv = [40, 3, 9], [40, 3000, 4], 1
+    starts, keys = np.cumsum([0] + new), np.cumsum([0] + sizes)
+    q, k, v = (rounded(O.fill_normal((m, h, dim), 33, s), dtype)
+               for m, h, s in ((starts[-1], 2, "q"), (keys[-1], kv, "k"), (keys[-1], kv, "v")))
+    q[..., 0] = np.abs(q[..., 0]) + 1
+    q = rounded(q, dtype)
+    k[0, 0, 0] = -np.inf                   # of the first document, its first key
+    k[keys[1]:keys[2], 0, 0] = -np.inf     # of the second, all; the third has five tokens before its keys
+    res = torch.full((starts[-1], 2, dim), 3.0, device="cuda", dtype=torch.bfloat16 if out == "bf16" else torch.float32)
+    tensors = dev(q, dtype), dev(k, dtype), dev(v, dtype), res
+    for alone in (False, True):
+        say("packed no weights", dim, dtype, out, alone)
+        # many documents' keys are few on average, the second one's by themselves enough to be split
+        for b in [slice(i, i + 1) for i in range(3)] if alone else [slice(0, 3)]:
+            at, ka = slice(starts[b.start], starts[b.stop]), slice(keys[b.start], keys[b.stop])
+            call = tensors[0][at], tensors[1][ka], tensors[2][ka], res[at]
+            how = dict(starts=vector((starts[b.start:b.stop + 1] - starts[b.start]).tolist()),
+                       key_starts=vector((keys[b.start:b.stop + 1] - keys[b.start]).tolist()))
+            assert (gpu.packed_attention_workspace(*call, **how).numel() > 0) == (alone and b.start == 1)
+            gpu.packed_attention(*call, **how)
+        got = host(res)
+        assert np.isnan(got[0]).all() and np.isnan(got[40:43]).all()
+        assert (got[43:48] == 0).all() and np.isfinite(got[48:]).all()
+        want, bound = document64(q[1:40], k[1:40], v[1:40], dtype, out)
+        assert (np.abs(got[1:40] - want) <= bound).all()
+        res.fill_(3.0)
+    pages = dev(k[keys[1]:keys[1] + 16], "bf16").reshape(1, 1, 16, dim)
+    one = torch.zeros((1, 2, dim), device="cuda")
+    gpu.paged_decode(dev(q[:1], "f32"), one, pages, pages.nan_to_num(neginf=0.0), vector([[0]]), vector([16]))
+    assert np.isnan(host(one)).all()
