@@ -735,7 +735,8 @@ typedef struct AiGpuPagedReadQ4 {
 AIGPU_ABI int aigpu_paged_read_q4(const AiGpuPagedReadQ4* args);
 
 /* As aigpu_paged_decode_scored, over 4-bit pages: fp32 throughout, the products taking
-   q and the weights in two fp16 terms each (22 bits) and the pages' values exactly. */
+   the pages' values exactly, q and the weights in two fp16 terms each: 22 bits, but
+   none below 2^-38 of the head's largest element of q and 2^-40 of its largest weight. */
 typedef struct AiGpuPagedDecodeQ4 {
     AiGpuPagedCacheQ4 cache;
     const void* q;

@@ -55,7 +55,8 @@ namespace {
                of a row, so its scales are two at most
       values   codes through registers into LDS, read back transposed, unpacked per column
       products v_mfma_f32_16x16x32_f16: the pages' values exactly, q and the weights in two
-               fp16 terms (22 bits), brought to a power of two where both hold
+               fp16 terms (22 bits), brought to a power of two where both hold down to
+               2^-38 and 2^-40 of the largest
     32 sequences of 1k to 32k under 32/4 heads of 128 (312 MB): 87 to 93 us, 3.3 to 3.6 TB/s;
     11 us with a position or two each, 4.4 us a slab of each wave on top. A slab is some 650
     vector instructions of a wave (420 of them unpack), 2.6 of those 4.4 us for a SIMD's two
@@ -862,7 +863,7 @@ __global__ __launch_bounds__(THREADS, occupancy(D, FORM)) void paged_attention_k
         }
     };
 
-    float m = -INFINITY, l = 0.0f;   // of head c16; l of this lane's positions
+    float m = -INFINITY, l = 0.0f;   // of head c16; l of this lane's positions; weights are 2^(score - m)
     floatx4 acc[CT];                 // [tile][r]: head 4 g + r, column 16 tile + c16
     bool bad = false, begun = false;
     float sv[KRB][4];                // scores: of head c16 at positions 16 rb + 4 g + i
@@ -952,10 +953,15 @@ __global__ __launch_bounds__(THREADS, occupancy(D, FORM)) void paged_attention_k
 #pragma unroll
             for (int i = 1; i < 16; ++i) top = fmaxf(top, sv[i >> 2][i & 3]);
             top = over_groups(top) * svBy;
-            // weights of 2^6, and up to 2^14 before the maximum is taken up anew (their sum
-            // carries it too): the second fp16 term of small ones stays above fp16's least
-            const bool grow = top > m + 8.0f;
-            const float next = grow ? top : m;
+            // Weights up to 2^15: their terms are whole numbers of 2^-24, so that a weight is off by
+            // its 22 bits or by 2^-40 of the largest, which many small ones add up to no more than
+            // fp32's own roundings do. m is what the weights are powers over, 15 below the
+            // largest score (7 below, where fp32 has no number there and 16 would be too much).
+            // Raising it only by 2^8 at a time, which leaves 2^-31, takes the same times.
+            const bool grow = top - m > 15.0f;
+            float next = top - 15.0f;
+            if (top - next > 15.0f) next = top - 7.0f;
+            next = grow ? next : m;
             if (__any(grow)) {
                 const float keep = grow ? __builtin_amdgcn_exp2f(m - next) : 1.0f;
                 l *= keep;
@@ -971,11 +977,11 @@ __global__ __launch_bounds__(THREADS, occupancy(D, FORM)) void paged_attention_k
 #pragma unroll
             for (int t = 0; t < CT; ++t) asm("" : "+v"(acc[t]));
             m = next;
-            const float under = (next == -INFINITY ? 0.0f : next) - 6.0f;
+            const float base = next == -INFINITY ? 0.0f : next;
             float pv[16], sum = 0.0f;
 #pragma unroll
             for (int i = 0; i < 16; ++i) {
-                pv[i] = __builtin_amdgcn_exp2f(fmaf(sv[i >> 2][i & 3], svBy, -under));
+                pv[i] = __builtin_amdgcn_exp2f(fmaf(sv[i >> 2][i & 3], svBy, -base));
                 sum += pv[i];
             }
             l += sum;
