@@ -835,7 +835,7 @@ __global__ __launch_bounds__(THREADS, occupancy(D, FORM)) void paged_attention_k
             top = fmaxf(top, __shfl_xor(top, 16, WAVE));
             top = fmaxf(top, __shfl_xor(top, 32, WAVE));
             int power = 14 - __builtin_amdgcn_frexp_expf(top);
-            power = power < -100 ? -100 : (power > 100 ? 100 : power);
+            power = power > 100 ? 100 : power;       // -114 for fp32's largest
             const float up = ldexpf(1.0f, power);
             qpow = ldexpf(1.0f, -power);
 #pragma unroll

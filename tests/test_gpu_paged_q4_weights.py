@@ -3,6 +3,8 @@ import numpy as np
 import pytest
 
 from gpu_util import dev_f32, host, say
+from oracle import oracle as O
+from paged_q4_util import CacheQ4
 
 pytestmark = pytest.mark.gpu
 
@@ -47,3 +49,25 @@ def test_many_small_weights_beside_a_large_one(gpu, dim, batch, n, kv, place):
     far = host(out)
     assert (np.abs(far[..., :dim // 2] - 7.0 * tail) <= 7.0 * (n * 2.0 ** -40 + tail * (score + alike + adds))).all()
     assert (np.abs(far[..., dim // 2:] - 7.0) <= 7.0 * (n * 2.0 ** -40 + alike + adds)).all()
+
+
+@pytest.mark.parametrize("dim", [64, 128, 256])
+@pytest.mark.parametrize("size", [1e34, 1e35, 1e36, 1e37])
+def test_queries_of_any_size(gpu, dim, size):
+    """queries near fp32's largest, over keys that keep the scores within it, pick one key; beside such a head, others
+    are as they are by themselves"""
+    cache = CacheQ4([130, 20], 2, 16, dim, 34, size=1e-3)
+    q = O.fill_normal((2, 4, dim), 8, "q")
+    large = q.copy()
+    large[:, 1::2] *= np.float32(size)
+    import torch
+    alone, got = (torch.empty((2, 4, dim), device="cuda") for _ in "ab")
+    say("decode_q4 large queries", dim, size)
+    gpu.paged_decode_q4(dev_f32(q), alone, *cache.device(), scale=1.0)
+    gpu.paged_decode_q4(dev_f32(large), got, *cache.device(), scale=1.0)
+    np.testing.assert_array_equal(host(got)[:, ::2], host(alone)[:, ::2])
+    for b in range(2):
+        keys, values = cache.rows(b)
+        for h in (1, 3):
+            best = (keys[:, h // 2] @ large[b, h].astype(np.float64)).argmax()
+            np.testing.assert_allclose(host(got)[b, h], values[best, h // 2], rtol=1e-6, atol=0)
