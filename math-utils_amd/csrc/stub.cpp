@@ -1,5 +1,5 @@
 // stub.cpp - the no-device backend: every entry point of
-// include/aigpu_attention.h answers "unavailable" (0 or null) and
+// include/aigpu_attention.h answers "unavailable" (0, null or its refusal) and
 // aigpu_last_error() says why, as the reference's src/gpu/Stub.cpp:18-66 does
 // for DeviceABI.h. Linked in place of libaigpu.so where there is no ROCm, so
 // callers take their CPU path through the same availability check they need
@@ -71,7 +71,7 @@ AIGPU_ABI int aigpu_paged_append(const AiGpuPagedAppend*) { return 0; }
 AIGPU_ABI int aigpu_paged_decode(const AiGpuPagedDecode*) { return 0; }
 AIGPU_ABI uint64_t aigpu_paged_decode_workspace(const AiGpuPagedDecode*) { return 0; }
 AIGPU_ABI int aigpu_packed_attention(const AiGpuPackedAttention*) { return 0; }
-AIGPU_ABI uint64_t aigpu_packed_attention_workspace(const AiGpuPackedAttention*) { return 0; }
+AIGPU_ABI uint64_t aigpu_packed_attention_workspace(const AiGpuPackedAttention*) { return UINT64_MAX; }   // 0: none needed
 AIGPU_ABI int aigpu_paged_decode_scored(const AiGpuPagedDecode*, const AiGpuScores*) { return 0; }
 AIGPU_ABI int aigpu_paged_append_q4(const AiGpuPagedAppendQ4*) { return 0; }
 AIGPU_ABI int aigpu_paged_read_q4(const AiGpuPagedReadQ4*) { return 0; }
