@@ -126,12 +126,13 @@ __device__ __forceinline__ void rotation64_at(uint32_t pos, float freq, double& 
     sn = turn == 0 ? s : (turn == 1 ? c : (turn == 2 ? -s : -c));
 }
 
-/* 1 / sqrt(x) in 64 bits: the instruction's 26 bits or so, twice improved */
+/* 1 / sqrt(x) in 64 bits: the instruction's 26 bits or so, twice improved; 0 for infinity,
+   which the steps would make NaN of: an element that is infinite is its own block's alone */
 __device__ __forceinline__ double inverse_root(double x) {
     double y = __builtin_amdgcn_rsq(x);
 #pragma unroll
     for (int i = 0; i < 2; ++i) y = fma(y * 0.5, fma(-x * y, y, 1.0), y);
-    return y;
+    return x == INFINITY ? 0.0 : y;
 }
 
 /* where a token's turn j stands: those that neighbouring lanes read together, together */
