@@ -800,9 +800,15 @@ typedef struct AiGpuPackedAttention {
     void* stream;
 } AiGpuPackedAttention;
 AIGPU_ABI int aigpu_packed_attention(const AiGpuPackedAttention* args);
-/* The workspace bytes of a call with these sizes (0: none; UINT64_MAX: refused, as the
-   call would be): few tokens over many keys are split over workgroups. It need not be zero-filled; calls that may run at once
-   need one each. A call captured into a graph has to bring one where this is not 0. */
+/* The workspace bytes of a call with these sizes and this window, no more than without
+   one (0: none; UINT64_MAX: refused, as the call would be): few tokens over many keys
+   are split over workgroups. How far, the sizes alone decide, as the starts are on the
+   device: keyCount / documents keys each, of which a window leaves its own, and one
+   workgroup of rows a kv head for each place, also those without tokens. A long history
+   among many short ones or many empty places is therefore split less or not at all, and
+   takes longer than by itself; a batch of chunks is best given without empty places.
+   The workspace need not be zero-filled; calls that may run at once need one each. A
+   call captured into a graph has to bring one where this is not 0. */
 AIGPU_ABI uint64_t aigpu_packed_attention_workspace(const AiGpuPackedAttention* args);
 
 /* ------------------------------------------------------------------------ */

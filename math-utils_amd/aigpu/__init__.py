@@ -1353,7 +1353,7 @@ def packed_attention(q, k, v, out, starts=None, key_starts=None, prefix=None, wi
 
 
 def packed_attention_workspace(q, k, v, out, starts=None, key_starts=None):
-    """a workspace (uint8 tensor, perhaps empty) for packed_attention calls of these sizes"""
+    """a workspace (uint8 tensor, perhaps empty) for packed_attention calls of these sizes, whatever their window"""
     args = _packed_attention(q, k, v, out, starts, key_starts, None, 0, 0.0, None, 0.0, None, 0)
     need = lib().aigpu_packed_attention_workspace(C.cast(C.c_char_p(args), C.POINTER(AiGpuPackedAttention)))
     _check(need != 2 ** 64 - 1)

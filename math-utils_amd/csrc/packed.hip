@@ -666,21 +666,28 @@ __global__ __launch_bounds__(THREADS) void packed_merge_kernel(PackedArgs a) {
 
 struct Shape { uint64_t slots, splits; };
 
-/* Few rows over many keys leave CUs idle: their keys are split over workgroups, two a CU,
-   whose records a second launch joins. How the rows lie in slots only the device knows: a
-   document has one at least. */
+/* Few rows over many keys leave CUs idle: their keys are split over workgroups, two a CU of
+   256 (fp32 rows from 96 channels on run one after the other there), whose records a second
+   launch joins. How rows and keys lie in documents only the device knows: a document is taken
+   to have one slot and the average's keys, so places without tokens and one long history among
+   short ones are split less than they could be. */
 Shape shape_of(const PackedParams& p) {
     const uint64_t group = p.heads / p.kvHeads, full = (uint64_t(p.count) * group + ROWS_WG - 1) / ROWS_WG;
     Shape s{};
     s.slots = p.starts ? uint64_t(p.count) * group / ROWS_WG + p.documents : full;
     const uint64_t busy = std::max<uint64_t>(full, std::min(p.documents, p.count)) * p.kvHeads, want = 512;
     s.splits = 1;
-    // A split of 512 keys at the least, were the documents alike. Us with splits and without,
+    // A split of 512 keys at the least, were the documents alike: of those that a window leaves
+    // a document's tokens. Us with splits and without,
     // 32/8 heads of 128, bf16 to fp32: four documents of 5 to 27 tokens behind 30011 keys 115 and
     // 865, 8 of 64 behind 2000 47 and 69, 512 behind 8000 141 and 252; 1000 alone 41.7 and 38, 512
     // alone 28 and 21, as the second launch costs what 500 keys do. Half or twice as many workgroups
     // take 148 and 122 for the first.
-    if (busy && busy * 2 <= want) s.splits = std::max<uint64_t>(std::min<uint64_t>(want / busy, p.keyCount / p.documents / 512), 1);
+    if (busy && busy * 2 <= want) {
+        uint64_t keys = p.keyCount / p.documents;
+        if (p.window && p.window < keys) keys = std::min<uint64_t>(keys, p.window + p.count / p.documents);
+        s.splits = std::max<uint64_t>(std::min<uint64_t>(want / busy, keys / 512), 1);
+    }
     return s;
 }
 
