@@ -49,8 +49,9 @@ __device__ __forceinline__ float load_elem(const void* base, size_t i, int type)
 __device__ __forceinline__ float softplus_of(float x) { return x > 20.0f ? x : log1pf(expf(x)); }
 __device__ __forceinline__ float sigmoid_of(float x) { return 1.0f / (1.0f + expf(-x)); }
 
-/* tanh to 2 units of fp32's last place: its series below 0.625 (five terms fitted over
-   that range), 1 - 2 / (e^2x + 1) past it */
+/* tanh to 2 units of fp32's last place, by a published scheme (S. L. Moshier, Methods and
+   Programs for Mathematical Functions): an odd polynomial below 0.625 (its five terms fitted
+   here over that range), 1 - 2 / (e^2x + 1) past it */
 __device__ __forceinline__ float tanh_of(float x) {
     const float t = x * x, a = fabsf(x);
     const float small =

@@ -25,17 +25,23 @@ namespace {
     The rows of a key tile stand in LDS in the order that makes a lane's 16 scores two runs
     of 8 keys, which is how the second product takes them.
 
-    bf16 in, bf16 out: the weights round to bf16, and the sum adds up the rounded ones.
+    bf16 in, bf16 out: the weights round to bf16, and the sum adds up the rounded ones. Next to
+    the result's own rounding (1.6e-3 of it rms, 2.0e-3 with both for a prompt of 2048) a second
+    term would spare little and cost 30%: 695 us in place of 535 for 8192 tokens of 128-wide
+    heads. Who needs the weights whole takes fp32 out.
     bf16 in, fp32 out: the weights in three bf16 terms, whose sum they are (two
-    leave 2^-16 of a weight, more than fp32's own roundings).
+    leave 2^-16 of a weight, more than fp32's own roundings do).
     fp32 in: fp32 products (v_mfma_f32_32x32x2_f32), for which the keys' order is the plain one.
 
-    Bounded by the matrix cores and the softmax's vector instructions, which take turns in a
-    wave and overlap between the two workgroups of a CU. A causal prompt of 8192 under 32/8
-    heads, bf16: heads of 64 345 us (800 TFLOP/s), 96 450 (915), 128 550 to 565 (970 to 1000),
-    192 775 (1065), 256 1170 (940, three pieces of the queries in scratch); capped 625 to
-    650 (865), 980 where every tile has scores past the series; biased 620; to fp32 865 (635;
-    its products are double). fp32 of 2048: 64 196 us (88), 128 326 (105 of 154).
+    bf16 is bounded by the matrix cores and the softmax's vector instructions, which take turns
+    in a wave and overlap between the two workgroups of a CU. A causal prompt of 8192 under 32/8
+    heads: heads of 64 330 to 345 us (800 to 840 TFLOP/s), 96 450 to 460 (900), 128 535 to 565
+    (970 to 1030), 192 775 to 815 (1010 to 1065), 256 1050 to 1140 (965 to 1045, eight registers
+    of the queries in scratch); capped 620 to 660 (835 to 885), 980 where every tile has scores
+    past the series; biased 620 to 640; to fp32 865 to 915 (600 to 635; its products are double).
+    fp32 is bounded by the matrix cores alone, whose products take eight times the softmax: 2048
+    tokens of 64 channels 197 us (87 TFLOP/s of 154), 96 243 (106), 128 327 (105). From 96
+    channels on one workgroup fits a CU, and nothing runs there while it waits at a tile's barrier.
 */
 constexpr int WAVES = 4, THREADS = 64 * WAVES, ROWS_WG = 32 * WAVES;
 enum Kind { BF16_OUT = 0, BF16_F32 = 1, FULL = 2 };
@@ -231,7 +237,8 @@ __global__ __launch_bounds__(THREADS, workgroups(D, KIND)) void packed_attention
     const int lane = threadIdx.x & 63, w = int(scalar(threadIdx.x >> 6)), g = lane >> 5, c = lane & 31;
 
     // consecutive workgroups go round the 8 XCDs: give each XCD a run of them, so that
-    // the rows that share a kv head's keys share an L2. Late rows, which see most, go first.
+    // the rows that share a kv head's keys share an L2, where the grid is a multiple of 8 (8 kv
+    // heads always; others go round as they come). Late rows, which see most, go first.
     uint32_t id = blockIdx.x;
     if (gridDim.x % 8 == 0) id = id % 8 * (gridDim.x / 8) + id / 8;
     const uint32_t split = id % a.splits, kvh = id / a.splits / a.slots, slot = a.slots - 1 - id / a.splits % a.slots;
@@ -469,7 +476,7 @@ __global__ __launch_bounds__(THREADS, workgroups(D, KIND)) void packed_attention
                     for (int r = 0; r < 16; ++r) {
                         const float y = s[kb][r] * a.factor;
                         if constexpr (KIND == BF16_OUT) {
-                            // both ways without a branch, which would take registers
+                            // tanh_of without its branch and division, which would take registers
                             const float large = 1.0f - 2.0f * __builtin_amdgcn_rcpf(__builtin_amdgcn_exp2f(2.0f * LOG2E * fabsf(y)) + 1.0f);
                             s[kb][r] = a.capLog2 * (fabsf(y) <= TANH_WITHIN ? y * tanh_series<6>(y * y, C) : copysignf(large, y));
                         } else {
@@ -765,7 +772,8 @@ bool launch_packed_attention(const PackedParams& p, void* work, hipStream_t stre
         for (int i = 0; i < series_terms(kind); ++i, power *= double(a.factor) * a.factor)
             a.series[i] = float((kind == BF16_OUT ? TANH4[i] : TANH6[i]) * power);
         float within = TANH_WITHIN;
-        // four terms are off by 7e-6 of a score: kept below 2^-10, as a weight's rounding to bf16 is
+        // four terms are off by 7e-6 of a score: kept below 2^-10, a quarter of a weight's
+        // rounding to bf16 (six terms for all: the same errors in three digits, 655 us in place of 620 at 8192)
         if (kind == BF16_OUT) within = std::min(within, 0x1p-10f / 7e-6f / p.cap);
         a.within = within / a.factor;
         // a cap far from 1 may leave terms that fp32 does not hold: then none are used

@@ -57,11 +57,11 @@ namespace {
       products v_mfma_f32_16x16x32_f16: the pages' values exactly, q and the weights in two
                fp16 terms (22 bits), brought to a power of two where both hold down to
                2^-38 and 2^-40 of the largest
-    32 sequences of 1k to 32k under 32/4 heads of 128 (312 MB): 87 to 93 us, 3.3 to 3.6 TB/s;
+    32 sequences of 1k to 32k under 32/4 heads of 128 (312 MB): 86 to 89 us, 3.5 to 3.6 TB/s;
     11 us with a position or two each, 4.4 us a slab of each wave on top. A slab is some 650
     vector instructions of a wave (420 of them unpack), 2.6 of those 4.4 us for a SIMD's two
-    waves, and 64 matrix ones: what is left is loads that two waves of one slab each do not
-    cover. One workgroup a CU takes 114 us, three (128 channels) spill and take twice the
+    waves, and 64 matrix ones: the 1.8 that are left, 30 us in all, are loads that two waves of
+    one slab each do not cover (a slab's keys are asked for behind the scores). One workgroup a CU takes 114 us, three (128 channels) spill and take twice the
     time; of 64 channels three fit.
 */
 constexpr bool scored(int form) { return form != PAGED_PLAIN; }
@@ -324,7 +324,8 @@ __device__ __forceinline__ void join_parts(const DecodeArgs& a, const Parts& par
     }
 }
 
-/* workgroups a CU: what registers and LDS hold without spilling */
+/* workgroups a CU: what registers and LDS hold (fp32 queries over 4-bit pages spill 5 registers at
+   128 channels and 10 at 256) */
 constexpr int occupancy(int D, int form) { return form == PAGED_CODES && D == 64 ? 3 : (D <= 128 ? 2 : 1); }
 
 /*
