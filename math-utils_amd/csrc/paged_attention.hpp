@@ -61,8 +61,9 @@ namespace {
     11 us with a position or two each, 4.4 us a slab of each wave on top. A slab is some 650
     vector instructions of a wave (420 of them unpack), 2.6 of those 4.4 us for a SIMD's two
     waves, and 64 matrix ones: the 1.8 that are left, 30 us in all, are loads that two waves of
-    one slab each do not cover (a slab's keys are asked for behind the scores). One workgroup a CU takes 114 us, three (128 channels) spill and take twice the
-    time; of 64 channels three fit.
+    one slab each do not cover (a slab's keys are asked for behind the scores). One workgroup a
+    CU takes 114 us, three (128 channels) spill and take twice the time; of 64 channels three
+    fit.
 */
 constexpr bool scored(int form) { return form != PAGED_PLAIN; }
 // positions of a slab: 4-bit rows are read 64 at a time, as their values are transposed in LDS
